@@ -16,6 +16,7 @@ from .lora import ExpertsLoRA
 from .arch.deepseek_v4 import DeepseekV4Experts4bit, DeepseekV4ExpertsNbit
 from .arch.gptoss import GptOssExperts4bit, GptOssExpertsMxfp4, GptOssExpertsNbit
 from .ops import gemm_4bit_grouped, gemm_mxfp4_grouped
+from .quant import quantize_mxfp4
 from .train import disable_fast_train, enable_fast_train
 
 __version__ = "0.1.0"
@@ -38,4 +39,5 @@ __all__ = [
     "gemm_4bit_grouped",
     "gemm_mxfp4_grouped",
     "normalize_quant_type",
+    "quantize_mxfp4",
 ]

@@ -66,6 +66,13 @@ E4B_DEV uint32_t pack2(uint16_t lo, uint16_t hi) {
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
+// Maximum over the aligned quad of lanes.
+E4B_DEV uint32_t quad_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
+  return v;
+}
+
 // ------------------------------------------------------------- fp16 operands of bf16 data
 // Power-of-two shift that puts values whose largest biased exponent (fp32 / bf16 field) is e
 // into [2^14, 2^15): below fp16's largest finite value, with fp16's 11 significant bits for

@@ -533,13 +533,7 @@ E4B_DEV void pair_chunk_dots(const uint4 (&qa)[CPL], const uint4 (&qb)[CPL], con
 }
 
 // bf16 -> scaled fp16 restaging of activations (up kernel, NF4 weights): bf16_exp_max gives a
-// 16-byte piece's largest exponent field.
-// Maximum over the aligned quad of lanes (the four pieces of one 32-value chunk).
-E4B_DEV uint32_t quad_max(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
-  return v;
-}
+// 16-byte piece's largest exponent field, quad_max that of the four pieces of one 32-value chunk.
 
 // Shift that puts a chunk whose largest biased exponent is e into [2^14, 2^15).
 E4B_DEV int chunk_shift(uint32_t exp_bits) { return exp_shift(static_cast<int>(exp_bits >> 7)); }

@@ -24,6 +24,7 @@
 #include "gemv.h"
 #include "lora.h"
 #include "lora_mfma.h"
+#include "mx.h"
 #include "quantize.h"
 #include "route.h"
 #include "scale.h"
@@ -475,6 +476,26 @@ int e4b_quantize_8bit(const float* values, const float* offset, int64_t rows, in
   hipLaunchKernelGGL(e4b::quantize8_kernel, dim3(static_cast<unsigned>(rows * blocks)), dim3(e4b::kQuant8Block), 0,
                      stream, values, offset, n, blocks, mids, zero_code, codes, absmax);
   return check_launch("quantize8_kernel");
+}
+
+int e4b_quantize_mxfp4(const void* x, int32_t dtype, int64_t values, void* blocks, void* scales, hipStream_t stream) {
+  if (values < 0 || values % e4b::kMxBlock)
+    return fail(E4B_EINVAL, "%lld values are not whole blocks of %d", (long long)values, e4b::kMxBlock);
+  if (!any_dtype_ok(dtype)) return fail(E4B_EINVAL, "bad dtype %d", dtype);
+  if (values == 0) return E4B_OK;
+  if (!x || !blocks || !scales) return fail(E4B_EINVAL, "x/blocks/scales pointer is NULL");
+  if (!aligned16(x) || !aligned16(blocks)) return fail(E4B_EINVAL, "x and blocks must be 16-byte aligned");
+  const int64_t pieces = values / 8, grid = cdiv(pieces, e4b::kMxThreads * e4b::kMxUnroll);
+  if (grid > 0x7fffffff) return fail(E4B_EUNSUPPORTED, "%lld values are more than one launch covers", (long long)values);
+  auto* c = static_cast<uint32_t*>(blocks);
+  auto* e = static_cast<uint8_t*>(scales);
+  const dim3 g(static_cast<unsigned>(grid)), b(e4b::kMxThreads);
+  switch (dtype) {
+    case E4B_FP32: hipLaunchKernelGGL(e4b::mx_quantize_kernel<E4B_FP32>, g, b, 0, stream, x, pieces, c, e); break;
+    case E4B_BF16: hipLaunchKernelGGL(e4b::mx_quantize_kernel<E4B_BF16>, g, b, 0, stream, x, pieces, c, e); break;
+    default: hipLaunchKernelGGL(e4b::mx_quantize_kernel<E4B_FP16>, g, b, 0, stream, x, pieces, c, e); break;
+  }
+  return check_launch("mx_quantize_kernel");
 }
 
 int e4b_route(const int64_t* top_k_index, int64_t tokens, int32_t top_k, int32_t num_experts, const e4b_routing* rt,

@@ -211,6 +211,26 @@ def quantize_8bit(values: torch.Tensor, offset: torch.Tensor, mids: torch.Tensor
     return codes, absmax
 
 
+def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``[..., k]`` dense values (``k`` a multiple of 32) -> MXFP4 (blocks uint8 ``[..., k/2]``, scales
+    e8m0 uint8 ``[..., k/32]``)."""
+    _require_cuda(w)
+    x = w.detach()
+    x = (x if x.dtype in _DT else x.float()).contiguous()
+    if x.data_ptr() % 16:  # a view that starts inside another tensor
+        x = x.clone()
+    k = x.shape[-1]
+    if k % 32:
+        raise ValueError(f"K={k} is not a multiple of 32")
+    blocks = torch.empty(*x.shape[:-1], k // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-1], k // 32, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        N.check("e4b_quantize_mxfp4",
+                N.lib().e4b_quantize_mxfp4(x.data_ptr(), dtype_code(x.dtype), x.numel(), blocks.data_ptr(),
+                                           scales.data_ptr(), _stream(x.device)))
+    return blocks, scales
+
+
 # ------------------------------------------------------------------------------ routing
 
 

@@ -235,7 +235,16 @@ def quantize_mxfp4(w: torch.Tensor, group: int = 32):
     """OCP MX e2m1 quantization of ``[..., K]`` rows: per 32 values an e8m0 exponent
     ``floor(log2(amax)) - 2 + 127`` (clamped to [0, 254]) and each value rounded to the nearest
     e2m1 magnitude (ties to the even code, saturating at 6). Low nibble = first value.
-    Returns ``(blocks [..., K/2] uint8, scales [..., K/32] uint8)``."""
+    Returns ``(blocks [..., K/2] uint8, scales [..., K/32] uint8)``. On a HIP device one pass of the
+    library's kernel, bit for bit the torch formulation below it."""
+    if group == 32 and w.dim() > 0 and w.numel() > 0 and w.shape[-1] % 32 == 0 and _plain_on_device(w):
+        from . import ops
+
+        return ops.quantize_mxfp4(w)
+    return _quantize_mxfp4_torch(w, group)
+
+
+def _quantize_mxfp4_torch(w: torch.Tensor, group: int = 32):
     w = w.float()
     K = w.shape[-1]
     if K % group:
@@ -245,7 +254,9 @@ def quantize_mxfp4(w: torch.Tensor, group: int = 32):
     safe = torch.where(amax > 0, amax, torch.ones_like(amax))
     X = torch.where(amax > 0, torch.floor(torch.log2(safe)) - 2, torch.full_like(amax, -127.0))
     e = torch.clamp(X + 127, 0, 254)
-    scaled = g.double() / torch.pow(2.0, (e - 127).double()).unsqueeze(-1)
+    # 2^(e - 127) from its bits: torch's fp64 pow on a HIP device is an ulp off at some powers of two,
+    # which moves values that lie exactly between two codes
+    scaled = g.double() / ((e.to(torch.int64) + (1023 - 127)) << 52).view(torch.float64).unsqueeze(-1)
     mag = scaled.abs()
     grid = torch.tensor(FP4_VALUES[:8], dtype=torch.float64, device=w.device)
     mids = (grid[:-1] + grid[1:]) / 2.0
