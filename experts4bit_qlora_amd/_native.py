@@ -40,6 +40,8 @@ EXPORTS = (
     "e4b_route_groups",
     "e4b_gather_rows",
     "e4b_grouped_gemm",
+    "e4b_mx_gemm_workspace_bytes",
+    "e4b_mx_grouped_gemm",
     "e4b_combine",
     "e4b_lora_delta",
     "e4b_lora_delta_epilogue",
@@ -151,6 +153,10 @@ def _bind(L):
     L.e4b_gather_rows.argtypes = [P, I64, I64, P, P, P, I32, I64, P, P]
     L.e4b_grouped_gemm.restype = ctypes.c_int
     L.e4b_grouped_gemm.argtypes = [P, I32, I32, QW, RT, I64, I64, I32, F32, F32, I32, P, I32, P]
+    L.e4b_mx_gemm_workspace_bytes.restype = ctypes.c_size_t
+    L.e4b_mx_gemm_workspace_bytes.argtypes = [I64, I64]
+    L.e4b_mx_grouped_gemm.restype = ctypes.c_int
+    L.e4b_mx_grouped_gemm.argtypes = [P, I32, ctypes.POINTER(ctypes.c_int64), I32, P, QW, P, ctypes.c_size_t, P, I32, P]
     L.e4b_combine.restype = ctypes.c_int
     L.e4b_combine.argtypes = [P, I32, P, P, I32, I64, I32, I64, P, I32, P]
     L.e4b_lora_delta.restype = ctypes.c_int

@@ -25,6 +25,7 @@
 #include "lora.h"
 #include "lora_mfma.h"
 #include "mx.h"
+#include "mx_launch.h"
 #include "quantize.h"
 #include "route.h"
 #include "scale.h"
@@ -224,6 +225,22 @@ int check_weight(const e4b_qweight* w) {
   }
   return E4B_OK;
 }
+
+// A weight stack of the microscaled products: MXFP4, k a multiple of its 32-value blocks.
+int check_mx_weight(const e4b_qweight* w) {
+  if (!w) return fail(E4B_EINVAL, "weight descriptor is NULL");
+  if (w->format != E4B_FMT_MXFP4) return fail(E4B_EUNSUPPORTED, "microscaled products take MXFP4 weights (format %d)", w->format);
+  if (w->num_experts <= 0 || w->n <= 0 || w->k <= 0)
+    return fail(E4B_EINVAL, "weight dims must be positive (E=%d n=%lld k=%lld)", w->num_experts, (long long)w->n,
+                (long long)w->k);
+  if (w->k % 32) return fail(E4B_EUNSUPPORTED, "k=%lld is not a multiple of 32", (long long)w->k);
+  if (w->n > 0x7fffffffLL || w->k > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "n or k exceeds int32");
+  if (!w->packed || !w->absmax) return fail(E4B_EINVAL, "packed/absmax pointer is NULL");
+  if (!aligned16(w->packed)) return fail(E4B_EINVAL, "packed weights must be 16-byte aligned");
+  return E4B_OK;
+}
+
+size_t mx_row_bytes(int64_t k) { return size_t(e4b::mx_chunks(k)) * (e4b::kMxChunk / 2); }
 
 int check_routing(const e4b_routing* rt, int64_t M) {
   if (!rt) return fail(E4B_EINVAL, "routing descriptor is NULL");
@@ -697,6 +714,58 @@ int e4b_grouped_gemm(const void* a, int32_t act_dtype, int32_t gather_k, const e
                      int32_t out_dtype, hipStream_t stream) {
   return grouped_gemm_impl(a, act_dtype, gather_k, w, rt, tokens, M, epilogue, alpha, limit, flags, out, out_dtype,
                            nullptr, stream);
+}
+
+size_t e4b_mx_gemm_workspace_bytes(int64_t rows, int64_t k) {
+  if (rows <= 0 || k <= 0) return 0;
+  return align256(size_t(rows) * mx_row_bytes(k)) + align256(size_t(rows) * e4b::mx_chunks(k) * 8);
+}
+
+int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, int32_t groups,
+                        const int64_t* expert_ids, const e4b_qweight* w, void* workspace, size_t workspace_bytes,
+                        void* out, int32_t out_dtype, hipStream_t stream) {
+  int rc = check_mx_weight(w);
+  if (rc) return rc;
+  if (!act_dtype_ok(act_dtype)) return fail(E4B_EINVAL, "act_dtype must be bf16 or fp16 (got %d)", act_dtype);
+  if (!any_dtype_ok(out_dtype)) return fail(E4B_EINVAL, "bad out_dtype %d", out_dtype);
+  if (groups < 0 || groups > e4b::kMxGroupsMax)
+    return fail(E4B_EUNSUPPORTED, "groups=%d outside [0, %d]", groups, e4b::kMxGroupsMax);
+  if (groups > 0 && (!sizes || !expert_ids)) return fail(E4B_EINVAL, "sizes/expert_ids is NULL");
+  e4b::MxGroups go{};
+  int64_t M = 0;
+  for (int g = 0; g < groups; ++g) {
+    if (sizes[g] < 0) return fail(E4B_EINVAL, "group %d has a negative size", g);
+    go.off[g] = static_cast<int32_t>(M);
+    M += sizes[g];
+    if (M > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "groups hold more than 2^31 - 1 rows");
+  }
+  for (int g = groups; g <= e4b::kMxGroupsMax; ++g) go.off[g] = static_cast<int32_t>(M);
+  if (M == 0) return E4B_OK;
+  if (!a || !out) return fail(E4B_EINVAL, "a/out is NULL");
+  if (!aligned16(a) || !aligned16(out)) return fail(E4B_EINVAL, "a and out must be 16-byte aligned");
+  const size_t need = e4b_mx_gemm_workspace_bytes(M, w->k);
+  if (!workspace || workspace_bytes < need)
+    return fail(E4B_ESPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(E4B_EINVAL, "workspace must be 16-byte aligned");
+  // one launch covers 2^31 - 1 workgroups: of the rows' quantization, and of 32-row x 32-column tiles
+  if (M * e4b::mx_chunks(w->k) / 8 >= 0x7fffffffLL ||
+      max_tiles_for(M, groups, 32) * cdiv(w->n, 32) >= 0x7fffffffLL)
+    return fail(E4B_EUNSUPPORTED, "%lld rows are more than one launch covers", (long long)M);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + align256(size_t(M) * mx_row_bytes(w->k));
+  e4b::launch_mx_rows(a, act_dtype, M, w->k, codes, scales, stream);
+  rc = check_launch("mx_rows_kernel");
+  if (rc) return rc;
+  e4b::MxGemmArgs args{};
+  args.a = codes;
+  args.as = scales;
+  args.w = *w;
+  args.ids = expert_ids;
+  args.groups = groups;
+  args.M = M;
+  args.out = out;
+  e4b::launch_mx_gemm_groups(args, go, out_dtype, stream);
+  return check_launch("mx_narrow_kernel");
 }
 
 int e4b_weight_shift(const e4b_qweight* w, int32_t* shift, hipStream_t stream) {

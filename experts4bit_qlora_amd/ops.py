@@ -734,12 +734,58 @@ def _nf4_code_on(device) -> torch.Tensor:
     return t
 
 
-def gemm_mxfp4_grouped(a: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, sizes, expert_ids) -> torch.Tensor:
+def gemm_mxfp4_grouped(a: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, sizes, expert_ids,
+                       act_quant: str | None = None) -> torch.Tensor:
     """Drop-in for ``mxfp4_grouped.gemm_mxfp4_grouped(a, blocks[E,N,K/2], scales[E,N,K/32], sizes, ids)``
-    (engines/nvme_experts.py:852-865); host or device ids as for gemm_4bit_grouped."""
+    (engines/nvme_experts.py:852-865); host or device ids as for gemm_4bit_grouped.
+
+    ``act_quant="mxfp4"`` (beyond the reference) quantizes the rows of ``a`` to MXFP4 as
+    ``quantize_mxfp4`` does and multiplies the two microscaled operands on the block-scaled matrix
+    cores (``e4b_mx_grouped_gemm``): ``[M, N]`` in ``a``'s dtype, up to 512 groups, K a multiple of 32."""
     E, n, kh = blocks.shape
     qw = mxfp4_qweight(blocks, scales, n, kh * 2, num_experts=E)
-    return _grouped_call(a, qw, sizes, expert_ids)
+    if act_quant is None:
+        return _grouped_call(a, qw, sizes, expert_ids)
+    if act_quant != "mxfp4":
+        raise ValueError(f"act_quant must be None or 'mxfp4', got {act_quant!r}")
+    return mx_grouped_gemm(a, qw, sizes, expert_ids)
+
+
+def mx_grouped_gemm(a: torch.Tensor, qw: QW, sizes, expert_ids) -> torch.Tensor:
+    """``gemm_mxfp4_grouped(..., act_quant="mxfp4")`` on a weight descriptor: ``[M, n]`` in ``a``'s dtype."""
+    _require_cuda(a, qw.packed)
+    G = len(sizes)
+    if torch.is_tensor(expert_ids) and expert_ids.is_cuda:
+        ids = expert_ids if expert_ids.dtype == torch.int64 else expert_ids.to(torch.int64)
+        ids = ids.contiguous()
+    else:
+        host = [int(e) for e in (expert_ids.tolist() if torch.is_tensor(expert_ids) else expert_ids)]
+        if any(not 0 <= e < qw.num_experts for e in host):
+            raise ValueError("bad expert ids")
+        ids = torch.tensor(host, dtype=torch.int64, device=a.device)
+    if ids.numel() != G:
+        raise ValueError("sizes and expert_ids differ in length")
+    host_sizes = (ctypes.c_int64 * max(G, 1))(*sizes)
+    M = sum(host_sizes[:G])
+    if a.dim() != 2 or a.shape[0] != M:
+        raise ValueError(f"a has {a.shape[0]} rows but sizes sum to {M}")
+    if a.shape[1] != qw.k:
+        raise ValueError(f"a has {a.shape[1]} columns but the weights have k={qw.k}")
+    for t in (ids, qw.packed, qw.absmax):
+        if t.device != a.device:
+            raise ValueError("a, the weights and expert_ids must be on one device")
+    L = N.lib()
+    x = a.detach().contiguous()
+    if x.data_ptr() % 16:  # a view that starts inside another tensor
+        x = x.clone()
+    dt = dtype_code(x.dtype)
+    out = torch.empty(M, qw.n, dtype=x.dtype, device=x.device)
+    ws = torch.empty(max(1, L.e4b_mx_gemm_workspace_bytes(M, qw.k)), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        N.check("e4b_mx_grouped_gemm",
+                L.e4b_mx_grouped_gemm(x.data_ptr(), dt, host_sizes, G, ids.data_ptr(), qw.ref(), ws.data_ptr(), ws.numel(),
+                                      out.data_ptr(), dt, _stream(x.device)))
+    return out
 
 
 def gather_rows(dst: torch.Tensor, src_addr: torch.Tensor, ident: torch.Tensor, have: torch.Tensor, n_bytes: int,

@@ -182,6 +182,24 @@ int e4b_grouped_gemm(const void* a, int32_t act_dtype, int32_t gather_k, const e
                      const e4b_routing* rt, int64_t tokens, int64_t M, int32_t epilogue, float alpha,
                      float limit, int32_t flags, void* out, int32_t out_dtype, hipStream_t stream);
 
+/* Bytes of workspace e4b_mx_grouped_gemm needs for `rows` activation rows of k values. */
+size_t e4b_mx_gemm_workspace_bytes(int64_t rows, int64_t k);
+
+/* Grouped product of microscaled operands (both e2m1 with one e8m0 scale per 32 values): the rows
+ * [sum(sizes[:g]), sum(sizes[:g + 1])) of a (E4B_BF16 / E4B_FP16 [M, w->k]) are quantized as
+ * e4b_quantize_mxfp4 does and multiplied by the MXFP4 weights of expert expert_ids[g] (int64 on the
+ * device, read only there, in any order):
+ *   out[m, n] = sum over blocks b of 2^(sa[m, b] + sw[n, b] - 254) * sum_{i < 32} a[m, b, i] * w[n, b, i],
+ * products exact, sums fp32, one rounding into out_dtype (E4B_BF16 / E4B_FP16 / E4B_FP32). A block of a row
+ * with an infinity or a NaN makes that row NaN, a weight scale byte of 255 its column's sums; rows of an id
+ * outside [0, E) are zero. sizes is a host array, read before the call returns; groups <= 512. w is MXFP4, k a
+ * multiple of 32, w->bias is not read; a, out and workspace are 16-byte aligned.
+ * The product of mxfp4_grouped.gemm_mxfp4_grouped (engines/nvme_experts.py:852-865) on the block-scaled
+ * matrix cores, with activations in the weights' format; the reference's activations stay 16-bit. */
+int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, int32_t groups,
+                        const int64_t* expert_ids, const e4b_qweight* w, void* workspace, size_t workspace_bytes,
+                        void* out, int32_t out_dtype, hipStream_t stream);
+
 /* Deterministic weighted combine back to token order:
  * out[t, :] = out_dtype( sum_{s<k} float(down[inv[t*k+s], :]) * float(top_k_weights[t, s]) ),
  * the slots summed in slot order in fp32 -- unique writes + a fixed-axis sum, never atomics.

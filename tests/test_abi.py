@@ -306,3 +306,41 @@ def test_integration_binding_matches_header_and_native():
 def test_routing_and_lora_structs_match_header():
     assert [f[0] for f in N.Routing._fields_] == _header_fields("e4b_routing")
     assert [f[0] for f in N.Lora._fields_] == _header_fields("e4b_lora")
+
+
+def test_quantize_mxfp4_rejects_bad_arguments():
+    L = N.lib()
+    assert L.e4b_quantize_mxfp4(4096, N.BF16, 48, 4096, 4096, None) == -1 and "blocks of 32" in _err()
+    assert L.e4b_quantize_mxfp4(4096, 7, 64, 4096, 4096, None) == -1 and "dtype" in _err()
+    assert L.e4b_quantize_mxfp4(None, N.BF16, 64, 4096, 4096, None) == -1 and "NULL" in _err()
+    assert L.e4b_quantize_mxfp4(4098, N.BF16, 64, 4096, 4096, None) == -1 and "aligned" in _err()
+    assert L.e4b_quantize_mxfp4(None, N.BF16, 0, None, None, None) == 0
+
+
+def test_mx_grouped_gemm_rejects_bad_arguments():
+    L = N.lib()
+    sizes = (ctypes.c_int64 * 2)(3, 2)
+    good = _qw(format=N.FMT_MXFP4, k=96)
+
+    def call(a=4096, dt=N.BF16, sizes=sizes, groups=2, ids=4096, w=good, ws=4096, ws_bytes=1 << 20, out=4096, od=N.BF16):
+        return L.e4b_mx_grouped_gemm(a, dt, sizes, groups, ids, None if w is None else ctypes.byref(w), ws, ws_bytes, out,
+                                     od, None)
+
+    assert call(w=None) == -1 and "NULL" in _err()
+    assert call(w=_qw(format=N.FMT_NF4)) == -2 and "MXFP4" in _err()
+    assert call(w=_qw(format=N.FMT_MXFP4, k=48)) == -2 and "multiple of 32" in _err()
+    assert call(w=_qw(format=N.FMT_MXFP4, n=0)) == -1 and "positive" in _err()
+    assert call(w=_qw(format=N.FMT_MXFP4, packed=4104)) == -1 and "aligned" in _err()
+    assert call(dt=N.FP32) == -1 and "act_dtype" in _err()
+    assert call(od=9) == -1 and "out_dtype" in _err()
+    assert call(groups=-1) == -2 and call(groups=513) == -2 and "groups" in _err()
+    assert call(sizes=None) == -1 and call(ids=None) == -1
+    assert call(sizes=(ctypes.c_int64 * 2)(3, -2)) == -1 and "negative" in _err()
+    assert call(sizes=(ctypes.c_int64 * 2)(1 << 31, 2)) == -2 and "2^31" in _err()
+    assert call(a=None) == -1 and call(out=None) == -1
+    assert call(a=4104) == -1 and call(out=4104) == -1 and call(ws=4104) == -1 and "aligned" in _err()
+    need = L.e4b_mx_gemm_workspace_bytes(5, 96)
+    assert need >= 5 * (48 + 3)
+    assert call(ws_bytes=need - 1) == -4 and call(ws=None) == -4 and "workspace" in _err()
+    assert call(sizes=(ctypes.c_int64 * 2)(0, 0), a=None, out=None, ws=None) == 0
+    assert L.e4b_mx_gemm_workspace_bytes(0, 96) == 0
