@@ -17,6 +17,7 @@ from .arch.deepseek_v4 import DeepseekV4Experts4bit, DeepseekV4ExpertsNbit
 from .arch.gptoss import GptOssExperts4bit, GptOssExpertsMxfp4, GptOssExpertsNbit
 from .ops import gemm_4bit_grouped, gemm_mxfp4_grouped
 from .quant import quantize_mxfp4
+from .router import balance_loss, router_topk
 from .train import disable_fast_train, enable_fast_train
 
 __version__ = "0.1.0"
@@ -30,6 +31,7 @@ __all__ = [
     "GptOssExperts4bit",
     "GptOssExpertsNbit",
     "GptOssExpertsMxfp4",
+    "balance_loss",
     "dequantize_mxfp4",
     "disable_fast",
     "disable_fast_train",
@@ -40,4 +42,5 @@ __all__ = [
     "gemm_mxfp4_grouped",
     "normalize_quant_type",
     "quantize_mxfp4",
+    "router_topk",
 ]

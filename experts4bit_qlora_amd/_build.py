@@ -2,7 +2,7 @@
 
 ``python -m experts4bit_qlora_amd._build`` (or ``__graft_entry__.build()``) compiles
 ``csrc/e4b_amd.hip`` (entry points and the routing / dequant / GEMV / LoRA / training kernels),
-``csrc/mx_gemm.hip`` (the products of microscaled operands), and ``csrc/decode_inst.hip`` and ``csrc/gemm_inst.hip`` once per (activation dtype, weight format)
+``csrc/mx_gemm.hip`` (the products of microscaled operands), ``csrc/gate.hip`` (the router's kernels), and ``csrc/decode_inst.hip`` and ``csrc/gemm_inst.hip`` once per (activation dtype, weight format)
 pair, all in parallel, then links them into ``experts4bit_qlora_amd/libe4b_amd.so``. The output is written to a temporary
 name and renamed, so a failed build never leaves a half-written library behind.
 """
@@ -20,6 +20,7 @@ SRC = os.path.join(CSRC, "e4b_amd.hip")
 DECODE_SRC = os.path.join(CSRC, "decode_inst.hip")
 GEMM_SRC = os.path.join(CSRC, "gemm_inst.hip")
 MX_SRC = os.path.join(CSRC, "mx_gemm.hip")
+GATE_SRC = os.path.join(CSRC, "gate.hip")
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include")
 # (E4B_INST_DT, E4B_INST_FMT): bf16/fp16 x NF4/NF4_DQ/MXFP4
 DECODE_PAIRS = [(dt, fmt) for dt in (0, 1) for fmt in (0, 1, 2)]
@@ -67,7 +68,7 @@ def build(verbose: bool = False) -> str:
     inc = [f"-I{CSRC}", f"-I{INCLUDE}"]
     with tempfile.TemporaryDirectory(prefix="e4b_build_") as tmpdir:
         objs, cmds = [], []
-        for name, src in (("e4b_amd.o", SRC), ("mx_gemm.o", MX_SRC)):
+        for name, src in (("e4b_amd.o", SRC), ("mx_gemm.o", MX_SRC), ("gate.o", GATE_SRC)):
             obj = os.path.join(tmpdir, name)
             cmds.append([cc, *FLAGS, *inc, "-c", "-o", obj, src])
             objs.append(obj)

@@ -22,6 +22,7 @@ BF16, FP16, FP32 = 0, 1, 2
 EPI_NONE, EPI_SWIGLU, EPI_ACT, EPI_CLAMP_SWIGLU, EPI_GPTOSS = 0, 1, 2, 3, 4
 # e4b_probe_site: launch sites of the prefill path that e4b_set_probe can watch
 PROBE_OFF, PROBE_GATE_UP_BIG, PROBE_GATE_UP_TAIL, PROBE_DOWN_BIG, PROBE_DOWN_TAIL = 0, 1, 2, 3, 4
+SCORE_ALL, SCORE_CHOSEN = 0, 1
 PATH_AUTO, PATH_GEMV, PATH_MFMA = 0, 1, 2
 NOALLOC_WORKSPACE_BYTES = 64 << 20  # E4B_NOALLOC_WORKSPACE_BYTES
 
@@ -37,6 +38,11 @@ EXPORTS = (
     "e4b_weight_shift",
     "e4b_route_scratch_ints",
     "e4b_route",
+    "e4b_router_topk",
+    "e4b_router_topk_backward",
+    "e4b_balance_workspace_bytes",
+    "e4b_balance_loss",
+    "e4b_balance_loss_backward",
     "e4b_route_groups",
     "e4b_gather_rows",
     "e4b_grouped_gemm",
@@ -147,6 +153,16 @@ def _bind(L):
     L.e4b_route_scratch_ints.argtypes = [I64, I32]
     L.e4b_route.restype = ctypes.c_int
     L.e4b_route.argtypes = [P, I64, I32, I32, RT, P]
+    L.e4b_router_topk.restype = ctypes.c_int
+    L.e4b_router_topk.argtypes = [P, I32, I64, I32, I32, I32, P, P, I32, P]
+    L.e4b_router_topk_backward.restype = ctypes.c_int
+    L.e4b_router_topk_backward.argtypes = [P, I32, I64, I32, I32, I32, P, P, I32, P, P]
+    L.e4b_balance_workspace_bytes.restype = ctypes.c_size_t
+    L.e4b_balance_workspace_bytes.argtypes = [I32, I64, I32]
+    L.e4b_balance_loss.restype = ctypes.c_int
+    L.e4b_balance_loss.argtypes = [P, I32, I32, I64, I32, P, I32, P, I64, P, ctypes.c_size_t, P, P, P, P]
+    L.e4b_balance_loss_backward.restype = ctypes.c_int
+    L.e4b_balance_loss_backward.argtypes = [P, I32, I32, I64, I32, P, I64, P, P, P, P, P]
     L.e4b_route_groups.restype = ctypes.c_int
     L.e4b_route_groups.argtypes = [ctypes.POINTER(ctypes.c_int64), I32, P, I32, RT, P]
     L.e4b_gather_rows.restype = ctypes.c_int

@@ -18,6 +18,7 @@
 #include "decode.h"
 #include "decode_launch.h"
 #include "dequant.h"
+#include "gate_launch.h"
 #include "gather.h"
 #include "gemm.h"
 #include "gemm_launch.h"
@@ -237,6 +238,43 @@ int check_mx_weight(const e4b_qweight* w) {
   if (w->n > 0x7fffffffLL || w->k > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "n or k exceeds int32");
   if (!w->packed || !w->absmax) return fail(E4B_EINVAL, "packed/absmax pointer is NULL");
   if (!aligned16(w->packed)) return fail(E4B_EINVAL, "packed weights must be 16-byte aligned");
+  return E4B_OK;
+}
+
+// The router kernels' shared checks; a takes the sizes.
+int check_gate(int32_t dtype, int64_t tokens, int32_t num_experts, int32_t top_k, int32_t scoring, int32_t weight_dtype,
+               e4b::GateArgs& a) {
+  if (!any_dtype_ok(dtype) || !any_dtype_ok(weight_dtype))
+    return fail(E4B_EINVAL, "bad dtype %d / weight_dtype %d", dtype, weight_dtype);
+  if (tokens < 0) return fail(E4B_EINVAL, "negative tokens");
+  if (num_experts <= 0 || num_experts > e4b::kGateMaxExperts)
+    return fail(E4B_EUNSUPPORTED, "num_experts=%d outside [1, %d]", num_experts, e4b::kGateMaxExperts);
+  if (top_k <= 0 || top_k > num_experts) return fail(E4B_EINVAL, "top_k=%d outside [1, %d]", top_k, num_experts);
+  if (top_k > e4b::kGateMaxK) return fail(E4B_EUNSUPPORTED, "top_k=%d > %d", top_k, e4b::kGateMaxK);
+  if (scoring != E4B_SCORE_ALL && scoring != E4B_SCORE_CHOSEN) return fail(E4B_EINVAL, "bad scoring %d", scoring);
+  if (tokens > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "tokens exceeds int32");
+  a.dtype = dtype;
+  a.T = tokens;
+  a.E = num_experts;
+  a.k = top_k;
+  a.over_chosen = scoring == E4B_SCORE_CHOSEN;
+  a.wdtype = weight_dtype;
+  return E4B_OK;
+}
+
+int check_balance(int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts, int64_t mask_stride,
+                  e4b::BalanceArgs& a) {
+  if (!any_dtype_ok(dtype)) return fail(E4B_EINVAL, "bad dtype %d", dtype);
+  if (layers < 0 || tokens < 0 || mask_stride < 0) return fail(E4B_EINVAL, "negative sizes");
+  if (layers > 65535) return fail(E4B_EUNSUPPORTED, "layers=%d > 65535", layers);
+  if (num_experts <= 0 || num_experts > e4b::kGateMaxExperts)
+    return fail(E4B_EUNSUPPORTED, "num_experts=%d outside [1, %d]", num_experts, e4b::kGateMaxExperts);
+  if (tokens > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "tokens exceeds int32");
+  a.dtype = dtype;
+  a.T = tokens;
+  a.L = layers;
+  a.E = num_experts;
+  a.mask_stride = mask_stride;
   return E4B_OK;
 }
 
@@ -579,6 +617,91 @@ int route_impl(const int64_t* top_k_index, int64_t tokens, int32_t top_k, int32_
 }  // namespace
 
 extern "C" {
+
+int e4b_router_topk(const void* logits, int32_t dtype, int64_t tokens, int32_t num_experts, int32_t top_k,
+                    int32_t scoring, int64_t* top_k_index, void* top_k_weights, int32_t weight_dtype,
+                    hipStream_t stream) {
+  e4b::GateArgs a{};
+  int rc = check_gate(dtype, tokens, num_experts, top_k, scoring, weight_dtype, a);
+  if (rc || tokens == 0) return rc;
+  if (!logits || !top_k_index || !top_k_weights) return fail(E4B_EINVAL, "logits/top_k_index/top_k_weights is NULL");
+  a.logits = logits;
+  a.index = top_k_index;
+  a.weights = top_k_weights;
+  e4b::launch_gate(a, stream);
+  return check_launch("gate_kernel");
+}
+
+int e4b_router_topk_backward(const void* logits, int32_t dtype, int64_t tokens, int32_t num_experts, int32_t top_k,
+                             int32_t scoring, const int64_t* top_k_index, const void* grad_weights,
+                             int32_t weight_dtype, void* grad_logits, hipStream_t stream) {
+  e4b::GateArgs a{};
+  int rc = check_gate(dtype, tokens, num_experts, top_k, scoring, weight_dtype, a);
+  if (rc || tokens == 0) return rc;
+  if (!logits || !top_k_index || !grad_weights || !grad_logits)
+    return fail(E4B_EINVAL, "logits/top_k_index/grad_weights/grad_logits is NULL");
+  a.logits = logits;
+  a.index = const_cast<int64_t*>(top_k_index);
+  a.weights = const_cast<void*>(grad_weights);
+  a.grad = grad_logits;
+  e4b::launch_gate_backward(a, stream);
+  return check_launch("gate_backward_kernel");
+}
+
+size_t e4b_balance_workspace_bytes(int32_t layers, int64_t tokens, int32_t num_experts) {
+  if (layers <= 0 || tokens <= 0 || num_experts <= 0 || num_experts > e4b::kGateMaxExperts) return 0;
+  const size_t parts = size_t(layers) * e4b::balance_chunks(tokens, layers, num_experts);
+  return align256(sizeof(float) * parts * num_experts) + align256(sizeof(int32_t) * parts * (num_experts + 1));
+}
+
+int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
+                     const int64_t* top_k_index, int32_t top_k, const uint8_t* mask, int64_t mask_stride,
+                     void* workspace, size_t workspace_bytes, float* loss, int64_t* counts, int64_t* valid,
+                     hipStream_t stream) {
+  e4b::BalanceArgs a{};
+  int rc = check_balance(dtype, layers, tokens, num_experts, mask_stride, a);
+  if (rc || layers == 0) return rc;
+  if (top_k <= 0) return fail(E4B_EINVAL, "top_k must be positive");
+  if (!loss || !counts || !valid) return fail(E4B_EINVAL, "loss/counts/valid is NULL");
+  if (tokens > 0 && (!logits || !top_k_index)) return fail(E4B_EINVAL, "logits/top_k_index is NULL");
+  // counts are summed in 32 bits per chunk
+  if (tokens > 0x7fffffffLL / top_k) return fail(E4B_EUNSUPPORTED, "tokens*top_k exceeds int32");
+  const size_t need = e4b_balance_workspace_bytes(layers, tokens, num_experts);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(E4B_ESPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(E4B_EINVAL, "workspace must be 16-byte aligned");
+  a.logits = logits;
+  a.k = top_k;
+  a.index = top_k_index;
+  a.mask = mask;
+  a.chunks = tokens ? e4b::balance_chunks(tokens, layers, num_experts) : 0;
+  a.part = static_cast<float*>(workspace);
+  a.part_counts = reinterpret_cast<int32_t*>(
+      static_cast<char*>(workspace) + align256(sizeof(float) * size_t(layers) * a.chunks * num_experts));
+  a.loss = loss;
+  a.counts = counts;
+  a.valid = valid;
+  e4b::launch_balance(a, stream);
+  return check_launch("balance_kernel");
+}
+
+int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
+                              const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
+                              const float* grad_loss, void* grad_logits, hipStream_t stream) {
+  e4b::BalanceArgs a{};
+  int rc = check_balance(dtype, layers, tokens, num_experts, mask_stride, a);
+  if (rc || layers == 0 || tokens == 0) return rc;
+  if (!logits || !counts || !valid || !grad_loss || !grad_logits)
+    return fail(E4B_EINVAL, "logits/counts/valid/grad_loss/grad_logits is NULL");
+  a.logits = logits;
+  a.mask = mask;
+  a.counts = const_cast<int64_t*>(counts);
+  a.valid = const_cast<int64_t*>(valid);
+  a.grad_loss = grad_loss;
+  a.grad = grad_logits;
+  e4b::launch_balance_backward(a, stream);
+  return check_launch("balance_backward_kernel");
+}
 
 int e4b_route_groups(const int64_t* sizes, int32_t groups, const int64_t* expert_ids, int32_t num_experts,
                      const e4b_routing* rt, hipStream_t stream) {

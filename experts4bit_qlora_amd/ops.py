@@ -7,6 +7,7 @@ here synchronises the device, and none computes anything itself: a missing libra
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 import threading
@@ -38,6 +39,14 @@ def _stream(device: torch.device) -> int:
     the accessor torch's own kernel launchers use, ~0.3 us against ~4 us for
     ``torch.cuda.current_stream(device).cuda_stream``, which an eager decode call pays each time."""
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """``torch.cuda.device(device)`` where it is not the current one (entering it costs ~4 us)."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _require_cuda(*ts):
@@ -224,7 +233,7 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"K={k} is not a multiple of 32")
     blocks = torch.empty(*x.shape[:-1], k // 2, dtype=torch.uint8, device=x.device)
     scales = torch.empty(*x.shape[:-1], k // 32, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         N.check("e4b_quantize_mxfp4",
                 N.lib().e4b_quantize_mxfp4(x.data_ptr(), dtype_code(x.dtype), x.numel(), blocks.data_ptr(),
                                            scales.data_ptr(), _stream(x.device)))
@@ -299,6 +308,72 @@ def route(top_k_index: torch.Tensor, num_experts: int, tile_m: int | None = None
     rs = rb.struct()
     N.check("e4b_route", L.e4b_route(idx.data_ptr(), T, k, num_experts, ctypes.byref(rs), _stream(dev)))
     return rb
+
+
+# ------------------------------------------------------------------------------- router
+
+
+def router_topk(logits: torch.Tensor, top_k: int, scoring: int, weight_dtype: torch.dtype):
+    """``[T, E]`` logits -> (index int64 ``[T, k]``, weights ``[T, k]``) by ``e4b_router_topk``."""
+    _require_cuda(logits)
+    T, E = logits.shape
+    dev = logits.device
+    index = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+    weights = torch.empty(T, top_k, dtype=weight_dtype, device=dev)
+    with _on(dev):
+        N.check("e4b_router_topk",
+                N.lib().e4b_router_topk(logits.data_ptr(), dtype_code(logits.dtype), T, E, top_k, scoring,
+                                        index.data_ptr(), weights.data_ptr(), dtype_code(weight_dtype), _stream(dev)))
+    return index, weights
+
+
+def router_topk_backward(logits: torch.Tensor, index: torch.Tensor, grad: torch.Tensor, scoring: int) -> torch.Tensor:
+    """dL/dlogits ``[T, E]`` from dL/dweights ``[T, k]`` (``e4b_router_topk_backward``)."""
+    _require_cuda(logits, index, grad)
+    T, E = logits.shape
+    dev = logits.device
+    out = torch.empty_like(logits)
+    with _on(dev):
+        N.check("e4b_router_topk_backward",
+                N.lib().e4b_router_topk_backward(logits.data_ptr(), dtype_code(logits.dtype), T, E, index.shape[1], scoring,
+                                                 index.data_ptr(), grad.data_ptr(), dtype_code(grad.dtype),
+                                                 out.data_ptr(), _stream(dev)))
+    return out
+
+
+def balance_loss(logits: torch.Tensor, index: torch.Tensor, mask: torch.Tensor | None):
+    """``[L, T, E]`` logits, ``[L, T, k]`` index, bool mask ``[T]`` or ``[L, T]`` -> (loss fp32 ``[L]``, counts int64
+    ``[L, E]``, valid tokens int64 ``[L]``) by ``e4b_balance_loss``."""
+    _require_cuda(logits, index, mask)
+    L_, T, E = logits.shape
+    dev = logits.device
+    lib = N.lib()
+    loss = torch.empty(L_, dtype=torch.float32, device=dev)
+    counts = torch.empty(L_, E + 1, dtype=torch.int64, device=dev)  # the counts and, behind them, the valid tokens
+    counts, valid = counts.view(-1)[:L_ * E].view(L_, E), counts.view(-1)[L_ * E:]
+    ws = torch.empty(max(1, lib.e4b_balance_workspace_bytes(L_, T, E)), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        N.check("e4b_balance_loss",
+                lib.e4b_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), L_, T, E, index.data_ptr(),
+                                     index.shape[2], _ptr(mask), 0 if mask is None or mask.dim() == 1 else T,
+                                     ws.data_ptr(), ws.numel(), loss.data_ptr(), counts.data_ptr(), valid.data_ptr(),
+                                     _stream(dev)))
+    return loss, counts, valid
+
+
+def balance_loss_backward(logits: torch.Tensor, mask: torch.Tensor | None, counts: torch.Tensor, valid: torch.Tensor,
+                          grad: torch.Tensor) -> torch.Tensor:
+    """dL/dlogits from dL/dloss fp32 ``[L]`` (``e4b_balance_loss_backward``)."""
+    _require_cuda(logits, mask, counts, valid, grad)
+    L_, T, E = logits.shape
+    dev = logits.device
+    out = torch.empty_like(logits)
+    with _on(dev):
+        N.check("e4b_balance_loss_backward",
+                N.lib().e4b_balance_loss_backward(logits.data_ptr(), dtype_code(logits.dtype), L_, T, E, _ptr(mask),
+                                                  0 if mask is None or mask.dim() == 1 else T, counts.data_ptr(),
+                                                  valid.data_ptr(), grad.data_ptr(), out.data_ptr(), _stream(dev)))
+    return out
 
 
 # -------------------------------------------------------------------------------- GEMMs
@@ -781,7 +856,7 @@ def mx_grouped_gemm(a: torch.Tensor, qw: QW, sizes, expert_ids) -> torch.Tensor:
     dt = dtype_code(x.dtype)
     out = torch.empty(M, qw.n, dtype=x.dtype, device=x.device)
     ws = torch.empty(max(1, L.e4b_mx_gemm_workspace_bytes(M, qw.k)), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         N.check("e4b_mx_grouped_gemm",
                 L.e4b_mx_grouped_gemm(x.data_ptr(), dt, host_sizes, G, ids.data_ptr(), qw.ref(), ws.data_ptr(), ws.numel(),
                                       out.data_ptr(), dt, _stream(x.device)))

@@ -50,6 +50,9 @@ enum e4b_epilogue {
                                after adding the per-expert gate_up bias */
 };
 
+/* What the router's softmax runs over: all logits, or the chosen ones (which equals renormalising). */
+enum e4b_scoring { E4B_SCORE_ALL = 0, E4B_SCORE_CHOSEN = 1 };
+
 /* Kernel-path selection flags for the grouped GEMMs (0 = automatic by token count). */
 enum e4b_flags { E4B_PATH_AUTO = 0, E4B_PATH_GEMV = 1, E4B_PATH_MFMA = 2 };
 
@@ -146,6 +149,48 @@ int64_t e4b_route_scratch_ints(int64_t M, int32_t num_experts);
  * nothing is copied to the host. Ids outside [0, E) are dropped (counted in meta[2]). */
 int e4b_route(const int64_t* top_k_index, int64_t tokens, int32_t top_k, int32_t num_experts,
               const e4b_routing* rt, hipStream_t stream);
+
+/* The router's top-k gate. top_k_index [tokens, top_k] int64: each row's top_k largest logits in
+ * descending order, ties to the lower index (-0 equals 0, a NaN above infinity); top_k_weights [tokens,
+ * top_k] in weight_dtype: the softmax over all logits at those (E4B_SCORE_ALL), or over the chosen ones
+ * (E4B_SCORE_CHOSEN), fp32 and rounded once. A row whose logits are all -inf gets zero weights.
+ * logits [tokens, num_experts] in dtype; num_experts <= 1024, top_k <= 64.
+ * Replaces: the routing epilogue of engines/cpu_router.py:100-120 (and the torch ops of the models'
+ * own routers: softmax, topk, renormalisation). */
+int e4b_router_topk(const void* logits, int32_t dtype, int64_t tokens, int32_t num_experts, int32_t top_k,
+                    int32_t scoring, int64_t* top_k_index, void* top_k_weights, int32_t weight_dtype,
+                    hipStream_t stream);
+
+/* Its backward: grad_logits [tokens, num_experts] in dtype from grad_weights [tokens, top_k] in
+ * weight_dtype and the forward's top_k_index (distinct entries per row):
+ *   E4B_SCORE_ALL:    dz_j = p_j (g_j [j chosen] - sum over chosen of g_s p_s)
+ *   E4B_SCORE_CHOSEN: dz_j = w_j (g_j - sum over chosen of g_s w_s), 0 where not chosen. */
+int e4b_router_topk_backward(const void* logits, int32_t dtype, int64_t tokens, int32_t num_experts, int32_t top_k,
+                             int32_t scoring, const int64_t* top_k_index, const void* grad_weights,
+                             int32_t weight_dtype, void* grad_logits, hipStream_t stream);
+
+/* Bytes of workspace e4b_balance_loss needs. */
+size_t e4b_balance_workspace_bytes(int32_t layers, int64_t tokens, int32_t num_experts);
+
+/* Load-balance loss and per-expert counts, one of each per layer. Over a layer's valid tokens (all, or
+ * those with mask[layer * mask_stride + t] != 0; mask_stride 0 shares one mask), N of them:
+ * counts[e] = number of top_k_index entries equal to e (entries outside [0, num_experts) count
+ * nowhere), P_e = mean softmax probability of e, loss = num_experts * sum_e counts[e] / N * P_e (0 when N
+ * is 0). logits [layers, tokens, num_experts] in dtype, top_k_index [layers, tokens, top_k] int64;
+ * loss fp32 [layers], counts int64 [layers, num_experts], valid int64 [layers] (N, for the backward).
+ * A row whose logits are all -inf adds no probability. Deterministic.
+ * Has no counterpart in the reference, whose models take transformers' load_balancing_loss_func; the
+ * definition is that one's, per layer. */
+int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
+                     const int64_t* top_k_index, int32_t top_k, const uint8_t* mask, int64_t mask_stride,
+                     void* workspace, size_t workspace_bytes, float* loss, int64_t* counts, int64_t* valid,
+                     hipStream_t stream);
+
+/* Its backward (the counts are constants): grad_logits[t, j] = grad_loss * num_experts / N^2 * p_tj *
+ * (counts[j] - sum_e counts[e] p_te) at valid tokens, 0 elsewhere; grad_loss fp32 [layers]. */
+int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
+                              const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
+                              const float* grad_loss, void* grad_logits, hipStream_t stream);
 
 /* Routing of row groups with host sizes and device expert ids: group g holds the input rows
  * [sum(sizes[:g]), sum(sizes[:g+1])) for expert expert_ids[g] (int64, on the device, read only

@@ -344,3 +344,39 @@ def test_mx_grouped_gemm_rejects_bad_arguments():
     assert call(ws_bytes=need - 1) == -4 and call(ws=None) == -4 and "workspace" in _err()
     assert call(sizes=(ctypes.c_int64 * 2)(0, 0), a=None, out=None, ws=None) == 0
     assert L.e4b_mx_gemm_workspace_bytes(0, 96) == 0
+
+
+def test_router_entry_points_reject_bad_arguments():
+    L = N.lib()
+
+    def gate(z=4096, dt=N.BF16, T=4, E=8, k=2, scoring=N.SCORE_ALL, index=4096, w=4096, wd=N.FP32):
+        a = L.e4b_router_topk(z, dt, T, E, k, scoring, index, w, wd, None)
+        b = L.e4b_router_topk_backward(z, dt, T, E, k, scoring, index, w, wd, 4096, None)
+        assert a == b
+        return a
+
+    assert gate(dt=5) == -1 and gate(wd=5) == -1 and "dtype" in _err()
+    assert gate(T=-1) == -1 and gate(k=0) == -1 and gate(k=9) == -1 and "top_k" in _err()
+    assert gate(E=0) == -2 and gate(E=1025) == -2 and "num_experts" in _err()
+    assert gate(E=100, k=65) == -2 and gate(T=1 << 31) == -2
+    assert gate(scoring=2) == -1 and "scoring" in _err()
+    assert gate(z=None) == -1 and gate(index=None) == -1 and gate(w=None) == -1 and "NULL" in _err()
+    assert gate(T=0, z=None, index=None, w=None) == 0
+    assert L.e4b_router_topk_backward(4096, N.BF16, 4, 8, 2, 0, 4096, 4096, N.FP32, None, None) == -1
+
+    def balance(z=4096, dt=N.BF16, layers=2, T=40, E=8, index=4096, k=2, mask=None, stride=0, ws=4096, ws_bytes=1 << 20,
+                loss=4096, counts=4096, valid=4096):
+        return L.e4b_balance_loss(z, dt, layers, T, E, index, k, mask, stride, ws, ws_bytes, loss, counts, valid, None)
+
+    assert balance(dt=4) == -1 and balance(layers=-1) == -1 and balance(T=-1) == -1 and balance(stride=-1) == -1
+    assert balance(layers=65536) == -2 and balance(E=0) == -2 and balance(E=1025) == -2 and balance(T=1 << 31) == -2
+    assert balance(k=0) == -1 and balance(T=(1 << 31) - 1, k=2) == -2
+    assert balance(z=None) == -1 and balance(index=None) == -1 and "NULL" in _err()
+    assert balance(loss=None) == -1 and balance(counts=None) == -1 and balance(valid=None) == -1
+    need = L.e4b_balance_workspace_bytes(2, 40, 8)
+    assert need > 0 and balance(ws_bytes=need - 1) == -4 and balance(ws=None) == -4 and balance(ws=4104) == -1
+    assert balance(layers=0, z=None) == 0
+    assert L.e4b_balance_workspace_bytes(2, 0, 8) == 0
+    back = lambda z=4096, c=4096, v=4096, g=4096, out=4096: L.e4b_balance_loss_backward(
+        z, N.BF16, 2, 40, 8, None, 0, c, v, g, out, None)
+    assert back(z=None) == back(c=None) == back(v=None) == back(g=None) == back(out=None) == -1
