@@ -12,7 +12,6 @@ The reference leaves both to the models (its CPU engine restates the gate,
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import ops
@@ -32,6 +31,13 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _once():
+    """Refuse a backward that is itself to be differentiated (torch's ``once_differentiable`` does it at
+    ~10 us a call)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("router_topk and balance_loss are differentiable once: no create_graph=True on the device")
+
+
 # -------------------------------------------------------------------------------- gate
 
 
@@ -42,11 +48,14 @@ class _Gate(torch.autograd.Function):
         ctx.save_for_backward(logits, index)
         ctx.scoring = scoring
         ctx.mark_non_differentiable(index)
+        ctx.set_materialize_grads(False)  # no zeros in the place of the index's gradient
         return index, weights
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _, grad):
+        if grad is None:
+            return None, None, None, None
+        _once()
         logits, index = ctx.saved_tensors
         return ops.router_topk_backward(logits, index, _aligned(grad), ctx.scoring), None, None, None
 
@@ -110,10 +119,10 @@ class _Balance(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
             return None, None, None
+        _once()
         logits, mask, counts, valid = ctx.saved_tensors
         return ops.balance_loss_backward(logits, mask, counts, valid, _aligned(grad)), None, None
 

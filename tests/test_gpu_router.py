@@ -246,9 +246,23 @@ def test_formulations_agree_where_the_kernel_does_not_reach():
 def test_second_derivatives_are_refused():
     z = _logits((4, 16), torch.float32, 9).to(DEV).requires_grad_()
     _, w = e4b.router_topk(z, 2)
-    (g,) = torch.autograd.grad(w.square().sum(), z, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(g.sum(), z)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(w.square().sum(), z, create_graph=True)
+    loss, _ = e4b.balance_loss(z, _choices(z, 2))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(loss, z, create_graph=True)
+
+
+def test_an_output_changed_in_place_is_refused():
+    z = _logits((2, 4, 16), torch.float32, 9).to(DEV).requires_grad_()
+    index, w = e4b.router_topk(z[0], 2)
+    index.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(w.sum(), z)
+    loss, counts = e4b.balance_loss(z, _choices(z, 2))
+    counts.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(loss.sum(), z)
 
 
 def test_captured_and_replayed():
