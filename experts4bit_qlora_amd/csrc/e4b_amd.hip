@@ -235,7 +235,8 @@ int check_mx_weight(const e4b_qweight* w) {
     return fail(E4B_EINVAL, "weight dims must be positive (E=%d n=%lld k=%lld)", w->num_experts, (long long)w->n,
                 (long long)w->k);
   if (w->k % 32) return fail(E4B_EUNSUPPORTED, "k=%lld is not a multiple of 32", (long long)w->k);
-  if (w->n > 0x7fffffffLL || w->k > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "n or k exceeds int32");
+  // offsets within a 256-row tile of weights are 32 bits
+  if (w->n > 0x7fffffffLL || w->k > (1 << 24)) return fail(E4B_EUNSUPPORTED, "n exceeds int32 or k 2^24");
   if (!w->packed || !w->absmax) return fail(E4B_EINVAL, "packed/absmax pointer is NULL");
   if (!aligned16(w->packed)) return fail(E4B_EINVAL, "packed weights must be 16-byte aligned");
   return E4B_OK;
@@ -859,8 +860,8 @@ int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, 
   for (int g = 0; g < groups; ++g) {
     if (sizes[g] < 0) return fail(E4B_EINVAL, "group %d has a negative size", g);
     go.off[g] = static_cast<int32_t>(M);
-    M += sizes[g];
-    if (M > 0x7fffffffLL) return fail(E4B_EUNSUPPORTED, "groups hold more than 2^31 - 1 rows");
+    if (sizes[g] > e4b::kMxRowsMax || (M += sizes[g]) > e4b::kMxRowsMax)
+      return fail(E4B_EUNSUPPORTED, "groups hold more than %lld rows", (long long)e4b::kMxRowsMax);
   }
   for (int g = groups; g <= e4b::kMxGroupsMax; ++g) go.off[g] = static_cast<int32_t>(M);
   if (M == 0) return E4B_OK;

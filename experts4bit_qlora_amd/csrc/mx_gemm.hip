@@ -3,6 +3,8 @@
 
 #include "mx_launch.h"
 
+#include <algorithm>
+
 namespace e4b {
 
 namespace {
@@ -22,20 +24,55 @@ void launch_mx_rows(const void* x, int dtype, int64_t rows, int64_t k, uint8_t* 
   else launch_rows<E4B_FP16>(x, rows, k, codes, scales, s);
 }
 
-void launch_mx_gemm_groups(MxGemmArgs a, const MxGroups& g, int out_dtype, hipStream_t s) {
-  a.tiles = 0;
-  a.one = 1;
-  for (int i = 0; i < a.groups; ++i) {
-    const int tiles = (g.off[i + 1] - g.off[i] + kMxTileM - 1) / kMxTileM;
-    a.tiles += tiles;
-    a.one &= tiles == 1;
+namespace {
+
+int group_tiles(const MxTiling& tl, int size) {
+  if (tl.rest_only) {
+    const int rest = size % tl.big;
+    return rest > 0 && rest <= tl.tm ? 1 : 0;
   }
-  a.n_blocks = static_cast<int>((a.w.n + 31) / 32);
-  const dim3 grid(static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.n_blocks)), b(kMxNarrowWaves * kWave);
+  return size / tl.tm + (size % tl.tm > tl.rest_above ? 1 : 0);
+}
+
+template <class K>
+void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl, int columns, hipStream_t s) {
+  a.tl = tl;
+  a.tl.one = 1;
+  int tiles = 0;
+  for (int i = 0; i < a.groups; ++i) {
+    g.tile[i] = static_cast<uint16_t>(tiles);
+    const int n = group_tiles(tl, g.off[i + 1] - g.off[i]);
+    tiles += n;
+    a.tl.one &= n == 1;
+  }
+  for (int i = a.groups; i <= kMxGroupsMax; ++i) g.tile[i] = static_cast<uint16_t>(tiles);
+  if (!tiles) return;
+  a.tiles = tiles;
+  a.n_blocks = static_cast<int>((a.w.n + columns - 1) / columns);
+  const unsigned total = static_cast<unsigned>(tiles) * static_cast<unsigned>(a.n_blocks);
+  hipLaunchKernelGGL(kernel, dim3((total + 7) / 8 * 8), dim3(threads), 0, s, a, g);
+}
+
+template <int ODT>
+void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
+  int largest = 0;
+  for (int i = 0; i < a.groups; ++i) largest = std::max(largest, g.off[i + 1] - g.off[i]);
+  const int threads = kMxNarrowWaves * kWave;
+  if (largest <= kMxTileM) {
+    launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 0, 1, 0}, 32, s);
+    return;
+  }
+  launch_tiles(mx_wide_kernel<ODT>, kMxWideThreads, a, g, {kMxWideTile, kMxTileM, 0, 1, 0}, kMxWideTile, s);
+  launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 1, kMxWideTile, 0}, 32, s);
+}
+
+}  // namespace
+
+void launch_mx_gemm_groups(const MxGemmArgs& a, MxGroups& g, int out_dtype, hipStream_t s) {
   switch (out_dtype) {
-    case E4B_BF16: hipLaunchKernelGGL(mx_narrow_kernel<E4B_BF16>, grid, b, 0, s, a, g); break;
-    case E4B_FP16: hipLaunchKernelGGL(mx_narrow_kernel<E4B_FP16>, grid, b, 0, s, a, g); break;
-    default: hipLaunchKernelGGL(mx_narrow_kernel<E4B_FP32>, grid, b, 0, s, a, g); break;
+    case E4B_BF16: return launch_groups<E4B_BF16>(a, g, s);
+    case E4B_FP16: return launch_groups<E4B_FP16>(a, g, s);
+    default: return launch_groups<E4B_FP32>(a, g, s);
   }
 }
 

@@ -16,8 +16,19 @@ inline int64_t mx_chunks(int64_t k) { return (k + kMxChunk - 1) / kMxChunk; }
 
 // Row groups given by the host: group g holds rows off[g] .. off[g + 1] - 1 for the expert ids[g].
 constexpr int kMxGroupsMax = 512;
+// tile: a launch's first row tile of each group.
 struct MxGroups {
   int32_t off[kMxGroupsMax + 1];
+  uint16_t tile[kMxGroupsMax + 1];
+};
+constexpr int64_t kMxRowsMax = int64_t(1) << 23;  // below 2^16 tiles of 256 rows, one more per group
+
+// How a launch cuts the groups into row tiles. With tiles of tm rows it takes of each group its whole tiles
+// and its last rows where more than rest_above are left, or (rest_only) only those last rows where at
+// most tm are left past whole tiles of `big` rows: together the two launches cover every row once.
+struct MxTiling {
+  int tm, rest_above, rest_only, big;
+  int one;  // every group is one tile
 };
 
 struct MxGemmArgs {
@@ -28,16 +39,16 @@ struct MxGemmArgs {
   int groups;
   int64_t M;
   void* out;  // [M, n] in the kernel's output type
-  int n_blocks;  // column blocks of the launch
+  MxTiling tl;
   int tiles;     // row tiles of the launch
-  int one;       // every group is one row tile
+  int n_blocks;  // column blocks of the launch
 };
 
 // Rows [rows, k] of dtype to padded codes and scale bytes; a block with an infinity or a NaN takes the
 // scale byte 255, which makes its products NaN.
 void launch_mx_rows(const void* x, int dtype, int64_t rows, int64_t k, uint8_t* codes, uint8_t* scales, hipStream_t s);
 
-// One launch over all row tiles and column blocks of the group form.
-void launch_mx_gemm_groups(MxGemmArgs a, const MxGroups& g, int out_dtype, hipStream_t s);
+// The whole product of the group form (g.tile is filled for each launch).
+void launch_mx_gemm_groups(const MxGemmArgs& a, MxGroups& g, int out_dtype, hipStream_t s);
 
 }  // namespace e4b
