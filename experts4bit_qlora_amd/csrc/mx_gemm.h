@@ -33,9 +33,9 @@ E4B_DEV mx_acc_t mx_mfma(const u32x4_t& w, const u32x4_t& a, uint32_t ws, uint32
                                                          static_cast<int>(as));
 }
 
-// Four (eight) scale bytes of a weight row from block b on. Rows of scale bytes start at any address and are
-// read in whole words: one that would pass the row's end is read back from it and shifted. Blocks past
-// the end, whose activation codes are zero, get byte 0.
+// Four scale bytes of a weight row from block b on. Rows of scale bytes start at any address and are read in
+// whole words: one that would pass the row's end is read back from it and shifted. Blocks past the end,
+// whose activation codes are zero, get byte 0.
 E4B_DEV uint32_t mx_scales4(const uint8_t* row, int b, int blocks) {
   uint32_t v = 0;
   if (blocks >= 4) {
@@ -47,18 +47,6 @@ E4B_DEV uint32_t mx_scales4(const uint8_t* row, int b, int blocks) {
   for (int j = 0; b + j < blocks; ++j) v |= static_cast<uint32_t>(row[b + j]) << (8 * j);
   return v;
 }
-E4B_DEV u32x2_t mx_scales8(const uint8_t* row, int b, int blocks) {
-  uint64_t v = 0;
-  if (blocks >= 8) {
-    const int past = max(b + 8 - blocks, 0);  // at most 7: a chunk has a block
-    __builtin_memcpy(&v, row + (b - past), 8);
-    v >>= 8 * past;
-  } else {
-    for (int j = 0; b + j < blocks; ++j) v |= static_cast<uint64_t>(row[b + j]) << (8 * j);
-  }
-  return __builtin_bit_cast(u32x2_t, v);
-}
-
 constexpr int kMxRowThreads = 256;
 
 // Activation rows to padded codes and scale bytes (a block with an infinity or a NaN: 255). Thread =
@@ -105,8 +93,8 @@ struct MxTile {
 // Items (row tile, column block) in group order, within a group the row tiles of one column block
 // next to each other; the launch's items are cut into eight equal runs, one per XCD (workgroups go
 // round-robin over the XCDs), so the tiles that share weights share an L2.
+constexpr int kXcds = 8;
 E4B_DEV bool mx_tile(const MxGemmArgs& p, const MxGroups& go, MxTile& o) {
-  constexpr int kXcds = 8;
   const int total = p.tiles * p.n_blocks;
   const int per = (total + kXcds - 1) / kXcds;
   const int w = static_cast<int>(blockIdx.x % kXcds) * per + static_cast<int>(blockIdx.x / kXcds);
@@ -169,7 +157,7 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
   mx_acc_t acc = {};
   if (e >= 0) {
     const int blocks = static_cast<int>(p.w.k / kMxBlock);
-    const int64_t wrow = int64_t(e) * n + min(n0 + r32, n - 1);  // rows past n are not stored
+    const int64_t wrow = int64_t(e) * n + min(static_cast<int>(n0) + r32, static_cast<int>(n) - 1);  // rows past n are not stored
     const uint8_t* wc = p.w.packed + wrow * (p.w.k / 2);
     const uint8_t* ws = static_cast<const uint8_t*>(p.w.absmax) + wrow * blocks;
     const int64_t arow = min(row0 + r32, end - 1);  // columns past the tile's rows are not stored
@@ -204,8 +192,8 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
     for (int w = 0; w < kMxNarrowWaves; ++w) s += red[w][c0 + j][tid >> 3];
     v[j] = s;
   }
-  const int64_t left = n - (n0 + c0);
-  if (left > 0) mx_store4<ODT>(p.out, int64_t(row) * n + n0 + c0, static_cast<int>(min<int64_t>(left, 4)), n % 4 == 0, v);
+  const int left = static_cast<int>(n - n0) - c0;
+  if (left > 0) mx_store4<ODT>(p.out, int64_t(row) * n + n0 + c0, left, n % 4 == 0, v);
 }
 
 // ---- large groups
@@ -221,206 +209,274 @@ E4B_DEV void mx_for(F&& f) {
   mx_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-constexpr int kMxWideThreads = 512;
-constexpr int kMxWideTile = 256;
+constexpr int kMxWideThreads = 256;
 
-// Sixteen 16-bit outputs of one row, columns c0 + 8 (i / 4) + 4 half + i % 4 (an MFMA block's sums of a lane):
-// v_permlane32_swap joins the halves' runs of four into eight neighbouring columns, one 16-byte store.
+// An MFMA block's sums of a lane, columns 8 (i / 4) + 4 half + i % 4 of one row, to the row's outputs from `at`
+// on, `left` of them. For a 16-bit type v_permlane32_swap joins the halves' runs of four into eight
+// neighbouring columns, one 16-byte store where the row's addresses allow (vec).
 template <int ODT>
-E4B_DEV void mx_store_block(void* out, int64_t at, int64_t left, bool vec, bool live, int half, const mx_acc_t& v) {
-  if (ODT != E4B_FP32 && vec && left >= 32) {
+E4B_DEV void mx_store_block(void* out, int64_t at, int left, bool vec, int half, const mx_acc_t& v) {
+  if constexpr (ODT == E4B_FP32) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 8 * g + 4 * half;
+      float* o = static_cast<float*>(out) + at + c;
+      if (vec && left >= 32) {
+        *reinterpret_cast<float4*>(o) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < left) o[j] = v[4 * g + j];
+      }
+    }
+  } else {
 #pragma unroll
     for (int g = 0; g < 4; g += 2) {
       uint32_t lo[2], hi[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        lo[j] = pack2(from_f<ODT == E4B_FP32 ? E4B_BF16 : ODT>(v[4 * g + 2 * j]),
-                      from_f<ODT == E4B_FP32 ? E4B_BF16 : ODT>(v[4 * g + 2 * j + 1]));
-        hi[j] = pack2(from_f<ODT == E4B_FP32 ? E4B_BF16 : ODT>(v[4 * g + 4 + 2 * j]),
-                      from_f<ODT == E4B_FP32 ? E4B_BF16 : ODT>(v[4 * g + 4 + 2 * j + 1]));
+        lo[j] = pack2(from_f<ODT>(v[4 * g + 2 * j]), from_f<ODT>(v[4 * g + 2 * j + 1]));
+        hi[j] = pack2(from_f<ODT>(v[4 * g + 4 + 2 * j]), from_f<ODT>(v[4 * g + 4 + 2 * j + 1]));
       }
       const auto a = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
       const auto b = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);
-      const u32x4_t o = {a[0], b[0], a[1], b[1]};
-      if (live) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + at + 8 * g + 8 * half) = o;
+      u32x4_t o = {a[0], b[0], a[1], b[1]};
+      const int c = 8 * g + 8 * half;
+      uint16_t* dst = static_cast<uint16_t*>(out) + at + c;
+      if (vec && left >= 32) {
+        *reinterpret_cast<u32x4_t*>(dst) = o;
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < 8 && c + j < left; ++j) {
+          dst[j] = static_cast<uint16_t>(o[0]);
+          o[0] = __builtin_amdgcn_alignbit(o[1], o[0], 16);
+          o[1] = __builtin_amdgcn_alignbit(o[2], o[1], 16);
+          o[2] = __builtin_amdgcn_alignbit(o[3], o[2], 16);
+          o[3] >>= 16;
+        }
+      }
     }
-    return;
-  }
-  if (!live) return;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int c = 8 * g + 4 * half;
-    const float f[4] = {v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
-    if (c < left) mx_store4<ODT>(out, at + c, static_cast<int>(min<int64_t>(left - c, 4)), vec, f);
   }
 }
 
-// A tile of 256 rows times 256 weight rows per workgroup, eight waves of 64 rows x 128 weight rows (two per
-// SIMD). Both operands pass through LDS a chunk of 256 values at a time: 128-byte rows whose eight 16-byte
-// pieces are stored in the order piece ^ (row & 7), so that the stores (eight lanes a row) and the fragment
-// reads (one piece of 32 rows) fall in distinct banks. Chunk c is computed from one buffer while chunk c + 1
-// goes from registers into the other, and a register that is stored takes its piece of chunk c + 2: every
-// load has a whole chunk's time. Fragments are read a step ahead (two sets); the one barrier per chunk
-// stands before its last step, which then reads the next chunk's first fragments.
-// A wave whose 64 rows lie past the tile's end only moves data: a tile of at most 128 rows leaves one
-// computing wave per SIMD.
+// `size` bytes from base on; 16 of them at offset + uniform, zeros at and past the end.
+E4B_DEV __amdgpu_buffer_rsrc_t mx_rows_of(const uint8_t* base, int64_t size) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, static_cast<int>(size), 0x00027000);
+}
+E4B_DEV u32x4_t mx_piece(__amdgpu_buffer_rsrc_t rows, uint32_t offset, uint32_t uniform) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rows, static_cast<int>(offset), static_cast<int>(uniform), 0);
+}
+
+// A tile of 256 rows times 256 weight rows, four waves (one per SIMD) of 128 x 128. Both operands pass through LDS
+// a chunk of 256 values at a time: 128-byte rows whose eight 16-byte pieces are stored in the order piece ^ (row
+// & 7), so that the stores (eight lanes a row) and the fragment reads (one piece of 32 rows) fall in distinct
+// banks. Chunk g is computed from one buffer while chunk g + 1 goes from registers into the other, and a register
+// that is stored takes its piece of chunk g + 2: every load has a whole chunk's time. Fragments are read a
+// step ahead (two sets); the one barrier per chunk stands before its last step, which then reads the next
+// chunk's first fragments. The order is pinned: left to the compiler, the fragments are read right before
+// their use.
+// The workgroups (one per CU) stay, and the chunks of a workgroup's tiles are one stream: the first chunks of its
+// next tile are loaded while the last ones of this tile are computed, and a tile's stores drain while the next one
+// is computed. (Started tile by tile, all CUs load, compute and store at the same time: 16,384 rows over 32
+// experts of 5,760 x 2,880 took 230 us, 42 of them for the stores and ~50 before the first products.)
+constexpr int kMxWideM = 256, kMxWideN = 256;
+
 template <int ODT>
-__global__ void __launch_bounds__(kMxWideThreads, 2) mx_wide_kernel(MxGemmArgs p, MxGroups go) {
-  constexpr int TN = kMxWideTile, TM = kMxWideTile, NA = 4, NB = 2, P = 4;
+__global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p, MxGroups go) {
+  constexpr int NA = 4, NB = 4, TN = kMxWideN, TM = kMxWideM;
+  constexpr int PW = TN / 32, PA = TM / 32;  // 16-byte pieces per thread and chunk
   __shared__ u32x4_t wl[2][TN * 8];
   __shared__ u32x4_t al[2][TM * 8];
-  __shared__ u32x2_t scl[2][TN + TM];  // the weight rows' scale bytes, then the activation rows'
-  MxTile t;
-  if (!mx_tile(p, go, t)) return;
+  __shared__ u32x2_t wsl[2][TN], asl[2][TM];
+  __shared__ int tab[3][kMxGroupsMax + 1];  // first row, first tile and expert (-1: none) of each group
   const int tid = threadIdx.x;
+  for (int i = tid; i <= p.groups; i += kMxWideThreads) {
+    tab[0][i] = go.off[i];
+    tab[1][i] = go.tile[i];
+    const int64_t id = i < p.groups ? p.ids[i] : -1;
+    tab[2][i] = id >= 0 && id < p.w.num_experts ? static_cast<int>(id) : -1;
+  }
+  __syncthreads();
+  // the workgroup's items: of its XCD's run, every 32nd or as many as workgroups there are
+  const int total = p.tiles * p.n_blocks, per = (total + kXcds - 1) / kXcds;
+  const int xcd = static_cast<int>(blockIdx.x) % kXcds;
+  const int stride = static_cast<int>(gridDim.x) / kXcds;
+  const int last = min((xcd + 1) * per, total);
+  int item = xcd * per + static_cast<int>(blockIdx.x) / kXcds;
+  if (item >= last) return;
+
   const int lane = tid & (kWave - 1);
   const int wid = __builtin_amdgcn_readfirstlane(tid) / kWave;
   const int wn = wid & 1, wm = wid >> 1;  // the wave's columns and rows of the tile
   const int half = lane >> 5, r32 = lane & 31;
-  const int64_t n = p.w.n, n0 = int64_t(t.nb) * TN;
+  const int64_t n = p.w.n;
   const int blocks = static_cast<int>(p.w.k / kMxBlock);
-  const int chunks = (blocks + 7) / 8;
-  const int e = max(t.e, 0);  // a group without an expert computes on expert 0 and stores zeros
-  const uint8_t* wbase = p.w.packed + (int64_t(e) * n + n0) * (16 * int64_t(blocks));
-  const uint8_t* wsbase = static_cast<const uint8_t*>(p.w.absmax) + (int64_t(e) * n + n0) * blocks;
-  const uint8_t* abase = p.a + int64_t(t.row0) * (chunks * 128);
-  const uint8_t* asbase = p.as + int64_t(t.row0) * (chunks * 8);
-  // rows past the ends repeat the last one; their sums are not stored
-  const int wlast = static_cast<int>(min<int64_t>(n - n0, TN)) - 1, alast = t.end - t.row0 - 1;
-  const int part = tid & 7, prow = tid >> 3;
-  uint32_t woff[P], aoff[P];
-  mx_for<P>([&](auto i) {
-    woff[i()] = static_cast<uint32_t>(min(64 * i() + prow, wlast)) * static_cast<uint32_t>(16 * blocks);
-    aoff[i()] = static_cast<uint32_t>(min(64 * i() + prow, alast)) * static_cast<uint32_t>(chunks * 128) + 16 * part;
-  });
-  // waves 0..3 carry the weights' scale bytes, 4..7 the activations', eight bytes per thread and chunk
-  const bool ws_wave = wid < 4;
-  const uint32_t srow = static_cast<uint32_t>(min(tid & (TN - 1), ws_wave ? wlast : alast));
-  const uint8_t* sbase = ws_wave ? wsbase + srow * static_cast<uint32_t>(blocks) : asbase + srow * static_cast<uint32_t>(chunks * 8);
-  const int sblocks = ws_wave ? blocks : 8 * chunks;
+  const int chunks = (blocks + 7) / 8;  // two at least: the loads are two ahead, at most one tile
+  const uint32_t wstride = 16 * blocks, astride = 128 * chunks;
 
-  u32x4_t wr[P], ar[P];
-  u32x2_t sr;
-  auto load_w = [&](auto i, int c) {
-    const int b = 8 * c + part;  // past the row's end: its first block, against zero codes
-    wr[i()] = *reinterpret_cast<const u32x4_t*>(wbase + (woff[i()] + 16 * (b < blocks ? b : 0)));
+  auto tile_of = [&](int w) {
+    const int t = __builtin_amdgcn_readfirstlane(w / p.n_blocks);
+    int lo = 0, hi = p.groups;  // the group whose tiles hold t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (__builtin_amdgcn_readfirstlane(tab[1][mid]) <= t) lo = mid;
+      else hi = mid;
+    }
+    const int first = __builtin_amdgcn_readfirstlane(tab[1][lo]);
+    const int count = __builtin_amdgcn_readfirstlane(tab[1][lo + 1]) - first;
+    const int i = w - first * p.n_blocks;
+    MxTile o;
+    o.e = __builtin_amdgcn_readfirstlane(tab[2][lo]);
+    o.nb = __builtin_amdgcn_readfirstlane(i / count);
+    o.row0 = __builtin_amdgcn_readfirstlane(tab[0][lo]) + (i - o.nb * count) * TM;
+    o.end = min(o.row0 + TM, __builtin_amdgcn_readfirstlane(tab[0][lo + 1]));
+    return o;
   };
-  auto load_a = [&](auto i, int c) { ar[i()] = *reinterpret_cast<const u32x4_t*>(abase + 128 * c + aoff[i()]); };
-  auto load_s = [&](int c) { sr = mx_scales8(sbase, 8 * c, sblocks); };
-  const int slot = prow * 8 + (part ^ (prow & 7));  // of rows 64 i + prow: 64 rows apart, the same order
-  auto store_w = [&](auto i, int buf) { wl[buf][512 * i() + slot] = wr[i()]; };
-  auto store_a = [&](auto i, int buf) { al[buf][512 * i() + slot] = ar[i()]; };
-  auto store_s = [&](int buf) { scl[buf][tid] = sr; };
+  // a tile's operands. Rows past the ends and pieces past the last row's end are zeros; a piece past another
+  // row's end is the next row's first, against zero codes. A group without an expert computes on expert 0 and
+  // stores zeros.
+  struct Source {
+    __amdgpu_buffer_rsrc_t w, a;
+    const uint8_t *ws, *as;
+    int wrows, arows;
+  };
+  auto source_of = [&](const MxTile& t) {
+    Source o;
+    const int64_t n0 = int64_t(t.nb) * TN, first = int64_t(max(t.e, 0)) * n + n0;
+    o.wrows = min(static_cast<int>(n) - t.nb * TN, TN);
+    o.arows = t.end - t.row0;
+    o.w = mx_rows_of(p.w.packed + first * wstride, int64_t(o.wrows) * wstride);
+    o.a = mx_rows_of(p.a + int64_t(t.row0) * astride, int64_t(o.arows) * astride);
+    o.ws = static_cast<const uint8_t*>(p.w.absmax) + first * blocks;
+    o.as = p.as + int64_t(t.row0) * (chunks * 8);
+    return o;
+  };
+
+  const int part = tid & 7, prow = tid >> 3;
+  const uint32_t woff = prow * wstride + 16 * part, aoff = prow * astride + 16 * part;
+  u32x4_t wr[PW], ar[PA];
+  u32x2_t wsr, asr;
+  int wpast = 0;
+  const int slot = prow * 8 + (part ^ (prow & 7));  // of rows 32 i + prow: 32 rows apart, the same order
+  // eight scale bytes of a weight row as mx_scales4 reads four, shifted where they are stored: the load is
+  // not waited for here
+  auto load_s = [&](const Source& f, int c) {
+    wpast = max(8 * c + 8 - blocks, 0);
+    __builtin_memcpy(&wsr, f.ws + (static_cast<uint32_t>(min(tid, f.wrows - 1)) * static_cast<uint32_t>(blocks) + (8 * c - wpast)), 8);
+    asr = *reinterpret_cast<const u32x2_t*>(f.as + (static_cast<uint32_t>(min(tid, f.arows - 1)) * (chunks * 8) + 8 * c));
+  };
+  auto store_s = [&](int buf) {
+    wsl[buf][tid] = __builtin_bit_cast(u32x2_t, __builtin_bit_cast(uint64_t, wsr) >> (8 * wpast));
+    asl[buf][tid] = asr;
+  };
+  auto load = [&](auto i, const Source& f, int c) {  // piece i of the thread: the weights' first
+    if constexpr (i() < PW) wr[i()] = mx_piece(f.w, woff, 32 * i() * wstride + 128 * c);
+    else ar[i() - PW] = mx_piece(f.a, aoff, 32 * (i() - PW) * astride + 128 * c);
+  };
+  auto store = [&](auto i, int buf) {
+    if constexpr (i() < PW) wl[buf][256 * i() + slot] = wr[i()];
+    else al[buf][256 * (i() - PW) + slot] = ar[i() - PW];
+  };
 
   mx_acc_t acc[NA][NB];
   mx_for<NA>([&](auto a) { mx_for<NB>([&](auto b) { acc[a()][b()] = mx_acc_t{}; }); });
   u32x4_t wf[2][NA], af[2][NB];
-  uint32_t ws[2][NA], as[2][NB];
+  uint32_t ws[NA], as[NB], wsn[NA], asn[NB];
   const int wrow = 32 * NA * wn + r32, arow = 32 * NB * wm + r32;
-  const bool live = 32 * NB * wm <= alast;  // the wave has rows
   auto frags = [&](auto set, int buf, int q) {
-    const int x = (q ^ (r32 & 7));
+    const int x = q ^ (r32 & 7);
     mx_for<NA>([&](auto a) { wf[set()][a()] = wl[buf][(wrow + 32 * a()) * 8 + x]; });
     mx_for<NB>([&](auto b) { af[set()][b()] = al[buf][(arow + 32 * b()) * 8 + x]; });
   };
-  auto scales = [&](auto set, int buf) {
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(scl[buf]) + half;
-    mx_for<NA>([&](auto a) { ws[set()][a()] = s[2 * (wrow + 32 * a())]; });
-    mx_for<NB>([&](auto b) { as[set()][b()] = s[2 * (TN + arow + 32 * b())]; });
+  auto scales = [&](int buf) {
+    mx_for<NA>([&](auto a) { wsn[a()] = reinterpret_cast<const uint32_t*>(wsl[buf])[2 * (wrow + 32 * a()) + half]; });
+    mx_for<NB>([&](auto b) { asn[b()] = reinterpret_cast<const uint32_t*>(asl[buf])[2 * (arow + 32 * b()) + half]; });
   };
-  auto products = [&](auto set, auto sset, auto j, auto from, auto to) {
-    mx_for<to() - from()>([&](auto i) {
-      constexpr int a = (from() + i()) / NB, b = (from() + i()) % NB;
-      acc[a][b] = mx_mfma<j()>(wf[set()][a], af[set()][b], ws[sset()][a], as[sset()][b], acc[a][b]);
-    });
-  };
-  constexpr std::integral_constant<int, 0> c0;
-  constexpr std::integral_constant<int, 1> c1;
-  constexpr std::integral_constant<int, 2> c2;
-  constexpr std::integral_constant<int, 3> c3;
-  constexpr std::integral_constant<int, 4> c4;
-  constexpr std::integral_constant<int, 8> c8;
-  // one piece moved on: into the other buffer, its register to the chunk after
-  auto move_w = [&](auto i, int buf, int c) { store_w(i, buf ^ 1); load_w(i, c); };
-  auto move_a = [&](auto i, int buf, int c) { store_a(i, buf ^ 1); load_a(i, c); };
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
 
-  mx_for<P>([&](auto i) { load_w(i, 0); load_a(i, 0); });
-  load_s(0);
-  {
-    const int c = min(1, chunks - 1);
-    mx_for<P>([&](auto i) {
-      store_w(i, 0);
-      load_w(i, c);
-      store_a(i, 0);
-      load_a(i, c);
-    });
-    store_s(0);
-    load_s(c);
-  }
-  __syncthreads();
-  frags(c0, 0, 4 * half);
-  scales(c0, 0);
-  // a chunk whose scales are in set s; the next chunk's go to set 1 - s
-  auto chunk = [&](auto s, auto s1, int c) {
-    const int buf = c & 1, cn = min(c + 2, chunks - 1);  // past the last chunk: again the last one, never stored
-    frags(c1, buf, 4 * half + 1);
-    if (live) products(c0, s, c0, c0, c4);
-    move_w(c0, buf, cn);
-    move_w(c1, buf, cn);
-    if (live) products(c0, s, c0, c4, c8);
-    move_w(c2, buf, cn);
-    frags(c0, buf, 4 * half + 2);
-    if (live) products(c1, s, c1, c0, c4);
-    move_w(c3, buf, cn);
-    move_a(c0, buf, cn);
-    if (live) products(c1, s, c1, c4, c8);
-    move_a(c1, buf, cn);
-    frags(c1, buf, 4 * half + 3);
-    if (live) products(c0, s, c2, c0, c4);
-    move_a(c2, buf, cn);
-    move_a(c3, buf, cn);
-    store_s(buf ^ 1);
-    load_s(cn);
-    if (live) products(c0, s, c2, c4, c8);
-    __syncthreads();
-    frags(c0, buf ^ 1, 4 * half);
-    scales(s1, buf ^ 1);
-    if (live) products(c1, s, c3, c0, c8);
-  };
-  int c = 0;
-  for (; c + 2 < chunks; c += 2) {
-    chunk(c0, c1, c);
-    chunk(c1, c0, c + 1);
-  }
-  if (c + 1 < chunks) chunk(c0, c1, c++);
-  // the last chunk's blocks in (left + 1) / 2 steps: step j takes blocks j and steps + j
-  if (live) {
-    const int buf = c & 1, left = blocks - 8 * c, steps = (left + 1) / 2;
-    uint32_t wz[NA], az[NB];
-    auto bytes = [&](int row) {  // the scale bytes of the half's blocks, the first lowest
-      return static_cast<uint32_t>(__builtin_bit_cast(uint64_t, scl[buf][row]) >> (half ? 8 * steps : 0));
-    };
-    mx_for<NA>([&](auto a) { wz[a()] = bytes(wrow + 32 * a()); });
-    mx_for<NB>([&](auto b) { az[b()] = bytes(TN + arow + 32 * b()); });
-    for (int j = 0; j < steps; ++j) {
-      frags(c0, buf, steps * half + j);
-      mx_for<NA>([&](auto a) {
-        mx_for<NB>([&](auto b) { acc[a()][b()] = mx_mfma<0>(wf[0][a()], af[0][b()], wz[a()], az[b()], acc[a()][b()]); });
-      });
-      mx_for<NA>([&](auto a) { wz[a()] >>= 8; });
-      mx_for<NB>([&](auto b) { az[b()] >>= 8; });
+  MxTile now = tile_of(item), then = now;
+  Source from = source_of(now);
+  int lc = 0;  // the next chunk to load, of the tile that `from` describes
+  auto advance = [&] {
+    if (++lc < chunks) return;
+    lc = 0;
+    item += stride;
+    if (item < last) {
+      then = tile_of(item);
+      from = source_of(then);
+    } else {
+      then.nb = -1;  // no tile: `from` is loaded once more, and not computed
     }
-  }
-  const bool vec = n % 8 == 0;
-  mx_for<NB>([&](auto b) {
-    const int row = t.row0 + arow + 32 * b();
-    mx_for<NA>([&](auto a) {
-      const int64_t col = n0 + 32 * (NA * wn + a());
-      mx_acc_t v = acc[a()][b()];
-      if (t.e < 0) v = mx_acc_t{};
-      if (col < n) mx_store_block<ODT>(p.out, int64_t(row) * n + col, n - col, vec, row < t.end, half, v);
-    });
+  };
+  mx_for<PW + PA>([&](auto i) { load(i, from, 0); });
+  load_s(from, 0);
+  advance();
+  mx_for<PW + PA>([&](auto i) {
+    store(i, 0);
+    load(i, from, lc);
   });
+  store_s(0);
+  load_s(from, lc);
+  __syncthreads();
+  frags(std::integral_constant<int, 0>{}, 0, 4 * half);
+  scales(0);
+  const bool vec = n % 8 == 0;
+  int buf = 0;
+  auto chunk = [&] {  // one chunk, from LDS buffer `buf`
+    const int other = 1 - buf;
+    advance();
+    mx_for<NA>([&](auto a) { ws[a()] = wsn[a()]; });
+    mx_for<NB>([&](auto b) { as[b()] = asn[b()]; });
+    mx_for<4>([&](auto j) {
+      constexpr std::integral_constant<int, j() & 1> set;
+      constexpr std::integral_constant<int, 1 - (j() & 1)> next;
+      if constexpr (j() < 3) {
+        frags(next, buf, 4 * half + j() + 1);
+      } else {
+        __syncthreads();
+        scales(other);
+        frags(next, other, 4 * half);
+      }
+      pin();
+      mx_for<NA>([&](auto a) {
+        mx_for<NB>([&](auto b) {
+          acc[a()][b()] = mx_mfma<j()>(wf[set()][a()], af[set()][b()], ws[a()], as[b()], acc[a()][b()]);
+        });
+        pin();
+        if constexpr (j() < 3) {  // the pieces of twelve slots
+          constexpr int at = NA * j() + a(), lo = at * (PW + PA) / 12, hi = (at + 1) * (PW + PA) / 12;
+          mx_for<hi - lo>([&](auto i) {
+            constexpr std::integral_constant<int, lo + i()> piece;
+            store(piece, other);
+            load(piece, from, lc);
+          });
+          if constexpr (at == 11) {
+            store_s(other);
+            load_s(from, lc);
+          }
+          pin();
+        }
+      });
+    });
+    buf = other;
+  };
+  for (;;) {
+    for (int c = 0; c < chunks; ++c) chunk();
+    mx_for<NB>([&](auto b) {
+      const int row = now.row0 + arow + 32 * b();
+      mx_for<NA>([&](auto a) {
+        const int col = now.nb * TN + 32 * (NA * wn + a());
+        mx_acc_t v = acc[a()][b()];
+        if (now.e < 0) v = mx_acc_t{};
+        // (the last columns' and rows' blocks: nothing to store)
+        mx_store_block<ODT>(p.out, int64_t(row) * n + col, row < now.end ? static_cast<int>(n) - col : 0, vec, half, v);
+        acc[a()][b()] = mx_acc_t{};
+        pin();
+      });
+    });
+    if (then.nb < 0) return;
+    now = then;
+  }
 }
 
 }  // namespace e4b

@@ -4,6 +4,7 @@
 #include "mx_launch.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace e4b {
 
@@ -35,7 +36,8 @@ int group_tiles(const MxTiling& tl, int size) {
 }
 
 template <class K>
-void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl, int columns, hipStream_t s) {
+void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl, int columns, hipStream_t s,
+                  unsigned most = 0x7fffffff) {
   a.tl = tl;
   a.tl.one = 1;
   int tiles = 0;
@@ -50,7 +52,7 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
   a.tiles = tiles;
   a.n_blocks = static_cast<int>((a.w.n + columns - 1) / columns);
   const unsigned total = static_cast<unsigned>(tiles) * static_cast<unsigned>(a.n_blocks);
-  hipLaunchKernelGGL(kernel, dim3((total + 7) / 8 * 8), dim3(threads), 0, s, a, g);
+  hipLaunchKernelGGL(kernel, dim3(std::min((total + 7) / 8 * 8, most)), dim3(threads), 0, s, a, g);
 }
 
 template <int ODT>
@@ -62,8 +64,14 @@ void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
     launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 0, 1, 0}, 32, s);
     return;
   }
-  launch_tiles(mx_wide_kernel<ODT>, kMxWideThreads, a, g, {kMxWideTile, kMxTileM, 0, 1, 0}, kMxWideTile, s);
-  launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 1, kMxWideTile, 0}, 32, s);
+  if (largest <= kMxTileM || a.w.k <= kMxChunk) {
+    launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 0, 1, 0}, 32, s);
+    return;
+  }
+  const char* env = getenv("MXT");
+  const int rest = env ? atoi(env) : 32;
+  launch_tiles(mx_wide_kernel<ODT>, kMxWideThreads, a, g, {kMxWideM, rest, 0, 1, 0}, kMxWideN, s, 256);
+  if (rest) launch_tiles(mx_narrow_kernel<ODT>, threads, a, g, {kMxTileM, 0, 1, kMxWideM, 0}, 32, s);
 }
 
 }  // namespace
