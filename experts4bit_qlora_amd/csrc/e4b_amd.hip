@@ -235,8 +235,8 @@ int check_mx_weight(const e4b_qweight* w) {
     return fail(E4B_EINVAL, "weight dims must be positive (E=%d n=%lld k=%lld)", w->num_experts, (long long)w->n,
                 (long long)w->k);
   if (w->k % 32) return fail(E4B_EUNSUPPORTED, "k=%lld is not a multiple of 32", (long long)w->k);
-  // offsets within a 256-row tile of weights are 32 bits
-  if (w->n > 0x7fffffffLL || w->k > (1 << 24)) return fail(E4B_EUNSUPPORTED, "n exceeds int32 or k 2^24");
+  // byte offsets within 256 rows of weights or outputs are 32 bits
+  if (w->n >= (1 << 22) || w->k >= (1 << 24)) return fail(E4B_EUNSUPPORTED, "n exceeds 2^22 or k 2^24");
   if (!w->packed || !w->absmax) return fail(E4B_EINVAL, "packed/absmax pointer is NULL");
   if (!aligned16(w->packed)) return fail(E4B_EINVAL, "packed weights must be 16-byte aligned");
   return E4B_OK;

@@ -106,7 +106,7 @@ E4B_DEV bool mx_tile(const MxGemmArgs& p, const MxGroups& go, MxTile& o) {
   const int64_t id = p.ids[g];
   o.e = id >= 0 && id < p.w.num_experts ? static_cast<int>(id) : -1;
   const int lo = go.off[g], hi = go.off[g + 1];
-  o.row0 = p.tl.rest_only ? hi - (hi - lo) % p.tl.big : lo + (i % count) * p.tl.tm;
+  o.row0 = lo + (i % count) * p.tl.tm;
   o.end = min(o.row0 + p.tl.tm, hi);
   return true;
 }
@@ -211,66 +211,86 @@ E4B_DEV void mx_for(F&& f) {
 
 constexpr int kMxWideThreads = 256;
 
-// An MFMA block's sums of a lane, columns 8 (i / 4) + 4 half + i % 4 of one row, to the row's outputs from `at`
-// on, `left` of them. For a 16-bit type v_permlane32_swap joins the halves' runs of four into eight
-// neighbouring columns, one 16-byte store where the row's addresses allow (vec).
-template <int ODT>
-E4B_DEV void mx_store_block(void* out, int64_t at, int left, bool vec, int half, const mx_acc_t& v) {
-  if constexpr (ODT == E4B_FP32) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = 8 * g + 4 * half;
-      float* o = static_cast<float*>(out) + at + c;
-      if (vec && left >= 32) {
-        *reinterpret_cast<float4*>(o) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < left) o[j] = v[4 * g + j];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      uint32_t lo[2], hi[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        lo[j] = pack2(from_f<ODT>(v[4 * g + 2 * j]), from_f<ODT>(v[4 * g + 2 * j + 1]));
-        hi[j] = pack2(from_f<ODT>(v[4 * g + 4 + 2 * j]), from_f<ODT>(v[4 * g + 4 + 2 * j + 1]));
-      }
-      const auto a = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
-      const auto b = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);
-      u32x4_t o = {a[0], b[0], a[1], b[1]};
-      const int c = 8 * g + 8 * half;
-      uint16_t* dst = static_cast<uint16_t*>(out) + at + c;
-      if (vec && left >= 32) {
-        *reinterpret_cast<u32x4_t*>(dst) = o;
-      } else {
-#pragma unroll 1
-        for (int j = 0; j < 8 && c + j < left; ++j) {
-          dst[j] = static_cast<uint16_t>(o[0]);
-          o[0] = __builtin_amdgcn_alignbit(o[1], o[0], 16);
-          o[1] = __builtin_amdgcn_alignbit(o[2], o[1], 16);
-          o[2] = __builtin_amdgcn_alignbit(o[3], o[2], 16);
-          o[3] >>= 16;
-        }
-      }
-    }
-  }
-}
-
 // `size` bytes from base on; 16 of them at offset + uniform, zeros at and past the end.
 E4B_DEV __amdgpu_buffer_rsrc_t mx_rows_of(const uint8_t* base, int64_t size) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, static_cast<int>(size), 0x00027000);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, static_cast<int>(static_cast<uint32_t>(size)), 0x00027000);
 }
 E4B_DEV u32x4_t mx_piece(__amdgpu_buffer_rsrc_t rows, uint32_t offset, uint32_t uniform) {
   return __builtin_amdgcn_raw_buffer_load_b128(rows, static_cast<int>(offset), static_cast<int>(uniform), 0);
 }
 
+// Two sums as a pair of 16-bit outputs.
+template <int ODT>
+E4B_DEV uint32_t mx_pair(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t v = {a, b};
+  if constexpr (ODT == E4B_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+
+// An MFMA block's sums of a lane, columns 8 (i / 4) + 4 half + i % 4 of row l % 32, to a tile's output rows, the
+// block's first output at byte `uniform` of the buffer (rows past the tile's last lie past its end).
+// All 32 columns of 16-bit outputs: v_permlane32_swap joins the halves' runs of four into eight neighbouring
+// columns, v_permlane16_swap hands a lane's second eight to the lane sixteen rows on for that lane's first
+// eight: four lanes then write a row's whole 64 bytes, sixteen rows per store. `offset`: of row l % 16,
+// columns 16 (l / 16 % 2) + 8 half.
+template <int ODT>
+E4B_DEV void mx_store_whole(__amdgpu_buffer_rsrc_t out, uint32_t offset, uint32_t uniform, uint32_t row_bytes,
+                            const mx_acc_t& v) {
+  uint32_t o[2][4];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const auto s = __builtin_amdgcn_permlane32_swap(mx_pair<ODT>(v[8 * g + 2 * j], v[8 * g + 2 * j + 1]),
+                                                      mx_pair<ODT>(v[8 * g + 4 + 2 * j], v[8 * g + 5 + 2 * j]), false, false);
+      o[g][j] = s[0];
+      o[g][2 + j] = s[1];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const auto s = __builtin_amdgcn_permlane16_swap(o[0][j], o[1][j], false, false);
+    o[0][j] = s[0];
+    o[1][j] = s[1];
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{o[g][0], o[g][1], o[g][2], o[g][3]}, out, static_cast<int>(offset),
+                                           static_cast<int>(uniform + 16 * g * row_bytes), 0);
+}
+// The first `left` of the 32 columns, or fp32 outputs. `offset`: of row l % 32, column 4 half.
+template <int ODT>
+E4B_DEV void mx_store_part(__amdgpu_buffer_rsrc_t out, uint32_t offset, uint32_t uniform, int left, int half,
+                           const mx_acc_t& v) {
+  constexpr int kOut = ODT == E4B_FP32 ? 4 : 2;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    u32x4_t o;  // the next output lowest
+    if constexpr (ODT == E4B_FP32)
+      o = u32x4_t{__float_as_uint(v[4 * g]), __float_as_uint(v[4 * g + 1]), __float_as_uint(v[4 * g + 2]),
+                  __float_as_uint(v[4 * g + 3])};
+    else
+      o = u32x4_t{mx_pair<ODT>(v[4 * g], v[4 * g + 1]), mx_pair<ODT>(v[4 * g + 2], v[4 * g + 3]), 0, 0};
+    const int c = 8 * g + 4 * half, at = static_cast<int>(uniform + 8 * g * kOut);
+#pragma unroll 1
+    for (int j = 0; j < 4 && c + j < left; ++j) {
+      const int to = static_cast<int>(offset + kOut * j);
+      if constexpr (ODT == E4B_FP32) {
+        __builtin_amdgcn_raw_buffer_store_b32(o[0], out, to, at, 0);
+        o = u32x4_t{o[1], o[2], o[3], 0};
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(o[0]), out, to, at, 0);
+        o = u32x4_t{__builtin_amdgcn_alignbit(o[1], o[0], 16), o[1] >> 16, 0, 0};
+      }
+    }
+  }
+}
+
 // A tile of 256 rows times 256 weight rows, four waves (one per SIMD) of 128 x 128. Both operands pass through LDS
 // a chunk of 256 values at a time: 128-byte rows whose eight 16-byte pieces are stored in the order piece ^ (row
-// & 7), so that the stores (eight lanes a row) and the fragment reads (one piece of 32 rows) fall in distinct
-// banks. Chunk g is computed from one buffer while chunk g + 1 goes from registers into the other, and a register
+// / 2 & 7): a row is half of the 64 banks, and sixteen rows' reads of one piece fall in distinct ones, as do the
+// stores (eight lanes a row). Chunk g is computed from one buffer while chunk g + 1 goes from registers into the other, and a register
 // that is stored takes its piece of chunk g + 2: every load has a whole chunk's time. Fragments are read a
 // step ahead (two sets); the one barrier per chunk stands before its last step, which then reads the next
 // chunk's first fragments. The order is pinned: left to the compiler, the fragments are read right before
@@ -289,6 +309,8 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   __shared__ u32x4_t al[2][TM * 8];
   __shared__ u32x2_t wsl[2][TN], asl[2][TM];
   __shared__ int tab[3][kMxGroupsMax + 1];  // first row, first tile and expert (-1: none) of each group
+  constexpr int kItems = 128;
+  __shared__ int4 items[kItems];
   const int tid = threadIdx.x;
   for (int i = tid; i <= p.groups; i += kMxWideThreads) {
     tab[0][i] = go.off[i];
@@ -314,23 +336,29 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   const int chunks = (blocks + 7) / 8;  // two at least: the loads are two ahead, at most one tile
   const uint32_t wstride = 16 * blocks, astride = 128 * chunks;
 
-  auto tile_of = [&](int w) {
-    const int t = __builtin_amdgcn_readfirstlane(w / p.n_blocks);
-    int lo = 0, hi = p.groups;  // the group whose tiles hold t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (__builtin_amdgcn_readfirstlane(tab[1][mid]) <= t) lo = mid;
-      else hi = mid;
+  // the workgroup's next kItems tiles, one per thread, from the tables: a tile is then one broadcast read
+  auto fill = [&](int first_item) {
+    const int w = first_item + tid * stride;
+    if (tid < kItems && w < last) {
+      const int t = w / p.n_blocks;
+      int lo = 0, hi = p.groups;  // the group whose tiles hold t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (tab[1][mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int first = tab[1][lo], count = tab[1][lo + 1] - first, i = w - first * p.n_blocks;
+      const int nb = i / count, row0 = tab[0][lo] + (i - nb * count) * TM;
+      items[tid] = make_int4(tab[2][lo], nb, row0, min(row0 + TM, tab[0][lo + 1]));
     }
-    const int first = __builtin_amdgcn_readfirstlane(tab[1][lo]);
-    const int count = __builtin_amdgcn_readfirstlane(tab[1][lo + 1]) - first;
-    const int i = w - first * p.n_blocks;
-    MxTile o;
-    o.e = __builtin_amdgcn_readfirstlane(tab[2][lo]);
-    o.nb = __builtin_amdgcn_readfirstlane(i / count);
-    o.row0 = __builtin_amdgcn_readfirstlane(tab[0][lo]) + (i - o.nb * count) * TM;
-    o.end = min(o.row0 + TM, __builtin_amdgcn_readfirstlane(tab[0][lo + 1]));
-    return o;
+  };
+  int filled = item;  // the first item of the table
+  fill(filled);
+  __syncthreads();
+  auto tile_of = [&](int w) {
+    const int4 v = items[(w - filled) / stride];
+    return MxTile{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.z),
+                  __builtin_amdgcn_readfirstlane(v.w), __builtin_amdgcn_readfirstlane(v.y)};
   };
   // a tile's operands. Rows past the ends and pieces past the last row's end are zeros; a piece past another
   // row's end is the next row's first, against zero codes. A group without an expert computes on expert 0 and
@@ -357,7 +385,7 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   u32x4_t wr[PW], ar[PA];
   u32x2_t wsr, asr;
   int wpast = 0;
-  const int slot = prow * 8 + (part ^ (prow & 7));  // of rows 32 i + prow: 32 rows apart, the same order
+  const int slot = prow * 8 + (part ^ ((prow >> 1) & 7));  // of rows 32 i + prow: 32 rows apart, the same order
   // eight scale bytes of a weight row as mx_scales4 reads four, shifted where they are stored: the load is
   // not waited for here
   auto load_s = [&](const Source& f, int c) {
@@ -384,7 +412,7 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   uint32_t ws[NA], as[NB], wsn[NA], asn[NB];
   const int wrow = 32 * NA * wn + r32, arow = 32 * NB * wm + r32;
   auto frags = [&](auto set, int buf, int q) {
-    const int x = q ^ (r32 & 7);
+    const int x = q ^ ((r32 >> 1) & 7);
     mx_for<NA>([&](auto a) { wf[set()][a()] = wl[buf][(wrow + 32 * a()) * 8 + x]; });
     mx_for<NB>([&](auto b) { af[set()][b()] = al[buf][(arow + 32 * b()) * 8 + x]; });
   };
@@ -402,6 +430,12 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
     lc = 0;
     item += stride;
     if (item < last) {
+      if (item - filled == kItems * stride) {  // (uniform; every wave has read the table's last tile)
+        __syncthreads();
+        filled = item;
+        fill(filled);
+        __syncthreads();
+      }
       then = tile_of(item);
       from = source_of(then);
     } else {
@@ -420,7 +454,6 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   __syncthreads();
   frags(std::integral_constant<int, 0>{}, 0, 4 * half);
   scales(0);
-  const bool vec = n % 8 == 0;
   int buf = 0;
   auto chunk = [&] {  // one chunk, from LDS buffer `buf`
     const int other = 1 - buf;
@@ -462,18 +495,28 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   };
   for (;;) {
     for (int c = 0; c < chunks; ++c) chunk();
-    mx_for<NB>([&](auto b) {
-      const int row = now.row0 + arow + 32 * b();
+    constexpr uint32_t kOut = ODT == E4B_FP32 ? 4 : 2;
+    const uint32_t ostride = static_cast<uint32_t>(n) * kOut;
+    const auto out = mx_rows_of(static_cast<uint8_t*>(p.out) + (int64_t(now.row0) * n + now.nb * TN) * kOut,
+                                int64_t(now.end - now.row0) * ostride - now.nb * TN * kOut);
+    if (now.e < 0) mx_for<NA>([&](auto a) { mx_for<NB>([&](auto b) { acc[a()][b()] = mx_acc_t{}; }); });
+    const int left = static_cast<int>(n) - now.nb * TN - 32 * NA * wn;
+    auto write = [&](auto&& block) {
       mx_for<NA>([&](auto a) {
-        const int col = now.nb * TN + 32 * (NA * wn + a());
-        mx_acc_t v = acc[a()][b()];
-        if (now.e < 0) v = mx_acc_t{};
-        // (the last columns' and rows' blocks: nothing to store)
-        mx_store_block<ODT>(p.out, int64_t(row) * n + col, row < now.end ? static_cast<int>(n) - col : 0, vec, half, v);
-        acc[a()][b()] = mx_acc_t{};
-        pin();
+        mx_for<NB>([&](auto b) {
+          block(acc[a()][b()], (32 * (NB * wm + b())) * ostride + 32 * (NA * wn + a()) * kOut, left - 32 * a());
+          pin();  // (else all of the tile's sums are read ahead)
+        });
       });
-    });
+    };
+    if (ODT != E4B_FP32 && n % 8 == 0 && left >= 32 * NA) {
+      const uint32_t o = (lane & 15) * ostride + 2 * (lane & 16) + 16 * half;
+      write([&](const mx_acc_t& v, uint32_t at, int) { mx_store_whole<ODT == E4B_FP32 ? E4B_BF16 : ODT>(out, o, at, ostride, v); });
+    } else {
+      const uint32_t o = r32 * ostride + 4 * kOut * half;
+      write([&](const mx_acc_t& v, uint32_t at, int l) { mx_store_part<ODT>(out, o, at, l, half, v); });
+    }
+    mx_for<NA>([&](auto a) { mx_for<NB>([&](auto b) { acc[a()][b()] = mx_acc_t{}; }); });
     if (then.nb < 0) return;
     now = then;
   }

@@ -23,11 +23,9 @@ struct MxGroups {
 };
 constexpr int64_t kMxRowsMax = int64_t(1) << 23;  // below 2^16 tiles of 256 rows, one more per group
 
-// How a launch cuts the groups into row tiles. With tiles of tm rows it takes of each group its whole tiles
-// and its last rows where more than rest_above are left, or (rest_only) only those last rows where at
-// most tm are left past whole tiles of `big` rows: together the two launches cover every row once.
+// A launch's row tiles: tiles of tm rows over the groups of above lo and at most hi rows.
 struct MxTiling {
-  int tm, rest_above, rest_only, big;
+  int tm, lo, hi;
   int one;  // every group is one tile
 };
 
