@@ -856,12 +856,13 @@ int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, 
     return fail(E4B_EUNSUPPORTED, "groups=%d outside [0, %d]", groups, e4b::kMxGroupsMax);
   if (groups > 0 && (!sizes || !expert_ids)) return fail(E4B_EINVAL, "sizes/expert_ids is NULL");
   e4b::MxGroups go{};
+  const int64_t rows_max = e4b::mx_rows_max(w->k);
   int64_t M = 0;
   for (int g = 0; g < groups; ++g) {
     if (sizes[g] < 0) return fail(E4B_EINVAL, "group %d has a negative size", g);
     go.off[g] = static_cast<int32_t>(M);
-    if (sizes[g] > e4b::kMxRowsMax || (M += sizes[g]) > e4b::kMxRowsMax)
-      return fail(E4B_EUNSUPPORTED, "groups hold more than %lld rows", (long long)e4b::kMxRowsMax);
+    if (sizes[g] > rows_max || (M += sizes[g]) > rows_max)
+      return fail(E4B_EUNSUPPORTED, "groups hold more than %lld rows", (long long)rows_max);
   }
   for (int g = groups; g <= e4b::kMxGroupsMax; ++g) go.off[g] = static_cast<int32_t>(M);
   if (M == 0) return E4B_OK;
@@ -871,25 +872,22 @@ int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, 
   if (!workspace || workspace_bytes < need)
     return fail(E4B_ESPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
   if (!aligned16(workspace)) return fail(E4B_EINVAL, "workspace must be 16-byte aligned");
-  // one launch covers 2^31 - 1 workgroups: of the rows' quantization, and of 32-row x 32-column tiles
-  if (M * e4b::mx_chunks(w->k) / 8 >= 0x7fffffffLL ||
+  // 32-bit chunk numbers in the rows' quantization; one launch covers 2^31 - 1 tiles of 32 x 32
+  if (M * e4b::mx_chunks(w->k) >= 0x7fffffffLL ||
       max_tiles_for(M, groups, 32) * cdiv(w->n, 32) >= 0x7fffffffLL)
     return fail(E4B_EUNSUPPORTED, "%lld rows are more than one launch covers", (long long)M);
-  uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* scales = codes + align256(size_t(M) * mx_row_bytes(w->k));
-  e4b::launch_mx_rows(a, act_dtype, M, w->k, codes, scales, stream);
-  rc = check_launch("mx_rows_kernel");
-  if (rc) return rc;
   e4b::MxGemmArgs args{};
-  args.a = codes;
-  args.as = scales;
+  args.x = a;
+  args.act_dtype = act_dtype;
+  args.a = static_cast<uint8_t*>(workspace);
+  args.as = args.a + align256(size_t(M) * mx_row_bytes(w->k));
   args.w = *w;
   args.ids = expert_ids;
   args.groups = groups;
   args.M = M;
   args.out = out;
   e4b::launch_mx_gemm_groups(args, go, out_dtype, stream);
-  return check_launch("mx_narrow_kernel");
+  return check_launch("the microscaled product");
 }
 
 int e4b_weight_shift(const e4b_qweight* w, int32_t* shift, hipStream_t stream) {

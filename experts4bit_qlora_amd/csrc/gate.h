@@ -324,33 +324,61 @@ __global__ void __launch_bounds__(kGateThreads) balance_kernel(BalanceArgs p, in
   }
 }
 
-// A layer's chunks joined, in chunk order and 64 bits: counts, valid tokens, loss.
-__global__ void __launch_bounds__(kGateThreads) balance_join_kernel(BalanceArgs p) {
-  __shared__ double terms[kGateThreads];
+// A layer's chunks joined, in a fixed order and 64 bits: counts, valid tokens, loss. Bound by the latency of
+// its loads: `lanes` threads (a power of two from 32, the layer's experts or 1,024 of them) per part of the chunks, every
+// 1024 / lanes'th, so that a thread's serial loads are few.
+constexpr int kJoinThreads = 1024;
+E4B_DEV double wave_sum(double v) {
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(BalanceArgs p, int lanes) {
+  __shared__ double part[kJoinThreads];
+  __shared__ int count[kJoinThreads];
   const int tid = threadIdx.x, layer = blockIdx.x;
-  int64_t n = 0;
-  for (int c = 0; c < p.chunks; ++c) n += p.part_counts[(int64_t(layer) * p.chunks + c) * (p.E + 1) + p.E];
-  double mine = 0.0;
-  for (int e = tid; e < p.E; e += kGateThreads) {
-    double s = 0.0;
-    int64_t count = 0;
-    for (int c = 0; c < p.chunks; ++c) {
-      const int64_t part = int64_t(layer) * p.chunks + c;
-      s += p.part[part * p.E + e];
-      count += p.part_counts[part * (p.E + 1) + e];
+  const int e = tid & (lanes - 1), from = tid / lanes, step = kJoinThreads / lanes;
+  const float* sums = p.part + int64_t(layer) * p.chunks * p.E + e;
+  const int32_t* counts = p.part_counts + int64_t(layer) * p.chunks * (p.E + 1);
+  double s = 0.0;
+  int n = 0, valid = 0;  // at most T * k of them: 32 bits
+  if (e < p.E) {
+#pragma unroll 8
+    for (int c = from; c < p.chunks; c += step) {
+      s += sums[int64_t(c) * p.E];
+      n += counts[int64_t(c) * (p.E + 1) + e];
     }
-    p.counts[int64_t(layer) * p.E + e] = count;
-    mine += static_cast<double>(count) * s;
   }
-  terms[tid] = mine;
+  for (int c = tid; c < p.chunks; c += kJoinThreads) valid += counts[int64_t(c) * (p.E + 1) + p.E];
+  part[tid] = s;
+  count[tid] = n;
   __syncthreads();
-  for (int o = kGateThreads / 2; o > 0; o >>= 1) {
-    if (tid < o) terms[tid] += terms[tid + o];
-    __syncthreads();
+  double mine = 0.0;
+  if (tid < p.E) {  // (lanes >= E: its parts are tid + lanes * i)
+    for (int i = 1; i < step; ++i) {
+      s += part[tid + lanes * i];
+      n += count[tid + lanes * i];
+    }
+    p.counts[int64_t(layer) * p.E + tid] = n;
+    mine = static_cast<double>(n) * s;
   }
+  __syncthreads();
+  mine = wave_sum(mine);
+  const double all = wave_sum(static_cast<double>(valid));  // exact: at most 2^31
+  double* const valids = part + kJoinThreads / kWave;
+  if (tid % kWave == 0) {
+    part[tid / kWave] = mine;
+    valids[tid / kWave] = all;
+  }
+  __syncthreads();
   if (tid == 0) {
-    p.valid[layer] = n;
-    p.loss[layer] = n ? static_cast<float>(terms[0] * p.E / (static_cast<double>(n) * static_cast<double>(n))) : 0.0f;
+    double terms = 0.0, tokens = 0.0;
+    for (int i = 0; i < kJoinThreads / kWave; ++i) {
+      terms += part[i];
+      tokens += valids[i];
+    }
+    p.valid[layer] = static_cast<int64_t>(tokens);
+    p.loss[layer] = tokens > 0.0 ? static_cast<float>(terms * p.E / (tokens * tokens)) : 0.0f;
   }
 }
 

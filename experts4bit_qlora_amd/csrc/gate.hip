@@ -79,7 +79,9 @@ void launch_balance(const BalanceArgs& a, hipStream_t s) {
                        sizeof(float) * kGateThreads * vpl(), s, a, vec_rows(a.logits, a.dtype, a.E),
                        cdiv(a.T, a.chunks));
   });
-  hipLaunchKernelGGL(balance_join_kernel, dim3(static_cast<unsigned>(a.L)), dim3(kGateThreads), 0, s, a);
+  int lanes = 32;
+  while (lanes < a.E) lanes *= 2;
+  hipLaunchKernelGGL(balance_join_kernel, dim3(static_cast<unsigned>(a.L)), dim3(kJoinThreads), 0, s, a, lanes);
 }
 
 void launch_balance_backward(const BalanceArgs& a, hipStream_t s) {

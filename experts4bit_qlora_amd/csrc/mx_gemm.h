@@ -34,33 +34,40 @@ E4B_DEV mx_acc_t mx_mfma(const u32x4_t& w, const u32x4_t& a, uint32_t ws, uint32
 }
 
 // Four scale bytes of a weight row from block b on. Rows of scale bytes start at any address and are read in
-// whole words: one that would pass the row's end is read back from it and shifted. Blocks past the end,
-// whose activation codes are zero, get byte 0.
-E4B_DEV uint32_t mx_scales4(const uint8_t* row, int b, int blocks) {
-  uint32_t v = 0;
+// whole words: one that would pass the row's end is read back from it and shifted where it is used (`past` bytes;
+// blocks past the end, whose activation codes are zero, get byte 0). Rows of fewer than four: by bytes.
+struct MxScales {
+  uint32_t word;
+  int past;
+};
+E4B_DEV MxScales mx_scales4(const uint8_t* row, int b, int blocks) {
+  MxScales s = {0, 0};
   if (blocks >= 4) {
-    const int past = b + 4 - blocks;
-    if (past >= 4) return 0;
-    __builtin_memcpy(&v, row + (past > 0 ? blocks - 4 : b), 4);
-    return v >> (past > 0 ? 8 * past : 0);
+    s.past = min(max(b + 4 - blocks, 0), 4);
+    __builtin_memcpy(&s.word, row + min(b, blocks - 4), 4);
+  } else {
+    for (int j = 0; b + j < blocks; ++j) s.word |= static_cast<uint32_t>(row[b + j]) << (8 * j);
   }
-  for (int j = 0; b + j < blocks; ++j) v |= static_cast<uint32_t>(row[b + j]) << (8 * j);
-  return v;
+  return s;
 }
+E4B_DEV uint32_t mx_scale_word(const MxScales& s) { return s.past < 4 ? s.word >> (8 * s.past) : 0u; }
+
 constexpr int kMxRowThreads = 256;
 
 // Activation rows to padded codes and scale bytes (a block with an infinity or a NaN: 255). Thread =
-// piece of eight values; pieces past k are zero.
+// piece of eight values; 32 threads take a chunk of a row, pieces past k are zero.
 template <int DT>
-__global__ void __launch_bounds__(kMxRowThreads) mx_rows_kernel(const void* __restrict__ x, int64_t k, int row_pieces,
-                                                                int64_t pieces, uint32_t* __restrict__ codes,
+__global__ void __launch_bounds__(kMxRowThreads) mx_rows_kernel(const void* __restrict__ x, int row_values, uint32_t row_chunks,
+                                                                uint32_t chunks, uint32_t* __restrict__ codes,
                                                                 uint8_t* __restrict__ scales) {
+  constexpr int kPieces = kMxChunk / 8;
+  const uint32_t chunk = blockIdx.x * (kMxRowThreads / kPieces) + threadIdx.x / kPieces;
+  if (chunk >= chunks) return;
+  const uint32_t row = chunk / row_chunks;
+  const int q = static_cast<int>(chunk - row * row_chunks) * kPieces + threadIdx.x % kPieces;
   const int64_t p = int64_t(blockIdx.x) * kMxRowThreads + threadIdx.x;
-  if (p >= pieces) return;  // whole quads: a row's pieces are a multiple of 32
-  const int64_t row = p / row_pieces;
-  const int q = static_cast<int>(p - row * row_pieces);
-  const bool in = q < k / 8;
-  MxPiece<DT> v = mx_load<DT>(x, row * (k / 8) + (in ? q : 0));
+  const bool in = q < row_values / 8;
+  MxPiece<DT> v = mx_load<DT>(x, int64_t(row) * (row_values / 8) + (in ? q : 0));
   const uint32_t m = quad_max(mx_amax<DT>(v));
   const uint32_t e = mx_scale_byte<DT>(m, true);
   const uint32_t c = mx_codes<DT>(v, e);
@@ -137,14 +144,16 @@ E4B_DEV void mx_store4(void* out, int64_t at, int left, bool vec, const float (&
 }
 
 // A tile of at most 32 rows times 32 weight rows per workgroup: each of the four waves takes every
-// fourth chunk of K straight into the operand registers, their sums join in LDS. Bound by the weights'
-// bytes: each is read once per tile.
+// fourth chunk of K straight into the operand registers, the next one's loads in flight while it computes; their
+// sums join in LDS. Bound by the weights' bytes: each is read once per tile.
+// DT >= 0: the workgroup quantizes its rows itself into LDS, from values of type DT.
 constexpr int kMxTileM = 32;
 constexpr int kMxNarrowWaves = 4;
 
-template <int ODT>
+template <int ODT, int DT>
 __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemmArgs p, MxGroups go) {
   __shared__ float red[kMxNarrowWaves][32][33];
+  extern __shared__ u32x4_t own[];  // DT >= 0: the rows' codes, 8 * chunks pieces each, then their scale bytes
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wid = __builtin_amdgcn_readfirstlane(tid) / kWave;
@@ -160,23 +169,58 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
     const int64_t wrow = int64_t(e) * n + min(static_cast<int>(n0) + r32, static_cast<int>(n) - 1);  // rows past n are not stored
     const uint8_t* wc = p.w.packed + wrow * (p.w.k / 2);
     const uint8_t* ws = static_cast<const uint8_t*>(p.w.absmax) + wrow * blocks;
-    const int64_t arow = min(row0 + r32, end - 1);  // columns past the tile's rows are not stored
-    const uint8_t* ac = p.a + arow * (chunks * 128);
-    const uint8_t* as = p.as + arow * (chunks * 8);
-    for (int c = wid; c < chunks; c += kMxNarrowWaves) {
-      u32x4_t wv[4], av[4];
+    const int arow = min(r32, end - row0 - 1);  // columns past the tile's rows are not stored
+    const uint8_t* ac = p.a + int64_t(row0 + arow) * (chunks * 128);
+    const uint8_t* as = p.as + int64_t(row0 + arow) * (chunks * 8);
+    struct Part {
+      u32x4_t w[4], a[4];
+      MxScales ws;
+      uint32_t as;
+    } even, odd;
+    auto load = [&](Part& f, int c) {
+      const int b0 = 8 * c + 4 * half;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int b = 8 * c + 4 * half + j;
-        wv[j] = *reinterpret_cast<const u32x4_t*>(wc + 16 * (b < blocks ? b : 0));
-        av[j] = *reinterpret_cast<const u32x4_t*>(ac + 16 * b);
+        f.w[j] = *reinterpret_cast<const u32x4_t*>(wc + 16 * (b0 + j < blocks ? b0 + j : 0));
+        if constexpr (DT < 0) f.a[j] = *reinterpret_cast<const u32x4_t*>(ac + 16 * (b0 + j));
       }
-      const uint32_t wsc = mx_scales4(ws, 8 * c + 4 * half, blocks);
-      const uint32_t asc = *reinterpret_cast<const uint32_t*>(as + 8 * c + 4 * half);
-      acc = mx_mfma<0>(wv[0], av[0], wsc, asc, acc);
-      acc = mx_mfma<1>(wv[1], av[1], wsc, asc, acc);
-      acc = mx_mfma<2>(wv[2], av[2], wsc, asc, acc);
-      acc = mx_mfma<3>(wv[3], av[3], wsc, asc, acc);
+      f.ws = mx_scales4(ws, b0, blocks);
+      if constexpr (DT < 0) f.as = *reinterpret_cast<const uint32_t*>(as + b0);
+    };
+    uint8_t* const own_scales = reinterpret_cast<uint8_t*>(own + (end - row0) * 8 * chunks);
+    auto add = [&](Part& f, int c) {
+      if constexpr (DT >= 0) {
+        const int b0 = 8 * (arow * chunks + c) + 4 * half;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.a[j] = own[b0 + j];
+        f.as = *reinterpret_cast<const uint32_t*>(own_scales + b0);
+      }
+      const uint32_t wsc = mx_scale_word(f.ws);
+      acc = mx_mfma<0>(f.w[0], f.a[0], wsc, f.as, acc);
+      acc = mx_mfma<1>(f.w[1], f.a[1], wsc, f.as, acc);
+      acc = mx_mfma<2>(f.w[2], f.a[2], wsc, f.as, acc);
+      acc = mx_mfma<3>(f.w[3], f.a[3], wsc, f.as, acc);
+    };
+    if (wid < chunks) load(even, wid);
+    if constexpr (DT >= 0) {
+      const int pieces = 32 * chunks, in = static_cast<int>(p.w.k / 8);  // of eight values, padded and given
+      for (int r = 0; r < end - row0; ++r) {
+        for (int q = tid; q < pieces; q += kMxNarrowWaves * kWave) {  // whole quads: a block's four pieces
+          const MxPiece<DT> v = mx_load<DT>(p.x, int64_t(row0 + r) * in + (q < in ? q : 0));
+          const uint32_t s = mx_scale_byte<DT>(quad_max(mx_amax<DT>(v)), true);
+          reinterpret_cast<uint32_t*>(own)[r * pieces + q] = q < in ? mx_codes<DT>(v, s) : 0u;
+          if ((q & 3) == 0) own_scales[(r * pieces + q) >> 2] = q < in ? static_cast<uint8_t>(s) : 0;
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = wid; c < chunks; c += 2 * kMxNarrowWaves) {
+      const int d = c + kMxNarrowWaves;
+      if (d < chunks) load(odd, d);
+      add(even, c);
+      if (d >= chunks) break;
+      if (d + kMxNarrowWaves < chunks) load(even, d + kMxNarrowWaves);
+      add(odd, d);
     }
   }
 #pragma unroll

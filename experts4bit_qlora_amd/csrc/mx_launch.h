@@ -21,7 +21,8 @@ struct MxGroups {
   int32_t off[kMxGroupsMax + 1];
   uint16_t tile[kMxGroupsMax + 1];
 };
-constexpr int64_t kMxRowsMax = int64_t(1) << 23;  // below 2^16 tiles of 256 rows, one more per group
+// Fewer than 2^16 row tiles, one more than the rows fill per group: of 256 rows, or of 32 where K is one chunk.
+inline int64_t mx_rows_max(int64_t k) { return int64_t(1) << (k > kMxChunk ? 23 : 20); }
 
 // A launch's row tiles: tiles of tm rows over the groups of above lo and at most hi rows.
 struct MxTiling {
@@ -30,8 +31,10 @@ struct MxTiling {
 };
 
 struct MxGemmArgs {
-  const uint8_t* a;   // codes [rows, 128 * chunks]
-  const uint8_t* as;  // scale bytes [rows, 8 * chunks]
+  const void* x;      // the rows [rows, k] as given, of type act_dtype
+  int act_dtype;
+  uint8_t* a;         // workspace: codes [rows, 128 * chunks]
+  uint8_t* as;        // workspace: scale bytes [rows, 8 * chunks]
   e4b_qweight w;
   const int64_t* ids;  // group form: the groups' experts (device); a group outside [0, E) gets zero rows
   int groups;
@@ -42,11 +45,7 @@ struct MxGemmArgs {
   int n_blocks;  // column blocks of the launch
 };
 
-// Rows [rows, k] of dtype to padded codes and scale bytes; a block with an infinity or a NaN takes the
-// scale byte 255, which makes its products NaN.
-void launch_mx_rows(const void* x, int dtype, int64_t rows, int64_t k, uint8_t* codes, uint8_t* scales, hipStream_t s);
-
-// The whole product of the group form (g.tile is filled for each launch).
+// The whole product of the group form, the rows' quantization included (g.tile is filled for each launch).
 void launch_mx_gemm_groups(const MxGemmArgs& a, MxGroups& g, int out_dtype, hipStream_t s);
 
 }  // namespace e4b

@@ -73,9 +73,11 @@ class QW:
     shift: torch.Tensor | None = None  # NF4: per-expert exponents of the fp16 matrix-core mode
 
     def __setattr__(self, name, value):  # a changed field invalidates the cached descriptor
-        self.__dict__.pop("_struct", None)
-        self.__dict__.pop("_ref", None)
-        object.__setattr__(self, name, value)
+        d = self.__dict__
+        if "_struct" in d:
+            del d["_struct"]
+            d.pop("_ref", None)
+        d[name] = value
 
     def struct(self) -> N.QWeight:
         """The C descriptor, built once per field state: the tensors it points at are held by this
@@ -349,8 +351,8 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, mask: torch.Tensor |
     dev = logits.device
     lib = N.lib()
     loss = torch.empty(L_, dtype=torch.float32, device=dev)
-    counts = torch.empty(L_, E + 1, dtype=torch.int64, device=dev)  # the counts and, behind them, the valid tokens
-    counts, valid = counts.view(-1)[:L_ * E].view(L_, E), counts.view(-1)[L_ * E:]
+    counts = torch.empty(L_, E, dtype=torch.int64, device=dev)
+    valid = torch.empty(L_, dtype=torch.int64, device=dev)
     ws = torch.empty(max(1, lib.e4b_balance_workspace_bytes(L_, T, E)), dtype=torch.uint8, device=dev)
     with _on(dev):
         N.check("e4b_balance_loss",
@@ -840,12 +842,16 @@ def mx_grouped_gemm(a: torch.Tensor, qw: QW, sizes, expert_ids) -> torch.Tensor:
         ids = torch.tensor(host, dtype=torch.int64, device=a.device)
     if ids.numel() != G:
         raise ValueError("sizes and expert_ids differ in length")
+    sizes = [int(s) for s in sizes]
     host_sizes = (ctypes.c_int64 * max(G, 1))(*sizes)
-    M = sum(host_sizes[:G])
+    M = sum(sizes)
     if a.dim() != 2 or a.shape[0] != M:
         raise ValueError(f"a has {a.shape[0]} rows but sizes sum to {M}")
     if a.shape[1] != qw.k:
         raise ValueError(f"a has {a.shape[1]} columns but the weights have k={qw.k}")
+    values = qw.num_experts * qw.n * qw.k
+    if 2 * qw.packed.numel() != values or qw.k % 32 or 32 * qw.absmax.numel() != values:
+        raise ValueError(f"blocks and scales must be [{qw.num_experts}, {qw.n}, K/2] and [.., K/32] with K a multiple of 32")
     for t in (ids, qw.packed, qw.absmax):
         if t.device != a.device:
             raise ValueError("a, the weights and expert_ids must be on one device")

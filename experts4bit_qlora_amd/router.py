@@ -134,8 +134,8 @@ def balance_loss(logits: torch.Tensor, top_k_index: torch.Tensor,
 
     Over the valid tokens, N of them (``mask [T]`` or ``[..., T]``: nonzero is valid): ``counts[e]`` the choices
     of expert e (ids outside ``[0, E)`` count nowhere), ``P[e]`` the mean of the softmax probabilities, ``loss = E
-    * sum_e counts[e] / N * P[e]``, 0 where N is 0. This is transformers' ``load_balancing_loss_func`` per leading
-    index; for its loss over several layers' tokens together, pass them as one axis. The loss is
+    * sum_e counts[e] / N * P[e]``, 0 where N is 0. For one loss over several
+    layers' tokens together, pass them as one axis. The loss is
     differentiable with respect to the logits (once), the counts are constants to it."""
     if logits.dim() < 2 or not logits.is_floating_point():
         raise ValueError("logits must be a floating-point tensor [..., tokens, num_experts]")

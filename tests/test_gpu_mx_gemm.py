@@ -242,3 +242,29 @@ def test_refusals():
         call(a, b, s, [4, -1], ids, act_quant="mxfp4")
     with pytest.raises(ValueError, match="HIP device"):
         call(a.cpu(), b, s, [1, 2], ids, act_quant="mxfp4")
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("k", (32, 96, 224, 256, 288, 1216, 2880))
+@pytest.mark.parametrize("sizes", ([1], [4, 0, 1, 3]))
+def test_few_rows(sizes, k, dtype):
+    """Groups of at most four rows, whose tiles quantize the rows themselves, and the same rows in a call
+    with a larger group: the same bytes."""
+    E, n = 3, 72
+    b, s = _weights(E, n, k, k)
+    ids = [2, 1, 0, 2][:len(sizes)]
+    a = _rows(sum(sizes) + 5, k, dtype, k + 7)
+    a[0, :32] = 0
+    few = a[:sum(sizes)]
+    out = _run(few, b, s, sizes, ids)
+    _check(few, b, s, sizes, ids, out)
+    assert torch.equal(_run(a, b, s, sizes + [5], ids + [1])[:sum(sizes)], out)
+
+
+def test_refuses_stacks_that_do_not_fit():
+    b, s = _weights(2, 16, 64, 1)
+    a = _rows(3, 64, torch.bfloat16, 2)
+    with pytest.raises(ValueError, match="scales"):
+        _run(a, b, s[..., :1].contiguous(), [3], [0])
+    with pytest.raises(ValueError, match="columns"):
+        _run(a[:, :32].contiguous(), b, s, [3], [0])
