@@ -143,6 +143,27 @@ E4B_DEV void mx_store4(void* out, int64_t at, int left, bool vec, const float (&
   }
 }
 
+// Four pieces of 16 bytes per lane, piece 4 (i / 2) + l / 16 of row 16 (i % 2) + l % 16 in v[i] as loaded (64
+// contiguous bytes of a row by four lanes), to the operands' order: v[j] piece 4 (l / 32) + j of row l % 32. A
+// 4 x 4 transposition of registers and groups of 16 lanes, in two steps of 2 x 2.
+E4B_DEV void mx_to_rows(u32x4_t (&v)[4]) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto s = __builtin_amdgcn_permlane32_swap(v[i][d], v[2 + i][d], false, false);
+      v[i][d] = s[0];
+      v[2 + i][d] = s[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const auto s = __builtin_amdgcn_permlane16_swap(v[i][d], v[i + 1][d], false, false);
+      v[i][d] = s[0];
+      v[i + 1][d] = s[1];
+    }
+  }
+}
+
 // A tile of at most 32 rows times 32 weight rows per workgroup: each of the four waves takes every
 // fourth chunk of K straight into the operand registers, the next one's loads in flight while it computes; their
 // sums join in LDS. Bound by the weights' bytes: each is read once per tile.
@@ -151,7 +172,7 @@ constexpr int kMxTileM = 32;
 constexpr int kMxNarrowWaves = 4;
 
 template <int ODT, int DT>
-__global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemmArgs p, MxGroups go) {
+__global__ void __launch_bounds__(kMxNarrowWaves* kWave, 4) mx_narrow_kernel(MxGemmArgs p, MxGroups go) {
   __shared__ float red[kMxNarrowWaves][32][33];
   extern __shared__ u32x4_t own[];  // DT >= 0: the rows' codes, 8 * chunks pieces each, then their scale bytes
   const int tid = threadIdx.x;
@@ -167,10 +188,15 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
   if (e >= 0) {
     const int blocks = static_cast<int>(p.w.k / kMxBlock);
     const int64_t wrow = int64_t(e) * n + min(static_cast<int>(n0) + r32, static_cast<int>(n) - 1);  // rows past n are not stored
-    const uint8_t* wc = p.w.packed + wrow * (p.w.k / 2);
+    const int r16 = lane & 15, quarter = lane >> 4;
+    const uint8_t *wc[2], *ac[2];  // the rows of which the lane loads pieces
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      wc[i] = p.w.packed + (int64_t(e) * n + min(static_cast<int>(n0) + 16 * i + r16, static_cast<int>(n) - 1)) * (p.w.k / 2);
+      ac[i] = p.a + int64_t(row0 + min(16 * i + r16, end - row0 - 1)) * (chunks * 128);
+    }
     const uint8_t* ws = static_cast<const uint8_t*>(p.w.absmax) + wrow * blocks;
     const int arow = min(r32, end - row0 - 1);  // columns past the tile's rows are not stored
-    const uint8_t* ac = p.a + int64_t(row0 + arow) * (chunks * 128);
     const uint8_t* as = p.as + int64_t(row0 + arow) * (chunks * 8);
     struct Part {
       u32x4_t w[4], a[4];
@@ -181,8 +207,9 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
       const int b0 = 8 * c + 4 * half;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f.w[j] = *reinterpret_cast<const u32x4_t*>(wc + 16 * (b0 + j < blocks ? b0 + j : 0));
-        if constexpr (DT < 0) f.a[j] = *reinterpret_cast<const u32x4_t*>(ac + 16 * (b0 + j));
+        const int b = 8 * c + 4 * (j / 2) + quarter;
+        f.w[j] = *reinterpret_cast<const u32x4_t*>(wc[j % 2] + 16 * (b < blocks ? b : 0));
+        if constexpr (DT < 0) f.a[j] = *reinterpret_cast<const u32x4_t*>(ac[j % 2] + 16 * b);
       }
       f.ws = mx_scales4(ws, b0, blocks);
       if constexpr (DT < 0) f.as = *reinterpret_cast<const uint32_t*>(as + b0);
@@ -194,7 +221,10 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave) mx_narrow_kernel(MxGemm
 #pragma unroll
         for (int j = 0; j < 4; ++j) f.a[j] = own[b0 + j];
         f.as = *reinterpret_cast<const uint32_t*>(own_scales + b0);
+      } else {
+        mx_to_rows(f.a);
       }
+      mx_to_rows(f.w);
       const uint32_t wsc = mx_scale_word(f.ws);
       acc = mx_mfma<0>(f.w[0], f.a[0], wsc, f.as, acc);
       acc = mx_mfma<1>(f.w[1], f.a[1], wsc, f.as, acc);
