@@ -150,22 +150,26 @@ constexpr int kTaken = -0x7fffffff - 1;
 // -inf). A NaN or +inf makes the row NaN, as in torch's softmax.
 template <int GL, int VPL>
 E4B_DEV float row_exp(const float (&z)[VPL], float m, float (&e)[VPL]) {
+  const float base = m == kNoLogit ? 0.0f : m;
   float sum = 0.0f;
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
-    e[j] = m == kNoLogit ? 0.0f : expf(z[j] - m);
+    e[j] = expf(z[j] - base);
     sum += e[j];
   }
   return lanes_sum<GL>(sum);
 }
 
+// The largest logit; NaN are passed over as long as a lane has another (row_exp finds them).
 template <int GL, int VPL>
 E4B_DEV float row_max(const float (&z)[VPL]) {
-  int m = logit_key(z[0]);
+  float m = z[0];
 #pragma unroll
-  for (int j = 1; j < VPL; ++j) m = max(m, logit_key(z[j]));
-  return key_logit(lanes_max<GL>(m));
+  for (int j = 1; j < VPL; ++j) m = fmaxf(m, z[j]);
+  return key_logit(lanes_max<GL>(logit_key(m)));
 }
+// 1 / the sum of a row's exponentials, 0 for a row without probabilities (any other row's sum is 1 at least).
+E4B_DEV float row_inv(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
 // ---- gate
 
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs p,
 #pragma unroll
   for (int j = 0; j < VPL; ++j) g[j] = 0.0f;
   for (int s = 0; s < p.k; ++s) {
-    const int64_t i = p.index[r * p.k + s] - VPL * gl;
+    const int i = static_cast<int>(p.index[r * p.k + s]) - VPL * gl;
     const float gs = load_dt(p.weights, p.wdtype, r * p.k + s);
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs p,
     }
     sum = lanes_sum<GL>(sum);
   }
-  const float inv = m == kNoLogit ? 0.0f : 1.0f / sum;
+  const float inv = row_inv(sum);
   float mean = 0.0f;
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(kGateThreads) balance_kernel(BalanceArgs p, in
     if (valid && gl == 0) atomicAdd(&cnt[p.E], 1);
     const float m = row_max<GL, VPL>(z);
     const float sum = row_exp<GL, VPL>(z, m, e);
-    const float inv = m == kNoLogit ? 0.0f : 1.0f / sum;
+    const float inv = row_inv(sum);
 #pragma unroll
     for (int j = 0; j < VPL; ++j) acc[j] = valid ? acc[j] + e[j] * inv : acc[j];
   }
@@ -382,36 +386,38 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(BalanceArgs 
   }
 }
 
+// dL/dz[t, e] = f P[t, e] (c[e] - sum_i c[i] P[t, i]), f = dL/dloss E / N^2. A workgroup takes every gridDim.x'th
+// group of rows, so that a lane reads its experts' counts once.
 template <int DT, int GL, int VPL>
 __global__ void __launch_bounds__(kGateThreads) balance_backward_kernel(BalanceArgs p, int vec) {
+  constexpr int NG = kGateThreads / GL;
   const int gl = threadIdx.x & (GL - 1);
   const int layer = blockIdx.y;
-  const int64_t t = int64_t(blockIdx.x) * (kGateThreads / GL) + threadIdx.x / GL;
-  const bool live = t < p.T;
-  const int64_t tc = live ? t : p.T - 1, row = layer * p.T + tc;
-  float z[VPL], e[VPL];
-  load_logits<DT, VPL>(p.logits, row, p.E, gl, vec, z);
-  const bool valid = !p.mask || p.mask[layer * p.mask_stride + tc];
-  float c[VPL];
+  float c[VPL];  // (counts of at most T * k choices: 32 bits)
 #pragma unroll
   for (int j = 0; j < VPL; ++j)
-    c[j] = VPL * gl + j < p.E ? static_cast<float>(p.counts[int64_t(layer) * p.E + VPL * gl + j]) : 0.0f;
+    c[j] = VPL * gl + j < p.E ? static_cast<float>(static_cast<int>(p.counts[int64_t(layer) * p.E + VPL * gl + j])) : 0.0f;
+  // the factor in two divisions: N^2 passes fp32's 24 bits long before N does (N = 0: no row is valid)
   const float n = static_cast<float>(p.valid[layer]);
-  const float m = row_max<GL, VPL>(z);
-  const float sum = row_exp<GL, VPL>(z, m, e);
-  const float inv = m == kNoLogit ? 0.0f : 1.0f / sum;
-  float dot = 0.0f;
+  const float f = p.grad_loss[layer] * (static_cast<float>(p.E) / n) / n;
+  for (int64_t t = int64_t(blockIdx.x) * NG + threadIdx.x / GL; t < p.T; t += int64_t(gridDim.x) * NG) {
+    const int64_t row = layer * p.T + t;
+    float z[VPL], e[VPL];
+    load_logits<DT, VPL>(p.logits, row, p.E, gl, vec, z);
+    const bool valid = !p.mask || p.mask[layer * p.mask_stride + t];
+    const float m = row_max<GL, VPL>(z);
+    const float inv = row_inv(row_exp<GL, VPL>(z, m, e));
+    float dot = 0.0f;
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    e[j] *= inv;
-    dot += VPL * gl + j < p.E ? c[j] * e[j] : 0.0f;
+    for (int j = 0; j < VPL; ++j) {
+      e[j] *= inv;
+      dot += VPL * gl + j < p.E ? c[j] * e[j] : 0.0f;
+    }
+    dot = lanes_sum<GL>(dot);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) e[j] = valid ? f * e[j] * (c[j] - dot) : 0.0f;
+    store_row<DT, VPL>(p.grad, row, p.E, gl, vec, e);
   }
-  dot = lanes_sum<GL>(dot);
-  // valid: N >= 1. The factor in two divisions: N^2 passes fp32's 24 bits long before N does
-  const float f = valid ? p.grad_loss[layer] * (static_cast<float>(p.E) / n) / n : 0.0f;
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) e[j] = valid ? f * e[j] * (c[j] - dot) : 0.0f;
-  if (live) store_row<DT, VPL>(p.grad, row, p.E, gl, vec, e);
 }
 
 }  // namespace e4b
