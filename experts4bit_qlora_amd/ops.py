@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
+import functools
 import threading
 from dataclasses import dataclass
 
@@ -343,20 +344,24 @@ def router_topk_backward(logits: torch.Tensor, index: torch.Tensor, grad: torch.
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _balance_ws_bytes(layers: int, tokens: int, experts: int) -> int:
+    return max(1, N.lib().e4b_balance_workspace_bytes(layers, tokens, experts))
+
+
 def balance_loss(logits: torch.Tensor, index: torch.Tensor, mask: torch.Tensor | None):
     """``[L, T, E]`` logits, ``[L, T, k]`` index, bool mask ``[T]`` or ``[L, T]`` -> (loss fp32 ``[L]``, counts int64
     ``[L, E]``, valid tokens int64 ``[L]``) by ``e4b_balance_loss``."""
     _require_cuda(logits, index, mask)
     L_, T, E = logits.shape
     dev = logits.device
-    lib = N.lib()
     loss = torch.empty(L_, dtype=torch.float32, device=dev)
     counts = torch.empty(L_, E, dtype=torch.int64, device=dev)
     valid = torch.empty(L_, dtype=torch.int64, device=dev)
-    ws = torch.empty(max(1, lib.e4b_balance_workspace_bytes(L_, T, E)), dtype=torch.uint8, device=dev)
+    ws = torch.empty(_balance_ws_bytes(L_, T, E), dtype=torch.uint8, device=dev)
     with _on(dev):
         N.check("e4b_balance_loss",
-                lib.e4b_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), L_, T, E, index.data_ptr(),
+                N.lib().e4b_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), L_, T, E, index.data_ptr(),
                                      index.shape[2], _ptr(mask), 0 if mask is None or mask.dim() == 1 else T,
                                      ws.data_ptr(), ws.numel(), loss.data_ptr(), counts.data_ptr(), valid.data_ptr(),
                                      _stream(dev)))

@@ -68,7 +68,8 @@ def router_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax_then_t
     ``"softmax_then_topk"`` the softmax over all logits (``renorm``: divided by their sum),
     ``"topk_then_softmax"`` the softmax over the chosen logits; fp32, rounded once into ``weight_dtype``
     (default: the logits' dtype). A row whose logits are all ``-inf`` gets zero weights. The weights are
-    differentiable with respect to the logits (once)."""
+    differentiable with respect to the logits (once). A backward pass is captured into a graph like any other
+    of torch's: with no eager graph of the same leaves alive."""
     if scoring not in _SCORING:
         raise ValueError(f"scoring must be one of {sorted(_SCORING)}, got {scoring!r}")
     if logits.dim() < 1 or not logits.is_floating_point():

@@ -178,16 +178,16 @@ size_t e4b_balance_workspace_bytes(int32_t layers, int64_t tokens, int32_t num_e
  * nowhere), P_e = mean softmax probability of e, loss = num_experts * sum_e counts[e] / N * P_e (0 when N
  * is 0). logits [layers, tokens, num_experts] in dtype, top_k_index [layers, tokens, top_k] int64;
  * loss fp32 [layers], counts int64 [layers, num_experts], valid int64 [layers] (N, for the backward).
- * A row whose logits are all -inf adds no probability. Deterministic.
- * Has no counterpart in the reference, whose models take transformers' load_balancing_loss_func; the
- * definition is that one's, per layer. */
+ * A row whose logits are all -inf adds no probability. Deterministic. layers <= 65535, tokens * top_k below
+ * 2^31, num_experts <= 1024. Has no counterpart in the reference. */
 int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                      const int64_t* top_k_index, int32_t top_k, const uint8_t* mask, int64_t mask_stride,
                      void* workspace, size_t workspace_bytes, float* loss, int64_t* counts, int64_t* valid,
                      hipStream_t stream);
 
 /* Its backward (the counts are constants): grad_logits[t, j] = grad_loss * num_experts / N^2 * p_tj *
- * (counts[j] - sum_e counts[e] p_te) at valid tokens, 0 elsewhere; grad_loss fp32 [layers]. */
+ * (counts[j] - sum_e counts[e] p_te) at valid tokens, 0 elsewhere; grad_loss fp32 [layers], counts and valid as
+ * the forward wrote them. */
 int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                               const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
                               const float* grad_loss, void* grad_logits, hipStream_t stream);
@@ -238,7 +238,10 @@ size_t e4b_mx_gemm_workspace_bytes(int64_t rows, int64_t k);
  * products exact, sums fp32, one rounding into out_dtype (E4B_BF16 / E4B_FP16 / E4B_FP32). A block of a row
  * with an infinity or a NaN makes that row NaN, a weight scale byte of 255 its column's sums; rows of an id
  * outside [0, E) are zero. sizes is a host array, read before the call returns; groups <= 512. w is MXFP4, k a
- * multiple of 32, w->bias is not read; a, out and workspace are 16-byte aligned.
+ * multiple of 32, w->bias is not read; a, out and workspace are 16-byte aligned. n < 2^22, k < 2^24, at most 2^23
+ * rows (2^20 where k <= 256), fewer than 2^31 chunks of 256 values. Nothing past the last row is written. A
+ * captured graph keeps the sizes; the ids may change between replays. The workspace holds the rows' codes until the
+ * product has run: calls that may overlap (other streams, graphs replayed side by side) need one each.
  * The product of mxfp4_grouped.gemm_mxfp4_grouped (engines/nvme_experts.py:852-865) on the block-scaled
  * matrix cores, with activations in the weights' format; the reference's activations stay 16-bit. */
 int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, int32_t groups,

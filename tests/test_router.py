@@ -88,15 +88,17 @@ def test_balance_values_gradients_and_layers():
         assert abs((ends[0] - ends[1]) / 2e-5 - grad[1, 0, t, e].item()) < 1e-6
 
 
-def test_balance_equals_transformers():
-    """One layer of tokens against the models' own function."""
-    from transformers.models.olmoe.modeling_olmoe import load_balancing_loss_func
-
-    z = torch.randn(40, 8, generator=torch.Generator().manual_seed(4))
+def test_balance_of_layers_as_one_axis():
+    """Several layers' tokens passed as one axis: the loss of all of them together."""
+    z = torch.randn(3, 40, 8, generator=torch.Generator().manual_seed(4))
     index, _ = e4b.router_topk(z, 2)
-    loss, _ = e4b.balance_loss(z, index)
-    want = load_balancing_loss_func((z,), num_experts=8, top_k=2)
+    loss, counts = e4b.balance_loss(z.reshape(120, 8), index.reshape(120, 2))
+    p, each = torch.softmax(z.double(), -1), torch.zeros(8, dtype=torch.float64)
+    for e in index.flatten():
+        each[e] += 1
+    want = 8 * ((each / 120) * p.mean((0, 1))).sum()
     assert loss.shape == () and abs(loss.item() - want.item()) <= 1e-5 * want.item()
+    assert torch.equal(counts, each.long())
 
 
 def test_no_tokens():
