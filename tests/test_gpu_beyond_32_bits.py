@@ -1,0 +1,70 @@
+"""The microscaled operators and the router on tensors whose offsets pass 32 bits: the last rows of a large call
+equal the same rows in a call of their own."""
+import pytest
+import torch
+
+import experts4bit_qlora_amd as e4b
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _bytes(*shape, lo=0, hi=256):
+    return torch.randint(lo, hi, shape, dtype=torch.uint8, device=DEV)
+
+
+@pytest.mark.parametrize("rows,n,k", [(300_001, 8200, 64), (280_001, 8200, 288)])
+def test_product_outputs(rows, n, k):
+    """More than 2^31 outputs, by 32-row tiles (K of one chunk) and by 256-row tiles."""
+    assert rows * n > 2 ** 31
+    b, s = _bytes(2, n, k // 2), _bytes(2, n, k // 32, lo=120, hi=130)
+    a = torch.randn(rows, k, device=DEV, dtype=torch.bfloat16)
+    ids = torch.tensor([1, 0], device=DEV)
+    out = e4b.gemm_mxfp4_grouped(a, b, s, [100, rows - 100], ids, act_quant="mxfp4")
+    part = e4b.gemm_mxfp4_grouped(a[-300:].contiguous(), b, s, [300], ids[1:], act_quant="mxfp4")
+    assert torch.equal(out[-300:], part)
+
+
+@pytest.mark.parametrize("size", (2, 9, 40))
+def test_product_weights(size):
+    """A stack of more than 2^32 bytes: the last expert."""
+    E, n, k = 33, 16384, 16384
+    assert E * n * k // 2 > 2 ** 32
+    b, s = _bytes(E, n, k // 2), _bytes(E, n, k // 32, lo=120, hi=130)
+    a = torch.randn(size, k, device=DEV, dtype=torch.bfloat16)
+    out = e4b.gemm_mxfp4_grouped(a, b, s, [size], torch.tensor([E - 1], device=DEV), act_quant="mxfp4")
+    alone = e4b.gemm_mxfp4_grouped(a, b[-1:].clone(), s[-1:].clone(), [size], torch.tensor([0], device=DEV),
+                                   act_quant="mxfp4")
+    assert torch.equal(out, alone)
+
+
+def test_quantize():
+    x = torch.randn(70_000, 65_536, device=DEV, dtype=torch.bfloat16)
+    assert x.numel() > 2 ** 32
+    blocks, scales = e4b.quantize_mxfp4(x)
+    last = e4b.quantize_mxfp4(x[-3:].clone())
+    assert torch.equal(blocks[-3:], last[0]) and torch.equal(scales[-3:], last[1])
+
+
+def test_router():
+    T, E, k = 2_200_003, 1000, 2
+    assert T * E > 2 ** 31
+    z = torch.randn(T, E, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    index, weights = e4b.router_topk(z, k)
+    (grad,) = torch.autograd.grad(weights, z, torch.ones_like(weights))
+    tail = z.detach()[-5:].clone().requires_grad_()
+    i, w = e4b.router_topk(tail, k)
+    assert torch.equal(index[-5:], i) and torch.equal(weights[-5:], w)
+    assert torch.equal(grad[-5:], torch.autograd.grad(w, tail, torch.ones_like(w))[0])
+    del grad
+    # only the last rows are valid: what the loss reads and writes lies past 2^31
+    mask = torch.zeros(T, dtype=torch.bool, device=DEV)
+    mask[-5:] = True
+    loss, counts = e4b.balance_loss(z[None], index[None], mask)
+    (grad,) = torch.autograd.grad(loss.sum(), z)
+    own, each = e4b.balance_loss(tail[None], i[None])
+    (want,) = torch.autograd.grad(own.sum(), tail)
+    assert torch.equal(counts, each)
+    # five probabilities per expert, summed in another order: 2^-20 is sixteen fp32 roundings
+    assert torch.allclose(loss, own, rtol=2.0 ** -20, atol=0)
+    assert torch.equal(grad[-5:], want) and not grad[:-5].any()

@@ -3,10 +3,14 @@
 Tolerance of one output, from the arithmetic: the rounding into the output type, half a step of the
 value (``eps / 2``), and the fp32 sums: K products (exact) added in any order, one error of at most 2^-23 of the
 running sum's bound per addition (a truncating adder), so K 2^-23 times the sum of the magnitudes."""
+import ctypes
+
 import pytest
 import torch
 
 import experts4bit_qlora_amd as e4b
+from experts4bit_qlora_amd import _native as N
+from experts4bit_qlora_amd import ops
 from experts4bit_qlora_amd import quant as Q
 
 pytestmark = pytest.mark.gpu
@@ -268,3 +272,58 @@ def test_refuses_stacks_that_do_not_fit():
         _run(a, b, s[..., :1].contiguous(), [3], [0])
     with pytest.raises(ValueError, match="columns"):
         _run(a[:, :32].contiguous(), b, s, [3], [0])
+
+
+def _entry(a, blocks, scales, sizes, ids, out, workspace):
+    """e4b_mx_grouped_gemm itself, on the caller's buffers."""
+    E, n, kh = blocks.shape
+    qw = ops.mxfp4_qweight(blocks, scales, n, 2 * kh)
+    return N.lib().e4b_mx_grouped_gemm(a.data_ptr(), ops.dtype_code(a.dtype), (ctypes.c_int64 * len(sizes))(*sizes),
+                                       len(sizes), ids.data_ptr(), qw.ref(), workspace.data_ptr(), workspace.numel(),
+                                       out.data_ptr(), ops.dtype_code(out.dtype),
+                                       torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("out_dtype", (torch.float32, torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("n", (72, 267))
+@pytest.mark.parametrize("sizes", ([1, 3], [2, 7], [40, 260]))
+def test_entry_point_output_types_and_what_it_leaves(sizes, n, out_dtype):
+    """The entry point's other output types; bytes behind the last row and behind the workspace it asked for stay."""
+    E, k, ids, M = 3, 352, [2, 0], sum(sizes)
+    b, s = _weights(E, n, k, 40)
+    a = _rows(M, k, torch.bfloat16, 41)
+    need = N.lib().e4b_mx_gemm_workspace_bytes(M, k)
+    ws = torch.full((need + 256,), 0xA5, dtype=torch.uint8, device=DEV)
+    out = torch.full((M + 2, n), 77.0, dtype=out_dtype, device=DEV)
+    assert _entry(a.to(DEV), b.to(DEV), s.to(DEV), sizes, torch.tensor(ids, device=DEV), out, ws[:need]) == 0
+    torch.cuda.synchronize()
+    assert (out[M:] == 77).all() and (ws[need:] == 0xA5).all()
+    ab, asc = Q._quantize_mxfp4_torch(a)
+    av, wv, r = _values(ab, asc), _values(b, s), 0
+    for size, e in zip(sizes, ids):
+        want = av[r:r + size] @ wv[e].T
+        bound = torch.finfo(out_dtype).eps / 2 * want.abs() + k * 2.0 ** -23 * (av[r:r + size].abs() @ wv[e].abs().T)
+        bound += torch.finfo(out_dtype).smallest_normal * torch.finfo(out_dtype).eps / 2 + 2.0 ** -126
+        top = torch.finfo(out_dtype).max  # a value past fp16's range is infinite
+        got = out[r:r + size].double().cpu()
+        fine = want.abs() < top
+        assert ((got - want).abs()[fine] <= bound[fine]).all() and got[~fine].abs().ge(top / 2).all()
+        r += size
+
+
+@pytest.mark.parametrize("sizes", ([1, 2], [9, 5], [300, 20]))
+def test_two_calls_at_once(sizes):
+    """Calls on two streams, each with rows of its own, over the same weights."""
+    E, n, k, ids = 4, 320, 704, torch.tensor([3, 1], device=DEV)
+    b, s = (t.to(DEV) for t in _weights(E, n, k, 50))
+    a = [_rows(sum(sizes), k, torch.bfloat16, 51 + i).to(DEV) for i in range(2)]
+    want = [e4b.gemm_mxfp4_grouped(x, b, s, sizes, ids, act_quant="mxfp4") for x in a]
+    streams = [torch.cuda.Stream() for _ in a]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for x, stream in zip(a, streams):
+            with torch.cuda.stream(stream):
+                got.append(e4b.gemm_mxfp4_grouped(x, b, s, sizes, ids, act_quant="mxfp4"))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
