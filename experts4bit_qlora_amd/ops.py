@@ -86,19 +86,9 @@ class QW:
         cached = self.__dict__.get("_struct")
         if cached is not None:
             return cached
-        s = N.QWeight()
-        s.format = self.fmt
-        s.num_experts = self.num_experts
-        s.n = self.n
-        s.k = self.k
-        s.packed = _ptr(self.packed)
-        s.absmax = _ptr(self.absmax)
-        s.absmax2 = _ptr(self.absmax2)
-        s.offset = _ptr(self.offset)
-        s.code = _ptr(self.code)
-        s.code2 = _ptr(self.code2)
-        s.bias = _ptr(self.bias)
-        s.shift = _ptr(self.shift)
+        s = N.QWeight(self.fmt, self.num_experts, self.n, self.k, _ptr(self.packed), _ptr(self.absmax),
+                      _ptr(self.absmax2), _ptr(self.offset), _ptr(self.code), _ptr(self.code2), _ptr(self.bias),
+                      _ptr(self.shift))
         self.__dict__["_struct"] = s
         self.__dict__["_ref"] = ctypes.byref(s)
         return s
@@ -824,53 +814,58 @@ def gemm_mxfp4_grouped(a: torch.Tensor, blocks: torch.Tensor, scales: torch.Tens
     ``act_quant="mxfp4"`` (beyond the reference) quantizes the rows of ``a`` to MXFP4 as
     ``quantize_mxfp4`` does and multiplies the two microscaled operands on the block-scaled matrix
     cores (``e4b_mx_grouped_gemm``): ``[M, N]`` in ``a``'s dtype, up to 512 groups, K a multiple of 32."""
-    E, n, kh = blocks.shape
-    qw = mxfp4_qweight(blocks, scales, n, kh * 2, num_experts=E)
     if act_quant is None:
-        return _grouped_call(a, qw, sizes, expert_ids)
+        E, n, kh = blocks.shape
+        return _grouped_call(a, mxfp4_qweight(blocks, scales, n, kh * 2, num_experts=E), sizes, expert_ids)
     if act_quant != "mxfp4":
         raise ValueError(f"act_quant must be None or 'mxfp4', got {act_quant!r}")
-    return mx_grouped_gemm(a, qw, sizes, expert_ids)
+    return mx_grouped_gemm(a, blocks, scales, sizes, expert_ids)
 
 
-def mx_grouped_gemm(a: torch.Tensor, qw: QW, sizes, expert_ids) -> torch.Tensor:
-    """``gemm_mxfp4_grouped(..., act_quant="mxfp4")`` on a weight descriptor: ``[M, n]`` in ``a``'s dtype."""
-    _require_cuda(a, qw.packed)
-    G = len(sizes)
+@functools.lru_cache(maxsize=1024)
+def _mx_ws_bytes(rows: int, k: int) -> int:
+    return max(1, N.lib().e4b_mx_gemm_workspace_bytes(rows, k))
+
+
+def mx_grouped_gemm(a: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, sizes, expert_ids) -> torch.Tensor:
+    """``gemm_mxfp4_grouped(..., act_quant="mxfp4")``. The descriptor is filled here and not kept: a call of a few
+    rows is bound by the host."""
+    _require_cuda(a, blocks, scales)
+    E, n, kh = blocks.shape
+    k, G, dev = 2 * kh, len(sizes), a.device
+    if k % 32 or 32 * scales.numel() != E * n * k:
+        raise ValueError(f"blocks and scales must be [{E}, {n}, K/2] and [{E}, {n}, K/32] with K a multiple of 32")
     if torch.is_tensor(expert_ids) and expert_ids.is_cuda:
         ids = expert_ids if expert_ids.dtype == torch.int64 else expert_ids.to(torch.int64)
         ids = ids.contiguous()
     else:
         host = [int(e) for e in (expert_ids.tolist() if torch.is_tensor(expert_ids) else expert_ids)]
-        if any(not 0 <= e < qw.num_experts for e in host):
+        if any(not 0 <= e < E for e in host):
             raise ValueError("bad expert ids")
-        ids = torch.tensor(host, dtype=torch.int64, device=a.device)
+        ids = torch.tensor(host, dtype=torch.int64, device=dev)
     if ids.numel() != G:
         raise ValueError("sizes and expert_ids differ in length")
     sizes = [int(s) for s in sizes]
-    host_sizes = (ctypes.c_int64 * max(G, 1))(*sizes)
     M = sum(sizes)
     if a.dim() != 2 or a.shape[0] != M:
         raise ValueError(f"a has {a.shape[0]} rows but sizes sum to {M}")
-    if a.shape[1] != qw.k:
-        raise ValueError(f"a has {a.shape[1]} columns but the weights have k={qw.k}")
-    values = qw.num_experts * qw.n * qw.k
-    if 2 * qw.packed.numel() != values or qw.k % 32 or 32 * qw.absmax.numel() != values:
-        raise ValueError(f"blocks and scales must be [{qw.num_experts}, {qw.n}, K/2] and [.., K/32] with K a multiple of 32")
-    for t in (ids, qw.packed, qw.absmax):
-        if t.device != a.device:
-            raise ValueError("a, the weights and expert_ids must be on one device")
-    L = N.lib()
-    x = a.detach().contiguous()
+    if a.shape[1] != k:
+        raise ValueError(f"a has {a.shape[1]} columns but the weights have k={k}")
+    if not ids.device == blocks.device == scales.device == dev:
+        raise ValueError("a, the weights and expert_ids must be on one device")
+    x = a.detach() if a.requires_grad else a
+    x, blocks, scales = x.contiguous(), blocks.contiguous(), scales.contiguous()
     if x.data_ptr() % 16:  # a view that starts inside another tensor
         x = x.clone()
     dt = dtype_code(x.dtype)
-    out = torch.empty(M, qw.n, dtype=x.dtype, device=x.device)
-    ws = torch.empty(max(1, L.e4b_mx_gemm_workspace_bytes(M, qw.k)), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
+    out = x.new_empty((M, n))
+    ws_bytes = _mx_ws_bytes(M, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    w = N.QWeight(N.FMT_MXFP4, E, n, k, blocks.data_ptr(), scales.data_ptr())
+    with _on(dev):
         N.check("e4b_mx_grouped_gemm",
-                L.e4b_mx_grouped_gemm(x.data_ptr(), dt, host_sizes, G, ids.data_ptr(), qw.ref(), ws.data_ptr(), ws.numel(),
-                                      out.data_ptr(), dt, _stream(x.device)))
+                N.lib().e4b_mx_grouped_gemm(x.data_ptr(), dt, (ctypes.c_int64 * G)(*sizes), G, ids.data_ptr(),
+                                            ctypes.byref(w), ws.data_ptr(), ws_bytes, out.data_ptr(), dt, _stream(dev)))
     return out
 
 
