@@ -172,9 +172,9 @@ E4B_DEV void mx_to_rows(u32x4_t (&v)[4]) {
 // 148 rows over 32 experts of 2,880 x 2,880 (141 MB of weights and scales): 30.4 us, 4.6 TB/s; with each lane
 // loading its own row's 64 bytes 31.0, at three waves per SIMD instead of four 32.0, without the next chunk's
 // loads in flight 33.6.
-// DT >= 0: the workgroup quantizes its rows itself into LDS, from values of type DT: one launch instead of two
-// (four experts of 5,760 x 2,880: one row each 9.3 us, against 2.1 + 8.7 and the gap between two launches; four
-// rows each 11.4 against 2.3 + 9.0; eight rows each 14.7 against 2.2 + 9.4).
+// DT >= 0: the workgroup quantizes its rows itself into LDS, from values of type DT, and takes p.run column blocks one
+// after the other with them, each block's first loads in flight while the one before is joined (the 148 rows: 30.4
+// us for everything, against 4.4 + 30.4 in two kernels).
 constexpr int kMxTileM = 32;
 constexpr int kMxNarrowWaves = 4;
 
@@ -188,93 +188,121 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave, 4) mx_narrow_kernel(MxG
   const int half = lane >> 5, r32 = lane & 31;
   MxTile t;
   if (!mx_tile(p, go, t)) return;
-  const int e = t.e, row0 = t.row0, end = t.end;
-  const int64_t n = p.w.n, n0 = int64_t(t.nb) * 32;
-  const int chunks = static_cast<int>((p.w.k + kMxChunk - 1) / kMxChunk);
-  mx_acc_t acc = {};
-  if (e >= 0) {
-    const int blocks = static_cast<int>(p.w.k / kMxBlock);
-    const int64_t wrow = int64_t(e) * n + min(static_cast<int>(n0) + r32, static_cast<int>(n) - 1);  // rows past n are not stored
-    const int r16 = lane & 15, quarter = lane >> 4;
-    const uint8_t *wc[2], *ac[2];  // the rows of which the lane loads pieces
+  const int e = t.e, row0 = t.row0, end = t.end, rows = end - row0;
+  const int n = static_cast<int>(p.w.n);
+  const int blocks = static_cast<int>(p.w.k / kMxBlock);
+  const int chunks = (blocks + 7) / 8;
+  const int run = DT < 0 ? 1 : p.run;  // the workgroup's column blocks
+  const int first = t.nb * run, last = min(first + run, (n + 31) / 32);
+  const int r16 = lane & 15, quarter = lane >> 4;
+  const int arow = min(r32, rows - 1);  // columns past the tile's rows are not stored
+  const uint8_t *wc[2], *ac[2];         // the rows of which the lane loads pieces
+  const uint8_t *ws, *as = p.as + int64_t(row0 + arow) * (chunks * 8);
+  auto aim = [&](int nb) {  // at a column block's weights; rows past n are not stored
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      wc[i] = p.w.packed + (int64_t(e) * n + min(static_cast<int>(n0) + 16 * i + r16, static_cast<int>(n) - 1)) * (p.w.k / 2);
-      ac[i] = p.a + int64_t(row0 + min(16 * i + r16, end - row0 - 1)) * (chunks * 128);
+    for (int i = 0; i < 2; ++i)
+      wc[i] = p.w.packed + (int64_t(e) * n + min(32 * nb + 16 * i + r16, n - 1)) * (16 * blocks);
+    ws = static_cast<const uint8_t*>(p.w.absmax) + (int64_t(e) * n + min(32 * nb + r32, n - 1)) * blocks;
+  };
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ac[i] = p.a + int64_t(row0 + min(16 * i + r16, rows - 1)) * (chunks * 128);
+  struct Part {
+    u32x4_t w[4], a[4];
+    MxScales ws;
+    uint32_t as;
+  } even, odd;
+  auto load = [&](Part& f, int c) {
+    const int b0 = 8 * c + 4 * half;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = 8 * c + 4 * (j / 2) + quarter;
+      f.w[j] = *reinterpret_cast<const u32x4_t*>(wc[j % 2] + 16 * (b < blocks ? b : 0));
+      if constexpr (DT < 0) f.a[j] = *reinterpret_cast<const u32x4_t*>(ac[j % 2] + 16 * b);
     }
-    const uint8_t* ws = static_cast<const uint8_t*>(p.w.absmax) + wrow * blocks;
-    const int arow = min(r32, end - row0 - 1);  // columns past the tile's rows are not stored
-    const uint8_t* as = p.as + int64_t(row0 + arow) * (chunks * 8);
-    struct Part {
-      u32x4_t w[4], a[4];
-      MxScales ws;
-      uint32_t as;
-    } even, odd;
-    auto load = [&](Part& f, int c) {
-      const int b0 = 8 * c + 4 * half;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int b = 8 * c + 4 * (j / 2) + quarter;
-        f.w[j] = *reinterpret_cast<const u32x4_t*>(wc[j % 2] + 16 * (b < blocks ? b : 0));
-        if constexpr (DT < 0) f.a[j] = *reinterpret_cast<const u32x4_t*>(ac[j % 2] + 16 * b);
-      }
-      f.ws = mx_scales4(ws, b0, blocks);
-      if constexpr (DT < 0) f.as = *reinterpret_cast<const uint32_t*>(as + b0);
-    };
-    uint8_t* const own_scales = reinterpret_cast<uint8_t*>(own + (end - row0) * 8 * chunks);
-    auto add = [&](Part& f, int c) {
-      if constexpr (DT >= 0) {
-        const int b0 = 8 * (arow * chunks + c) + 4 * half;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f.a[j] = own[b0 + j];
-        f.as = *reinterpret_cast<const uint32_t*>(own_scales + b0);
-      } else {
-        mx_to_rows(f.a);
-      }
-      mx_to_rows(f.w);
-      const uint32_t wsc = mx_scale_word(f.ws);
-      acc = mx_mfma<0>(f.w[0], f.a[0], wsc, f.as, acc);
-      acc = mx_mfma<1>(f.w[1], f.a[1], wsc, f.as, acc);
-      acc = mx_mfma<2>(f.w[2], f.a[2], wsc, f.as, acc);
-      acc = mx_mfma<3>(f.w[3], f.a[3], wsc, f.as, acc);
-    };
-    if (wid < chunks) load(even, wid);
+    f.ws = mx_scales4(ws, b0, blocks);
+    if constexpr (DT < 0) f.as = *reinterpret_cast<const uint32_t*>(as + b0);
+  };
+  uint8_t* const own_scales = reinterpret_cast<uint8_t*>(own + rows * 8 * chunks);
+  mx_acc_t acc;
+  auto add = [&](Part& f, int c) {
     if constexpr (DT >= 0) {
-      const int pieces = 32 * chunks, in = static_cast<int>(p.w.k / 8);  // of eight values, padded and given
-      for (int r = 0; r < end - row0; ++r) {
-        for (int q = tid; q < pieces; q += kMxNarrowWaves * kWave) {  // whole quads: a block's four pieces
-          const MxPiece<DT> v = mx_load<DT>(p.x, int64_t(row0 + r) * in + (q < in ? q : 0));
-          const uint32_t s = mx_scale_byte<DT>(quad_max(mx_amax<DT>(v)), true);
-          reinterpret_cast<uint32_t*>(own)[r * pieces + q] = q < in ? mx_codes<DT>(v, s) : 0u;
-          if ((q & 3) == 0) own_scales[(r * pieces + q) >> 2] = q < in ? static_cast<uint8_t>(s) : 0;
+      const int b0 = 8 * (arow * chunks + c) + 4 * half;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f.a[j] = own[b0 + j];
+      f.as = *reinterpret_cast<const uint32_t*>(own_scales + b0);
+    } else {
+      mx_to_rows(f.a);
+    }
+    mx_to_rows(f.w);
+    const uint32_t wsc = mx_scale_word(f.ws);
+    acc = mx_mfma<0>(f.w[0], f.a[0], wsc, f.as, acc);
+    acc = mx_mfma<1>(f.w[1], f.a[1], wsc, f.as, acc);
+    acc = mx_mfma<2>(f.w[2], f.a[2], wsc, f.as, acc);
+    acc = mx_mfma<3>(f.w[3], f.a[3], wsc, f.as, acc);
+  };
+  const bool busy = e >= 0 && wid < chunks;
+  if (busy) {
+    aim(first);
+    load(even, wid);
+  }
+  if constexpr (DT >= 0) {
+    constexpr int kThreads = kMxNarrowWaves * kWave, kAhead = 4;
+    const int pieces = 32 * chunks, in = 4 * blocks;  // of a row, eight values each: padded and given
+    for (int q0 = tid; q0 < rows * pieces; q0 += kAhead * kThreads) {  // whole quads: a block's four pieces
+      MxPiece<DT> v[kAhead];
+      bool some[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int q = min(q0 + u * kThreads, rows * pieces - 1), r = q / pieces;
+        some[u] = q - r * pieces < in;
+        v[u] = mx_load<DT>(p.x, int64_t(row0 + r) * in + (some[u] ? q - r * pieces : 0));
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int q = q0 + u * kThreads;
+        const uint32_t s = mx_scale_byte<DT>(quad_max(mx_amax<DT>(v[u])), true);
+        const uint32_t code = mx_codes<DT>(v[u], s);
+        if (q < rows * pieces) {
+          reinterpret_cast<uint32_t*>(own)[q] = some[u] ? code : 0u;
+          if ((q & 3) == 0) own_scales[q >> 2] = some[u] ? static_cast<uint8_t>(s) : 0;
         }
       }
-      __syncthreads();
     }
-    for (int c = wid; c < chunks; c += 2 * kMxNarrowWaves) {
-      const int d = c + kMxNarrowWaves;
-      if (d < chunks) load(odd, d);
-      add(even, c);
-      if (d >= chunks) break;
-      if (d + kMxNarrowWaves < chunks) load(even, d + kMxNarrowWaves);
-      add(odd, d);
+    __syncthreads();
+  }
+  for (int nb = first; nb < (DT < 0 ? first + 1 : last); ++nb) {
+    acc = mx_acc_t{};
+    if (busy) {
+      for (int c = wid; c < chunks; c += 2 * kMxNarrowWaves) {
+        const int d = c + kMxNarrowWaves;
+        if (d < chunks) load(odd, d);
+        add(even, c);
+        if (d >= chunks) break;
+        if (d + kMxNarrowWaves < chunks) load(even, d + kMxNarrowWaves);
+        add(odd, d);
+      }
+      if (DT >= 0 && nb + 1 < last) {  // the next block's first chunk, in flight while this one is joined
+        aim(nb + 1);
+        load(even, wid);
+      }
+    }
+    if (DT >= 0 && nb > first) __syncthreads();  // the previous block's sums have been read
+#pragma unroll
+    for (int i = 0; i < 16; ++i) red[wid][8 * (i / 4) + 4 * half + i % 4][r32] = acc[i];
+    __syncthreads();
+    const int row = tid >> 3, c0 = 4 * (tid & 7), left = n - 32 * nb - c0;
+    if (row < rows && left > 0) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kMxNarrowWaves; ++w) s += red[w][c0 + j][row];
+        v[j] = s;
+      }
+      mx_store4<ODT>(p.out, int64_t(row0 + row) * n + 32 * nb + c0, left, n % 4 == 0, v);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) red[wid][8 * (i / 4) + 4 * half + i % 4][r32] = acc[i];
-  __syncthreads();
-  const int row = row0 + (tid >> 3), c0 = 4 * (tid & 7);
-  if (row >= end) return;
-  float v[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kMxNarrowWaves; ++w) s += red[w][c0 + j][tid >> 3];
-    v[j] = s;
-  }
-  const int left = static_cast<int>(n - n0) - c0;
-  if (left > 0) mx_store4<ODT>(p.out, int64_t(row) * n + n0 + c0, left, n % 4 == 0, v);
 }
 
 // ---- large groups

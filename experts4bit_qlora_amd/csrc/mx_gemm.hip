@@ -40,15 +40,22 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
   hipLaunchKernelGGL(kernel, dim3(std::min((total + 7) / 8 * 8, most)), dim3(threads), lds, s, a, g);
 }
 
+
 // Groups of more than 32 rows take 256-row tiles; smaller ones 32-row tiles, unless there are only a few beside
 // larger groups: a tile of either kind costs about its weights' bytes (5,760 x 2,880: 3.1 us of the card in
 // the 256-row launch, 2 in the other), a launch 5 us. K of at most one chunk has no 256-row kernel.
-// Where no group has more than kDirect rows, and their codes fit 16 KB (four workgroups per CU with the 17 KB of
-// partial sums), the 32-row tiles quantize their rows themselves: four experts of 5,760 x 2,880 take 11.4 us so at
-// four rows each, 11.3 and a launch more in two kernels; at eight 14.7 and 11.6.
+//
+// Small groups all round quantize their rows inside the 32-row tiles, without a launch for that: up to eight rows
+// each, up to sixteen where there are tiles enough for runs of column blocks (more than twice 1,024), which share
+// the quantized rows (one row or four are cheaper quantized again for every block than runs are). Per call in us,
+// against the rows' kernel and the product's (and a gap between them):
+//   experts x rows of 5,760 x 2,880: 4 x 1 8.6 (4.4 + 9.7); 4 x 8 12.1 (4.4 + 9.4); 4 x 16 16.9 (4.4 + 10.4);
+//   32 x 1 56.8 (4.4 + 61.7); 32 x 4 63.5 (4.3 + 66.9), in runs 66.3; 32 x 12 72.3 (4.4 + 76.7), without runs 84.0;
+//   32 x 16 75.6 (4.5 + 80.7); 32 x 24 87.8 (4.5 + 88.5); of 2,880 x 2,880: 32 x 16 38.9 (4.5 + 37.5)
 template <int ODT>
 void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
-  constexpr int kAll = 0x7fffffff, kFew = 5, kDirect = 4;
+  constexpr int kAll = 0x7fffffff, kFew = 5, kNarrowThreads = kMxNarrowWaves * kWave;
+  constexpr int kDirect = 8, kDirectInRuns = 16, kDirectLds = 32768, kOnce = 4, kRunItems = 1024, kRunMost = 4;
   int small = 0, large = 0, most = 0;
   for (int i = 0; i < a.groups; ++i) {
     const int size = g.off[i + 1] - g.off[i];
@@ -56,14 +63,14 @@ void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
     large += size > kMxTileM;
     most = std::max(most, size);
   }
-  const int threads = kMxNarrowWaves * kWave;
-  const MxTiling tiles32 = {kMxTileM, 0, kAll, 0};
   const bool bf16 = a.act_dtype == E4B_BF16;
   const int64_t lds = most * mx_chunks(a.w.k) * (kMxChunk / 2 + kMxChunk / kMxBlock);
-  if (most <= kDirect && lds <= 16384) {
-    const unsigned all = 0x7fffffff;
-    if (bf16) launch_tiles(mx_narrow_kernel<ODT, E4B_BF16>, threads, a, g, tiles32, 32, s, all, static_cast<int>(lds));
-    else launch_tiles(mx_narrow_kernel<ODT, E4B_FP16>, threads, a, g, tiles32, 32, s, all, static_cast<int>(lds));
+  const int64_t run = std::clamp<int64_t>(small * ((a.w.n + 31) / 32) / kRunItems, 1, kRunMost);
+  if (most <= (run > 1 ? kDirectInRuns : kDirect) && lds <= kDirectLds) {
+    MxGemmArgs d = a;
+    d.run = most > kOnce ? static_cast<int>(run) : 1;
+    const auto kernel = bf16 ? mx_narrow_kernel<ODT, E4B_BF16> : mx_narrow_kernel<ODT, E4B_FP16>;
+    launch_tiles(kernel, kNarrowThreads, d, g, {kMxTileM, 0, kAll, 0}, 32 * d.run, s, 0x7fffffff, static_cast<int>(lds));
     return;
   }
   if (bf16) launch_rows<E4B_BF16>(a, s);
@@ -71,7 +78,7 @@ void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
   const bool wide = large && a.w.k > kMxChunk;
   const int narrow_to = !wide ? kAll : small > kFew ? kMxTileM : 0;
   if (wide) launch_tiles(mx_wide_kernel<ODT>, kMxWideThreads, a, g, {kMxWideM, narrow_to, kAll, 0}, kMxWideN, s, 256);
-  if (narrow_to) launch_tiles(mx_narrow_kernel<ODT, -1>, threads, a, g, {kMxTileM, 0, narrow_to, 0}, 32, s);
+  if (narrow_to) launch_tiles(mx_narrow_kernel<ODT, -1>, kNarrowThreads, a, g, {kMxTileM, 0, narrow_to, 0}, 32, s);
 }
 
 }  // namespace

@@ -42,7 +42,8 @@ struct MxGemmArgs {
   void* out;  // [M, n] in the kernel's output type
   MxTiling tl;
   int tiles;     // row tiles of the launch
-  int n_blocks;  // column blocks of the launch
+  int n_blocks;  // columns of the launch's tiles
+  int run;       // 32-row tiles: column blocks of 32 that a workgroup takes one after the other
 };
 
 // The whole product of the group form, the rows' quantization included (g.tile is filled for each launch).

@@ -327,3 +327,20 @@ def test_two_calls_at_once(sizes):
                 got.append(e4b.gemm_mxfp4_grouped(x, b, s, sizes, ids, act_quant="mxfp4"))
         torch.cuda.synchronize()
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("n", (1408, 2064))
+@pytest.mark.parametrize("most", (4, 8, 16))
+def test_many_small_groups(most, n):
+    """Groups of up to four, eight and sixteen rows, enough of them (2,064 weight rows: 65 column blocks of 48
+    groups) for a workgroup to take several column blocks: the bytes of a call that has a larger group beside them."""
+    E, k, G = 4, 320, 48
+    b, s = (t.to(DEV) for t in _weights(E, n, k, 60))
+    sizes = [most, 0] + [1 + i % most for i in range(G - 2)]
+    ids = [i % E for i in range(G)]
+    ids[5] = E  # zero rows
+    a = _rows(sum(sizes) + 17, k, torch.bfloat16, 61)
+    few = a[:sum(sizes)]
+    out = _run(few, b, s, sizes, ids)
+    _check(few, b.cpu(), s.cpu(), sizes, ids, out)
+    assert torch.equal(_run(a, b, s, sizes + [17], ids + [1])[:sum(sizes)], out)
