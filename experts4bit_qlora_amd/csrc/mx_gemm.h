@@ -622,12 +622,17 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
         });
       });
     };
-    if (ODT != E4B_FP32 && n % 8 == 0 && left >= 32 * NA) {
+    if (ODT != E4B_FP32) {
       const uint32_t o = (lane & 15) * ostride + 2 * (lane & 16) + 16 * half;
-      write([&](const mx_acc_t& v, uint32_t at, int) { mx_store_whole<ODT == E4B_FP32 ? E4B_BF16 : ODT>(out, o, at, ostride, v); });
-    } else {
+      write([&](const mx_acc_t& v, uint32_t at, int l) {
+        if (l >= 32) mx_store_whole<ODT == E4B_FP32 ? E4B_BF16 : ODT>(out, o, at, ostride, v);
+      });
+    }
+    if (ODT == E4B_FP32 || (left < 32 * NA && left % 32)) {  // (a whole block's stores must not be repeated by parts)
       const uint32_t o = r32 * ostride + 4 * kOut * half;
-      write([&](const mx_acc_t& v, uint32_t at, int l) { mx_store_part<ODT>(out, o, at, l, half, v); });
+      write([&](const mx_acc_t& v, uint32_t at, int l) {
+        if (ODT == E4B_FP32 || l < 32) mx_store_part<ODT>(out, o, at, l, half, v);
+      });
     }
     mx_for<NA>([&](auto a) { mx_for<NB>([&](auto b) { acc[a()][b()] = mx_acc_t{}; }); });
     if (then.nb < 0) return;
