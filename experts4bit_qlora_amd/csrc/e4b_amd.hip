@@ -856,7 +856,7 @@ int e4b_mx_grouped_gemm(const void* a, int32_t act_dtype, const int64_t* sizes, 
     return fail(E4B_EUNSUPPORTED, "groups=%d outside [0, %d]", groups, e4b::kMxGroupsMax);
   if (groups > 0 && (!sizes || !expert_ids)) return fail(E4B_EINVAL, "sizes/expert_ids is NULL");
   e4b::MxGroups go{};
-  const int64_t rows_max = e4b::mx_rows_max(w->k);
+  const int64_t rows_max = e4b::mx_rows_max(*w);
   int64_t M = 0;
   for (int g = 0; g < groups; ++g) {
     if (sizes[g] < 0) return fail(E4B_EINVAL, "group %d has a negative size", g);

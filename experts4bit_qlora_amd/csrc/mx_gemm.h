@@ -119,13 +119,13 @@ E4B_DEV bool mx_tile(const MxGemmArgs& p, const MxGroups& go, MxTile& o) {
   return true;
 }
 
-// Four sums of a row to the output's columns n .. n + 3.
+// Four sums of a row to the output's columns n .. n + 3, at any address.
 template <int ODT>
-E4B_DEV void mx_store4(void* out, int64_t at, int left, bool vec, const float (&v)[4]) {
+E4B_DEV void mx_store4(void* out, int64_t at, int left, const float (&v)[4]) {
   if constexpr (ODT == E4B_FP32) {
     float* o = static_cast<float*>(out) + at;
-    if (vec && left >= 4) {
-      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    if (left >= 4) {
+      __builtin_memcpy(o, v, 16);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -134,8 +134,8 @@ E4B_DEV void mx_store4(void* out, int64_t at, int left, bool vec, const float (&
   } else {
     uint16_t* o = static_cast<uint16_t*>(out) + at;
     const uint16_t h[4] = {from_f<ODT>(v[0]), from_f<ODT>(v[1]), from_f<ODT>(v[2]), from_f<ODT>(v[3])};
-    if (vec && left >= 4) {
-      *reinterpret_cast<uint2*>(o) = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
+    if (left >= 4) {
+      __builtin_memcpy(o, h, 8);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave, 4) mx_narrow_kernel(MxG
   const int e = t.e, row0 = t.row0, end = t.end, rows = end - row0;
   const int n = static_cast<int>(p.w.n);
   const int blocks = static_cast<int>(p.w.k / kMxBlock);
-  const int chunks = (blocks + 7) / 8;
+  const int chunks = static_cast<int>(mx_chunks(p.w.k));
   const int run = DT < 0 ? 1 : p.run;  // the workgroup's column blocks
   const int first = t.nb * run, last = min(first + run, (n + 31) / 32);
   const int r16 = lane & 15, quarter = lane >> 4;
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave, 4) mx_narrow_kernel(MxG
         for (int w = 0; w < kMxNarrowWaves; ++w) s += red[w][c0 + j][row];
         v[j] = s;
       }
-      mx_store4<ODT>(p.out, int64_t(row0 + row) * n + 32 * nb + c0, left, n % 4 == 0, v);
+      mx_store4<ODT>(p.out, int64_t(row0 + row) * n + 32 * nb + c0, left, v);
     }
   }
 }
@@ -382,6 +382,10 @@ E4B_DEV void mx_store_part(__amdgpu_buffer_rsrc_t out, uint32_t offset, uint32_t
     else
       o = u32x4_t{mx_pair<ODT>(v[4 * g], v[4 * g + 1]), mx_pair<ODT>(v[4 * g + 2], v[4 * g + 3]), 0, 0};
     const int c = 8 * g + 4 * half, at = static_cast<int>(uniform + 8 * g * kOut);
+    if (ODT == E4B_FP32 && c + 4 <= left) {
+      __builtin_amdgcn_raw_buffer_store_b128(o, out, static_cast<int>(offset), at, 0);
+      continue;
+    }
 #pragma unroll 1
     for (int j = 0; j < 4 && c + j < left; ++j) {
       const int to = static_cast<int>(offset + kOut * j);
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   const int half = lane >> 5, r32 = lane & 31;
   const int64_t n = p.w.n;
   const int blocks = static_cast<int>(p.w.k / kMxBlock);
-  const int chunks = (blocks + 7) / 8;  // two at least: the loads are two ahead, at most one tile
+  const int chunks = static_cast<int>(mx_chunks(p.w.k));  // two at least: the loads are two ahead, at most one tile
   const uint32_t wstride = 16 * blocks, astride = 128 * chunks;
 
   // the workgroup's next kItems tiles, one per thread, from the tables: a tile is then one broadcast read
@@ -478,8 +482,8 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   // stores zeros.
   struct Source {
     __amdgpu_buffer_rsrc_t w, a;
-    const uint8_t *ws, *as;
-    int wrows, arows;
+    const uint8_t *ws, *as;  // ws: `before` bytes (8, fewer at the stack's start) before the tile's first
+    int wrows, arows, before;
   };
   auto source_of = [&](const MxTile& t) {
     Source o;
@@ -488,7 +492,8 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
     o.arows = t.end - t.row0;
     o.w = mx_rows_of(p.w.packed + first * wstride, int64_t(o.wrows) * wstride);
     o.a = mx_rows_of(p.a + int64_t(t.row0) * astride, int64_t(o.arows) * astride);
-    o.ws = static_cast<const uint8_t*>(p.w.absmax) + first * blocks;
+    o.before = first * blocks < 8 ? static_cast<int>(first * blocks) : 8;
+    o.ws = static_cast<const uint8_t*>(p.w.absmax) + (first * blocks - o.before);
     o.as = p.as + int64_t(t.row0) * (chunks * 8);
     return o;
   };
@@ -497,17 +502,21 @@ __global__ void __launch_bounds__(kMxWideThreads, 1) mx_wide_kernel(MxGemmArgs p
   const uint32_t woff = prow * wstride + 16 * part, aoff = prow * astride + 16 * part;
   u32x4_t wr[PW], ar[PA];
   u32x2_t wsr, asr;
-  int wpast = 0;
+  int wshift = 0;
+  uint64_t wmask = 0;
   const int slot = prow * 8 + (part ^ ((prow >> 1) & 7));  // of rows 32 i + prow: 32 rows apart, the same order
-  // eight scale bytes of a weight row as mx_scales4 reads four, shifted where they are stored: the load is
-  // not waited for here
+  // eight scale bytes of a weight row, those that would pass the row's end read back from it (in a row of fewer, at the
+  // stack's start, from there); shifted and cut to the row's where they are stored: the load is not waited for here
   auto load_s = [&](const Source& f, int c) {
-    wpast = max(8 * c + 8 - blocks, 0);
-    __builtin_memcpy(&wsr, f.ws + (static_cast<uint32_t>(min(tid, f.wrows - 1)) * static_cast<uint32_t>(blocks) + (8 * c - wpast)), 8);
+    const int left = blocks - 8 * c, past = max(8 - left, 0);
+    const int at = min(tid, f.wrows - 1) * blocks + (8 * c - past + f.before);
+    __builtin_memcpy(&wsr, f.ws + static_cast<uint32_t>(max(at, 0)), 8);
+    wshift = 8 * (past + min(at, 0)) & 63;
+    wmask = left >= 8 ? ~0ull : (1ull << (8 * max(left, 0))) - 1;
     asr = *reinterpret_cast<const u32x2_t*>(f.as + (static_cast<uint32_t>(min(tid, f.arows - 1)) * (chunks * 8) + 8 * c));
   };
   auto store_s = [&](int buf) {
-    wsl[buf][tid] = __builtin_bit_cast(u32x2_t, __builtin_bit_cast(uint64_t, wsr) >> (8 * wpast));
+    wsl[buf][tid] = __builtin_bit_cast(u32x2_t, (__builtin_bit_cast(uint64_t, wsr) >> wshift) & wmask);
     asl[buf][tid] = asr;
   };
   auto load = [&](auto i, const Source& f, int c) {  // piece i of the thread: the weights' first

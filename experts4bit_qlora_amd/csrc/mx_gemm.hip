@@ -41,9 +41,15 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
 }
 
 
-// Groups of more than 32 rows take 256-row tiles; smaller ones 32-row tiles, unless there are only a few beside
-// larger groups: a tile of either kind costs about its weights' bytes (5,760 x 2,880: 3.1 us of the card in
-// the 256-row launch, 2 in the other), a launch 5 us. K of at most one chunk has no 256-row kernel.
+// Calls of at most kNarrowTiles tiles of 32 x 32 (2.5 for each workgroup that the card holds) take those alone: they
+// spread over the CUs and start at once, where a 256-row tile keeps one CU for ~10 us and longer. Both grow alike
+// with K, so the bound holds for any: in us, 32-row tiles / 256-row tiles,
+//   2,880 tiles: K 128 11.3 / 11.6, 256 12.8 / 10.4, 1,024 19.9 / 13.6, 2,880 29.9 / 24.8
+//   1,664 to 1,792: K 128 8.3 / 12.4, 512 9.6 / 11.2, 1,024 13.0 / 15.4, 2,880 20.2 / 27.0
+//   832: K 512 6.0 / 11.9, 2,880 12.8 / 25.4;  23,040: K 128 64.9 / 23.4, 2,880 206.9 / 60.2
+// In larger calls the groups of more than 32 rows take 256-row tiles, smaller ones 32-row tiles, unless there are only
+// a few: a tile of either kind costs about its weights' bytes (5,760 x 2,880: 3.1 us of the card in the 256-row
+// launch, 2 in the other), a launch 5 us.
 //
 // Small groups all round quantize their rows inside the 32-row tiles, without a launch for that: up to eight rows
 // each, up to sixteen where there are tiles enough for runs of column blocks (more than twice 1,024), which share
@@ -55,17 +61,20 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
 template <int ODT>
 void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
   constexpr int kAll = 0x7fffffff, kFew = 5, kNarrowThreads = kMxNarrowWaves * kWave;
-  constexpr int kDirect = 8, kDirectInRuns = 16, kDirectLds = 32768, kOnce = 4, kRunItems = 1024, kRunMost = 4;
+  constexpr int kDirect = 8, kDirectInRuns = 16, kDirectLds = 32768, kOnce = 4, kRunItems = 1024, kRunMost = 4, kNarrowTiles = 2560;
   int small = 0, large = 0, most = 0;
+  int64_t tiles = 0;
   for (int i = 0; i < a.groups; ++i) {
     const int size = g.off[i + 1] - g.off[i];
     small += size > 0 && size <= kMxTileM;
     large += size > kMxTileM;
     most = std::max(most, size);
+    tiles += (size + kMxTileM - 1) / kMxTileM;
   }
   const bool bf16 = a.act_dtype == E4B_BF16;
+  const int64_t blocks = (a.w.n + 31) / 32;
   const int64_t lds = most * mx_chunks(a.w.k) * (kMxChunk / 2 + kMxChunk / kMxBlock);
-  const int64_t run = std::clamp<int64_t>(small * ((a.w.n + 31) / 32) / kRunItems, 1, kRunMost);
+  const int64_t run = std::clamp<int64_t>(tiles * blocks / kRunItems, 1, kRunMost);
   if (most <= (run > 1 ? kDirectInRuns : kDirect) && lds <= kDirectLds) {
     MxGemmArgs d = a;
     d.run = most > kOnce ? static_cast<int>(run) : 1;
@@ -75,7 +84,7 @@ void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
   }
   if (bf16) launch_rows<E4B_BF16>(a, s);
   else launch_rows<E4B_FP16>(a, s);
-  const bool wide = large && a.w.k > kMxChunk;
+  const bool wide = large && tiles * blocks > kNarrowTiles && mx_wide(a.w);
   const int narrow_to = !wide ? kAll : small > kFew ? kMxTileM : 0;
   if (wide) launch_tiles(mx_wide_kernel<ODT>, kMxWideThreads, a, g, {kMxWideM, narrow_to, kAll, 0}, kMxWideN, s, 256);
   if (narrow_to) launch_tiles(mx_narrow_kernel<ODT, -1>, kNarrowThreads, a, g, {kMxTileM, 0, narrow_to, 0}, 32, s);

@@ -9,10 +9,10 @@
 
 namespace e4b {
 
-// Activation rows are quantized into the workspace with K padded to whole chunks of 256 (zero codes):
-// a chunk is 128 bytes of codes and 8 scale bytes.
+// Activation rows are quantized into the workspace with K padded to whole chunks of 256, two at least (zero codes,
+// scale bytes 0): a chunk is 128 bytes of codes and 8 scale bytes.
 constexpr int kMxChunk = 256;
-inline int64_t mx_chunks(int64_t k) { return (k + kMxChunk - 1) / kMxChunk; }
+__host__ __device__ inline int64_t mx_chunks(int64_t k) { return k > kMxChunk ? (k + kMxChunk - 1) / kMxChunk : 2; }
 
 // Row groups given by the host: group g holds rows off[g] .. off[g + 1] - 1 for the expert ids[g].
 constexpr int kMxGroupsMax = 512;
@@ -21,8 +21,10 @@ struct MxGroups {
   int32_t off[kMxGroupsMax + 1];
   uint16_t tile[kMxGroupsMax + 1];
 };
-// Fewer than 2^16 row tiles, one more than the rows fill per group: of 256 rows, or of 32 where K is one chunk.
-inline int64_t mx_rows_max(int64_t k) { return int64_t(1) << (k > kMxChunk ? 23 : 20); }
+// The 256-row tiles read scale bytes eight at a time.
+inline bool mx_wide(const e4b_qweight& w) { return w.num_experts * w.n * (w.k / 32) >= 8; }
+// Fewer than 2^16 row tiles, one more than the rows fill per group: of 256 rows, or of 32 for stacks so small.
+inline int64_t mx_rows_max(const e4b_qweight& w) { return int64_t(1) << (mx_wide(w) ? 23 : 20); }
 
 // A launch's row tiles: tiles of tm rows over the groups of above lo and at most hi rows.
 struct MxTiling {

@@ -345,10 +345,10 @@ def test_mx_grouped_gemm_rejects_bad_arguments():
     assert call(ws_bytes=need - 1) == -4 and call(ws=None) == -4 and "workspace" in _err()
     assert call(sizes=(ctypes.c_int64 * 2)(0, 0), a=None, out=None, ws=None) == 0
     assert L.e4b_mx_gemm_workspace_bytes(0, 96) == 0
-    # K of one chunk has 32-row tiles only: 2^20 rows at most
-    many = dict(a=None, out=None, ws=None)
-    assert call(sizes=(ctypes.c_int64 * 2)(1 << 20, 1), **many) == -2 and "1048576 rows" in _err()
-    assert call(sizes=(ctypes.c_int64 * 2)(1 << 20, 0), **many) == -1 and "NULL" in _err()
+    # stacks of fewer than eight scale bytes have 32-row tiles only: 2^20 rows at most
+    many, tiny = dict(a=None, out=None, ws=None), _qw(format=N.FMT_MXFP4, n=1, k=96)
+    assert call(sizes=(ctypes.c_int64 * 2)(1 << 20, 1), w=tiny, **many) == -2 and "1048576 rows" in _err()
+    assert call(sizes=(ctypes.c_int64 * 2)(1 << 20, 0), w=tiny, **many) == -1 and "NULL" in _err()
     longer = _qw(format=N.FMT_MXFP4, k=288)
     assert call(sizes=(ctypes.c_int64 * 2)(1 << 23, 1), w=longer, **many) == -2 and "8388608 rows" in _err()
     assert call(sizes=(ctypes.c_int64 * 2)(1 << 23, 0), w=longer, **many) == -1 and "NULL" in _err()

@@ -25,7 +25,7 @@ def test_product_outputs(rows, n, k):
     assert torch.equal(out[-300:], part)
 
 
-@pytest.mark.parametrize("size", (2, 9, 40))
+@pytest.mark.parametrize("size", (2, 9, 40, 200))
 def test_product_weights(size):
     """A stack of more than 2^32 bytes: the last expert."""
     E, n, k = 33, 16384, 16384

@@ -60,6 +60,17 @@ def _rows(M, k, dtype, seed):
     return (torch.randn(M, k, generator=g) * torch.exp(torch.randn(M, 1, generator=g))).to(dtype)
 
 
+def _check_both(a, blocks, scales, sizes, ids):
+    """The call, and, where a group has more than 32 rows, the same beside a group of zero rows without an expert that
+    is large enough (2,700 tiles of 32 x 32) for the 256-row tiles to take them all."""
+    _check(a, blocks, scales, sizes, ids, _run(a, blocks, scales, sizes, ids))
+    if max(sizes) > 32:
+        more = 32 * -(-2700 // -(-blocks.shape[1] // 32))
+        out = _run(torch.cat([a, a.new_zeros(more, a.shape[1])]), blocks, scales, [*sizes, more], [*ids, -1])
+        assert not out[len(a):].any()
+        _check(a, blocks, scales, sizes, ids, out[:len(a)])
+
+
 def _run(a, blocks, scales, sizes, ids, **kw):
     return e4b.gemm_mxfp4_grouped(a.to(DEV), blocks.to(DEV), scales.to(DEV), sizes, torch.tensor(ids, device=DEV),
                                   act_quant="mxfp4", **kw)
@@ -72,7 +83,7 @@ def test_depths(k, dtype):
     E, n, sizes, ids = 3, 80, [1, 5, 33], [2, 0, 1]
     b, s = _weights(E, n, k, k)
     a = _rows(sum(sizes), k, dtype, k + 1)
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
 
 
 @pytest.mark.parametrize("n", (1, 3, 31, 32, 33, 127, 130, 256, 257, 516))
@@ -80,7 +91,7 @@ def test_widths(n):
     E, k, sizes, ids = 2, 320, [2, 40], [1, 0]
     b, s = _weights(E, n, k, n)
     a = _rows(sum(sizes), k, torch.bfloat16, n)
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
 
 
 @pytest.mark.parametrize("sizes", ([1], [31], [32], [33], [64], [1, 1, 1, 1], [0, 3, 0], [127, 1, 129], [255], [256],
@@ -90,7 +101,7 @@ def test_group_sizes(sizes):
     ids = [(3 * g + 1) % E for g in range(len(sizes))]
     b, s = _weights(E, n, k, 4)
     a = _rows(sum(sizes), k, torch.bfloat16, len(sizes))
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
 
 
 def test_512_groups_and_one_more():
@@ -98,7 +109,7 @@ def test_512_groups_and_one_more():
     sizes, ids = [g % 4 for g in range(512)], [g % E for g in range(512)]
     b, s = _weights(E, n, k, 6)
     a = _rows(sum(sizes), k, torch.bfloat16, 6)
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
     with pytest.raises(RuntimeError, match="groups=513"):
         _run(a, b, s, sizes + [0], ids + [0])
 
@@ -109,9 +120,9 @@ def test_ids_in_any_order_repeated_and_out_of_range(sizes):
     E, n, k, ids = 4, 96, 256, [3, -1, 3, 4]
     b, s = _weights(E, n, k, 7)
     a = _rows(sum(sizes), k, torch.bfloat16, 7)
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
     ids = [2, 1 << 40, 0, -(1 << 40)]
-    _check(a, b, s, sizes, ids, _run(a, b, s, sizes, ids))
+    _check_both(a, b, s, sizes, ids)
 
 
 def test_host_ids_and_no_rows():
@@ -131,7 +142,7 @@ def test_infinities_and_nan_reach_their_rows_only(rows):
     b, s = _weights(E, n, k, 9)
     a = _rows(rows, k, torch.bfloat16, 9)
     a[0, 17], a[1, 300], a[rows - 1, k - 1] = float("nan"), float("inf"), -float("inf")
-    _check(a, b, s, [rows], [1], _run(a, b, s, [rows], [1]))
+    _check_both(a, b, s, [rows], [1])
 
 
 @pytest.mark.parametrize("rows", (3, 300))
@@ -141,7 +152,7 @@ def test_weight_scales_at_the_ends(rows):
     b, s = _weights(E, n, k, 10)
     s[0, 3], s[0, 4, 2], s[0, 5], s[0, 6, 5] = 0, 1, 200, 255
     a = _rows(rows, k, torch.bfloat16, 10)
-    _check(a, b, s, [rows], [0], _run(a, b, s, [rows], [0]))
+    _check_both(a, b, s, [rows], [0])
 
 
 def test_zero_rows():
@@ -149,7 +160,7 @@ def test_zero_rows():
     b, s = _weights(E, n, k, 11)
     a = torch.zeros(5, k, dtype=torch.bfloat16)
     a[3] = _rows(1, k, torch.bfloat16, 11)[0]
-    _check(a, b, s, [5], [0], _run(a, b, s, [5], [0]))
+    _check_both(a, b, s, [5], [0])
 
 
 def test_views():
@@ -166,7 +177,7 @@ def test_views():
         _check(a, b, s, [3, 1], [1, 0], out)
 
 
-@pytest.mark.parametrize("sizes", ([1, 2], [300, 20]))
+@pytest.mark.parametrize("sizes", ([1, 2], [300, 20], [300, 17_000]))
 def test_captured_and_replayed(sizes):
     """Replays on new inputs in place equal the eager calls bit for bit; two graphs of one pool alternate."""
     E, n, k, ids = 4, 160, 512, torch.tensor([3, 1], device=DEV)
@@ -217,7 +228,7 @@ def test_another_stream_and_no_synchronization():
 def test_repeats_are_bit_equal():
     E, n, k = 4, 400, 704
     b, s = (t.to(DEV) for t in _weights(E, n, k, 15))
-    for sizes in ([2, 1], [700, 90]):
+    for sizes in ([2, 1], [700, 90], [700, 6000]):
         a, ids = _rows(sum(sizes), k, torch.bfloat16, 15).to(DEV), torch.tensor([0, 2], device=DEV)
         first = e4b.gemm_mxfp4_grouped(a, b, s, sizes, ids, act_quant="mxfp4")
         assert all(torch.equal(first, e4b.gemm_mxfp4_grouped(a, b, s, sizes, ids, act_quant="mxfp4")) for _ in range(10))
@@ -286,7 +297,7 @@ def _entry(a, blocks, scales, sizes, ids, out, workspace):
 
 @pytest.mark.parametrize("out_dtype", (torch.float32, torch.float16, torch.bfloat16))
 @pytest.mark.parametrize("n", (72, 267))
-@pytest.mark.parametrize("sizes", ([1, 3], [2, 7], [40, 260]))
+@pytest.mark.parametrize("sizes", ([1, 3], [2, 7], [40, 260], [40, 29_000]))
 def test_entry_point_output_types_and_what_it_leaves(sizes, n, out_dtype):
     """The entry point's other output types; bytes behind the last row and behind the workspace it asked for stay."""
     E, k, ids, M = 3, 352, [2, 0], sum(sizes)
@@ -311,7 +322,7 @@ def test_entry_point_output_types_and_what_it_leaves(sizes, n, out_dtype):
         r += size
 
 
-@pytest.mark.parametrize("sizes", ([1, 2], [9, 5], [300, 20]))
+@pytest.mark.parametrize("sizes", ([1, 2], [9, 5], [300, 20], [300, 9000]))
 def test_two_calls_at_once(sizes):
     """Calls on two streams, each with rows of its own, over the same weights."""
     E, n, k, ids = 4, 320, 704, torch.tensor([3, 1], device=DEV)
@@ -344,3 +355,17 @@ def test_many_small_groups(most, n):
     out = _run(few, b, s, sizes, ids)
     _check(few, b.cpu(), s.cpu(), sizes, ids, out)
     assert torch.equal(_run(a, b, s, sizes + [17], ids + [1])[:sum(sizes)], out)
+
+
+@pytest.mark.parametrize("E", (1, 3))
+@pytest.mark.parametrize("n", (1, 2, 7, 40, 300))
+@pytest.mark.parametrize("k", (32, 64, 96, 224, 256))
+def test_short_rows_in_large_groups(k, n, E):
+    """Rows of fewer than eight scale bytes, from the stack's first byte to its last, in 256-row tiles where the stack
+    has eight bytes; a byte of 255 makes its own column NaN and no neighbour."""
+    b, s = _weights(E, n, k, k + n)
+    g = torch.Generator().manual_seed(k * n)
+    s[torch.rand(s.shape, generator=g) < 0.1] = 255
+    sizes, ids = [300, 45], [E - 1, 0]
+    a = _rows(sum(sizes), k, torch.bfloat16, k + n + 1)
+    _check_both(a, b, s, sizes, ids)
