@@ -47,9 +47,10 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
 //   2,880 tiles: K 128 11.3 / 11.6, 256 12.8 / 10.4, 1,024 19.9 / 13.6, 2,880 29.9 / 24.8
 //   1,664 to 1,792: K 128 8.3 / 12.4, 512 9.6 / 11.2, 1,024 13.0 / 15.4, 2,880 20.2 / 27.0
 //   832: K 512 6.0 / 11.9, 2,880 12.8 / 25.4;  23,040: K 128 64.9 / 23.4, 2,880 206.9 / 60.2
-// In larger calls the groups of more than 32 rows take 256-row tiles, smaller ones 32-row tiles, unless there are only
-// a few: a tile of either kind costs about its weights' bytes (5,760 x 2,880: 3.1 us of the card in the 256-row
-// launch, 2 in the other), a launch 5 us.
+// In larger calls the groups of more than 32 rows take 256-row tiles, and smaller ones ride along unless there are
+// many: a launch of 32-row tiles for them gains only where it is mostly their weights (us a call, own launch /
+// along: 24 groups of 30 rows + 8 of 300, 2,880 x 2,880 79.6 / 67.7, 1,408 x 1,216 31.4 / 25.2; 8 of 8 + 24 of 200 84.2
+// / 74.1, 29.7 / 25.6; 26 of 2 + 6 of 500 68.5 / 72.5, 30.2 / 25.5).
 //
 // Small groups all round quantize their rows inside the 32-row tiles, without a launch for that: up to eight rows
 // each, up to sixteen where there are tiles enough for runs of column blocks (more than twice 1,024), which share
@@ -60,7 +61,7 @@ void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl,
 //   32 x 16 75.6 (4.5 + 80.7); 32 x 24 87.8 (4.5 + 88.5); of 2,880 x 2,880: 32 x 16 38.9 (4.5 + 37.5)
 template <int ODT>
 void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
-  constexpr int kAll = 0x7fffffff, kFew = 5, kNarrowThreads = kMxNarrowWaves * kWave;
+  constexpr int kAll = 0x7fffffff, kFew = 32, kNarrowThreads = kMxNarrowWaves * kWave;
   constexpr int kDirect = 8, kDirectInRuns = 16, kDirectLds = 32768, kOnce = 4, kRunItems = 1024, kRunMost = 4, kNarrowTiles = 2560;
   int small = 0, large = 0, most = 0;
   int64_t tiles = 0;

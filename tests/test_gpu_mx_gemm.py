@@ -95,7 +95,7 @@ def test_widths(n):
 
 
 @pytest.mark.parametrize("sizes", ([1], [31], [32], [33], [64], [1, 1, 1, 1], [0, 3, 0], [127, 1, 129], [255], [256],
-                                   [257, 300], [513, 30, 290], [1] * 40, [7] * 100, [900]))
+                                   [257, 300], [513, 30, 290], [3] * 40 + [300], [1] * 40, [7] * 100, [900]))
 def test_group_sizes(sizes):
     E, n, k = 5, 272, 544
     ids = [(3 * g + 1) % E for g in range(len(sizes))]
