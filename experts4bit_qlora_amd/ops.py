@@ -56,7 +56,7 @@ def _require_cuda(*ts):
             raise ValueError("the MI355X kernels need tensors on the HIP device")
 
 
-@dataclass
+@dataclass(init=False)
 class QW:
     """A 4-bit weight stack as the kernels see it (tensors kept alive alongside the struct)."""
 
@@ -72,6 +72,12 @@ class QW:
     code2: torch.Tensor | None = None
     bias: torch.Tensor | None = None
     shift: torch.Tensor | None = None  # NF4: per-expert exponents of the fp16 matrix-core mode
+
+    def __init__(self, fmt, num_experts, n, k, packed, absmax, absmax2=None, offset=None, code=None, code2=None, bias=None,
+                 shift=None):
+        # (field by field through __setattr__ this is ~2 us of every call that takes plain tensors)
+        self.__dict__.update(fmt=fmt, num_experts=num_experts, n=n, k=k, packed=packed, absmax=absmax, absmax2=absmax2,
+                             offset=offset, code=code, code2=code2, bias=bias, shift=shift)
 
     def __setattr__(self, name, value):  # a changed field invalidates the cached descriptor
         d = self.__dict__
@@ -217,19 +223,19 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``[..., k]`` dense values (``k`` a multiple of 32) -> MXFP4 (blocks uint8 ``[..., k/2]``, scales
     e8m0 uint8 ``[..., k/32]``)."""
     _require_cuda(w)
-    x = w.detach()
+    x = w.detach() if w.requires_grad else w
     x = (x if x.dtype in _DT else x.float()).contiguous()
     if x.data_ptr() % 16:  # a view that starts inside another tensor
         x = x.clone()
-    k = x.shape[-1]
+    lead, k, dev = x.shape[:-1], x.shape[-1], x.device
     if k % 32:
         raise ValueError(f"K={k} is not a multiple of 32")
-    blocks = torch.empty(*x.shape[:-1], k // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], k // 32, dtype=torch.uint8, device=x.device)
-    with _on(x.device):
+    blocks = torch.empty((*lead, k // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*lead, k // 32), dtype=torch.uint8, device=dev)
+    with _on(dev):
         N.check("e4b_quantize_mxfp4",
                 N.lib().e4b_quantize_mxfp4(x.data_ptr(), dtype_code(x.dtype), x.numel(), blocks.data_ptr(),
-                                           scales.data_ptr(), _stream(x.device)))
+                                           scales.data_ptr(), _stream(dev)))
     return blocks, scales
 
 
@@ -833,8 +839,8 @@ def mx_grouped_gemm(a: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor,
     _require_cuda(a, blocks, scales)
     E, n, kh = blocks.shape
     k, G, dev = 2 * kh, len(sizes), a.device
-    if k % 32 or 32 * scales.numel() != E * n * k:
-        raise ValueError(f"blocks and scales must be [{E}, {n}, K/2] and [{E}, {n}, K/32] with K a multiple of 32")
+    if k % 32 or 32 * scales.numel() != E * n * k or blocks.element_size() != 1 or scales.element_size() != 1:
+        raise ValueError(f"blocks and scales must be bytes [{E}, {n}, K/2] and [{E}, {n}, K/32], K a multiple of 32")
     if torch.is_tensor(expert_ids) and expert_ids.is_cuda:
         ids = expert_ids if expert_ids.dtype == torch.int64 else expert_ids.to(torch.int64)
         ids = ids.contiguous()

@@ -281,6 +281,8 @@ def test_refuses_stacks_that_do_not_fit():
     a = _rows(3, 64, torch.bfloat16, 2)
     with pytest.raises(ValueError, match="scales"):
         _run(a, b, s[..., :1].contiguous(), [3], [0])
+    with pytest.raises(ValueError, match="bytes"):
+        _run(a, b.int(), s, [3], [0])
     with pytest.raises(ValueError, match="columns"):
         _run(a[:, :32].contiguous(), b, s, [3], [0])
 
