@@ -652,7 +652,8 @@ int e4b_router_topk_backward(const void* logits, int32_t dtype, int64_t tokens, 
 size_t e4b_balance_workspace_bytes(int32_t layers, int64_t tokens, int32_t num_experts) {
   if (layers <= 0 || tokens <= 0 || num_experts <= 0 || num_experts > e4b::kGateMaxExperts) return 0;
   const size_t parts = size_t(layers) * e4b::balance_chunks(tokens, layers, num_experts);
-  return align256(sizeof(float) * parts * num_experts) + align256(sizeof(int32_t) * parts * (num_experts + 1));
+  return align256(sizeof(int64_t) * layers * num_experts) + align256(sizeof(float) * parts * num_experts) +
+         align256(sizeof(int32_t) * parts * (num_experts + 1));
 }
 
 int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
@@ -676,9 +677,14 @@ int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t 
   a.index = top_k_index;
   a.mask = mask;
   a.chunks = tokens ? e4b::balance_chunks(tokens, layers, num_experts) : 0;
-  a.part = static_cast<float*>(workspace);
-  a.part_counts = reinterpret_cast<int32_t*>(
-      static_cast<char*>(workspace) + align256(sizeof(float) * size_t(layers) * a.chunks * num_experts));
+  if (a.chunks) {
+    char* at = static_cast<char*>(workspace);
+    a.kept = reinterpret_cast<int64_t*>(at);
+    at += align256(sizeof(int64_t) * layers * num_experts);
+    a.part = reinterpret_cast<float*>(at);
+    at += align256(sizeof(float) * size_t(layers) * a.chunks * num_experts);
+    a.part_counts = reinterpret_cast<int32_t*>(at);
+  }
   a.loss = loss;
   a.counts = counts;
   a.valid = valid;

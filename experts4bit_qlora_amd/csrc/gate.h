@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(BalanceArgs 
       n += count[tid + lanes * i];
     }
     p.counts[int64_t(layer) * p.E + tid] = n;
+    if (p.kept) p.kept[int64_t(layer) * p.E + tid] = n;
     mine = static_cast<double>(n) * s;
   }
   __syncthreads();

@@ -37,6 +37,7 @@ struct BalanceArgs {
   int32_t* part_counts;  // [L, chunks, E + 1] counts, then the valid tokens
   float* loss;           // [L]
   int64_t* counts;       // [L, E]
+  int64_t* kept;         // [L, E], NULL without tokens: the same, in the workspace
   int64_t* valid;        // [L] valid tokens
   const float* grad_loss;  // backward: [L]
   void* grad;              // backward: [L, T, E] in dtype

@@ -347,7 +347,7 @@ def _balance_ws_bytes(layers: int, tokens: int, experts: int) -> int:
 
 def balance_loss(logits: torch.Tensor, index: torch.Tensor, mask: torch.Tensor | None):
     """``[L, T, E]`` logits, ``[L, T, k]`` index, bool mask ``[T]`` or ``[L, T]`` -> (loss fp32 ``[L]``, counts int64
-    ``[L, E]``, valid tokens int64 ``[L]``) by ``e4b_balance_loss``."""
+    ``[L, E]``, valid tokens int64 ``[L]``, the workspace, which begins with the counts again) by ``e4b_balance_loss``."""
     _require_cuda(logits, index, mask)
     L_, T, E = logits.shape
     dev = logits.device
@@ -361,12 +361,13 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, mask: torch.Tensor |
                                      index.shape[2], _ptr(mask), 0 if mask is None or mask.dim() == 1 else T,
                                      ws.data_ptr(), ws.numel(), loss.data_ptr(), counts.data_ptr(), valid.data_ptr(),
                                      _stream(dev)))
-    return loss, counts, valid
+    return loss, counts, valid, ws
 
 
 def balance_loss_backward(logits: torch.Tensor, mask: torch.Tensor | None, counts: torch.Tensor, valid: torch.Tensor,
                           grad: torch.Tensor) -> torch.Tensor:
-    """dL/dlogits from dL/dloss fp32 ``[L]`` (``e4b_balance_loss_backward``)."""
+    """dL/dlogits from dL/dloss fp32 ``[L]`` (``e4b_balance_loss_backward``); ``counts``: those of ``balance_loss`` or
+    its workspace."""
     _require_cuda(logits, mask, counts, valid, grad)
     L_, T, E = logits.shape
     dev = logits.device

@@ -113,8 +113,10 @@ def _router_topk_torch(logits, top_k, scoring, weight_dtype):
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, mask):
-        loss, counts, valid = ops.balance_loss(logits, index, mask)
-        ctx.save_for_backward(logits, mask, counts, valid)
+        # The backward reads the counts that the workspace begins with: a collective may reduce the public ones over
+        # ranks meanwhile without raising autograd's version. They are saved so that an ordinary change is refused.
+        loss, counts, valid, kept = ops.balance_loss(logits, index, mask)
+        ctx.save_for_backward(logits, mask, counts, kept, valid)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
@@ -124,8 +126,8 @@ class _Balance(torch.autograd.Function):
         if grad is None:
             return None, None, None
         _once()
-        logits, mask, counts, valid = ctx.saved_tensors
-        return ops.balance_loss_backward(logits, mask, counts, valid, _aligned(grad)), None, None
+        logits, mask, _, kept, valid = ctx.saved_tensors
+        return ops.balance_loss_backward(logits, mask, kept, valid, _aligned(grad)), None, None
 
 
 def balance_loss(logits: torch.Tensor, top_k_index: torch.Tensor,
@@ -137,7 +139,10 @@ def balance_loss(logits: torch.Tensor, top_k_index: torch.Tensor,
     of expert e (ids outside ``[0, E)`` count nowhere), ``P[e]`` the mean of the softmax probabilities, ``loss = E
     * sum_e counts[e] / N * P[e]``, 0 where N is 0. For one loss over several
     layers' tokens together, pass them as one axis. The loss is
-    differentiable with respect to the logits (once), the counts are constants to it."""
+    differentiable with respect to the logits (once), the counts are constants to it: the gradient is that of this
+    call's own tokens also where a collective (``torch.distributed.all_reduce``) has summed ``counts`` over the ranks
+    before the backward. An ordinary change of ``counts`` in place before the backward goes to a copy (on the device
+    autograd refuses it)."""
     if logits.dim() < 2 or not logits.is_floating_point():
         raise ValueError("logits must be a floating-point tensor [..., tokens, num_experts]")
     lead, (T, E) = logits.shape[:-2], logits.shape[-2:]
@@ -161,7 +166,7 @@ def balance_loss(logits: torch.Tensor, top_k_index: torch.Tensor,
     if z.requires_grad and torch.is_grad_enabled():
         loss, counts = _Balance.apply(z, index, mask)
     else:
-        loss, counts, _ = ops.balance_loss(z, index, mask)
+        loss, counts, _, _ = ops.balance_loss(z, index, mask)
     return (loss, counts) if len(lead) == 1 else (loss.view(lead), counts.view(*lead, E))
 
 

@@ -179,15 +179,17 @@ size_t e4b_balance_workspace_bytes(int32_t layers, int64_t tokens, int32_t num_e
  * is 0). logits [layers, tokens, num_experts] in dtype, top_k_index [layers, tokens, top_k] int64;
  * loss fp32 [layers], counts int64 [layers, num_experts], valid int64 [layers] (N, for the backward).
  * A row whose logits are all -inf adds no probability. Deterministic. layers <= 65535, tokens * top_k below
- * 2^31, num_experts <= 1024. Has no counterpart in the reference. */
+ * 2^31, num_experts <= 1024. Where there are tokens the workspace begins with the counts a second time, int64
+ * [layers, num_experts]: a caller that keeps it until the backward may reduce `counts` over its ranks meanwhile.
+ * Has no counterpart in the reference. */
 int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                      const int64_t* top_k_index, int32_t top_k, const uint8_t* mask, int64_t mask_stride,
                      void* workspace, size_t workspace_bytes, float* loss, int64_t* counts, int64_t* valid,
                      hipStream_t stream);
 
 /* Its backward (the counts are constants): grad_logits[t, j] = grad_loss * num_experts / N^2 * p_tj *
- * (counts[j] - sum_e counts[e] p_te) at valid tokens, 0 elsewhere; grad_loss fp32 [layers], counts and valid as
- * the forward wrote them. */
+ * (counts[j] - sum_e counts[e] p_te) at valid tokens, 0 elsewhere; grad_loss fp32 [layers], counts (or the
+ * workspace that begins with them) and valid as the forward wrote them. */
 int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                               const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
                               const float* grad_loss, void* grad_logits, hipStream_t stream);

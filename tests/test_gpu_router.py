@@ -324,3 +324,19 @@ def test_no_tokens_on_the_device():
     loss, counts = e4b.balance_loss(z, torch.zeros(3, 0, 2, dtype=torch.int64, device=DEV))
     assert not loss.any() and not counts.any() and counts.shape == (3, 8)
     assert torch.autograd.grad(loss.sum(), z)[0].shape == (3, 0, 8)
+
+
+@pytest.mark.parametrize("L,T,E,k,masked", ((1, 1, 8, 2, False), (3, 200, 60, 4, True), (2, 5000, 128, 8, False), (1200, 5, 16, 2, True)))
+def test_counts_reduced_over_ranks_before_the_backward(L, T, E, k, masked):
+    """A collective writes its sum into ``counts`` without raising autograd's version (``.data`` does the same here): the
+    gradient is still that of this call's own tokens."""
+    z = _logits((L, T, E), torch.bfloat16, T).to(DEV).requires_grad_()
+    index, grad = _choices(z, k), torch.rand(L, generator=torch.Generator().manual_seed(T)).to(DEV)
+    mask = torch.rand(L, T, generator=torch.Generator().manual_seed(E)).to(DEV) > 0.3 if masked else None
+    loss, counts = e4b.balance_loss(z, index, mask)
+    (want,) = torch.autograd.grad(loss, z, grad)
+    loss, counts = e4b.balance_loss(z, index, mask)
+    counts.data.mul_(3).add_(torch.arange(E, device=DEV))
+    assert counts._version == 0
+    (got,) = torch.autograd.grad(loss, z, grad)
+    assert torch.equal(got, want)
