@@ -178,8 +178,10 @@ def _on_kernel_index(index: torch.Tensor, mask) -> bool:
 def _balance_loss_torch(logits, top_k_index, mask):
     z = logits if logits.dtype == torch.float64 else logits.float()
     T, E = z.shape[-2:]
-    p = _softmax_or_zero(z)
     valid = torch.ones(z.shape[:-1], dtype=torch.bool, device=z.device) if mask is None else mask.expand(z.shape[:-1])
+    if mask is not None:  # before the softmax, whose gradient at a NaN or an infinity is NaN whatever it is multiplied by
+        z = torch.where(valid.unsqueeze(-1), z, 0.0)
+    p = _softmax_or_zero(z)
     n = valid.sum(-1)
     i = top_k_index.to(torch.int64)
     held = valid.unsqueeze(-1) & (i >= 0) & (i < E)

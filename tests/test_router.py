@@ -126,3 +126,25 @@ def test_refusals():
         e4b.balance_loss(z, index, mask=torch.ones(5))
     with pytest.raises(ValueError, match="logits"):
         e4b.balance_loss(z[0], index[0])
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float64))
+def test_balance_values_behind_the_mask_have_no_influence(dtype):
+    """NaN and infinities in masked tokens: loss, counts and gradient are those of finite values there, the masked
+    tokens' gradient is zero."""
+    z = torch.randn(2, 20, 24, dtype=dtype, generator=torch.Generator().manual_seed(5))
+    index, _ = e4b.router_topk(z, 2)
+    one = torch.ones(20)
+    one[[1, 2, 5, 7]] = 0
+    each = one.expand(2, 20).clone()
+    each[1, 9] = 0
+    bad = z.clone()
+    bad[:, 1], bad[:, 2, 3], bad[:, 5], bad[:, 7, 4] = float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min
+    for mask in (one, each):
+        outs = []
+        for logits in (z, bad):
+            leaf = logits.clone().requires_grad_()
+            loss, counts = e4b.balance_loss(leaf, index, mask)
+            outs.append((loss, counts, torch.autograd.grad(loss.sum(), leaf)[0]))
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+        assert not outs[1][2][(mask == 0).expand(2, 20)].any() and outs[1][2].any()
