@@ -32,6 +32,7 @@ _FP4_RAW = (0.0, 0.0625, 8.0, 12.0, 4.0, 6.0, 2.0, 3.0, -0.0, -0.0625, -8.0, -12
 
 # e2m1 grid, index = nibble (formats/mxfp4.py:29-32)
 FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
+_E8M0_VALUES = tuple(2.0 ** (e - 127) for e in range(255))
 
 _DQ_BLOCKSIZE2 = 256
 
@@ -254,9 +255,10 @@ def _quantize_mxfp4_torch(w: torch.Tensor, group: int = 32):
     safe = torch.where(amax > 0, amax, torch.ones_like(amax))
     X = torch.where(amax > 0, torch.floor(torch.log2(safe)) - 2, torch.full_like(amax, -127.0))
     e = torch.clamp(X + 127, 0, 254)
-    # 2^(e - 127) from its bits: torch's fp64 pow on a HIP device is an ulp off at some powers of two,
-    # which moves values that lie exactly between two codes
-    scaled = g.double() / ((e.to(torch.int64) + (1023 - 127)) << 52).view(torch.float64).unsqueeze(-1)
+    # 2^(e - 127) from a table: torch's fp64 pow on a HIP device is an ulp off at some powers of two, which
+    # moves values that lie exactly between two codes
+    power = torch.tensor(_E8M0_VALUES, dtype=torch.float64, device=w.device)
+    scaled = g.double() / power[e.to(torch.int64)].unsqueeze(-1)
     mag = scaled.abs()
     grid = torch.tensor(FP4_VALUES[:8], dtype=torch.float64, device=w.device)
     mids = (grid[:-1] + grid[1:]) / 2.0

@@ -333,3 +333,11 @@ def test_evicted_storage_frees_the_cached_weights():
     mod2.down_proj = torch.nn.Parameter(torch.empty(0, dtype=torch.uint8), requires_grad=False)
     gc.collect()
     assert old2() is None
+
+
+def test_mxfp4_quantizer_under_vmap_and_trace():
+    w = torch.randn(4, 3, 64, generator=torch.Generator().manual_seed(1))
+    want = Q.quantize_mxfp4(w)
+    assert all(torch.equal(a, b) for a, b in zip(torch.func.vmap(Q.quantize_mxfp4)(w), want))
+    traced = torch.jit.trace(Q.quantize_mxfp4, (w * 3,))
+    assert all(torch.equal(a, b) for a, b in zip(traced(w), want))
