@@ -55,21 +55,13 @@ E4B_DEV uint32_t mx_amax(const MxPiece<DT>& p) {
   }
 }
 
-// The scale byte of a block whose largest magnitude has the fp32 bits m. An fp32 maximum a few ulp
-// below a power of two counts as that power where fp32's log2 rounds to it: `quantize_mxfp4` in quant.py
-// takes the logarithm in fp32 (bf16 and fp16 values are too coarse to come that close). A block with
-// an infinity or a NaN: 255, which makes the whole block NaN in a product (nan_scale), or the torch
+// The scale byte of a block whose largest magnitude has the fp32 bits m: floor(log2) is its exponent field. A block
+// with an infinity or a NaN: 255, which makes the whole block NaN in a product (nan_scale), or the torch
 // formulation's 254 and 0.
-template <int DT>
 E4B_DEV uint32_t mx_scale_byte(uint32_t m, bool nan_scale) {
   const uint32_t f = m >> 23;
   if (f == 255) return nan_scale ? 255u : (m == 0x7f800000u ? 254u : 0u);
-  uint32_t e = f > 2 ? f - 2 : 0;
-  if constexpr (DT == E4B_FP32) {
-    if ((m & 0x7fff00u) == 0x7fff00u && f > 1)
-      e = static_cast<uint32_t>(max(0, static_cast<int>(floorf(log2f(__uint_as_float(m)))) + 125));
-  }
-  return e;
+  return f > 2 ? f - 2 : 0;
 }
 
 // The eight codes of a piece under scale byte e (255 converts as 254; its codes are not read as values).
@@ -133,7 +125,7 @@ __global__ void __launch_bounds__(kMxThreads) mx_quantize_kernel(const void* __r
   for (int u = 0; u < kMxUnroll; ++u) {
     const int64_t p = first + u * kMxThreads;
     const uint32_t m = quad_max(mx_amax<DT>(raw[u]));
-    const uint32_t e = mx_scale_byte<DT>(m, false);
+    const uint32_t e = mx_scale_byte(m, false);
     uint32_t c = mx_codes<DT>(raw[u], e);
     if (m > 0x7f800000u) c = mx_nan_codes<DT>(raw[u], c);
     if (p < pieces) {

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kMxRowThreads) mx_rows_kernel(const void* __re
   const bool in = q < row_values / 8;
   MxPiece<DT> v = mx_load<DT>(x, int64_t(row) * (row_values / 8) + (in ? q : 0));
   const uint32_t m = quad_max(mx_amax<DT>(v));
-  const uint32_t e = mx_scale_byte<DT>(m, true);
+  const uint32_t e = mx_scale_byte(m, true);
   const uint32_t c = mx_codes<DT>(v, e);
   codes[p] = in ? c : 0u;
   if ((p & 3) == 0) scales[p >> 2] = in ? static_cast<uint8_t>(e) : 0;
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kMxNarrowWaves* kWave, 4) mx_narrow_kernel(MxG
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int q = q0 + u * kThreads;
-        const uint32_t s = mx_scale_byte<DT>(quad_max(mx_amax<DT>(v[u])), true);
+        const uint32_t s = mx_scale_byte(quad_max(mx_amax<DT>(v[u])), true);
         const uint32_t code = mx_codes<DT>(v[u], s);
         if (q < rows * pieces) {
           reinterpret_cast<uint32_t*>(own)[q] = some[u] ? code : 0u;

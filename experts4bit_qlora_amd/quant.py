@@ -33,6 +33,7 @@ _FP4_RAW = (0.0, 0.0625, 8.0, 12.0, 4.0, 6.0, 2.0, 3.0, -0.0, -0.0625, -8.0, -12
 # e2m1 grid, index = nibble (formats/mxfp4.py:29-32)
 FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
 _E8M0_VALUES = tuple(2.0 ** (e - 127) for e in range(255))
+_E8M0_FIRST = tuple(2.0 ** (e - 125) for e in range(1, 255))  # the smallest block maxima of scale bytes 1 to 254
 
 _DQ_BLOCKSIZE2 = 256
 
@@ -252,13 +253,13 @@ def _quantize_mxfp4_torch(w: torch.Tensor, group: int = 32):
         raise ValueError(f"K={K} is not a multiple of {group}")
     g = w.reshape(*w.shape[:-1], K // group, group)
     amax = g.abs().amax(dim=-1)
-    safe = torch.where(amax > 0, amax, torch.ones_like(amax))
-    X = torch.where(amax > 0, torch.floor(torch.log2(safe)) - 2, torch.full_like(amax, -127.0))
-    e = torch.clamp(X + 127, 0, 254)
-    # 2^(e - 127) from a table: torch's fp64 pow on a HIP device is an ulp off at some powers of two, which
-    # moves values that lie exactly between two codes
+    # e and 2^(e - 127) from tables: fp32's log2 is a whole number already a few ulp below some powers of two (differently
+    # on CPU and device), and torch's fp64 pow on a HIP device is an ulp off at some powers of two, which moves values
+    # that lie exactly between two codes
     power = torch.tensor(_E8M0_VALUES, dtype=torch.float64, device=w.device)
-    scaled = g.double() / power[e.to(torch.int64)].unsqueeze(-1)
+    first = torch.tensor(_E8M0_FIRST, dtype=torch.float64, device=w.device)
+    e = torch.bucketize(torch.where(amax > 0, amax, 0.0).double(), first, right=True)  # (a NaN counts as 0)
+    scaled = g.double() / power[e].unsqueeze(-1)
     mag = scaled.abs()
     grid = torch.tensor(FP4_VALUES[:8], dtype=torch.float64, device=w.device)
     mids = (grid[:-1] + grid[1:]) / 2.0

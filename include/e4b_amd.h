@@ -123,9 +123,9 @@ int e4b_quantize_8bit(const float* values, const float* offset, int64_t rows, in
                       int32_t zero_code, uint8_t* codes, float* absmax, hipStream_t stream);
 
 /* Quantize `values` dense values (E4B_BF16 / E4B_FP16 / E4B_FP32, a multiple of 32) to MXFP4 in blocks of
- * 32: scales[b] = clamp(floor(log2(largest magnitude)) - 2 + 127, 0, 254) (0 for a zero block; the
- * logarithm rounded to fp32), each value the e2m1 code nearest to value / 2^(scales[b] - 127), ties to
- * the even code, saturating at 6, a zero without a sign. blocks is u8 [values / 2], first value of a pair
+ * 32: scales[b] = clamp(floor(log2(largest magnitude)) - 2 + 127, 0, 254) (0 for a zero block), each
+ * value the e2m1 code nearest to value / 2^(scales[b] - 127), ties to the even code, saturating at 6, a
+ * zero without a sign. blocks is u8 [values / 2], first value of a pair
  * in the low nibble, scales u8 [values / 32]. A block with a NaN takes scale 0, one with an infinity 254;
  * a NaN's code is +6. x and blocks are 16-byte aligned.
  * Has no counterpart in the reference, which loads released MXFP4 bytes (formats/mxfp4.py:35-105). */

@@ -190,8 +190,8 @@ def quantize_mxfp4(w, group: int = 32):
         raise ValueError(f"K={K} is not a multiple of {group}")
     g = w.reshape(w.shape[:-1] + (K // group, group))
     amax = np.abs(g).max(axis=-1)
-    with np.errstate(divide="ignore"):
-        X = np.where(amax > 0, np.floor(np.log2(np.where(amax > 0, amax, 1.0))) - 2, -127)
+    X = np.where(amax > 0, np.frexp(amax)[1] - 3, -127)  # frexp: amax in [2^(exponent - 1), 2^exponent)
+    X = np.where(np.isinf(amax), 127, X)
     e = np.clip(X + 127, 0, 254).astype(np.int32)
     scaled = (g.astype(np.float64) / np.ldexp(1.0, e - 127)[..., None])
     mag = np.abs(scaled)

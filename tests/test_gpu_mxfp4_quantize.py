@@ -92,3 +92,19 @@ def test_another_stream():
     s.synchronize()
     want = Q._quantize_mxfp4_torch(w * 2)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_fp32_blocks_equal_the_cpu_formulation():
+    """Scale bytes are the floor of the exact logarithm on either side: maxima next to every power of two, random rows."""
+    exponent = torch.arange(0, 255, dtype=torch.int32)[:, None]
+    mantissa = torch.cat([torch.arange(512, dtype=torch.int32), 0x7FFFFF - torch.arange(512, dtype=torch.int32)])
+    bits = ((exponent << 23) | mantissa[None, :]).reshape(-1)
+    block = torch.zeros(bits.numel(), 32)
+    block[:, 31] = -bits.view(torch.float32)
+    block[:, 0] = bits.view(torch.float32) * 0.55
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn(4096, 32, generator=g) * torch.exp(20 * torch.randn(4096, 1, generator=g))
+    for w in (block, rows):
+        got, want = e4b.quantize_mxfp4(w.to(DEV)), Q._quantize_mxfp4_torch(w)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    assert torch.equal(e4b.quantize_mxfp4(block.to(DEV))[1].cpu()[:, 0].int(), ((bits >> 23) - 2).clamp(min=0))

@@ -341,3 +341,19 @@ def test_mxfp4_quantizer_under_vmap_and_trace():
     assert all(torch.equal(a, b) for a, b in zip(torch.func.vmap(Q.quantize_mxfp4)(w), want))
     traced = torch.jit.trace(Q.quantize_mxfp4, (w * 3,))
     assert all(torch.equal(a, b) for a, b in zip(traced(w), want))
+
+
+def test_mxfp4_scale_is_the_floor_of_the_logarithm():
+    """The 64 largest and smallest mantissas of every fp32 binade as a block's maximum (the logarithm rounded to fp32
+    is a whole number already below some powers of two), the ends, infinity and NaN."""
+    m = torch.cat([torch.arange(64, dtype=torch.int32), 0x7FFFFF - torch.arange(64, dtype=torch.int32)])
+    bits = ((torch.arange(255, dtype=torch.int32)[:, None] << 23) | m).reshape(-1)
+    top = bits.view(torch.float32)
+    block = torch.zeros(top.numel(), 32)
+    block[:, 31], block[:, 0] = -top, top * 0.55
+    codes, scales = Q._quantize_mxfp4_torch(block)
+    assert torch.equal(scales[:, 0].int(), ((bits >> 23) - 2).clamp(min=0))
+    ob, os_ = oq.quantize_mxfp4(block.numpy())
+    assert np.array_equal(scales.numpy(), os_) and np.array_equal(codes.numpy(), ob.reshape(len(top), 16))
+    for value, byte in ((float("inf"), 254), (float("nan"), 0), (0.0, 0)):
+        assert Q._quantize_mxfp4_torch(torch.full((32,), value))[1].item() == byte
