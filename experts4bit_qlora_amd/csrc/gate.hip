@@ -16,9 +16,10 @@ int lanes_of(int E) {
   return gl;
 }
 
+int dtype_bytes(int dtype) { return dtype == E4B_FP32 ? 4 : 2; }
+
 int vec_rows(const void* p, int dtype, int E) {
-  const int bytes = dtype == E4B_FP32 ? 4 : 2;
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (int64_t(E) * bytes) % 16 == 0;
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (int64_t(E) * dtype_bytes(dtype)) % 16 == 0;
 }
 
 // f(dtype, lanes, logits per lane) with all three known at compile time
@@ -47,21 +48,39 @@ void by_shape(int dtype, int E, F&& f) {
   }
 }
 
+// f(arguments of the rows, grid) for all rows in order, `per` a workgroup. A launch holds fewer than 2^32 work items
+// (2^26 rows of more than 256 experts are as many), so it takes 2^23 workgroups at most.
+template <class F>
+void by_rows(const GateArgs& a, int per, F&& f) {
+  const int64_t most = (int64_t(1) << 23) * per;
+  for (int64_t first = 0; first < a.T; first += most) {
+    GateArgs p = a;
+    p.T = std::min(most, a.T - first);
+    p.logits = static_cast<const char*>(a.logits) + first * a.E * dtype_bytes(a.dtype);
+    p.index = a.index + first * a.k;
+    p.weights = static_cast<char*>(a.weights) + first * a.k * dtype_bytes(a.wdtype);
+    if (a.grad) p.grad = static_cast<char*>(a.grad) + first * a.E * dtype_bytes(a.dtype);
+    f(p, dim3(static_cast<unsigned>(cdiv(p.T, per))));
+  }
+}
+
 }  // namespace
 
 void launch_gate(const GateArgs& a, hipStream_t s) {
   by_shape(a.dtype, a.E, [&](auto dt, auto gl, auto vpl) {
-    const dim3 grid(static_cast<unsigned>(cdiv(a.T, kGateThreads / gl())));
-    hipLaunchKernelGGL((gate_kernel<dt(), gl(), vpl()>), grid, dim3(kGateThreads), 0, s, a,
-                       vec_rows(a.logits, a.dtype, a.E));
+    by_rows(a, kGateThreads / gl(), [&](const GateArgs& p, dim3 grid) {
+      hipLaunchKernelGGL((gate_kernel<dt(), gl(), vpl()>), grid, dim3(kGateThreads), 0, s, p,
+                         vec_rows(p.logits, p.dtype, p.E));
+    });
   });
 }
 
 void launch_gate_backward(const GateArgs& a, hipStream_t s) {
   by_shape(a.dtype, a.E, [&](auto dt, auto gl, auto vpl) {
-    const dim3 grid(static_cast<unsigned>(cdiv(a.T, kGateThreads / gl())));
-    hipLaunchKernelGGL((gate_backward_kernel<dt(), gl(), vpl()>), grid, dim3(kGateThreads), 0, s, a,
-                       vec_rows(a.logits, a.dtype, a.E) && vec_rows(a.grad, a.dtype, a.E));
+    by_rows(a, kGateThreads / gl(), [&](const GateArgs& p, dim3 grid) {
+      hipLaunchKernelGGL((gate_backward_kernel<dt(), gl(), vpl()>), grid, dim3(kGateThreads), 0, s, p,
+                         vec_rows(p.logits, p.dtype, p.E) && vec_rows(p.grad, p.dtype, p.E));
+    });
   });
 }
 

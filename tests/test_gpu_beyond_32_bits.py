@@ -68,3 +68,34 @@ def test_router():
     # five probabilities per expert, summed in another order: 2^-20 is sixteen fp32 roundings
     assert torch.allclose(loss, own, rtol=2.0 ** -20, atol=0)
     assert torch.equal(grad[-5:], want) and not grad[:-5].any()
+
+
+def test_gate_of_more_work_items_than_a_launch_holds():
+    """2^26 rows of more than 256 experts (64 lanes each) in several launches: every row against one call of the rows
+    that repeat, new rows where one launch may end and at the end."""
+    E, k, rows = 257, 2, 1 << 16
+    T = (1 << 26) + 5
+    base = torch.randn(rows, E, device=DEV, dtype=torch.bfloat16)
+    z = base.repeat(1025, 1)[:T]
+    new = [slice(t - 2, t + 3) for t in (1 << 24, 1 << 25, (1 << 25) + (1 << 24))] + [slice(T - 5, T)]
+    for s in new:
+        z[s] = torch.randn(5, E, device=DEV, dtype=torch.bfloat16)
+    z.requires_grad_()
+    index, weights = e4b.router_topk(z, k)
+    (grad,) = torch.autograd.grad(weights, z, torch.ones_like(weights))
+
+    def own(t):
+        t = t.detach().clone().requires_grad_()
+        i, w = e4b.router_topk(t, k)
+        return i, w.detach(), torch.autograd.grad(w, t, torch.ones_like(w))[0]
+
+    for s in new:
+        assert all(torch.equal(a, b) for a, b in zip((index[s], weights.detach()[s], grad[s]), own(z[s])))
+    want = own(base)
+    for lo in range(0, T - 5, rows):
+        part = slice(lo, lo + rows)
+        for got, each in zip((index[part], weights.detach()[part], grad[part]), want):
+            other = (got != each).any(-1)
+            for s in new:  # (rows of their own, compared above)
+                other[max(s.start - lo, 0):max(s.stop - lo, 0)] = False
+            assert not other.any()
