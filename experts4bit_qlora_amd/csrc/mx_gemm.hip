@@ -9,13 +9,21 @@ namespace e4b {
 
 namespace {
 
+// A launch holds fewer than 2^32 work items: 2^26 chunks of the rows' kernel (32 threads each) and 2^24 workgroups of
+// 256 threads are taken per launch at most.
+constexpr int64_t kRowChunks = int64_t(1) << 26, kWorkgroups = (int64_t(1) << 24) - 8;
+
 template <int DT>
 void launch_rows(const MxGemmArgs& a, hipStream_t s) {
-  const int64_t row_chunks = mx_chunks(a.w.k), chunks = a.M * row_chunks;
+  const int64_t row_chunks = mx_chunks(a.w.k), most = kRowChunks / row_chunks;  // (k below 2^24: at least 2^10 rows)
   constexpr int kPer = kMxRowThreads / (kMxChunk / 8);
-  hipLaunchKernelGGL(mx_rows_kernel<DT>, dim3(static_cast<unsigned>((chunks + kPer - 1) / kPer)), dim3(kMxRowThreads), 0, s,
-                     a.x, static_cast<int>(a.w.k), static_cast<uint32_t>(row_chunks), static_cast<uint32_t>(chunks),
-                     reinterpret_cast<uint32_t*>(a.a), a.as);
+  for (int64_t row = 0; row < a.M; row += most) {
+    const int64_t chunks = std::min(most, a.M - row) * row_chunks, first = row * row_chunks;
+    hipLaunchKernelGGL(mx_rows_kernel<DT>, dim3(static_cast<unsigned>((chunks + kPer - 1) / kPer)), dim3(kMxRowThreads), 0, s,
+                       static_cast<const uint16_t*>(a.x) + row * a.w.k, static_cast<int>(a.w.k),
+                       static_cast<uint32_t>(row_chunks), static_cast<uint32_t>(chunks),
+                       reinterpret_cast<uint32_t*>(a.a) + first * (kMxChunk / 8), a.as + first * (kMxChunk / kMxBlock));
+  }
 }
 
 int group_tiles(const MxTiling& tl, int size) { return size > tl.lo && size <= tl.hi ? (size + tl.tm - 1) / tl.tm : 0; }

@@ -99,3 +99,33 @@ def test_gate_of_more_work_items_than_a_launch_holds():
             for s in new:  # (rows of their own, compared above)
                 other[max(s.start - lo, 0):max(s.stop - lo, 0)] = False
             assert not other.any()
+
+
+def test_product_of_more_chunks_than_a_launch_quantizes():
+    """2^27 chunks of 256 values and more (64 GiB of rows): every row against one call of the rows that repeat, new ones
+    where one launch may end and at the end."""
+    n, k, rows = 40, 32768, 1 << 12
+    M = (1 << 20) + 77
+    b, s = _bytes(1, n, k // 2), _bytes(1, n, k // 32, lo=120, hi=130)
+    ids = torch.tensor([0], device=DEV)
+    base = torch.randn(rows, k, device=DEV, dtype=torch.bfloat16)
+    x = base.repeat(257, 1)[:M]
+    new = [slice(r - 3, r + 4) for r in (1 << 18, 1 << 19, (1 << 19) + (1 << 18))] + [slice(M - 7, M)]
+    for part in new:
+        x[part] = torch.randn(7, k, device=DEV, dtype=torch.bfloat16)
+    out = e4b.gemm_mxfp4_grouped(x, b, s, [M], ids, act_quant="mxfp4")
+
+    def own(part):  # beside zero rows without an expert, enough for 256-row tiles, whose order of sums is the large call's
+        more = torch.zeros(50_000, k, device=DEV, dtype=torch.bfloat16)
+        return e4b.gemm_mxfp4_grouped(torch.cat([part, more]), b, s, [len(part), len(more)],
+                                      torch.tensor([0, -1], device=DEV), act_quant="mxfp4")[:len(part)]
+
+    want = own(base)
+    for part in new:
+        assert torch.equal(out[part], own(x[part.start - 300:part.stop])[300:])
+    for lo in range(0, M, rows):
+        got = out[lo:lo + rows]
+        other = (got != want[:got.shape[0]]).any(-1)
+        for part in new:
+            other[max(part.start - lo, 0):max(part.stop - lo, 0)] = False
+        assert not other.any()
