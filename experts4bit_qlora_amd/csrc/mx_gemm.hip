@@ -28,26 +28,34 @@ void launch_rows(const MxGemmArgs& a, hipStream_t s) {
 
 int group_tiles(const MxTiling& tl, int size) { return size > tl.lo && size <= tl.hi ? (size + tl.tm - 1) / tl.tm : 0; }
 
+// most: the workgroups of a launch, which stay and take all tiles; 0: one workgroup for every tile and column block,
+// in launches of as many groups as one holds. (No group alone passes that: one of more than 32 rows takes 256-row
+// tiles, unless its call has few tiles or its stack fewer than eight scale bytes, which are one column block.)
 template <class K>
-void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl, int columns, hipStream_t s,
-                  unsigned most = 0x7fffffff, int lds = 0) {
+void launch_tiles(K kernel, int threads, MxGemmArgs a, MxGroups& g, MxTiling tl, int columns, hipStream_t s, unsigned most = 0,
+                  int lds = 0) {
   a.tl = tl;
-  a.tl.one = 1;
-  int tiles = 0;
-  for (int i = 0; i < a.groups; ++i) {
-    g.tile[i] = static_cast<uint16_t>(tiles);
-    const int n = group_tiles(tl, g.off[i + 1] - g.off[i]);
-    tiles += n;
-    a.tl.one &= n == 1;
-  }
-  for (int i = a.groups; i <= kMxGroupsMax; ++i) g.tile[i] = static_cast<uint16_t>(tiles);
-  if (!tiles) return;
-  a.tiles = tiles;
   a.n_blocks = static_cast<int>((a.w.n + columns - 1) / columns);
-  const unsigned total = static_cast<unsigned>(tiles) * static_cast<unsigned>(a.n_blocks);
-  hipLaunchKernelGGL(kernel, dim3(std::min((total + 7) / 8 * 8, most)), dim3(threads), lds, s, a, g);
+  const int64_t fit = most ? int64_t(1) << 31 : kWorkgroups / a.n_blocks;
+  for (int from = 0; from < a.groups;) {
+    a.tl.one = from == 0;
+    a.tiles = 0;
+    int i = 0;
+    for (; i < a.groups; ++i) {
+      const int n = i < from ? 0 : group_tiles(tl, g.off[i + 1] - g.off[i]);
+      if (a.tiles && a.tiles + n > fit) break;
+      g.tile[i] = static_cast<uint16_t>(a.tiles);
+      a.tiles += n;
+      a.tl.one &= n == 1;
+    }
+    a.tl.one &= i == a.groups;
+    from = i;
+    for (; i <= kMxGroupsMax; ++i) g.tile[i] = static_cast<uint16_t>(a.tiles);
+    if (!a.tiles) return;
+    const unsigned total = (static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.n_blocks) + 7) / 8 * 8;
+    hipLaunchKernelGGL(kernel, dim3(most ? std::min(total, most) : total), dim3(threads), lds, s, a, g);
+  }
 }
-
 
 // Calls of at most kNarrowTiles tiles of 32 x 32 (2.5 for each workgroup that the card holds) take those alone: they
 // spread over the CUs and start at once, where a 256-row tile keeps one CU for ~10 us and longer. Both grow alike
@@ -88,7 +96,7 @@ void launch_groups(const MxGemmArgs& a, MxGroups& g, hipStream_t s) {
     MxGemmArgs d = a;
     d.run = most > kOnce ? static_cast<int>(run) : 1;
     const auto kernel = bf16 ? mx_narrow_kernel<ODT, E4B_BF16> : mx_narrow_kernel<ODT, E4B_FP16>;
-    launch_tiles(kernel, kNarrowThreads, d, g, {kMxTileM, 0, kAll, 0}, 32 * d.run, s, 0x7fffffff, static_cast<int>(lds));
+    launch_tiles(kernel, kNarrowThreads, d, g, {kMxTileM, 0, kAll, 0}, 32 * d.run, s, 0, static_cast<int>(lds));
     return;
   }
   if (bf16) launch_rows<E4B_BF16>(a, s);

@@ -129,3 +129,25 @@ def test_product_of_more_chunks_than_a_launch_quantizes():
         for part in new:
             other[max(part.start - lo, 0):max(part.stop - lo, 0)] = False
         assert not other.any()
+
+
+@pytest.mark.parametrize("size", (1, 17))
+def test_product_of_more_workgroups_than_a_launch_holds(size):
+    """512 groups times 2^16 column blocks and more, rows quantized inside the tiles and before them: groups of one
+    expert have the same rows and so the same outputs."""
+    n, k = (1 << 21) + 40, 32
+    b, s = _bytes(2, n, k // 2), _bytes(2, n, k // 32, lo=120, hi=130)
+    rows = torch.randn(2, size, k, device=DEV, dtype=torch.bfloat16)
+    ids = torch.arange(512, device=DEV) % 2
+    ids[300] = 2
+    sizes = [size] * 512
+    sizes[255], sizes[256] = 0, 0  # beside a launch's last group
+    x = torch.cat([rows[g % 2][:r] for g, r in enumerate(sizes)])
+    out = e4b.gemm_mxfp4_grouped(x, b, s, sizes, ids, act_quant="mxfp4")
+    want = e4b.gemm_mxfp4_grouped(rows.flatten(0, 1), b, s, [size] * 2, ids[:2], act_quant="mxfp4").view(2, size, n)
+    assert out.shape[0] == 510 * size and want.any()
+    at = 0
+    for g, r in enumerate(sizes):
+        got = out[at:at + r]
+        at += r
+        assert torch.equal(got, want[g % 2][:r]) if g != 300 else not got.any()
