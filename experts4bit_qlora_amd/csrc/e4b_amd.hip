@@ -542,7 +542,8 @@ int e4b_quantize_mxfp4(const void* x, int32_t dtype, int64_t values, void* block
   if (!x || !blocks || !scales) return fail(E4B_EINVAL, "x/blocks/scales pointer is NULL");
   if (!aligned16(x) || !aligned16(blocks)) return fail(E4B_EINVAL, "x and blocks must be 16-byte aligned");
   const int64_t pieces = values / 8, grid = cdiv(pieces, e4b::kMxThreads * e4b::kMxUnroll);
-  if (grid > 0x7fffffff) return fail(E4B_EUNSUPPORTED, "%lld values are more than one launch covers", (long long)values);
+  if (grid * e4b::kMxThreads >= int64_t(1) << 32)  // work items of a launch
+    return fail(E4B_EUNSUPPORTED, "%lld values are more than one launch covers", (long long)values);
   auto* c = static_cast<uint32_t*>(blocks);
   auto* e = static_cast<uint8_t*>(scales);
   const dim3 g(static_cast<unsigned>(grid)), b(e4b::kMxThreads);

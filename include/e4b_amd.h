@@ -127,7 +127,7 @@ int e4b_quantize_8bit(const float* values, const float* offset, int64_t rows, in
  * value the e2m1 code nearest to value / 2^(scales[b] - 127), ties to the even code, saturating at 6, a
  * zero without a sign. blocks is u8 [values / 2], first value of a pair
  * in the low nibble, scales u8 [values / 32]. A block with a NaN takes scale 0, one with an infinity 254;
- * a NaN's code is +6. x and blocks are 16-byte aligned.
+ * a NaN's code is +6. x and blocks are 16-byte aligned; up to 2^37 - 2^13 values.
  * Has no counterpart in the reference, which loads released MXFP4 bytes (formats/mxfp4.py:35-105). */
 int e4b_quantize_mxfp4(const void* x, int32_t dtype, int64_t values, void* blocks, void* scales, hipStream_t stream);
 

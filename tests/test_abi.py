@@ -389,3 +389,10 @@ def test_router_entry_points_reject_bad_arguments():
     back = lambda z=4096, c=4096, v=4096, g=4096, out=4096: L.e4b_balance_loss_backward(
         z, N.BF16, 2, 40, 8, None, 0, c, v, g, out, None)
     assert back(z=None) == back(c=None) == back(v=None) == back(g=None) == back(out=None) == -1
+
+
+def test_quantize_mxfp4_refuses_more_than_a_launch_covers():
+    """2^32 work items, each four pieces of eight values: refused before anything is launched."""
+    L = N.lib()
+    assert L.e4b_quantize_mxfp4(4096, N.BF16, 1 << 37, 4096, 4096, None) == -2 and "one launch" in _err()
+    assert L.e4b_quantize_mxfp4(4096, N.FP32, 1 << 42, 4096, 4096, None) == -2 and "one launch" in _err()
