@@ -3,8 +3,8 @@
 ``router_topk`` turns a router's logits into the ``(top_k_index, top_k_weights)`` that ``route`` and the
 expert modules take; ``balance_loss`` gives the auxiliary loss that keeps the experts in use, and the
 per-expert counts. On a HIP device each is a kernel each way (``csrc/gate.h``); tensors elsewhere, other
-dtypes, more than 1,024 experts or 64 choices, and tensors that a transform, a trace or forward-mode
-differentiation follows take the torch formulation, which is the definition.
+dtypes, more than 1,024 experts or 64 choices, rows (or a layer's choices) from 2^31 on, and tensors that a
+transform, a trace or forward-mode differentiation follows take the torch formulation, which is the definition.
 
 The reference leaves both to the models (its CPU engine restates the gate,
 ``experts4bit_qlora/engines/cpu_router.py:100-120``).
@@ -79,7 +79,7 @@ def router_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax_then_t
         raise ValueError(f"top_k={top_k} outside [1, {E}]")
     wd = logits.dtype if weight_dtype is None else weight_dtype
     code = N.SCORE_CHOSEN if renorm else _SCORING[scoring]
-    if not (E <= 1024 and top_k <= 64 and wd in ops._DT and _on_kernel(logits)):
+    if not (E <= 1024 and top_k <= 64 and logits.shape[:-1].numel() < 2 ** 31 and wd in ops._DT and _on_kernel(logits)):
         return _router_topk_torch(logits, top_k, code, wd)
     z = _aligned(logits) if logits.dim() == 2 else logits.reshape(-1, E).contiguous()
     if z.requires_grad and torch.is_grad_enabled():
@@ -156,7 +156,8 @@ def balance_loss(logits: torch.Tensor, top_k_index: torch.Tensor,
     if mask is not None and mask.dtype != torch.bool:
         mask = mask != 0
     layers = lead.numel()
-    if not (1 <= E <= 1024 and layers <= 65535 and _on_kernel(logits) and _on_kernel_index(top_k_index, mask)):
+    if not (1 <= E <= 1024 and layers <= 65535 and T * top_k_index.shape[-1] < 2 ** 31 and _on_kernel(logits)
+            and _on_kernel_index(top_k_index, mask)):
         return _balance_loss_torch(logits, top_k_index, mask)
     z = _aligned(logits) if len(lead) == 1 else logits.reshape(layers, T, E).contiguous()
     index = top_k_index if top_k_index.dtype == torch.int64 else top_k_index.to(torch.int64)

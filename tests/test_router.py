@@ -148,3 +148,23 @@ def test_balance_values_behind_the_mask_have_no_influence(dtype):
             outs.append((loss, counts, torch.autograd.grad(loss.sum(), leaf)[0]))
         assert all(torch.equal(a, b) for a, b in zip(*outs))
         assert not outs[1][2][(mask == 0).expand(2, 20)].any() and outs[1][2].any()
+
+
+def test_sizes_beyond_the_kernels_take_the_torch_formulation(monkeypatch):
+    """Choices and tokens that pass the kernels' 32 bits: broadcast tensors of one element, seen as device tensors."""
+    from experts4bit_qlora_amd import router as R
+
+    seen = []
+    monkeypatch.setattr(R, "_on_kernel", lambda t: True)
+    monkeypatch.setattr(R, "_aligned", lambda t: t)  # nothing of this size is made
+    monkeypatch.setattr(R.ops, "balance_loss", lambda *a: seen.append("kernel") or (torch.zeros(1), torch.zeros(1, 4), None, None))
+    monkeypatch.setattr(R.ops, "router_topk", lambda *a: seen.append("kernel") or (torch.zeros(1, 1), torch.zeros(1, 1)))
+    monkeypatch.setattr(R, "_balance_loss_torch", lambda *a: seen.append("torch"))
+    monkeypatch.setattr(R, "_router_topk_torch", lambda *a: seen.append("torch"))
+    z, index = torch.zeros(1, 1, 4), torch.zeros(1, 1, 1, dtype=torch.int64)
+    e4b.balance_loss(z, index)
+    e4b.balance_loss(z.expand(1, 1 << 29, 4), index.expand(1, 1 << 29, 4))
+    e4b.balance_loss(z.expand(1, 1 << 31, 4), index.expand(1, 1 << 31, 1))
+    e4b.router_topk(z[0], 1)
+    e4b.router_topk(z[0].expand(1 << 31, 4), 1)
+    assert seen == ["kernel", "torch", "torch", "kernel", "torch"]
