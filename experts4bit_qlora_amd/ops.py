@@ -81,9 +81,8 @@ class QW:
 
     def __setattr__(self, name, value):  # a changed field invalidates the cached descriptor
         d = self.__dict__
-        if "_struct" in d:
-            del d["_struct"]
-            d.pop("_ref", None)
+        d.pop("_struct", None)
+        d.pop("_ref", None)
         d[name] = value
 
     def struct(self) -> N.QWeight:

@@ -357,3 +357,18 @@ def test_mxfp4_scale_is_the_floor_of_the_logarithm():
     assert np.array_equal(scales.numpy(), os_) and np.array_equal(codes.numpy(), ob.reshape(len(top), 16))
     for value, byte in ((float("inf"), 254), (float("nan"), 0), (0.0, 0)):
         assert Q._quantize_mxfp4_torch(torch.full((32,), value))[1].item() == byte
+
+
+def test_weight_descriptor_follows_every_field():
+    """An assigned field drops the descriptor and its reference, also where another thread's assignment fell between
+    the two being kept."""
+    from experts4bit_qlora_amd import ops
+
+    t = [torch.zeros(4, dtype=torch.uint8) for _ in range(3)]
+    qw = ops.mxfp4_qweight(torch.zeros(1, 2, 16, dtype=torch.uint8), torch.zeros(1, 2, 1, dtype=torch.uint8), 2, 32)
+    for bias in t[:2]:
+        qw.bias = bias
+        assert qw.ref()._obj.bias == qw.struct().bias == bias.data_ptr()
+    del qw.__dict__["_struct"]
+    qw.bias = t[2]
+    assert qw.ref()._obj.bias == t[2].data_ptr()
