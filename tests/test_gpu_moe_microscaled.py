@@ -98,6 +98,70 @@ def test_layer(tokens, E, k, hidden, inter, dtype):
     assert (grad.double().cpu() - want).abs().max() <= 4 * hidden * tokens * 2.0 ** -23 * top
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("tokens,E,k,hidden,inter", [(1, 8, 2, 128, 96), (7, 5, 3, 96, 160), (150, 4, 2, 288, 128)])
+def test_layer_gradients_of_gate_and_loss(tokens, E, k, hidden, inter, dtype):
+    """The logits' gradient through the experts' weighted sum, through the balance loss and through both, against the
+    formulas in 64 bits on the same logits and expert outputs, element by element; the loss is weighted (by a power of
+    two) so that either part is far above the bound of their sum, so a sum without one of them, or with its sign
+    changed, is refused.
+
+    Bounds, with u = 2^-24 and `reach` the relative error of a probability, (largest distance from a row's maximum + E
+    + 8) u: a weight's gradient is torch's sum of `hidden` rounded products, (hidden + 1) u of their magnitudes (dg);
+    the gate turns it into w (g - mean), off by w (dg + mean of dg) and by w (|g| + mean of |g|) (3 reach + (k + 4) u);
+    the loss's part f p (c - dot) is off by f p (c + dot) (3 reach + 8 u). Each is rounded once, their sum once more;
+    products of these errors are below 2^-10 of them."""
+    layer = _Layer(E, hidden, inter, k, dtype, tokens + 40)
+    g = torch.Generator(device=DEV).manual_seed(tokens + 41)
+    x = torch.randn(tokens, hidden, generator=g, device=DEV).to(dtype)
+    mask = torch.rand(tokens, generator=g, device=DEV) < 0.8
+    mask[0] = True
+    logits = torch.nn.functional.linear(x.float(), layer.router).detach().requires_grad_()
+    index, weights = e4b.router_topk(logits, k, renorm=True)
+    loss, counts = e4b.balance_loss(logits[None], index[None], mask)
+    sizes, seen = torch.bincount(index.flatten(), minlength=E).tolist(), []
+    out = layer.experts(x, index, weights, sizes, seen)
+    down = seen[1][1]
+    into = torch.randn(tokens, hidden, generator=g, device=DEV) / down.float().square().mean().sqrt()
+
+    u = 2.0 ** -24
+    z = logits.detach().double().cpu()
+    chosen = torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :k]
+    each = torch.zeros(tokens * k, hidden, dtype=torch.float64)
+    each[torch.sort(chosen.flatten(), stable=True).indices] = down.double().cpu()
+    terms = each.view(tokens, k, hidden) * into.double().cpu().unsqueeze(1)
+    gw, dg = terms.sum(-1), (hidden + 1) * u * terms.abs().sum(-1)
+    p = torch.softmax(z, -1)
+    w = p.gather(-1, chosen)
+    w = w / w.sum(-1, keepdim=True)
+    reach = ((z.amax(-1, keepdim=True) - z).amax() + E + 8) * u
+    on = lambda v: torch.zeros_like(z).scatter(-1, chosen, v)
+    mean = lambda v: (w * v).sum(-1, keepdim=True)
+    gate = on(w * (gw - mean(gw)))
+    gate_off = on(w * (dg + mean(dg)) + w * (gw.abs() + mean(gw.abs())) * (3 * reach + (k + 4) * u)) + u * gate.abs()
+    valid = mask.cpu()
+    n, c = valid.sum().double(), torch.bincount(chosen[valid].flatten(), minlength=E).double()
+    dot = (p * c).sum(-1, keepdim=True)
+    f = E / n ** 2 * valid.double().unsqueeze(-1)
+    balance = f * p * (c - dot)
+    alpha = 2.0 ** round(torch.log2(gate.abs().max() / balance.abs().max()).item())
+    balance = alpha * balance
+    balance_off = alpha * f * p * (c + dot) * (3 * reach + 8 * u) + u * balance.abs()
+
+    def off(want, bound):  # whether an element is further off than its bound (2^-149: below fp32's normal range)
+        return ((got.double().cpu() - want).abs() > bound * (1 + 2.0 ** -10) + 2.0 ** -149).any()
+
+    (got,) = torch.autograd.grad(out, logits, into, retain_graph=True)
+    assert not off(gate, gate_off)
+    (got,) = torch.autograd.grad(alpha * loss.sum(), logits, retain_graph=True)
+    assert not off(balance, balance_off)
+    (got,) = torch.autograd.grad([out, alpha * loss.sum()], logits, [into, torch.ones((), device=DEV)])
+    bound = gate_off + balance_off + u * (gate + balance).abs()
+    assert not off(gate + balance, bound)
+    assert off(gate, bound) and off(balance, bound) and off(gate - balance, bound) and off(balance - gate, bound)
+    assert off(gate + 1.01 * balance, bound) and off(1.01 * gate + balance, bound)
+
+
 def test_layer_replayed():
     """The layer captured with fixed group sizes (every token to every expert), replayed on new inputs between
     eager runs."""
