@@ -151,3 +151,18 @@ def test_product_of_more_workgroups_than_a_launch_holds(size):
         got = out[at:at + r]
         at += r
         assert torch.equal(got, want[g % 2][:r]) if g != 300 else not got.any()
+
+
+@pytest.mark.parametrize("k", (64, 288))
+def test_product_outputs_of_small_groups(k):
+    """More than 2^31 outputs with the last ones written by 32-row tiles: more than 32 small groups behind a large one
+    take a launch of their own (in test_product_outputs the 256-row tiles take all rows)."""
+    n, sizes = 8200, [280_000] + [30] * 33
+    M = sum(sizes)
+    assert 280_000 * n > 2 ** 31
+    b, s = _bytes(2, n, k // 2), _bytes(2, n, k // 32, lo=120, hi=130)
+    a = torch.randn(M, k, device=DEV, dtype=torch.bfloat16)
+    ids = torch.arange(34, device=DEV) % 2
+    out = e4b.gemm_mxfp4_grouped(a, b, s, sizes, ids, act_quant="mxfp4")
+    part = e4b.gemm_mxfp4_grouped(a[280_000:].clone(), b, s, sizes[1:], ids[1:], act_quant="mxfp4")
+    assert torch.equal(out[280_000:], part)

@@ -371,3 +371,23 @@ def test_short_rows_in_large_groups(k, n, E):
     sizes, ids = [300, 45], [E - 1, 0]
     a = _rows(sum(sizes), k, torch.bfloat16, k + n + 1)
     _check_both(a, b, s, sizes, ids)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("k", (32, 96, 224, 256, 288, 1216, 2880))
+@pytest.mark.parametrize("sizes", ([1], [4, 0, 1, 3], [8, 5], [0, 7, 1, 2]))
+def test_rows_quantized_inside_the_tiles_and_before_them(sizes, k, dtype):
+    """Small groups, whose tiles quantize the rows themselves, and the same rows beside a group of more rows than a tile
+    holds, for which all are quantized before the product (test_few_rows adds five rows, which the tiles still
+    take): the same bytes."""
+    E, n = 3, 72
+    b, s = _weights(E, n, k, k)
+    ids = [2, 1, 0, 2][:len(sizes)]
+    a = _rows(sum(sizes) + 40, k, dtype, k + 9)
+    a[0, :32] = 0
+    few = a[:sum(sizes)]
+    out = _run(few, b, s, sizes, ids)
+    _check(few, b, s, sizes, ids, out)
+    all_rows = _run(a, b, s, sizes + [40], ids + [1])
+    _check(a, b, s, sizes + [40], ids + [1], all_rows)
+    assert torch.equal(all_rows[:len(few)], out)
