@@ -79,7 +79,7 @@ def router_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax_then_t
         raise ValueError(f"top_k={top_k} outside [1, {E}]")
     wd = logits.dtype if weight_dtype is None else weight_dtype
     code = N.SCORE_CHOSEN if renorm else _SCORING[scoring]
-    if not (E <= 1024 and top_k <= 64 and logits.shape[:-1].numel() < 2 ** 31 and wd in ops._DT and _on_kernel(logits)):
+    if not (E <= 1024 and top_k <= 64 and logits.numel() < E << 31 and wd in ops._DT and _on_kernel(logits)):
         return _router_topk_torch(logits, top_k, code, wd)
     z = _aligned(logits) if logits.dim() == 2 else logits.reshape(-1, E).contiguous()
     if z.requires_grad and torch.is_grad_enabled():
