@@ -109,7 +109,7 @@ constexpr int kMxUnroll = 4;  // pieces per thread, their loads in flight togeth
 //
 // Bound by HBM: 2 bytes of a bf16 value read, 17 / 32 written. A quad of lanes holds one block, so a
 // wave's loads and its code stores are contiguous. 32 experts of 5,760 x 2,880 in bf16 (1.34 GB): at the rate of a
-// large copy, 4.9 TB/s.
+// large copy, 4.9 TB/s; in fp32 (2.4 GB) 453 us, 5.3 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(kMxThreads) mx_quantize_kernel(const void* __restrict__ x, int64_t pieces,
                                                                  uint32_t* __restrict__ codes,

@@ -411,9 +411,10 @@ E4B_DEV void mx_store_part(__amdgpu_buffer_rsrc_t out, uint32_t offset, uint32_t
 // The workgroups (one per CU) stay, and the chunks of a workgroup's tiles are one stream: the first chunks of its
 // next tile are loaded while the last ones of this tile are computed, and a tile's stores drain while the next one
 // is computed.
-// 16,384 rows over 32 experts of 5,760 x 2,880: 246 us, 2.2 PFLOP/s. The products alone take 117 us (the card's
-// power limit: 105 for a loop of these instructions on random operands), 139 with the LDS reads; the loads and
-// LDS stores of the chunks bring it to 200, the output's 189 MB to 246. Tried against it: 128 x 256 tiles, two
+// 16,384 rows over 32 experts of 5,760 x 2,880: 242 to 250 us on most cards, medians of 270 to 290 on some (1.9 to 2.2
+// PFLOP/s). On one of the former the products alone take 117 us (the card's power limit: 105 for a loop of these
+// instructions on random operands), 139 with the LDS reads; the loads and LDS stores of the chunks bring it to 200, the
+// output's 189 MB to 246. Tried against it: 128 x 256 tiles, two
 // workgroups per CU, 270 us; the same tiles without persistent workgroups 258; fewer row blocks for the last,
 // mostly empty row tile of a group 250 (such a tile waits for its weights all the same).
 constexpr int kMxWideM = 256, kMxWideN = 256;

@@ -241,7 +241,8 @@ size_t e4b_mx_gemm_workspace_bytes(int64_t rows, int64_t k);
  * with an infinity or a NaN makes that row NaN, a weight scale byte of 255 its column's sums; rows of an id
  * outside [0, E) are zero. sizes is a host array, read before the call returns; groups <= 512. w is MXFP4, k a
  * multiple of 32, w->bias is not read; a, out and workspace are 16-byte aligned. n < 2^22, k < 2^24, at most 2^23
- * rows (2^20 for stacks of fewer than eight scale bytes), fewer than 2^31 chunks of 256 values. Nothing past the last row is written. A
+ * rows (2^20 for stacks of fewer than eight scale bytes), fewer than 2^31 chunks of 256 values and tiles of 32 x 32
+ * outputs. Nothing past the last row is written. A
  * captured graph keeps the sizes; the ids may change between replays. The workspace holds the rows' codes until the
  * product has run: calls that may overlap (other streams, graphs replayed side by side) need one each.
  * The product of mxfp4_grouped.gemm_mxfp4_grouped (engines/nvme_experts.py:852-865) on the block-scaled
