@@ -15,6 +15,7 @@ from .formats.mxfp4 import dequantize_mxfp4
 from .lora import ExpertsLoRA
 from .arch.deepseek_v4 import DeepseekV4Experts4bit, DeepseekV4ExpertsNbit
 from .arch.gptoss import GptOssExperts4bit, GptOssExpertsMxfp4, GptOssExpertsNbit
+from .losses import distill_loss, policy_loss, preference_loss, token_logprobs
 from .ops import gemm_4bit_grouped, gemm_mxfp4_grouped
 from .quant import quantize_mxfp4
 from .router import balance_loss, router_topk
@@ -35,12 +36,16 @@ __all__ = [
     "dequantize_mxfp4",
     "disable_fast",
     "disable_fast_train",
+    "distill_loss",
     "enable_fast",
     "enable_fast_train",
     "fast_available",
     "gemm_4bit_grouped",
     "gemm_mxfp4_grouped",
     "normalize_quant_type",
+    "policy_loss",
+    "preference_loss",
     "quantize_mxfp4",
     "router_topk",
+    "token_logprobs",
 ]

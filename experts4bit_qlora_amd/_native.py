@@ -23,6 +23,8 @@ EPI_NONE, EPI_SWIGLU, EPI_ACT, EPI_CLAMP_SWIGLU, EPI_GPTOSS = 0, 1, 2, 3, 4
 # e4b_probe_site: launch sites of the prefill path that e4b_set_probe can watch
 PROBE_OFF, PROBE_GATE_UP_BIG, PROBE_GATE_UP_TAIL, PROBE_DOWN_BIG, PROBE_DOWN_TAIL = 0, 1, 2, 3, 4
 SCORE_ALL, SCORE_CHOSEN = 0, 1
+PREFERENCE_SIGMOID, PREFERENCE_HINGE, PREFERENCE_IPO = 0, 1, 2
+REDUCE_NONE, REDUCE_SEQUENCE, REDUCE_MEAN = 0, 1, 2
 PATH_AUTO, PATH_GEMV, PATH_MFMA = 0, 1, 2
 NOALLOC_WORKSPACE_BYTES = 64 << 20  # E4B_NOALLOC_WORKSPACE_BYTES
 
@@ -43,6 +45,11 @@ EXPORTS = (
     "e4b_balance_workspace_bytes",
     "e4b_balance_loss",
     "e4b_balance_loss_backward",
+    "e4b_token_logprobs",
+    "e4b_preference_loss",
+    "e4b_policy_loss",
+    "e4b_distill_loss",
+    "e4b_loss_backward",
     "e4b_route_groups",
     "e4b_gather_rows",
     "e4b_grouped_gemm",
@@ -126,6 +133,23 @@ class Routing(ctypes.Structure):
     ]
 
 
+class Logits(ctypes.Structure):
+    """``e4b_logits``: logits ``[seqs, tokens, vocab]`` by their strides (elements), labels and mask."""
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("seqs", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("seq_stride", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("labels", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _load_error: str | None = None
 
@@ -163,6 +187,17 @@ def _bind(L):
     L.e4b_balance_loss.argtypes = [P, I32, I32, I64, I32, P, I32, P, I64, P, ctypes.c_size_t, P, P, P, P]
     L.e4b_balance_loss_backward.restype = ctypes.c_int
     L.e4b_balance_loss_backward.argtypes = [P, I32, I32, I64, I32, P, I64, P, P, P, P, P]
+    LG, PAIR = ctypes.POINTER(Logits), ctypes.POINTER(ctypes.c_int64)
+    L.e4b_token_logprobs.restype = ctypes.c_int
+    L.e4b_token_logprobs.argtypes = [LG, P, P, P]
+    L.e4b_preference_loss.restype = ctypes.c_int
+    L.e4b_preference_loss.argtypes = [LG, P, I32, I32, F32, F32, I32, P, P, P, P, P]
+    L.e4b_policy_loss.restype = ctypes.c_int
+    L.e4b_policy_loss.argtypes = [LG, P, P, I32, P, F32, F32, F32, I32, P, P, P, P, P, P, P]
+    L.e4b_distill_loss.restype = ctypes.c_int
+    L.e4b_distill_loss.argtypes = [LG, P, I32, P, I32, I32, P, P, P, P, P, P]
+    L.e4b_loss_backward.restype = ctypes.c_int
+    L.e4b_loss_backward.argtypes = [LG, P, P, I64, PAIR, P, PAIR, P, I64, P, P, I32, P, P]
     L.e4b_route_groups.restype = ctypes.c_int
     L.e4b_route_groups.argtypes = [ctypes.POINTER(ctypes.c_int64), I32, P, I32, RT, P]
     L.e4b_gather_rows.restype = ctypes.c_int

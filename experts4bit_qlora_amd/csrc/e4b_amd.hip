@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -25,6 +26,7 @@
 #include "gemv.h"
 #include "lora.h"
 #include "lora_mfma.h"
+#include "losses_launch.h"
 #include "mx.h"
 #include "mx_launch.h"
 #include "quantize.h"
@@ -277,6 +279,55 @@ int check_balance(int32_t dtype, int32_t layers, int64_t tokens, int32_t num_exp
   a.E = num_experts;
   a.mask_stride = mask_stride;
   return E4B_OK;
+}
+
+// A batch of vocabulary logits; rows = seqs * tokens.
+int check_logits(const e4b_logits* z, bool labels, const void* stats) {
+  if (!z) return fail(E4B_EINVAL, "logits descriptor is NULL");
+  if (!any_dtype_ok(z->dtype)) return fail(E4B_EINVAL, "bad dtype %d", z->dtype);
+  if (z->seqs < 0 || z->tokens < 0 || z->seq_stride < 0 || z->row_stride < 0 || z->mask_stride < 0)
+    return fail(E4B_EINVAL, "negative sizes or strides");
+  if (z->vocab < 1 || z->vocab > e4b::kLossMaxVocab)
+    return fail(E4B_EUNSUPPORTED, "vocab=%lld outside [1, 2^30]", (long long)z->vocab);
+  if (z->seqs > e4b::kLossMaxSeqs || (z->tokens && z->seqs > 0x7fffffffLL / z->tokens))
+    return fail(E4B_EUNSUPPORTED, "seqs exceeds 2^21 or seqs*tokens int32");
+  const float k = 1.4426950408889634f / z->temperature;
+  if (!(z->temperature > 0.0f) || !std::isnormal(k) || !std::isnormal(1.0f / z->temperature))
+    return fail(E4B_EINVAL, "temperature must be positive, it and its inverse finite");
+  if (z->seqs * z->tokens > 0 && (!z->logits || (labels && !z->labels) || !stats))
+    return fail(E4B_EINVAL, "logits/labels/stats is NULL");
+  if (reinterpret_cast<uintptr_t>(stats) & 7) return fail(E4B_EINVAL, "stats must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(z->logits) & (z->dtype == E4B_FP32 ? 3 : 1))
+    return fail(E4B_EINVAL, "logits are not aligned to their dtype");
+  return E4B_OK;
+}
+
+e4b::LossArgs loss_args(const e4b_logits& z, float* stats) {
+  e4b::LossArgs a{};
+  a.z = z;
+  a.scale2 = 1.4426950408889634f / z.temperature;
+  a.stats = reinterpret_cast<float2*>(stats);
+  return a;
+}
+
+// The join of the tokens' losses, and what it needs.
+int check_reduction(const e4b_logits& z, int32_t reduction, const float* token_loss, const float* loss, const float* inv) {
+  if (reduction < E4B_REDUCE_NONE || reduction > E4B_REDUCE_MEAN) return fail(E4B_EINVAL, "bad reduction %d", reduction);
+  if (reduction != E4B_REDUCE_NONE && (reduction == E4B_REDUCE_MEAN || z.seqs) && (!loss || !inv))
+    return fail(E4B_EINVAL, "loss/inv is NULL");
+  if (z.seqs * z.tokens > 0 && !token_loss) return fail(E4B_EINVAL, "token_loss is NULL");
+  return E4B_OK;
+}
+
+int reduce_tokens(const e4b_logits& z, int32_t reduction, const float* token_loss, const float* stats, float* loss,
+                  float* inv, hipStream_t stream) {
+  if (reduction == E4B_REDUCE_NONE) return E4B_OK;
+  const bool all = reduction == E4B_REDUCE_MEAN;
+  const e4b::MeanArgs m{token_loss, reinterpret_cast<const float2*>(stats), all ? 1 : z.seqs,
+                        all ? z.seqs * z.tokens : z.tokens, loss, inv};
+  if (m.groups == 0) return E4B_OK;
+  e4b::launch_loss_mean(m, stream);
+  return check_launch("loss_mean_kernel");
 }
 
 size_t mx_row_bytes(int64_t k) { return size_t(e4b::mx_chunks(k)) * (e4b::kMxChunk / 2); }
@@ -709,6 +760,125 @@ int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers,
   a.grad = grad_logits;
   e4b::launch_balance_backward(a, stream);
   return check_launch("balance_backward_kernel");
+}
+
+int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream) {
+  float2 none;  // stats may be NULL here
+  const int rc = check_logits(z, true, stats ? static_cast<const void*>(stats) : &none);
+  if (rc || z->seqs * z->tokens == 0) return rc;
+  if (!logps) return fail(E4B_EINVAL, "logps is NULL");
+  e4b::LossArgs a = loss_args(*z, stats);
+  a.logps = logps;
+  e4b::launch_loss_rows(e4b::kLogprobs, a, stream);
+  return check_launch("loss_rows_kernel");
+}
+
+int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_token, int32_t kind, float beta,
+                        float smoothing, int32_t average, float* loss, float* rewards, float* stats, float* coef,
+                        hipStream_t stream) {
+  int rc = check_logits(z, true, stats);
+  if (rc) return rc;
+  if (z->seqs % 2) return fail(E4B_EINVAL, "seqs=%lld is odd", (long long)z->seqs);
+  if (kind < E4B_PREFERENCE_SIGMOID || kind > E4B_PREFERENCE_IPO) return fail(E4B_EINVAL, "bad preference kind %d", kind);
+  if (!(beta > 0.0f) || !std::isfinite(beta)) return fail(E4B_EINVAL, "beta must be positive and finite");
+  if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return fail(E4B_EINVAL, "smoothing outside [0, 1]");
+  if (z->seqs == 0) return E4B_OK;
+  if (!loss || !rewards || !coef) return fail(E4B_EINVAL, "loss/rewards/coef is NULL");
+  e4b::LossArgs a = loss_args(*z, stats);
+  if (z->tokens) e4b::launch_loss_rows(e4b::kStats, a, stream);
+  const e4b::PairArgs p{*z, a.stats, ref, ref_per_token, kind, beta, smoothing, average, loss, rewards, coef};
+  e4b::launch_pairs(p, stream);
+  return check_launch("pairs_kernel");
+}
+
+int e4b_policy_loss(const e4b_logits* z, const float* old_logps, const float* advantages, int32_t adv_per_token,
+                    const float* ref_logps, float clip_lo, float clip_hi, float kl_coef, int32_t reduction, float* logps,
+                    float* token_loss, float* stats, float* coef, float* loss, float* inv, hipStream_t stream) {
+  int rc = check_logits(z, true, stats);
+  if (!rc) rc = check_reduction(*z, reduction, token_loss, loss, inv);
+  if (rc) return rc;
+  if (!(clip_lo <= clip_hi)) return fail(E4B_EINVAL, "clip_lo > clip_hi");
+  if (!std::isfinite(kl_coef)) return fail(E4B_EINVAL, "kl_coef is not finite");
+  if (z->seqs * z->tokens) {
+    if (!old_logps || !advantages || !logps || !coef) return fail(E4B_EINVAL, "old_logps/advantages/logps/coef is NULL");
+    e4b::LossArgs a = loss_args(*z, stats);
+    a.logps = logps;
+    a.old_logps = old_logps;
+    a.advantages = advantages;
+    a.adv_per_token = adv_per_token;
+    a.ref_logps = ref_logps;
+    a.clip_lo = clip_lo;
+    a.clip_hi = clip_hi;
+    a.kl_coef = kl_coef;
+    a.token_loss = token_loss;
+    a.coef = coef;
+    e4b::launch_loss_rows(e4b::kPolicy, a, stream);
+    rc = check_launch("loss_rows_kernel");
+    if (rc) return rc;
+  }
+  return reduce_tokens(*z, reduction, token_loss, stats, loss, inv, stream);
+}
+
+int e4b_distill_loss(const e4b_logits* z, const void* teacher, int32_t teacher_dtype, const int64_t* index, int32_t top,
+                     int32_t reduction, float* share, float* token_loss, float* stats, float* loss, float* inv,
+                     hipStream_t stream) {
+  int rc = check_logits(z, false, stats);
+  if (!rc) rc = check_reduction(*z, reduction, token_loss, loss, inv);
+  if (rc) return rc;
+  if (!any_dtype_ok(teacher_dtype)) return fail(E4B_EINVAL, "bad teacher_dtype %d", teacher_dtype);
+  if (top < 1) return fail(E4B_EINVAL, "top=%d < 1", top);
+  if (top > e4b::kLossMaxTop) return fail(E4B_EUNSUPPORTED, "top=%d > %d", top, e4b::kLossMaxTop);
+  if (z->seqs * z->tokens) {
+    if (!teacher || !index || !share) return fail(E4B_EINVAL, "teacher/index/share is NULL");
+    e4b::LossArgs a = loss_args(*z, stats);
+    a.z.labels = nullptr;
+    a.teacher = teacher;
+    a.teacher_dtype = teacher_dtype;
+    a.index = index;
+    a.top = top;
+    a.share = share;
+    a.token_loss = token_loss;
+    e4b::launch_loss_rows(e4b::kDistill, a, stream);
+    rc = check_launch("loss_rows_kernel");
+    if (rc) return rc;
+  }
+  return reduce_tokens(*z, reduction, token_loss, stats, loss, inv, stream);
+}
+
+int e4b_loss_backward(const e4b_logits* z, const float* stats, const float* grad_loss, int64_t grad_seqs,
+                      const int64_t grad_strides[2], const float* coef, const int64_t coef_strides[2], const float* inv,
+                      int64_t inv_stride, const int64_t* index, const float* share, int32_t top, void* grad_logits,
+                      hipStream_t stream) {
+  const int rc = check_logits(z, !index, stats);
+  if (rc || z->seqs * z->tokens == 0) return rc;
+  if (!grad_loss || !grad_strides || !grad_logits || (coef && !coef_strides))
+    return fail(E4B_EINVAL, "grad_loss/grad_logits or strides are NULL");
+  if (grad_seqs < 1) return fail(E4B_EINVAL, "grad_seqs must be positive");
+  if (index && (!share || top < 1)) return fail(E4B_EINVAL, "share is NULL or top < 1");
+  if (index && top > e4b::kLossMaxTop) return fail(E4B_EUNSUPPORTED, "top=%d > %d", top, e4b::kLossMaxTop);
+  if (!aligned16(grad_logits)) return fail(E4B_EINVAL, "grad_logits must be 16-byte aligned");
+  e4b::LossBackwardArgs a{};
+  a.z = *z;
+  a.scale2 = 1.4426950408889634f / z->temperature;
+  a.stats = reinterpret_cast<const float2*>(stats);
+  a.grad_loss = grad_loss;
+  a.grad_seqs = grad_seqs;
+  a.grad_ns = grad_strides[0];
+  a.grad_ts = grad_strides[1];
+  a.coef = coef;
+  if (coef) {
+    a.coef_ns = coef_strides[0];
+    a.coef_ts = coef_strides[1];
+  }
+  a.inv = inv;
+  a.inv_ns = inv_stride;
+  a.slope = index ? z->temperature : -1.0f / z->temperature;
+  a.index = index;
+  a.share = share;
+  a.top = top;
+  a.grad = grad_logits;
+  e4b::launch_loss_backward(a, stream);
+  return check_launch("loss_backward_kernel");
 }
 
 int e4b_route_groups(const int64_t* sizes, int32_t groups, const int64_t* expert_ids, int32_t num_experts,

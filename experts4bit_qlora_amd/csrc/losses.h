@@ -1,0 +1,478 @@
+// Losses over the vocabulary: log-probabilities of labels, preference pairs, the clipped policy loss, distillation
+// from a teacher's top logits, forward and backward.
+//
+// A row of logits z [V] at temperature tau: y = z / tau, m = max z, s = sum_j exp((z_j - m) / tau),
+// q_j = exp((z_j - m) / tau) / s, and for its label l
+//   lp = (z_l - m) / tau - log s,                    dlp / dz_j = ([j = l] - q_j) / tau.
+// Policy, r = exp(lp - old):  loss = -min(r A, clip(r) A) + kl (e^x - x - 1), x = ref - lp,
+//   dloss / dlp = -A r [r A <= clip(r) A] + kl (1 - e^x).
+// Teacher with probabilities p_k at the indices i_k:  loss = tau^2 sum_k p_k (log p_k - log q_{i_k}),
+//   dloss / dz_j = tau (q_j - sum of p_k with i_k = j).
+// Preference, S = sum of a sequence's lp (or their mean), d = (S_c - r_c) - (S_r - r_r):  a loss of d, whose slope is
+// every chosen token's dloss / dlp and, negated, every rejected one's.
+//
+// One workgroup takes a row: its threads run over 16-byte pieces with a running maximum and sum each, which are then
+// joined; a row's logits are read once in the forward and once in the backward, tokens that do not count are not
+// read. Differences to the maximum are taken before they are scaled: logits of the type's lowest value stay finite.
+#pragma once
+
+#include "common.h"
+#include "losses_launch.h"
+
+namespace e4b {
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLowest = -3.402823466e38f;
+
+// ---- 16-byte pieces of a row
+
+template <int DT>
+struct Piece {
+  static constexpr int kBytes = DT == E4B_FP32 ? 4 : 2;
+  static constexpr int kCount = 16 / kBytes;
+  static constexpr uint32_t kEmpty = DT == E4B_FP32 ? 0xff800000u : DT == E4B_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  using T = std::conditional_t<DT == E4B_FP32, float, uint16_t>;
+
+  static E4B_DEV float one(T v) {
+    if constexpr (DT == E4B_FP32) return v;
+    else return to_f<DT>(v);
+  }
+  static E4B_DEV T round(float f) {
+    if constexpr (DT == E4B_FP32) return f;
+    else return from_f<DT>(f);
+  }
+  static E4B_DEV void unpack(const uint4& v, float (&f)[kCount]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == E4B_FP32) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        f[2 * i] = lo_f<DT>(w[i]);
+        f[2 * i + 1] = hi_f<DT>(w[i]);
+      }
+    }
+  }
+  static E4B_DEV uint4 pack(const float (&f)[kCount]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == E4B_FP32) w[i] = __float_as_uint(f[i]);
+      else w[i] = pack2(from_f<DT>(f[2 * i]), from_f<DT>(f[2 * i + 1]));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// A row as `head` single values up to the first 16-byte address, `pieces` whole pieces, and what is left.
+template <int DT>
+struct Split {
+  int head, pieces, tail;  // tail: index of the first value behind the pieces
+  E4B_DEV Split(const void* p, int n) {
+    constexpr int C = Piece<DT>::kCount;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / Piece<DT>::kBytes;
+    head = min(n, (C - off) & (C - 1));
+    pieces = (n - head) / C;
+    tail = head + pieces * C;
+  }
+};
+
+// 16 bytes at any address that the type's values may have.
+E4B_DEV uint4 load16(const void* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// ---- running maximum m and sum s of exp2((x - m) k)
+
+struct Run {
+  float m = kLowest, s = 0.0f;
+  E4B_DEV void join(float om, float os, float k) {
+    const float n = fmaxf(m, om);
+    s = s * __builtin_amdgcn_exp2f((m - n) * k) + os * __builtin_amdgcn_exp2f((om - n) * k);
+    m = n;
+  }
+  template <int N>
+  E4B_DEV void add(const float (&x)[N], float k) {
+    float n = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n = fmaxf(n, x[i]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((x[i] - n) * k);
+    s = s * __builtin_amdgcn_exp2f((m - n) * k) + sum;
+    m = n;
+  }
+};
+
+// The maximum and the sum of a row, in every lane of the first wave.
+template <int DT, int NT>
+E4B_DEV Run row_run(const void* row, int V, float k) {
+  using P = Piece<DT>;
+  constexpr int U = 4;  // pieces in flight per thread
+  const typename P::T* p = static_cast<const typename P::T*>(row);
+  const Split<DT> at(row, V);
+  const int tid = threadIdx.x;
+  Run r;
+  float edge[2] = {-__builtin_inff(), -__builtin_inff()};
+  if (tid < at.head) edge[0] = P::one(p[tid]);
+  if (tid < V - at.tail) edge[1] = P::one(p[at.tail + tid]);
+  const uint4* v = reinterpret_cast<const uint4*>(p + at.head);
+  int i = tid;
+  for (; i + (U - 1) * NT < at.pieces; i += U * NT) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = v[i + u * NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[P::kCount];
+      P::unpack(w[u], x);
+      r.add(x, k);
+    }
+  }
+  for (; i < at.pieces; i += NT) {
+    float x[P::kCount];
+    P::unpack(v[i], x);
+    r.add(x, k);
+  }
+  r.add(edge, k);
+#pragma unroll
+  for (int off = 1; off < kWave; off *= 2) r.join(__shfl_xor(r.m, off), __shfl_xor(r.s, off), k);
+  if constexpr (NT > kWave) {
+    constexpr int W = NT / kWave;
+    __shared__ float2 part[W];
+    if ((tid & (kWave - 1)) == 0) part[tid / kWave] = make_float2(r.m, r.s);
+    __syncthreads();
+    if (tid < kWave) {
+      const float2 o = part[tid & (W - 1)];
+      r.m = o.x;
+      r.s = o.y;
+#pragma unroll
+      for (int off = 1; off < W; off *= 2) r.join(__shfl_xor(r.m, off), __shfl_xor(r.s, off), k);
+    }
+  }
+  return r;
+}
+
+E4B_DEV float any_float(const void* p, int dtype, int64_t i) {
+  if (dtype == E4B_FP32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  return dtype == E4B_BF16 ? to_f<E4B_BF16>(v) : to_f<E4B_FP16>(v);
+}
+
+E4B_DEV float wave_max(float v) {
+#pragma unroll
+  for (int off = 1; off < kWave; off *= 2) v = fmaxf(v, __shfl_xor(v, off));
+  return v;
+}
+E4B_DEV float wave_sum(float v) {
+#pragma unroll
+  for (int off = 1; off < kWave; off *= 2) v += __shfl_xor(v, off);
+  return v;
+}
+
+// The row of token `at`, and whether the token counts.
+struct Token {
+  const char* row;
+  int64_t n, t, label;
+  bool counts;
+  E4B_DEV Token(const e4b_logits& z, int64_t at, int bytes) {
+    n = at / z.tokens;
+    t = at - n * z.tokens;
+    row = static_cast<const char*>(z.logits) + (n * z.seq_stride + t * z.row_stride) * bytes;
+    label = z.labels ? z.labels[at] : 0;
+    counts = (!z.mask || z.mask[n * z.mask_stride + t]) && label >= 0 && label < z.vocab;
+  }
+};
+
+// The teacher's part of a row, by the first wave: probabilities over its usable entries (an index inside the
+// vocabulary, a value above -inf) and tau^2 sum_k p_k (log p_k - log q_k); zero where no entry is usable.
+template <int DT>
+E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, Run& r) {
+  const float tau = a.z.temperature, per = 1.0f / tau;
+  const int lane = threadIdx.x;
+  const int64_t first = at * a.top;
+  float most = -__builtin_inff();
+  bool bad = false;
+  for (int k = lane; k < a.top; k += kWave) {
+    const int64_t j = a.index[first + k];
+    if (j >= 0 && j < a.z.vocab) {
+      const float w = any_float(a.teacher, a.teacher_dtype, first + k);
+      most = fmaxf(most, w);
+      bad |= w != w;
+    }
+  }
+  most = wave_max(most);
+  const bool none = most == -__builtin_inff() && !__any(bad);
+  float norm = 0.0f;
+  if (!none)
+    for (int k = lane; k < a.top; k += kWave) {
+      const int64_t j = a.index[first + k];
+      if (j >= 0 && j < a.z.vocab) norm += expf((any_float(a.teacher, a.teacher_dtype, first + k) - most) * per);
+    }
+  norm = wave_sum(norm);
+  const float log_norm = logf(norm), log_s = logf(r.s), inv = 1.0f / norm;
+  float sum = 0.0f;
+  for (int k = lane; k < a.top; k += kWave) {
+    const int64_t j = a.index[first + k];
+    float p = 0.0f;
+    if (!none && j >= 0 && j < a.z.vocab) {
+      const float w = (any_float(a.teacher, a.teacher_dtype, first + k) - most) * per;
+      p = expf(w) * inv;
+      // log p - log q; an entry without probability adds nothing, whatever the student holds there
+      const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[j]) - r.m) * per - log_s;
+      if (!(p == 0.0f)) sum += p * ((w - log_norm) - lq);
+    }
+    a.share[first + k] = p;
+  }
+  if (none) r.s = 0.0f;  // nothing to differentiate
+  return tau * tau * wave_sum(sum);
+}
+
+template <int KIND, int DT, int NT>
+__global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin) {
+  using P = Piece<DT>;
+  const int64_t at = begin + blockIdx.x;
+  const Token tok(a.z, at, P::kBytes);
+  const bool lead = threadIdx.x == 0;
+  if (!tok.counts) {
+    if (lead) {
+      if (a.stats) a.stats[at] = make_float2(0.0f, -1.0f);
+      if (KIND == kLogprobs || KIND == kPolicy) a.logps[at] = 0.0f;
+      if (KIND == kPolicy || KIND == kDistill) a.token_loss[at] = 0.0f;
+      if (KIND == kPolicy) a.coef[at] = 0.0f;
+    }
+    return;
+  }
+  const typename P::T* row = reinterpret_cast<const typename P::T*>(tok.row);
+  float own = 0.0f;
+  if (KIND == kLogprobs || KIND == kPolicy) own = P::one(row[tok.label]);
+  Run r = row_run<DT, NT>(row, static_cast<int>(a.z.vocab), a.scale2);
+  if (threadIdx.x >= kWave) return;
+  if constexpr (KIND == kDistill) {
+    const float loss = teacher_loss<DT>(a, at, row, r);
+    if (lead) a.token_loss[at] = loss;
+  } else if (KIND != kStats && lead) {
+    // s is 0 where every logit is -inf: each label has probability 0
+    const float lp = r.s == 0.0f ? -__builtin_inff() : (own - r.m) / a.z.temperature - logf(r.s);
+    a.logps[at] = lp;
+    if constexpr (KIND == kPolicy) {
+      const float adv = a.advantages[a.adv_per_token ? at : tok.n];
+      const float ratio = expf(lp - a.old_logps[at]);
+      const float clipped = fminf(fmaxf(ratio, a.clip_lo), a.clip_hi);
+      const float free_gain = ratio * adv, held = clipped * adv;
+      const bool bad = free_gain != free_gain;
+      float loss = bad ? free_gain : -fminf(free_gain, held);
+      float slope = bad ? free_gain : free_gain <= held ? -free_gain : 0.0f;
+      if (a.ref_logps) {
+        const float x = a.ref_logps[at] - lp, e = expm1f(x);
+        loss += a.kl_coef * (e == __builtin_inff() ? e : e - x);
+        slope -= a.kl_coef * e;
+      }
+      a.token_loss[at] = loss;
+      a.coef[at] = slope;
+    }
+  }
+  if (lead && a.stats) a.stats[at] = make_float2(r.m, r.s);
+}
+
+// ---- joins over tokens
+
+constexpr int kJoin = 1024;
+
+E4B_DEV double block_sum(double v) {
+  __shared__ double part[kJoin / kWave];
+#pragma unroll
+  for (int off = 1; off < kWave; off *= 2) v += __shfl_xor(v, off);
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int w = 0; w < kJoin / kWave; ++w) v += part[w];
+  return v;
+}
+
+// A workgroup per group; sums in 64 bits, in an order that the sizes alone decide.
+__global__ __launch_bounds__(kJoin) void loss_mean_kernel(MeanArgs a) {
+  const int64_t first = blockIdx.x * a.per;
+  double sum = 0.0, n = 0.0;
+  for (int64_t t = threadIdx.x; t < a.per; t += kJoin)
+    if (!(a.stats[first + t].y < 0.0f)) {
+      sum += a.token_loss[first + t];
+      n += 1.0;
+    }
+  sum = block_sum(sum);
+  n = block_sum(n);
+  if (threadIdx.x == 0) {
+    a.loss[blockIdx.x] = n > 0.0 ? static_cast<float>(sum / n) : 0.0f;
+    a.inv[blockIdx.x] = n > 0.0 ? static_cast<float>(1.0 / n) : 0.0f;
+  }
+}
+
+// (sum of lp - ref over the counted tokens, their number) of a sequence, in 64 bits: the sums are long and their
+// differences short.
+E4B_DEV double2 sequence_sum(const PairArgs& a, int64_t n) {
+  const int bytes = a.z.dtype == E4B_FP32 ? 4 : 2;
+  double sum = 0.0, count = 0.0;
+  for (int64_t t = threadIdx.x; t < a.z.tokens; t += kJoin) {
+    const int64_t at = n * a.z.tokens + t;
+    const float2 st = a.stats[at];
+    if (st.y < 0.0f) continue;
+    const Token tok(a.z, at, bytes);
+    const float own = any_float(tok.row, a.z.dtype, tok.label);
+    count += 1.0;
+    sum += st.y == 0.0f ? -__builtin_inf() : (static_cast<double>(own) - st.x) / a.z.temperature - log(static_cast<double>(st.y));
+    if (a.ref && a.ref_per_token) sum -= a.ref[at];
+  }
+  return make_double2(block_sum(sum), block_sum(count));
+}
+
+__global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
+  const int64_t half = a.z.seqs / 2, b = blockIdx.x;
+  const double2 c = sequence_sum(a, b), r = sequence_sum(a, b + half);
+  if (threadIdx.x != 0) return;
+  double each[2] = {1.0, 1.0}, ratio[2] = {c.x, r.x};
+  for (int i = 0; i < 2; ++i) {
+    const double n = i ? r.y : c.y;
+    if (a.average && n > 0.0) {
+      each[i] = 1.0 / n;
+      ratio[i] *= each[i];
+    }
+    if (a.ref && !a.ref_per_token) ratio[i] -= a.ref[b + i * half];
+    a.rewards[b + i * half] = static_cast<float>(a.beta * ratio[i]);
+  }
+  const double d = ratio[0] - ratio[1], beta = a.beta, h = beta * d, eps = a.smoothing;
+  double loss, slope;
+  if (a.kind == E4B_PREFERENCE_SIGMOID) {
+    // log(1 + e^-|h|) once: -log sigmoid(h) = log1p + max(-h, 0), -log sigmoid(-h) = log1p + max(h, 0)
+    const double e = exp(-fabs(h)), soft = log1p(e), small = e / (1.0 + e), large = 1.0 / (1.0 + e);
+    loss = soft + (h < 0.0 ? (1.0 - eps) * -h : eps == 0.0 ? 0.0 : eps * h);
+    slope = beta * (eps * (h < 0.0 ? small : large) - (1.0 - eps) * (h < 0.0 ? large : small));
+  } else if (a.kind == E4B_PREFERENCE_HINGE) {
+    loss = h < 1.0 ? 1.0 - h : h != h ? h : 0.0;
+    slope = h < 1.0 ? -beta : h != h ? h : 0.0;
+  } else {
+    const double off = d - 0.5 / beta;
+    loss = off * off;
+    slope = 2.0 * off;
+  }
+  a.loss[b] = static_cast<float>(loss);
+  a.coef[b] = static_cast<float>(slope * each[0]);
+  a.coef[b + half] = static_cast<float>(-slope * each[1]);
+}
+
+// ---- backward
+
+constexpr int kBackThreads = 256;
+constexpr int kBackUnroll = 4;
+
+// A workgroup takes kBackThreads * kBackUnroll pieces of one row's gradient: A q_j - A p_k at the row's entries (a label:
+// one entry, A = -derivative / tau; a teacher: p_k, A = derivative * tau). Entries inside the workgroup's part are
+// listed in LDS in the order of k, and each thread takes those in its pieces before it rounds.
+template <int DT, bool TEACHER>
+__global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwardArgs a, int64_t begin, int parts) {
+  using P = Piece<DT>;
+  constexpr int C = P::kCount;
+  const int64_t at = begin + blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  const int V = static_cast<int>(a.z.vocab), tid = threadIdx.x;
+  typename P::T* out = static_cast<typename P::T*>(a.grad) + at * V;
+  const int64_t n = at / a.z.tokens, t = at - n * a.z.tokens;
+  const float2 st = a.stats[at];
+  float A = 0.0f;
+  if (st.y > 0.0f || st.y != st.y) {
+    A = a.grad_loss[n % a.grad_seqs * a.grad_ns + t * a.grad_ts] * a.slope;
+    if (a.coef) A *= a.coef[n * a.coef_ns + t * a.coef_ts];
+    if (a.inv) A *= a.inv[n * a.inv_ns];
+  }
+  const Split<DT> sp(out, V);
+  const int first = part * kBackThreads * kBackUnroll;
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
+  if (A == 0.0f) {  // nothing to differentiate: the logits are not read
+#pragma unroll
+    for (int u = 0; u < kBackUnroll; ++u) {
+      const int i = first + u * kBackThreads + tid;
+      if (i < sp.pieces) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (part == 0) {
+      if (tid < sp.head) out[tid] = P::round(0.0f);
+      if (tid < V - sp.tail) out[sp.tail + tid] = P::round(0.0f);
+    }
+    return;
+  }
+  const typename P::T* row = static_cast<const typename P::T*>(a.z.logits) + n * a.z.seq_stride + t * a.z.row_stride;
+  const typename P::T* body = row + sp.head;
+  uint4 w[kBackUnroll];
+#pragma unroll
+  for (int u = 0; u < kBackUnroll; ++u) {
+    const int i = first + u * kBackThreads + tid;
+    if (i < sp.pieces) w[u] = load16(body + static_cast<int64_t>(i) * C);
+  }
+  // the entries of this part: positions relative to its first value, head and tail among them in part 0
+  const int lo = sp.head + first * C, hi = min(sp.tail, lo + kBackThreads * kBackUnroll * C);
+  auto mine = [&](int64_t j) { return (j >= lo && j < hi) || (part == 0 && ((j >= 0 && j < sp.head) || (j >= sp.tail && j < V))); };
+  __shared__ int where[TEACHER ? kLossMaxTop : 1];
+  __shared__ float what[TEACHER ? kLossMaxTop : 1];
+  __shared__ int listed;
+  int count = 0, label = -1;
+  if constexpr (TEACHER) {
+    if (tid < kWave) {
+      int have = 0;
+      for (int k0 = 0; k0 < a.top; k0 += kWave) {
+        const int k = k0 + tid;
+        int64_t j = -1;
+        if (k < a.top) j = a.index[at * a.top + k];
+        const bool keep = mine(j);
+        const uint64_t held = __ballot(keep);
+        if (keep) {
+          const int slot = have + __popcll(held & ((uint64_t(1) << tid) - 1));
+          where[slot] = static_cast<int>(j);
+          what[slot] = A * a.share[at * a.top + k];
+        }
+        have += __popcll(held);
+      }
+      if (tid == 0) listed = have;
+    }
+    __syncthreads();
+    count = __builtin_amdgcn_readfirstlane(listed);
+  } else {
+    const int64_t j = a.z.labels[at];
+    if (mine(j)) label = static_cast<int>(j), count = 1;
+  }
+  auto entry = [&](int e) { return TEACHER ? where[e] : label; };
+  auto share = [&](int e) { return TEACHER ? what[e] : A; };
+  const float A_s = A / st.y;
+  auto value = [&](float z) { return A_s * __builtin_amdgcn_exp2f((z - st.x) * a.scale2); };
+#pragma unroll
+  for (int u = 0; u < kBackUnroll; ++u) {
+    const int i = first + u * kBackThreads + tid;
+    if (i >= sp.pieces) continue;
+    float x[C];
+    P::unpack(w[u], x);
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = value(x[c]);
+    const int j0 = sp.head + i * C;
+    for (int e = 0; e < count; ++e) {
+      const int off = entry(e) - j0;
+      if (off >= 0 && off < C) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c == off) x[c] -= share(e);
+      }
+    }
+    dst[i] = P::pack(x);
+  }
+  if (part == 0) {
+    for (int side = 0; side < 2; ++side) {
+      const int j = side ? sp.tail + tid : tid;
+      if (side ? j >= V : j >= sp.head) continue;
+      float x = value(P::one(row[j]));
+      for (int e = 0; e < count; ++e)
+        if (entry(e) == j) x -= share(e);
+      out[j] = P::round(x);
+    }
+  }
+}
+
+}  // namespace e4b

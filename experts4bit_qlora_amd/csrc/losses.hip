@@ -1,0 +1,79 @@
+// Launchers of the losses over the vocabulary's logits (losses.h).
+#include "losses.h"
+
+#include <algorithm>
+
+namespace e4b {
+
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// f(first row, rows) for all rows in order: a launch holds fewer than 2^32 work items, `per` workgroups of `threads` a row.
+template <class F>
+void by_launch(int64_t rows, int64_t per, int threads, F&& f) {
+  const int64_t most = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / threads / per);
+  for (int64_t first = 0; first < rows; first += most) f(first, std::min(most, rows - first));
+}
+
+template <int KIND, int DT>
+void rows_of(const LossArgs& a, hipStream_t s) {
+  constexpr int NT = 512;
+  by_launch(a.z.seqs * a.z.tokens, 1, NT, [&](int64_t first, int64_t rows) {
+    hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, NT>), dim3(static_cast<unsigned>(rows)), dim3(NT), 0, s, a, first);
+  });
+}
+
+template <int KIND>
+void rows_of(const LossArgs& a, hipStream_t s) {
+  switch (a.z.dtype) {
+    case E4B_FP32: return rows_of<KIND, E4B_FP32>(a, s);
+    case E4B_BF16: return rows_of<KIND, E4B_BF16>(a, s);
+    default: return rows_of<KIND, E4B_FP16>(a, s);
+  }
+}
+
+template <int DT, bool TEACHER>
+void backward_of(const LossBackwardArgs& a, hipStream_t s) {
+  const int64_t parts = std::max<int64_t>(1, cdiv(a.z.vocab, int64_t(kBackThreads) * kBackUnroll * Piece<DT>::kCount));
+  by_launch(a.z.seqs * a.z.tokens, parts, kBackThreads, [&](int64_t first, int64_t rows) {
+    hipLaunchKernelGGL((loss_backward_kernel<DT, TEACHER>), dim3(static_cast<unsigned>(rows * parts)), dim3(kBackThreads),
+                       0, s, a, first, static_cast<int>(parts));
+  });
+}
+
+template <bool TEACHER>
+void backward_of(const LossBackwardArgs& a, hipStream_t s) {
+  switch (a.z.dtype) {
+    case E4B_FP32: return backward_of<E4B_FP32, TEACHER>(a, s);
+    case E4B_BF16: return backward_of<E4B_BF16, TEACHER>(a, s);
+    default: return backward_of<E4B_FP16, TEACHER>(a, s);
+  }
+}
+
+}  // namespace
+
+void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s) {
+  switch (kind) {
+    case kStats: return rows_of<kStats>(a, s);
+    case kLogprobs: return rows_of<kLogprobs>(a, s);
+    case kPolicy: return rows_of<kPolicy>(a, s);
+    default: return rows_of<kDistill>(a, s);
+  }
+}
+
+// Both: groups and pairs number at most 2^21 (kLossMaxSeqs), so one launch holds their workgroups.
+void launch_loss_mean(const MeanArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(loss_mean_kernel, dim3(static_cast<unsigned>(a.groups)), dim3(kJoin), 0, s, a);
+}
+
+void launch_pairs(const PairArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(pairs_kernel, dim3(static_cast<unsigned>(a.z.seqs / 2)), dim3(kJoin), 0, s, a);
+}
+
+void launch_loss_backward(const LossBackwardArgs& a, hipStream_t s) {
+  if (a.index) return backward_of<true>(a, s);
+  return backward_of<false>(a, s);
+}
+
+}  // namespace e4b

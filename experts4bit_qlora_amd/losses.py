@@ -1,0 +1,428 @@
+"""Losses over the vocabulary's logits, with gradients: what the adapters of a training lane learn from.
+
+``token_logprobs`` (the log-probability of each label: what serving reports for a generated token, and what the losses take
+from an older or a reference model), ``preference_loss`` (paired log ratios of chosen and rejected answers),
+``policy_loss`` (clipped ratios with a KL term) and ``distill_loss`` (divergence from a teacher's top logits). On a HIP
+device each reads the logits once forward and once backward (``csrc/losses.h``) and keeps two floats per token
+between; tensors elsewhere, other dtypes, sizes beyond the kernels' limits, and tensors that a transform, a trace or
+forward-mode differentiation follows take the torch formulation, which is the definition.
+
+Logits are ``[..., tokens, vocab]``; the leading axes are sequences. They may be a view whose rows lie at any stride
+(``logits[:, :-1]`` is not copied). The gradient of such a view is copied into the whole's by autograd: shifting the
+labels instead (the last one ``-100``) saves that. A token counts iff its mask is nonzero (where a mask is given) and, in
+the three losses with labels, its label is inside ``[0, vocab)``; other tokens' logits have no influence, whatever they
+are, and get a zero gradient. A row whose logits are all ``-inf`` gives every label probability 0 and gets a zero
+gradient. Everything but the logits is a constant to the gradient.
+
+The reference has no losses of its own (its training lane starts at a model's, ``experts4bit_qlora/engines/fast.py:453-674``).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native as N
+from . import ops
+from .router import _aligned, _on_kernel
+
+_PREFERENCE = {"sigmoid": N.PREFERENCE_SIGMOID, "hinge": N.PREFERENCE_HINGE, "ipo": N.PREFERENCE_IPO}
+_REDUCTION = {"none": N.REDUCE_NONE, "sequence": N.REDUCE_SEQUENCE, "mean": N.REDUCE_MEAN}
+_MAX_TOP = 1024
+
+
+# ------------------------------------------------------------------------------- arguments
+
+
+def _sequences(logits: torch.Tensor):
+    """(logits as ``[seqs, tokens, vocab]``, leading axes)"""
+    if logits.dim() < 2 or not logits.is_floating_point() or not logits.shape[-1]:
+        raise ValueError("logits must be a floating-point tensor [..., tokens, vocab]")
+    if logits.dim() == 3:
+        return logits, logits.shape[:1]
+    return logits.reshape(logits.shape[:-2].numel(), *logits.shape[-2:]) if logits.dim() > 3 else logits.unsqueeze(0), logits.shape[:-2]
+
+
+def _integers(name: str, t: torch.Tensor, logits: torch.Tensor, shape) -> None:
+    if t.shape != shape or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise ValueError(f"{name} must be integers {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if t.device != logits.device:
+        raise ValueError(f"logits and {name} must be on one device")
+
+
+def _floats(name: str, t: torch.Tensor, logits: torch.Tensor, *shapes) -> None:
+    if t.shape not in shapes or not t.is_floating_point():
+        raise ValueError(f"{name} must be floating-point {' or '.join(str(list(s)) for s in shapes)}, got {t.dtype} "
+                         f"{list(t.shape)}")
+    if t.device != logits.device:
+        raise ValueError(f"logits and {name} must be on one device")
+
+
+def _mask(mask, logits: torch.Tensor, seqs: int):
+    """The mask as bool ``[tokens]`` or ``[seqs, tokens]``, or None."""
+    if mask is None:
+        return None
+    if mask.shape != logits.shape[:-1] and mask.shape != logits.shape[-2:-1]:
+        raise ValueError(f"mask must be {list(logits.shape[-2:-1])} or {list(logits.shape[:-1])}, got {list(mask.shape)}")
+    if mask.device != logits.device:
+        raise ValueError("logits and mask must be on one device")
+    if mask.dtype != torch.bool:
+        mask = mask != 0
+    return mask if mask.dim() == 1 else mask.reshape(seqs, logits.shape[-2])
+
+
+def _temperature(t: float) -> float:
+    if not (t > 0 and math.isfinite(t)):
+        raise ValueError(f"temperature={t} is not positive and finite")
+    return float(t)
+
+
+def _reduction(name: str) -> int:
+    if name not in _REDUCTION:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {name!r}")
+    return _REDUCTION[name]
+
+
+def _fits(z: torch.Tensor, temperature: float, *others) -> bool:
+    """Whether the kernels may take these: plain device tensors within the limits of ``e4b_logits``."""
+    seqs, tokens, vocab = z.shape
+    return (_on_kernel(z) and seqs <= 2 ** 21 and seqs * tokens < 2 ** 31 and vocab <= 2 ** 30
+            and 1e-30 < temperature < 1e30 and all(t is None or _plain(t) for t in others))
+
+
+def _plain(t: torch.Tensor) -> bool:
+    return not torch._C._functorch.is_functorch_wrapped_tensor(t)
+
+
+def _rows(z: torch.Tensor) -> torch.Tensor:
+    return z if z.stride(2) == 1 or z.shape[2] == 1 else z.contiguous()
+
+
+def _ints(t: torch.Tensor, *shape) -> torch.Tensor:
+    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    return _aligned(t if t.shape == shape else t.reshape(shape))
+
+
+def _fp32(t, *shape):
+    """A constant as contiguous fp32."""
+    if t is None:
+        return None
+    t = t.detach() if t.dtype == torch.float32 else t.detach().float()
+    return _aligned(t if t.shape == shape else t.reshape(shape))
+
+
+def _bools(mask):
+    return None if mask is None else _aligned(mask)
+
+
+def _once():
+    if torch.is_grad_enabled():
+        raise RuntimeError("the losses over logits are differentiable once: no create_graph=True on the device")
+
+
+def _differentiated(z: torch.Tensor) -> bool:
+    return z.requires_grad and torch.is_grad_enabled()
+
+
+# ----------------------------------------------------------------------- log-probabilities
+
+
+class _Logprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, labels, mask, temperature):
+        logps, saved = ops.token_logprobs(z, labels, mask, temperature)
+        ctx.save_for_backward(z, labels, mask, saved)
+        ctx.temperature = temperature
+        return logps
+
+    @staticmethod
+    def backward(ctx, grad):
+        _once()
+        z, labels, mask, saved = ctx.saved_tensors
+        return ops.loss_backward(z, labels, mask, ctx.temperature, saved, grad, N.REDUCE_NONE), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tensor | None = None,
+                   temperature: float = 1.0) -> torch.Tensor:
+    """Log-probability of each label under ``softmax(logits / temperature)``: logits ``[..., T, V]``, labels ``[..., T]``
+    integers, mask ``[T]`` or ``[..., T]`` -> fp32 ``[..., T]`` (fp64 for fp64 logits), 0 where a token does not count.
+    Differentiable with respect to the logits (once)."""
+    z, lead = _sequences(logits)
+    _integers("labels", labels, logits, logits.shape[:-1])
+    m, t = _mask(mask, logits, z.shape[0]), _temperature(temperature)
+    if not _fits(z, t, labels, m):
+        return _token_logprobs_torch(z, labels.reshape(z.shape[:2]), m, t)[0].view(logits.shape[:-1])
+    z, labels, m = _rows(z), _ints(labels, *z.shape[:2]), _bools(m)
+    if _differentiated(z):
+        logps = _Logprobs.apply(z, labels, m, t)
+    else:
+        logps, _ = ops.token_logprobs(z, labels, m, t, stats=False)
+    return logps if len(lead) == 1 else logps.view(logits.shape[:-1])
+
+
+def _wide(z: torch.Tensor) -> torch.Tensor:
+    return z if z.dtype == torch.float64 else z.float()
+
+
+def _log_softmax(z: torch.Tensor, counted: torch.Tensor, temperature: float) -> torch.Tensor:
+    """Of rows that count, -inf throughout where all logits are; zeros' elsewhere."""
+    z = torch.where(counted.unsqueeze(-1), _wide(z), 0.0)
+    empty = (z == -math.inf).all(-1, keepdim=True)
+    y = torch.where(empty, 0.0, z)
+    y = (y - y.detach().amax(-1, keepdim=True)) / temperature
+    return torch.log_softmax(y, -1).masked_fill(empty, -math.inf)
+
+
+def _token_logprobs_torch(z, labels, mask, temperature):
+    counted = (labels >= 0) & (labels < z.shape[-1])
+    if mask is not None:
+        counted = counted & mask
+    at = torch.where(counted, labels, 0).to(torch.int64).unsqueeze(-1)
+    logps = _log_softmax(z, counted, temperature).gather(-1, at).squeeze(-1)
+    return torch.where(counted, logps, 0.0), counted
+
+
+# ------------------------------------------------------------------------------ preference
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, labels, mask, ref, kind, beta, smoothing, average):
+        loss, rewards, saved = ops.preference_loss(z, labels, mask, ref, kind, beta, smoothing, average)
+        ctx.save_for_backward(z, labels, mask, saved)
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    def backward(ctx, grad, _):
+        none = (None,) * 7
+        if grad is None:
+            return None, *none
+        _once()
+        z, labels, mask, saved = ctx.saved_tensors
+        return ops.loss_backward(z, labels, mask, 1.0, saved, grad, N.REDUCE_SEQUENCE, coef="sequence"), *none
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor | None = None, beta: float = 0.1,
+                    loss_type: str = "sigmoid", label_smoothing: float = 0.0, average: bool = False,
+                    mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Preference loss of pairs: logits ``[2B, T, V]`` and labels ``[2B, T]``, the chosen answers in the first half and the
+    rejected ones in the second -> ``(loss fp32 [B], rewards fp32 [2B])``.
+
+    With ``S`` the sum of an answer's counted log-probabilities (``average``: their mean) and ``r`` the same under the
+    reference model, ``d = (S_c - r_c) - (S_r - r_r)`` and ``h = beta d``: ``"sigmoid"`` ``-(1 - e) log sigmoid(h) - e
+    log sigmoid(-h)`` with ``e = label_smoothing``, ``"hinge"`` ``max(0, 1 - h)``, ``"ipo"`` ``(d - 1 / (2 beta))^2``.
+    ``ref_logps``: per token ``[2B, T]`` as ``token_logprobs`` gives them (the difference is then summed in 64 bits
+    token by token), or the answers' sums (means) ``[2B]``; None: zeros. ``rewards = beta (S - r)``, constants to the
+    gradient. The loss is differentiable with respect to the logits (once)."""
+    if logits.dim() != 3 or logits.shape[0] % 2:
+        raise ValueError(f"logits must be [2 * pairs, tokens, vocab], got {list(logits.shape)}")
+    z, _ = _sequences(logits)
+    seqs, T, _ = z.shape
+    _integers("labels", labels, logits, logits.shape[:-1])
+    if ref_logps is not None:
+        _floats("ref_logps", ref_logps, logits, (seqs, T), (seqs,))
+    if loss_type not in _PREFERENCE:
+        raise ValueError(f"loss_type must be one of {sorted(_PREFERENCE)}, got {loss_type!r}")
+    if not (beta > 0 and math.isfinite(beta)):
+        raise ValueError(f"beta={beta} is not positive and finite")
+    if not 0 <= label_smoothing <= 1:
+        raise ValueError(f"label_smoothing={label_smoothing} outside [0, 1]")
+    if label_smoothing and loss_type != "sigmoid":
+        raise ValueError("label_smoothing belongs to loss_type='sigmoid'")
+    m = _mask(mask, logits, seqs)
+    kind = _PREFERENCE[loss_type]
+    if not (_fits(z, 1.0, labels, m, ref_logps) and 1e-30 < beta < 1e30):
+        return _preference_loss_torch(z, labels, m, ref_logps, kind, beta, label_smoothing, average)
+    z, labels, m = _rows(z), _ints(labels, seqs, T), _bools(m)
+    ref = None if ref_logps is None else _fp32(ref_logps, *ref_logps.shape)
+    args = (z, labels, m, ref, kind, float(beta), float(label_smoothing), bool(average))
+    if _differentiated(z):
+        return _Preference.apply(*args)
+    loss, rewards, _ = ops.preference_loss(*args)
+    return loss, rewards
+
+
+def _preference_loss_torch(z, labels, mask, ref, kind, beta, smoothing, average):
+    lp, counted = _token_logprobs_torch(z, labels, mask, 1.0)
+    lp = lp.double()
+    if ref is not None and ref.dim() == 2:
+        lp = lp - torch.where(counted, ref.detach(), 0.0).double()
+    ratio = lp.sum(-1)
+    if average:
+        ratio = ratio / counted.sum(-1).clamp(min=1)
+    if ref is not None and ref.dim() == 1:
+        ratio = ratio - ref.detach().double()
+    d = ratio[:len(ratio) // 2] - ratio[len(ratio) // 2:]
+    h = beta * d
+    if kind == N.PREFERENCE_SIGMOID:
+        loss = -(1 - smoothing) * torch.nn.functional.logsigmoid(h)
+        if smoothing:
+            loss = loss - smoothing * torch.nn.functional.logsigmoid(-h)
+    elif kind == N.PREFERENCE_HINGE:
+        loss = torch.relu(1 - h)
+    else:
+        loss = (d - 1 / (2 * beta)) ** 2
+    dtype = _wide(z[:0]).dtype
+    return loss.to(dtype), (beta * ratio).detach().to(dtype)
+
+
+# ---------------------------------------------------------------------------------- policy
+
+
+class _Policy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, labels, mask, old, advantages, ref, clip_lo, clip_hi, kl_coef, temperature, reduction):
+        loss, logps, saved = ops.policy_loss(z, labels, mask, old, advantages, ref, clip_lo, clip_hi, kl_coef, temperature,
+                                             reduction)
+        ctx.save_for_backward(z, labels, mask, saved)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        ctx.mark_non_differentiable(logps)
+        ctx.set_materialize_grads(False)
+        return loss, logps
+
+    @staticmethod
+    def backward(ctx, grad, _):
+        none = (None,) * 10
+        if grad is None:
+            return None, *none
+        _once()
+        z, labels, mask, saved = ctx.saved_tensors
+        return ops.loss_backward(z, labels, mask, ctx.temperature, saved, grad, ctx.reduction, coef="token"), *none
+
+
+def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
+                ref_logps: torch.Tensor | None = None, clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0,
+                mask: torch.Tensor | None = None, temperature: float = 1.0,
+                reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor]:
+    """Clipped policy loss: logits ``[..., T, V]``, labels (the sampled tokens) and ``old_logps`` ``[..., T]``, ``advantages``
+    ``[...]`` or ``[..., T]`` -> ``(loss fp32, logps fp32 [..., T])``.
+
+    With ``lp`` a token's log-probability at the temperature, ``r = exp(lp - old_logps)`` and ``x = ref_logps - lp``, a
+    counted token's loss is ``-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (e^x - x - 1)``; the KL term
+    needs ``ref_logps``. ``reduction``: ``"mean"`` over all counted tokens (one value), ``"sequence"`` over
+    each sequence's ``[...]``, ``"none"`` each token's ``[..., T]``; 0 where nothing counts. ``logps`` are constants
+    to the gradient. The loss is differentiable with respect to the logits (once)."""
+    z, lead = _sequences(logits)
+    seqs, T, _ = z.shape
+    _integers("labels", labels, logits, logits.shape[:-1])
+    _floats("old_logps", old_logps, logits, logits.shape[:-1])
+    _floats("advantages", advantages, logits, lead, logits.shape[:-1])
+    if ref_logps is not None:
+        _floats("ref_logps", ref_logps, logits, logits.shape[:-1])
+    elif kl_coef:
+        raise ValueError("kl_coef needs ref_logps")
+    if not math.isfinite(kl_coef):
+        raise ValueError(f"kl_coef={kl_coef} is not finite")
+    lo, hi = (float(c) for c in clip)
+    if not (0 <= lo <= 1 and 0 <= hi and math.isfinite(hi)):
+        raise ValueError(f"clip={tuple(clip)}: below in [0, 1], above not negative")
+    m, t, red = _mask(mask, logits, seqs), _temperature(temperature), _reduction(reduction)
+    ref = ref_logps if kl_coef else None
+    adv_shape = (seqs, T) if advantages.dim() > len(lead) else (seqs,)
+    if not _fits(z, t, labels, m, old_logps, advantages, ref):
+        loss, logps = _policy_loss_torch(z, labels.reshape(seqs, T), m, old_logps.reshape(seqs, T),
+                                         advantages.reshape(adv_shape), None if ref is None else ref.reshape(seqs, T),
+                                         1 - lo, 1 + hi, kl_coef, t, red)
+    else:
+        z = _rows(z)
+        args = (z, _ints(labels, seqs, T), _bools(m), _fp32(old_logps, seqs, T), _fp32(advantages, *adv_shape),
+                _fp32(ref, seqs, T), 1 - lo, 1 + hi, float(kl_coef), t, red)
+        loss, logps = _Policy.apply(*args) if _differentiated(z) else ops.policy_loss(*args)[:2]
+    return _unflatten(loss, lead, T, red), logps if len(lead) == 1 else logps.view(*lead, T)
+
+
+def _unflatten(loss: torch.Tensor, lead, T: int, reduction: int) -> torch.Tensor:
+    if reduction == N.REDUCE_MEAN or len(lead) == 1:
+        return loss
+    return loss.view(lead if reduction == N.REDUCE_SEQUENCE else (*lead, T))
+
+
+def _reduce_torch(each, counted, reduction):
+    if reduction == N.REDUCE_NONE:
+        return each
+    if reduction == N.REDUCE_SEQUENCE:
+        return (each.double().sum(-1) / counted.sum(-1).clamp(min=1)).to(each.dtype)
+    return (each.double().sum() / counted.sum().clamp(min=1)).to(each.dtype)
+
+
+def _policy_loss_torch(z, labels, mask, old, advantages, ref, clip_lo, clip_hi, kl_coef, temperature, reduction):
+    lp, counted = _token_logprobs_torch(z, labels, mask, temperature)
+    held = [torch.where(counted, t.detach().to(lp.dtype), 0.0) for t in
+            (old, advantages if advantages.dim() == 2 else advantages.unsqueeze(-1).expand_as(lp))]
+    ratio = torch.exp(lp - held[0])
+    # a minimum whose two sides are equal takes the unclipped side's derivative
+    free, kept = ratio * held[1], ratio.detach().clamp(clip_lo, clip_hi) * held[1]
+    each = -torch.where(free <= kept, free, torch.where(free.isnan(), free, kept))
+    if ref is not None:
+        x = torch.where(counted, ref.detach().to(lp.dtype), 0.0) - lp
+        e = torch.expm1(x)
+        each = each + kl_coef * torch.where(e == math.inf, e, e - x)
+    return _reduce_torch(torch.where(counted, each, 0.0), counted, reduction), lp.detach()
+
+
+# ---------------------------------------------------------------------------- distillation
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, mask, teacher, index, temperature, reduction):
+        loss, share, saved = ops.distill_loss(z, mask, teacher, index, temperature, reduction)
+        ctx.save_for_backward(z, mask, index, share, saved)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        _once()
+        z, mask, index, share, saved = ctx.saved_tensors
+        return (ops.loss_backward(z, None, mask, ctx.temperature, saved, grad, ctx.reduction, index=index, share=share),
+                None, None, None, None, None)
+
+
+def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                 mask: torch.Tensor | None = None, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """Distillation from a teacher's top logits: logits ``[..., T, V]``, ``teacher_logits`` and ``teacher_index`` ``[..., T,
+    K]`` (values, or log-probabilities, and where in the vocabulary they belong) -> loss fp32.
+
+    With ``p = softmax(teacher_logits / temperature)`` over a token's K entries and ``q = softmax(logits /
+    temperature)`` over the vocabulary, a counted token's loss is ``temperature^2 sum_k p_k (log p_k - log q[index_k])``.
+    Entries whose index is outside ``[0, V)`` or whose value is ``-inf`` have no probability; a token without any has
+    loss 0 (and counts, if its mask says so). ``reduction`` as in ``policy_loss``. Differentiable with respect to
+    the logits (once)."""
+    z, lead = _sequences(logits)
+    seqs, T, _ = z.shape
+    if teacher_index.dim() != logits.dim() or not teacher_index.shape[-1]:
+        raise ValueError(f"teacher_index must be {list(logits.shape[:-1])} and at least one entry, got "
+                         f"{list(teacher_index.shape)}")
+    K = teacher_index.shape[-1]
+    shape = (*logits.shape[:-1], K)
+    _integers("teacher_index", teacher_index, logits, shape)
+    _floats("teacher_logits", teacher_logits, logits, shape)
+    m, t, red = _mask(mask, logits, seqs), _temperature(temperature), _reduction(reduction)
+    if not (_fits(z, t, m, teacher_logits, teacher_index) and K <= _MAX_TOP and teacher_logits.dtype in ops._DT):
+        loss = _distill_loss_torch(z, m, teacher_logits.reshape(seqs, T, K), teacher_index.reshape(seqs, T, K), t, red)
+    else:
+        z = _rows(z)
+        values = teacher_logits.detach()
+        args = (z, _bools(m), _aligned(values if len(lead) == 1 else values.reshape(seqs, T, K)),
+                _ints(teacher_index, seqs, T, K), t, red)
+        loss = _Distill.apply(*args) if _differentiated(z) else ops.distill_loss(*args)[0]
+    return _unflatten(loss, lead, T, red)
+
+
+def _distill_loss_torch(z, mask, teacher, index, temperature, reduction):
+    counted = torch.ones(z.shape[:2], dtype=torch.bool, device=z.device) if mask is None else mask.expand(z.shape[:2])
+    log_q = _log_softmax(z, counted, temperature)
+    w = teacher.detach().to(log_q.dtype)
+    usable = (index >= 0) & (index < z.shape[-1]) & counted.unsqueeze(-1)
+    w = torch.where(usable, w, -math.inf)
+    none = (w == -math.inf).all(-1, keepdim=True)
+    top = torch.where(none, 0.0, w.amax(-1, keepdim=True))
+    y = (w - top) / temperature
+    log_p = torch.log_softmax(torch.where(none, 0.0, y), -1)
+    p = torch.exp(log_p).masked_fill(none, 0.0)
+    away = log_p - log_q.gather(-1, torch.where(usable, index, 0).to(torch.int64))
+    each = temperature ** 2 * torch.where(p == 0, 0.0, p * torch.where(p == 0, 0.0, away)).sum(-1)
+    return _reduce_torch(torch.where(counted, each, 0.0), counted, reduction)

@@ -53,6 +53,17 @@ enum e4b_epilogue {
 /* What the router's softmax runs over: all logits, or the chosen ones (which equals renormalising). */
 enum e4b_scoring { E4B_SCORE_ALL = 0, E4B_SCORE_CHOSEN = 1 };
 
+/* Losses of e4b_preference_loss over h = beta d: -(1-e) log sigmoid(h) - e log sigmoid(-h); max(0, 1 - h);
+ * (d - 1 / (2 beta))^2. */
+enum e4b_preference { E4B_PREFERENCE_SIGMOID = 0, E4B_PREFERENCE_HINGE = 1, E4B_PREFERENCE_IPO = 2 };
+
+/* What the losses over tokens reduce to. */
+enum e4b_reduction {
+  E4B_REDUCE_NONE = 0,     /* each token's loss [seqs, tokens] */
+  E4B_REDUCE_SEQUENCE = 1, /* the mean over each sequence's counted tokens [seqs] */
+  E4B_REDUCE_MEAN = 2      /* the mean over all counted tokens, one value */
+};
+
 /* Kernel-path selection flags for the grouped GEMMs (0 = automatic by token count). */
 enum e4b_flags { E4B_PATH_AUTO = 0, E4B_PATH_GEMV = 1, E4B_PATH_MFMA = 2 };
 
@@ -86,6 +97,20 @@ typedef struct e4b_routing {
   int32_t* scratch;     /* [e4b_route_scratch_ints(M, E)] per-chunk counts of the chunked route
                            (M > 4096); may be NULL when that size is 0 */
 } e4b_routing;
+
+/* A batch of logits over the vocabulary. Token t of sequence n has the row at
+ * logits + n * seq_stride + t * row_stride (elements; a row's own elements are adjacent). */
+typedef struct e4b_logits {
+  const void* logits;
+  int32_t dtype;         /* e4b_dtype */
+  float temperature;     /* the logits are divided by it; positive, finite, its inverse too */
+  int64_t seqs, tokens;  /* seqs <= 2^21, seqs * tokens < 2^31 */
+  int64_t vocab;         /* 1 .. 2^30 */
+  int64_t seq_stride, row_stride;
+  const int64_t* labels; /* [seqs, tokens]; a token whose label is outside [0, vocab) does not count */
+  const uint8_t* mask;   /* token (n, t) counts iff mask[n * mask_stride + t] != 0 (NULL: all do) */
+  int64_t mask_stride;   /* 0 shares one mask */
+} e4b_logits;
 
 /* Library version string and the last error message of the calling host thread. */
 const char* e4b_version(void);
@@ -193,6 +218,52 @@ int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t 
 int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                               const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
                               const float* grad_loss, void* grad_logits, hipStream_t stream);
+
+/* Log-probabilities of the labels: logps[n, t] = (z_l - max z) / temperature - log sum_j exp((z_j - max z) /
+ * temperature), 0 where the token does not count (its row is not read), -inf where the row's logits are all -inf.
+ * stats fp32 [seqs * tokens, 2] (8-byte aligned; the rows' maxima and sums, for e4b_loss_backward) may be NULL.
+ * Has no counterpart in the reference. */
+int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream);
+
+/* Preference loss of the pairs (sequence b, chosen; sequence b + seqs / 2, rejected): S_i the sum of the counted
+ * tokens' log-probabilities (their mean where `average`), d = (S_c - r_c) - (S_r - r_r). ref: log-probabilities under
+ * the reference model, per token [seqs, tokens] (then summed, or averaged, over the counted tokens like the model's) or
+ * per sequence [seqs] (taken as they are), NULL: zeros. loss fp32 [seqs / 2], rewards fp32 [seqs] = beta (S_i - r_i), coef fp32 [seqs]
+ * = the loss's derivative by each of a sequence's log-probabilities, stats as above (required). seqs is even. Sums in 64 bits, deterministic.
+ * Has no counterpart in the reference. */
+int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_token, int32_t kind, float beta,
+                        float smoothing, int32_t average, float* loss, float* rewards, float* stats, float* coef,
+                        hipStream_t stream);
+
+/* Clipped policy loss: with lp a token's log-probability, r = exp(lp - old_logps) and x = ref_logps - lp,
+ * -min(r A, min(max(r, clip_lo), clip_hi) A) + kl_coef (e^x - x - 1) at counted tokens, 0 elsewhere. advantages
+ * [seqs], or [seqs, tokens] with adv_per_token; ref_logps may be NULL (no KL term). loss: [seqs * tokens], [seqs] or one
+ * value by `reduction` (0 where nothing counts). logps, token_loss, coef (the derivative by lp) fp32 [seqs, tokens], stats as above; with a
+ * reduction, inv fp32 [seqs] or one value: 1 / the number of counted tokens. With E4B_REDUCE_NONE loss is
+ * token_loss and inv is not written. Has no counterpart in the reference. */
+int e4b_policy_loss(const e4b_logits* z, const float* old_logps, const float* advantages, int32_t adv_per_token,
+                    const float* ref_logps, float clip_lo, float clip_hi, float kl_coef, int32_t reduction, float* logps,
+                    float* token_loss, float* stats, float* coef, float* loss, float* inv, hipStream_t stream);
+
+/* Distillation from a teacher's top logits: p = softmax(teacher / temperature) over a token's usable entries (an index
+ * in [0, vocab), a value above -inf), temperature^2 sum_k p_k (log p_k - log q_{index k}) with q the softmax of the row at
+ * the temperature; 0 where the token does not count (by the mask alone) or no entry is usable. teacher [seqs, tokens, top] in
+ * teacher_dtype, index int64 [seqs, tokens, top], top <= 1024; an index may come several times. share fp32 [seqs, tokens,
+ * top] receives p. z->labels is not read. The others as in e4b_policy_loss. Has no counterpart in the reference. */
+int e4b_distill_loss(const e4b_logits* z, const void* teacher, int32_t teacher_dtype, const int64_t* index, int32_t top,
+                     int32_t reduction, float* share, float* token_loss, float* stats, float* loss, float* inv,
+                     hipStream_t stream);
+
+/* The gradient of each of these: grad_logits [seqs, tokens, vocab] (contiguous) in the logits' dtype, rounded once. A
+ * token's derivative is w = grad_loss[(n mod grad_seqs) * grad_strides[0] + t * grad_strides[1]] * coef[n * coef_strides[0] + t *
+ * coef_strides[1]] * inv[n * inv_stride] (coef and inv may be NULL: 1), and with q the row's softmax
+ *   labels (index NULL):  w / temperature ([j = label] - q_j)
+ *   a teacher:            w temperature (q_j - sum of share_k with index_k = j).
+ * Zero, without reading the row, where the token does not count or w is 0. stats, coef, inv, share: as the forward wrote them, z as it read it. */
+int e4b_loss_backward(const e4b_logits* z, const float* stats, const float* grad_loss, int64_t grad_seqs,
+                      const int64_t grad_strides[2], const float* coef, const int64_t coef_strides[2], const float* inv,
+                      int64_t inv_stride, const int64_t* index, const float* share, int32_t top, void* grad_logits,
+                      hipStream_t stream);
 
 /* Routing of row groups with host sizes and device expert ids: group g holds the input rows
  * [sum(sizes[:g]), sum(sizes[:g+1])) for expert expert_ids[g] (int64, on the device, read only

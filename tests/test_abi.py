@@ -396,3 +396,68 @@ def test_quantize_mxfp4_refuses_more_than_a_launch_covers():
     L = N.lib()
     assert L.e4b_quantize_mxfp4(4096, N.BF16, 1 << 37, 4096, 4096, None) == -2 and "one launch" in _err()
     assert L.e4b_quantize_mxfp4(4096, N.FP32, 1 << 42, 4096, 4096, None) == -2 and "one launch" in _err()
+
+
+def test_loss_entry_points_reject_bad_arguments():
+    """Everything is refused before a launch; the sizes and NULLs that are allowed return 0 without one."""
+    L = N.lib()
+    assert ctypes.sizeof(N.Logits) == 8 + 4 + 4 + 5 * 8 + 3 * 8
+
+    def z(p=4096, dt=N.BF16, tau=1.0, seqs=2, tokens=3, vocab=10, s0=30, s1=10, labels=4096, mask=None, stride=0):
+        return ctypes.byref(N.Logits(p, dt, tau, seqs, tokens, vocab, s0, s1, labels, mask, stride))
+
+    def logprobs(d, out=4096, stats=4096):
+        return L.e4b_token_logprobs(d, out, stats, None)
+
+    def pref(d, ref=None, kind=0, beta=0.1, smoothing=0.0, loss=4096, rewards=4096, stats=4096, coef=4096):
+        return L.e4b_preference_loss(d, ref, 0, kind, beta, smoothing, 0, loss, rewards, stats, coef, None)
+
+    def policy(d, old=4096, adv=4096, lo=0.8, hi=1.2, kl=0.0, red=2, logps=4096, each=4096, stats=4096, coef=4096, loss=4096,
+               inv=4096):
+        return L.e4b_policy_loss(d, old, adv, 0, None, lo, hi, kl, red, logps, each, stats, coef, loss, inv, None)
+
+    def distill(d, teacher=4096, tdt=N.FP32, index=4096, top=4, red=2, share=4096, each=4096, stats=4096, loss=4096, inv=4096):
+        return L.e4b_distill_loss(d, teacher, tdt, index, top, red, share, each, stats, loss, inv, None)
+
+    pair = (ctypes.c_int64 * 2)(1, 1)
+
+    def back(d, stats=4096, grad=4096, seqs=2, strides=pair, coef=None, cs=pair, index=None, share=None, top=0, out=4096):
+        return L.e4b_loss_backward(d, stats, grad, seqs, strides, coef, cs, None, 0, index, share, top, out, None)
+
+    for f in (logprobs, pref, policy, distill, back):
+        assert f(None) == -1 and "NULL" in _err()
+        assert f(z(dt=3)) == -1 and "dtype" in _err()
+        for bad in (dict(seqs=-2), dict(tokens=-1), dict(s0=-1), dict(s1=-1), dict(stride=-1)):
+            assert f(z(**bad)) == -1 and "negative" in _err()
+        for bad in (dict(vocab=0), dict(vocab=(1 << 30) + 1)):
+            assert f(z(**bad)) == -2 and "vocab" in _err()
+        for bad in (dict(seqs=(1 << 21) + 2), dict(tokens=1 << 30), dict(seqs=1 << 20, tokens=1 << 11)):
+            assert f(z(**bad)) == -2 and "seqs" in _err()
+        for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-39, 3e38):
+            assert f(z(tau=tau)) == -1 and "temperature" in _err()
+        assert f(z(p=None)) == -1 and f(z(p=4097)) == -1 and f(z(p=4098, dt=N.FP32)) == -1 and "aligned" in _err()
+        if f is not logprobs:
+            assert f(z(), stats=None) == -1
+        assert f(z(), stats=4100) == -1 and "stats" in _err()
+        if f is not distill:
+            assert f(z(labels=None)) == -1 and "labels" in _err()
+    assert logprobs(z(), out=None) == -1 and logprobs(z(seqs=0, p=None), None, None) == 0
+    assert pref(z(seqs=3)) == -1 and "odd" in _err()
+    assert pref(z(), kind=3) == -1 and pref(z(), kind=-1) == -1 and "kind" in _err()
+    for beta in (0.0, -1.0, float("inf"), float("nan")):
+        assert pref(z(), beta=beta) == -1 and "beta" in _err()
+    assert pref(z(), smoothing=-0.1) == pref(z(), smoothing=1.1) == -1 and "smoothing" in _err()
+    assert pref(z(), loss=None) == pref(z(), rewards=None) == pref(z(), coef=None) == -1
+    assert pref(z(seqs=0, p=None), stats=None, loss=None) == 0
+    assert policy(z(), lo=1.3) == -1 and policy(z(), kl=float("inf")) == -1 and policy(z(), red=3) == -1
+    for name in ("old", "adv", "logps", "each", "coef", "loss", "inv"):
+        assert policy(z(), **{name: None}) == -1, name
+    assert policy(z(seqs=0), red=0, loss=None, inv=None) == policy(z(seqs=0), red=1, loss=None, inv=None) == 0
+    assert distill(z(), tdt=7) == -1 and distill(z(), top=0) == -1 and distill(z(), top=1025) == -2 and distill(z(), red=-1) == -1
+    for name in ("teacher", "index", "share", "each", "loss", "inv"):
+        assert distill(z(), **{name: None}) == -1, name
+    assert distill(z(labels=None, seqs=0), red=0) == 0
+    assert back(z(), grad=None) == back(z(), out=None) == back(z(), strides=None) == back(z(), coef=4096, cs=None) == -1
+    assert back(z(), seqs=0) == -1 and back(z(), index=4096, share=None, top=4) == back(z(), index=4096, share=4096) == -1
+    assert back(z(), index=4096, share=4096, top=1025) == -2 and back(z(), out=4104) == -1 and "16-byte" in _err()
+    assert back(z(tokens=0, p=None)) == 0
