@@ -296,17 +296,25 @@ int check_logits(const e4b_logits* z, bool labels, const void* stats) {
     return fail(E4B_EINVAL, "temperature must be positive, it and its inverse finite");
   if (z->seqs * z->tokens > 0 && (!z->logits || (labels && !z->labels) || !stats))
     return fail(E4B_EINVAL, "logits/labels/stats is NULL");
-  if (reinterpret_cast<uintptr_t>(stats) & 7) return fail(E4B_EINVAL, "stats must be 8-byte aligned");
+  if (!aligned16(stats)) return fail(E4B_EINVAL, "stats must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(z->logits) & (z->dtype == E4B_FP32 ? 3 : 1))
     return fail(E4B_EINVAL, "logits are not aligned to their dtype");
   return E4B_OK;
 }
 
+// log2(e) / temperature in two parts, both positive: a difference of -inf keeps its sign in either product.
+float2 exponent_scale(float temperature) {
+  const double k = 1.4426950408889634 / temperature;
+  float hi = static_cast<float>(k);
+  if (hi >= k) hi = std::nextafterf(hi, 0.0f);
+  return make_float2(hi, static_cast<float>(k - hi));
+}
+
 e4b::LossArgs loss_args(const e4b_logits& z, float* stats) {
   e4b::LossArgs a{};
   a.z = z;
-  a.scale2 = 1.4426950408889634f / z.temperature;
-  a.stats = reinterpret_cast<float2*>(stats);
+  a.k = exponent_scale(z.temperature);
+  a.stats = reinterpret_cast<float4*>(stats);
   return a;
 }
 
@@ -323,7 +331,7 @@ int reduce_tokens(const e4b_logits& z, int32_t reduction, const float* token_los
                   float* inv, hipStream_t stream) {
   if (reduction == E4B_REDUCE_NONE) return E4B_OK;
   const bool all = reduction == E4B_REDUCE_MEAN;
-  const e4b::MeanArgs m{token_loss, reinterpret_cast<const float2*>(stats), all ? 1 : z.seqs,
+  const e4b::MeanArgs m{token_loss, reinterpret_cast<const float4*>(stats), all ? 1 : z.seqs,
                         all ? z.seqs * z.tokens : z.tokens, loss, inv};
   if (m.groups == 0) return E4B_OK;
   e4b::launch_loss_mean(m, stream);
@@ -763,8 +771,8 @@ int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers,
 }
 
 int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream) {
-  float2 none;  // stats may be NULL here
-  const int rc = check_logits(z, true, stats ? static_cast<const void*>(stats) : &none);
+  alignas(16) const char none[16] = {};  // stats may be NULL here
+  const int rc = check_logits(z, true, stats ? static_cast<const void*>(stats) : none);
   if (rc || z->seqs * z->tokens == 0) return rc;
   if (!logps) return fail(E4B_EINVAL, "logps is NULL");
   e4b::LossArgs a = loss_args(*z, stats);
@@ -786,7 +794,7 @@ int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_t
   if (!loss || !rewards || !coef) return fail(E4B_EINVAL, "loss/rewards/coef is NULL");
   e4b::LossArgs a = loss_args(*z, stats);
   if (z->tokens) e4b::launch_loss_rows(e4b::kStats, a, stream);
-  const e4b::PairArgs p{*z, a.stats, ref, ref_per_token, kind, beta, smoothing, average, loss, rewards, coef};
+  const e4b::PairArgs p{z->seqs, z->tokens, a.stats, ref, ref_per_token, kind, beta, smoothing, average, loss, rewards, coef};
   e4b::launch_pairs(p, stream);
   return check_launch("pairs_kernel");
 }
@@ -859,8 +867,8 @@ int e4b_loss_backward(const e4b_logits* z, const float* stats, const float* grad
   if (!aligned16(grad_logits)) return fail(E4B_EINVAL, "grad_logits must be 16-byte aligned");
   e4b::LossBackwardArgs a{};
   a.z = *z;
-  a.scale2 = 1.4426950408889634f / z->temperature;
-  a.stats = reinterpret_cast<const float2*>(stats);
+  a.k = exponent_scale(z->temperature);
+  a.stats = reinterpret_cast<const float4*>(stats);
   a.grad_loss = grad_loss;
   a.grad_seqs = grad_seqs;
   a.grad_ns = grad_strides[0];

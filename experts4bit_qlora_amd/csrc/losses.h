@@ -8,6 +8,9 @@
 //   dloss / dlp = -A r [r A <= clip(r) A] + kl (1 - e^x).
 // Teacher with probabilities p_k at the indices i_k:  loss = tau^2 sum_k p_k (log p_k - log q_{i_k}),
 //   dloss / dz_j = tau (q_j - sum of p_k with i_k = j).
+// The label's own exponential is left out of the row's sum and joined at the end: with rest = sum over j != l of
+// exp((z_j - z_l) / tau), lp = -log(1 + rest) keeps its precision where the label is nearly certain, and so does the
+// label's derivative 1 - q_l = 1 - e^lp.
 // Preference, S = sum of a sequence's lp (or their mean), d = (S_c - r_c) - (S_r - r_r):  a loss of d, whose slope is
 // every chosen token's dloss / dlp and, negated, every rejected one's.
 //
@@ -77,47 +80,70 @@ struct Split {
   }
 };
 
-// 16 bytes at any address that the type's values may have.
-E4B_DEV uint4 load16(const void* p) {
-  uint4 v;
-  __builtin_memcpy(&v, p, 16);
-  return v;
+// 16 bytes at any address that the type's values may have, and to an aligned one. The backward's logits are read for the
+// last time and its gradient is larger than the caches: past them, both (1,500 x 128,000 bf16: 143 -> 122 us, the stores
+// alone 125; 5,500 x 50,257: 184 -> 185; 252 x 50,257, which the caches would hold: 13.7 -> 12.2).
+E4B_DEV uint4 load16_once(const void* p) {
+  typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+  const Any v = __builtin_nontemporal_load(static_cast<const Any*>(p));
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+E4B_DEV void store16_once(uint4* p, const uint4& v) {
+  typedef uint32_t Vec __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(Vec{v.x, v.y, v.z, v.w}, reinterpret_cast<Vec*>(p));
 }
 
 // ---- running maximum m and sum s of exp2((x - m) k)
 
+// k = log2(e) / temperature in two parts: with one, the exponents of all rows are off the same way by 2^-25 or so of
+// their size, which a sequence's sum of log-probabilities adds up (820 tokens: 2e-4).
+E4B_DEV float exp_of(float d, float2 k) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.x, d * k.y)); }
+
 struct Run {
   float m = kLowest, s = 0.0f;
-  E4B_DEV void join(float om, float os, float k) {
+  E4B_DEV void join(float om, float os, float2 k) {
     const float n = fmaxf(m, om);
-    s = s * __builtin_amdgcn_exp2f((m - n) * k) + os * __builtin_amdgcn_exp2f((om - n) * k);
+    s = s * exp_of(m - n, k) + os * exp_of(om - n, k);
     m = n;
   }
   template <int N>
-  E4B_DEV void add(const float (&x)[N], float k) {
+  E4B_DEV void add(const float (&x)[N], float2 k) {
     float n = m;
 #pragma unroll
     for (int i = 0; i < N; ++i) n = fmaxf(n, x[i]);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((x[i] - n) * k);
-    s = s * __builtin_amdgcn_exp2f((m - n) * k) + sum;
+    for (int i = 0; i < N; ++i) sum += exp_of(x[i] - n, k);
+    s = s * exp_of(m - n, k) + sum;
     m = n;
   }
 };
 
-// The maximum and the sum of a row, in every lane of the first wave.
-template <int DT, int NT>
-E4B_DEV Run row_run(const void* row, int V, float k) {
+constexpr int kRowUnroll = 4;  // pieces in flight per thread
+
+// The maximum and the sum of a row without its element `skip` (-1: of all), in every lane of the first wave.
+template <int DT, int NT, int U>
+E4B_DEV Run row_run(const void* row, int V, int skip, float2 k) {
   using P = Piece<DT>;
-  constexpr int U = 4;  // pieces in flight per thread
   const typename P::T* p = static_cast<const typename P::T*>(row);
   const Split<DT> at(row, V);
   const int tid = threadIdx.x;
   Run r;
   float edge[2] = {-__builtin_inff(), -__builtin_inff()};
-  if (tid < at.head) edge[0] = P::one(p[tid]);
-  if (tid < V - at.tail) edge[1] = P::one(p[at.tail + tid]);
+  if (tid < at.head && tid != skip) edge[0] = P::one(p[tid]);
+  if (tid < V - at.tail && at.tail + tid != skip) edge[1] = P::one(p[at.tail + tid]);
+  // the skipped element's piece (one that no thread takes where it is none) and its place there
+  const int skip_at = skip < at.head ? -1 : (skip - at.head) / P::kCount, skip_off = (skip - at.head) % P::kCount;
+  auto take = [&](const uint4& w, int i) {
+    float x[P::kCount];
+    P::unpack(w, x);
+    if (i == skip_at) {
+#pragma unroll
+      for (int c = 0; c < P::kCount; ++c)
+        if (c == skip_off) x[c] = -__builtin_inff();
+    }
+    return r.add(x, k);
+  };
   const uint4* v = reinterpret_cast<const uint4*>(p + at.head);
   int i = tid;
   for (; i + (U - 1) * NT < at.pieces; i += U * NT) {
@@ -125,17 +151,9 @@ E4B_DEV Run row_run(const void* row, int V, float k) {
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = v[i + u * NT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[P::kCount];
-      P::unpack(w[u], x);
-      r.add(x, k);
-    }
+    for (int u = 0; u < U; ++u) take(w[u], i + u * NT);
   }
-  for (; i < at.pieces; i += NT) {
-    float x[P::kCount];
-    P::unpack(v[i], x);
-    r.add(x, k);
-  }
+  for (; i < at.pieces; i += NT) take(v[i], i);
   r.add(edge, k);
 #pragma unroll
   for (int off = 1; off < kWave; off *= 2) r.join(__shfl_xor(r.m, off), __shfl_xor(r.s, off), k);
@@ -230,7 +248,7 @@ E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<D
   return tau * tau * wave_sum(sum);
 }
 
-template <int KIND, int DT, int NT>
+template <int KIND, int DT, int NT, int U>
 __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin) {
   using P = Piece<DT>;
   const int64_t at = begin + blockIdx.x;
@@ -238,7 +256,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   const bool lead = threadIdx.x == 0;
   if (!tok.counts) {
     if (lead) {
-      if (a.stats) a.stats[at] = make_float2(0.0f, -1.0f);
+      if (a.stats) a.stats[at] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);
       if (KIND == kLogprobs || KIND == kPolicy) a.logps[at] = 0.0f;
       if (KIND == kPolicy || KIND == kDistill) a.token_loss[at] = 0.0f;
       if (KIND == kPolicy) a.coef[at] = 0.0f;
@@ -247,16 +265,29 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   }
   const typename P::T* row = reinterpret_cast<const typename P::T*>(tok.row);
   float own = 0.0f;
-  if (KIND == kLogprobs || KIND == kPolicy) own = P::one(row[tok.label]);
-  Run r = row_run<DT, NT>(row, static_cast<int>(a.z.vocab), a.scale2);
+  if (KIND != kDistill) own = P::one(row[tok.label]);
+  Run r = row_run<DT, NT, U>(row, static_cast<int>(a.z.vocab), KIND == kDistill ? -1 : static_cast<int>(tok.label), a.k);
   if (threadIdx.x >= kWave) return;
   if constexpr (KIND == kDistill) {
     const float loss = teacher_loss<DT>(a, at, row, r);
     if (lead) a.token_loss[at] = loss;
-  } else if (KIND != kStats && lead) {
-    // s is 0 where every logit is -inf: each label has probability 0
-    const float lp = r.s == 0.0f ? -__builtin_inff() : (own - r.m) / a.z.temperature - logf(r.s);
-    a.logps[at] = lp;
+    if (lead) a.stats[at] = make_float4(r.m, r.s, 0.0f, 0.0f);
+  } else if (lead) {
+    // join the label; (own - m) / tau also where it is 0, for a label of +inf. The sum is 0 where every logit is -inf: each
+    // label has probability 0
+    const float m = fmaxf(r.m, own), rest = r.s * exp_of(r.m - m, a.k), s = rest + exp_of(own - m, a.k);
+    float lp, low = 0.0f;
+    if constexpr (KIND == kStats) {  // for long sums, in 64 bits
+      const double d = (static_cast<double>(own) - m) / a.z.temperature;
+      const double l = d - (own == m ? log1p(static_cast<double>(rest)) : log(rest + exp(d)));
+      lp = static_cast<float>(l);
+      low = lp - lp == 0.0f ? static_cast<float>(l - lp) : 0.0f;
+    } else {
+      lp = (own - m) / a.z.temperature - (own == m ? log1pf(rest) : logf(s));
+    }
+    if (s == 0.0f) lp = -__builtin_inff();
+    if (KIND != kStats) a.logps[at] = lp;
+    if (a.stats) a.stats[at] = make_float4(m, s, lp, low);
     if constexpr (KIND == kPolicy) {
       const float adv = a.advantages[a.adv_per_token ? at : tok.n];
       const float ratio = expf(lp - a.old_logps[at]);
@@ -274,64 +305,75 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
       a.coef[at] = slope;
     }
   }
-  if (lead && a.stats) a.stats[at] = make_float2(r.m, r.s);
 }
 
 // ---- joins over tokens
 
 constexpr int kJoin = 1024;
 
-E4B_DEV double block_sum(double v) {
-  __shared__ double part[kJoin / kWave];
+// The sums of N values over the workgroup, in the first thread.
+template <int N>
+E4B_DEV void block_sums(double (&v)[N]) {
+  constexpr int W = kJoin / kWave;
+  __shared__ double part[W][N];
 #pragma unroll
-  for (int off = 1; off < kWave; off *= 2) v += __shfl_xor(v, off);
+  for (int off = 1; off < kWave; off *= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
+  }
+  const int lane = threadIdx.x & (kWave - 1);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[threadIdx.x / kWave][i] = v[i];
+  }
   __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < kJoin / kWave; ++w) v += part[w];
-  return v;
+  if (threadIdx.x >= kWave) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = part[lane & (W - 1)][i];
+#pragma unroll
+  for (int off = 1; off < W; off *= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
+  }
 }
 
 // A workgroup per group; sums in 64 bits, in an order that the sizes alone decide.
 __global__ __launch_bounds__(kJoin) void loss_mean_kernel(MeanArgs a) {
   const int64_t first = blockIdx.x * a.per;
-  double sum = 0.0, n = 0.0;
+  double v[2] = {0.0, 0.0};
   for (int64_t t = threadIdx.x; t < a.per; t += kJoin)
     if (!(a.stats[first + t].y < 0.0f)) {
-      sum += a.token_loss[first + t];
-      n += 1.0;
+      v[0] += a.token_loss[first + t];
+      v[1] += 1.0;
     }
-  sum = block_sum(sum);
-  n = block_sum(n);
+  block_sums(v);
   if (threadIdx.x == 0) {
+    const double sum = v[0], n = v[1];
     a.loss[blockIdx.x] = n > 0.0 ? static_cast<float>(sum / n) : 0.0f;
     a.inv[blockIdx.x] = n > 0.0 ? static_cast<float>(1.0 / n) : 0.0f;
   }
 }
 
-// (sum of lp - ref over the counted tokens, their number) of a sequence, in 64 bits: the sums are long and their
+// A workgroup per pair. The tokens' log-probabilities and their sums are in 64 bits: the sums are long, their
 // differences short.
-E4B_DEV double2 sequence_sum(const PairArgs& a, int64_t n) {
-  const int bytes = a.z.dtype == E4B_FP32 ? 4 : 2;
-  double sum = 0.0, count = 0.0;
-  for (int64_t t = threadIdx.x; t < a.z.tokens; t += kJoin) {
-    const int64_t at = n * a.z.tokens + t;
-    const float2 st = a.stats[at];
-    if (st.y < 0.0f) continue;
-    const Token tok(a.z, at, bytes);
-    const float own = any_float(tok.row, a.z.dtype, tok.label);
-    count += 1.0;
-    sum += st.y == 0.0f ? -__builtin_inf() : (static_cast<double>(own) - st.x) / a.z.temperature - log(static_cast<double>(st.y));
-    if (a.ref && a.ref_per_token) sum -= a.ref[at];
-  }
-  return make_double2(block_sum(sum), block_sum(count));
-}
-
 __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
-  const int64_t half = a.z.seqs / 2, b = blockIdx.x;
-  const double2 c = sequence_sum(a, b), r = sequence_sum(a, b + half);
+  const int64_t half = a.seqs / 2, b = blockIdx.x;
+  double v[4] = {0.0, 0.0, 0.0, 0.0};  // sum of lp - ref over the counted tokens, their number; of both sequences
+  for (int64_t i = threadIdx.x; i < 2 * a.tokens; i += kJoin) {
+    const bool second = i >= a.tokens;
+    const int64_t at = second ? (b + half) * a.tokens + i - a.tokens : b * a.tokens + i;
+    const float4 st = a.stats[at];
+    if (st.y < 0.0f) continue;
+    double lp = static_cast<double>(st.z) + st.w;
+    if (a.ref && a.ref_per_token) lp -= a.ref[at];
+    v[0] += second ? 0.0 : lp;
+    v[1] += second ? 0.0 : 1.0;
+    v[2] += second ? lp : 0.0;
+    v[3] += second ? 1.0 : 0.0;
+  }
+  block_sums(v);
   if (threadIdx.x != 0) return;
+  const double2 c = make_double2(v[0], v[1]), r = make_double2(v[2], v[3]);
   double each[2] = {1.0, 1.0}, ratio[2] = {c.x, r.x};
   for (int i = 0; i < 2; ++i) {
     const double n = i ? r.y : c.y;
@@ -365,10 +407,10 @@ __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
 // ---- backward
 
 constexpr int kBackThreads = 256;
-constexpr int kBackUnroll = 4;
+constexpr int kBackUnroll = 2;  // 5,500 x 128,000 bf16: 1 / 2 / 4 / 8 pieces a thread 505 / 509 / 542 / 554 us, 50,257: 210 / 184 / 200 / 226
 
 // A workgroup takes kBackThreads * kBackUnroll pieces of one row's gradient: A q_j - A p_k at the row's entries (a label:
-// one entry, A = -derivative / tau; a teacher: p_k, A = derivative * tau). Entries inside the workgroup's part are
+// one entry with p = 1, A = -derivative / tau; a teacher: p_k, A = derivative * tau). Entries inside the workgroup's part are
 // listed in LDS in the order of k, and each thread takes those in its pieces before it rounds.
 template <int DT, bool TEACHER>
 __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwardArgs a, int64_t begin, int parts) {
@@ -379,7 +421,7 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
   const int V = static_cast<int>(a.z.vocab), tid = threadIdx.x;
   typename P::T* out = static_cast<typename P::T*>(a.grad) + at * V;
   const int64_t n = at / a.z.tokens, t = at - n * a.z.tokens;
-  const float2 st = a.stats[at];
+  const float4 st = a.stats[at];
   float A = 0.0f;
   if (st.y > 0.0f || st.y != st.y) {
     A = a.grad_loss[n % a.grad_seqs * a.grad_ns + t * a.grad_ts] * a.slope;
@@ -393,7 +435,7 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
 #pragma unroll
     for (int u = 0; u < kBackUnroll; ++u) {
       const int i = first + u * kBackThreads + tid;
-      if (i < sp.pieces) dst[i] = make_uint4(0, 0, 0, 0);
+      if (i < sp.pieces) store16_once(dst + i, make_uint4(0, 0, 0, 0));
     }
     if (part == 0) {
       if (tid < sp.head) out[tid] = P::round(0.0f);
@@ -407,7 +449,7 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
 #pragma unroll
   for (int u = 0; u < kBackUnroll; ++u) {
     const int i = first + u * kBackThreads + tid;
-    if (i < sp.pieces) w[u] = load16(body + static_cast<int64_t>(i) * C);
+    if (i < sp.pieces) w[u] = load16_once(body + static_cast<int64_t>(i) * C);
   }
   // the entries of this part: positions relative to its first value, head and tail among them in part 0
   const int lo = sp.head + first * C, hi = min(sp.tail, lo + kBackThreads * kBackUnroll * C);
@@ -441,9 +483,9 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
     if (mine(j)) label = static_cast<int>(j), count = 1;
   }
   auto entry = [&](int e) { return TEACHER ? where[e] : label; };
-  auto share = [&](int e) { return TEACHER ? what[e] : A; };
+  const float rest = TEACHER ? 0.0f : A * expm1f(st.z);  // the label's A (q_l - 1)
   const float A_s = A / st.y;
-  auto value = [&](float z) { return A_s * __builtin_amdgcn_exp2f((z - st.x) * a.scale2); };
+  auto value = [&](float z) { return A_s * exp_of(z - st.x, a.k); };
 #pragma unroll
   for (int u = 0; u < kBackUnroll; ++u) {
     const int i = first + u * kBackThreads + tid;
@@ -458,10 +500,10 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
       if (off >= 0 && off < C) {
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          if (c == off) x[c] -= share(e);
+          if (c == off) x[c] = TEACHER ? x[c] - what[e] : rest;
       }
     }
-    dst[i] = P::pack(x);
+    store16_once(dst + i, P::pack(x));
   }
   if (part == 0) {
     for (int side = 0; side < 2; ++side) {
@@ -469,7 +511,7 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
       if (side ? j >= V : j >= sp.head) continue;
       float x = value(P::one(row[j]));
       for (int e = 0; e < count; ++e)
-        if (entry(e) == j) x -= share(e);
+        if (entry(e) == j) x = TEACHER ? x - what[e] : rest;
       out[j] = P::round(x);
     }
   }

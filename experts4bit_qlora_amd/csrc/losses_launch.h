@@ -18,9 +18,11 @@ enum LossKind { kStats = 0, kLogprobs = 1, kPolicy = 2, kDistill = 3 };
 
 struct LossArgs {
   e4b_logits z;
-  float scale2;     // log2(e) / temperature
+  float2 k;         // log2(e) / temperature, its high and low part
   float* logps;     // [R] log-probabilities of the labels, 0 where a token does not count (kLogprobs, kPolicy)
-  float2* stats;    // [R] (row maximum, sum of the row's exponentials); (0, -1) where a token does not count
+  // [R] (row maximum, sum of the row's exponentials, label's log-probability in two parts: the second for kStats only);
+  // (0, -1, 0, 0) where a token does not count
+  float4* stats;
   // kPolicy
   const float* old_logps;   // [R]
   const float* advantages;  // [seqs] or [R]
@@ -42,7 +44,7 @@ void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s);
 // loss[i] = mean of token_loss over the counted tokens of group i, inv[i] = 1 / their number (0 where none counts)
 struct MeanArgs {
   const float* token_loss;
-  const float2* stats;
+  const float4* stats;
   int64_t groups, per;  // groups of `per` consecutive tokens
   float* loss;
   float* inv;
@@ -50,8 +52,8 @@ struct MeanArgs {
 void launch_loss_mean(const MeanArgs& a, hipStream_t s);
 
 struct PairArgs {
-  e4b_logits z;  // the first half of the sequences are the chosen ones
-  const float2* stats;
+  int64_t seqs, tokens;  // the first half of the sequences are the chosen ones
+  const float4* stats;
   const float* ref;  // [R], [seqs] or NULL
   int ref_per_token;
   int kind;  // e4b_preference
@@ -65,8 +67,8 @@ void launch_pairs(const PairArgs& a, hipStream_t s);
 
 struct LossBackwardArgs {
   e4b_logits z;
-  float scale2;
-  const float2* stats;
+  float2 k;
+  const float4* stats;
   // a token's derivative: grad_loss[n, t] * coef[n, t] * inv[n], each at its own strides; coef and inv may be NULL
   const float* grad_loss;
   int64_t grad_seqs, grad_ns, grad_ts;  // sequence n has that of n mod grad_seqs

@@ -221,7 +221,7 @@ int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers,
 
 /* Log-probabilities of the labels: logps[n, t] = (z_l - max z) / temperature - log sum_j exp((z_j - max z) /
  * temperature), 0 where the token does not count (its row is not read), -inf where the row's logits are all -inf.
- * stats fp32 [seqs * tokens, 2] (8-byte aligned; the rows' maxima and sums, for e4b_loss_backward) may be NULL.
+ * stats fp32 [seqs * tokens, 4] (16-byte aligned: what e4b_loss_backward needs of each row) may be NULL.
  * Has no counterpart in the reference. */
 int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream);
 

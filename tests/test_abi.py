@@ -438,7 +438,7 @@ def test_loss_entry_points_reject_bad_arguments():
         assert f(z(p=None)) == -1 and f(z(p=4097)) == -1 and f(z(p=4098, dt=N.FP32)) == -1 and "aligned" in _err()
         if f is not logprobs:
             assert f(z(), stats=None) == -1
-        assert f(z(), stats=4100) == -1 and "stats" in _err()
+        assert f(z(), stats=4104) == -1 and "stats" in _err()
         if f is not distill:
             assert f(z(labels=None)) == -1 and "labels" in _err()
     assert logprobs(z(), out=None) == -1 and logprobs(z(seqs=0, p=None), None, None) == 0
