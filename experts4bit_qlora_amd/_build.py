@@ -4,7 +4,9 @@
 ``csrc/e4b_amd.hip`` (entry points and the routing / dequant / GEMV / LoRA / training kernels),
 ``csrc/mx_gemm.hip`` (the products of microscaled operands), ``csrc/gate.hip`` (the router's kernels), ``csrc/losses.hip`` (the losses over the vocabulary), and ``csrc/decode_inst.hip`` and ``csrc/gemm_inst.hip`` once per (activation dtype, weight format)
 pair, all in parallel, then links them into ``experts4bit_qlora_amd/libe4b_amd.so``. The output is written to a temporary
-name and renamed, so a failed build never leaves a half-written library behind.
+name and renamed, so a failed build never leaves a half-written library behind. ``csrc/torch_losses.cpp``, host code that calls
+the library from torch's autograd, becomes ``experts4bit_qlora_amd/libe4b_torch.so`` the same way, with the host compiler and
+torch's headers.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -22,10 +25,12 @@ GEMM_SRC = os.path.join(CSRC, "gemm_inst.hip")
 MX_SRC = os.path.join(CSRC, "mx_gemm.hip")
 GATE_SRC = os.path.join(CSRC, "gate.hip")
 LOSSES_SRC = os.path.join(CSRC, "losses.hip")
+TORCH_SRC = os.path.join(CSRC, "torch_losses.cpp")
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include")
 # (E4B_INST_DT, E4B_INST_FMT): bf16/fp16 x NF4/NF4_DQ/MXFP4
 DECODE_PAIRS = [(dt, fmt) for dt in (0, 1) for fmt in (0, 1, 2)]
 OUT = os.path.join(_HERE, "libe4b_amd.so")
+TORCH_OUT = os.path.join(_HERE, "libe4b_torch.so")
 ARCH = os.environ.get("E4B_OFFLOAD_ARCH", "gfx950")
 
 FLAGS = [
@@ -64,6 +69,19 @@ def _run_all(cmds):
     return msgs
 
 
+def _torch_commands(obj: str, out: str):
+    """(compile, link) of the extension that binds the library to torch's autograd."""
+    from torch.utils import cpp_extension
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    inc = [f"-I{p}" for p in (INCLUDE, *cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"])]
+    libs = [f"-L{p}" for p in cpp_extension.library_paths("cuda")] + [
+        "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip"]
+    compile_ = [cxx, "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", *inc, "-c", "-o", obj, TORCH_SRC]
+    link = [cxx, "-shared", "-o", out, obj, *libs, f"-L{_HERE}", "-l:libe4b_amd.so", "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def build(verbose: bool = False) -> str:
     cc = hipcc()
     inc = [f"-I{CSRC}", f"-I{INCLUDE}"]
@@ -83,12 +101,15 @@ def build(verbose: bool = False) -> str:
             cmds.append([cc, *FLAGS, *inc, f"-DE4B_INST_DT={dt}", f"-DE4B_INST_FMT={fmt}", "-c", "-o", obj,
                          GEMM_SRC])
             objs.append(obj)
-        msgs = _run_all(cmds)
+        torch_compile, torch_link = _torch_commands(os.path.join(tmpdir, "torch_losses.o"), TORCH_OUT + ".tmp")
+        msgs = _run_all([torch_compile, *cmds])
         tmp = OUT + ".tmp"
         msgs += _run_all([[cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]])
+        os.replace(tmp, OUT)
+        msgs += _run_all([torch_link])
+        os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     if verbose and msgs:
         print("\n".join(msgs), file=sys.stderr)
-    os.replace(tmp, OUT)
     return OUT
 
 

@@ -9,11 +9,15 @@ library's own message.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libe4b_amd.so"
 LIB_PATH = os.path.join(_HERE, LIB_NAME)
+TORCH_LIB_NAME = "libe4b_torch"  # the autograd functions over the library (csrc/torch_losses.cpp)
+TORCH_LIB_PATH = os.path.join(_HERE, TORCH_LIB_NAME + ".so")
 
 # enums mirrored from include/e4b_amd.h
 E4B_OK = 0
@@ -280,6 +284,24 @@ def lib():
     if L is None:
         raise NativeUnavailable(f"the MI355X kernel library is unavailable: {_load_error}")
     return L
+
+
+_torch_lib = None
+
+
+def torch_lib():
+    """The extension module of ``csrc/torch_losses.cpp`` (loaded once); raises :class:`NativeUnavailable` like :func:`lib`."""
+    global _torch_lib
+    if _torch_lib is None:
+        lib()
+        try:
+            loader = importlib.machinery.ExtensionFileLoader(TORCH_LIB_NAME, TORCH_LIB_PATH)
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader(TORCH_LIB_NAME, loader))
+            loader.exec_module(mod)
+        except ImportError as e:
+            raise NativeUnavailable(f"cannot load {TORCH_LIB_PATH} (run __graft_entry__.build()): {e}") from None
+        _torch_lib = mod
+    return _torch_lib
 
 
 def check(fn: str, status: int) -> None:

@@ -24,7 +24,7 @@ import torch
 
 from . import _native as N
 from . import ops
-from .router import _aligned, _on_kernel
+from .router import _on_kernel
 
 _PREFERENCE = {"sigmoid": N.PREFERENCE_SIGMOID, "hinge": N.PREFERENCE_HINGE, "ipo": N.PREFERENCE_IPO}
 _REDUCTION = {"none": N.REDUCE_NONE, "sequence": N.REDUCE_SEQUENCE, "mean": N.REDUCE_MEAN}
@@ -35,16 +35,18 @@ _MAX_TOP = 1024
 
 
 def _sequences(logits: torch.Tensor):
-    """(logits as ``[seqs, tokens, vocab]``, leading axes)"""
-    if logits.dim() < 2 or not logits.is_floating_point() or not logits.shape[-1]:
+    """(logits as ``[seqs, tokens, vocab]``, their shape up to the vocabulary)"""
+    shape = logits.shape
+    if len(shape) < 2 or not shape[-1] or not logits.is_floating_point():
         raise ValueError("logits must be a floating-point tensor [..., tokens, vocab]")
-    if logits.dim() == 3:
-        return logits, logits.shape[:1]
-    return logits.reshape(logits.shape[:-2].numel(), *logits.shape[-2:]) if logits.dim() > 3 else logits.unsqueeze(0), logits.shape[:-2]
+    if len(shape) == 3:
+        return logits, shape[:2]
+    z = logits.unsqueeze(0) if len(shape) == 2 else logits.reshape(shape[:-2].numel(), *shape[-2:])
+    return z, shape[:-1]
 
 
 def _integers(name: str, t: torch.Tensor, logits: torch.Tensor, shape) -> None:
-    if t.shape != shape or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+    if t.shape != shape or t.is_floating_point() or t.dtype == torch.bool:
         raise ValueError(f"{name} must be integers {list(shape)}, got {t.dtype} {list(t.shape)}")
     if t.device != logits.device:
         raise ValueError(f"logits and {name} must be on one device")
@@ -58,17 +60,17 @@ def _floats(name: str, t: torch.Tensor, logits: torch.Tensor, *shapes) -> None:
         raise ValueError(f"logits and {name} must be on one device")
 
 
-def _mask(mask, logits: torch.Tensor, seqs: int):
+def _mask(mask, logits: torch.Tensor, shape):
     """The mask as bool ``[tokens]`` or ``[seqs, tokens]``, or None."""
     if mask is None:
         return None
-    if mask.shape != logits.shape[:-1] and mask.shape != logits.shape[-2:-1]:
-        raise ValueError(f"mask must be {list(logits.shape[-2:-1])} or {list(logits.shape[:-1])}, got {list(mask.shape)}")
+    if mask.shape != shape and mask.shape != shape[-1:]:
+        raise ValueError(f"mask must be {list(shape[-1:])} or {list(shape)}, got {list(mask.shape)}")
     if mask.device != logits.device:
         raise ValueError("logits and mask must be on one device")
     if mask.dtype != torch.bool:
         mask = mask != 0
-    return mask if mask.dim() == 1 else mask.reshape(seqs, logits.shape[-2])
+    return mask if mask.dim() <= 2 else mask.reshape(shape[:-1].numel(), shape[-1])
 
 
 def _temperature(t: float) -> float:
@@ -85,61 +87,38 @@ def _reduction(name: str) -> int:
 
 def _fits(z: torch.Tensor, temperature: float, *others) -> bool:
     """Whether the kernels may take these: plain device tensors within the limits of ``e4b_logits``."""
+    if not _on_kernel(z):
+        return False
+    wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+    for t in others:
+        if t is not None and wrapped(t):
+            return False
     seqs, tokens, vocab = z.shape
-    return (_on_kernel(z) and seqs <= 2 ** 21 and seqs * tokens < 2 ** 31 and vocab <= 2 ** 30
-            and 1e-30 < temperature < 1e30 and all(t is None or _plain(t) for t in others))
-
-
-def _plain(t: torch.Tensor) -> bool:
-    return not torch._C._functorch.is_functorch_wrapped_tensor(t)
+    return seqs <= 2 ** 21 and seqs * tokens < 2 ** 31 and vocab <= 2 ** 30 and 1e-30 < temperature < 1e30
 
 
 def _rows(z: torch.Tensor) -> torch.Tensor:
     return z if z.stride(2) == 1 or z.shape[2] == 1 else z.contiguous()
 
 
-def _ints(t: torch.Tensor, *shape) -> torch.Tensor:
-    t = t if t.dtype == torch.int64 else t.to(torch.int64)
-    return _aligned(t if t.shape == shape else t.reshape(shape))
+def _contiguous(mask):
+    return mask if mask is None or mask.is_contiguous() else mask.contiguous()
 
 
-def _fp32(t, *shape):
-    """A constant as contiguous fp32."""
+def _constant(t, dtype, shape):
+    """A constant of the gradient, contiguous and of one dtype (or None)."""
     if t is None:
         return None
-    t = t.detach() if t.dtype == torch.float32 else t.detach().float()
-    return _aligned(t if t.shape == shape else t.reshape(shape))
-
-
-def _bools(mask):
-    return None if mask is None else _aligned(mask)
-
-
-def _once():
-    if torch.is_grad_enabled():
-        raise RuntimeError("the losses over logits are differentiable once: no create_graph=True on the device")
-
-
-def _differentiated(z: torch.Tensor) -> bool:
-    return z.requires_grad and torch.is_grad_enabled()
+    if t.requires_grad:
+        t = t.detach()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if t.shape != shape:
+        t = t.reshape(shape)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # ----------------------------------------------------------------------- log-probabilities
-
-
-class _Logprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, labels, mask, temperature):
-        logps, saved = ops.token_logprobs(z, labels, mask, temperature)
-        ctx.save_for_backward(z, labels, mask, saved)
-        ctx.temperature = temperature
-        return logps
-
-    @staticmethod
-    def backward(ctx, grad):
-        _once()
-        z, labels, mask, saved = ctx.saved_tensors
-        return ops.loss_backward(z, labels, mask, ctx.temperature, saved, grad, N.REDUCE_NONE), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tensor | None = None,
@@ -147,17 +126,15 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tenso
     """Log-probability of each label under ``softmax(logits / temperature)``: logits ``[..., T, V]``, labels ``[..., T]``
     integers, mask ``[T]`` or ``[..., T]`` -> fp32 ``[..., T]`` (fp64 for fp64 logits), 0 where a token does not count.
     Differentiable with respect to the logits (once)."""
-    z, lead = _sequences(logits)
-    _integers("labels", labels, logits, logits.shape[:-1])
-    m, t = _mask(mask, logits, z.shape[0]), _temperature(temperature)
-    if not _fits(z, t, labels, m):
-        return _token_logprobs_torch(z, labels.reshape(z.shape[:2]), m, t)[0].view(logits.shape[:-1])
-    z, labels, m = _rows(z), _ints(labels, *z.shape[:2]), _bools(m)
-    if _differentiated(z):
-        logps = _Logprobs.apply(z, labels, m, t)
+    z, shape = _sequences(logits)
+    _integers("labels", labels, logits, shape)
+    m, t = _mask(mask, logits, shape), _temperature(temperature)
+    flat = z.shape[:2]
+    if _fits(z, t, labels, m):
+        logps = N.torch_lib().token_logprobs(_rows(z), _constant(labels, torch.int64, flat), _contiguous(m), t)
     else:
-        logps, _ = ops.token_logprobs(z, labels, m, t, stats=False)
-    return logps if len(lead) == 1 else logps.view(logits.shape[:-1])
+        logps = _token_logprobs_torch(z, labels.reshape(flat), m, t)[0]
+    return logps if len(shape) == 2 else logps.view(shape)
 
 
 def _wide(z: torch.Tensor) -> torch.Tensor:
@@ -185,25 +162,6 @@ def _token_logprobs_torch(z, labels, mask, temperature):
 # ------------------------------------------------------------------------------ preference
 
 
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, labels, mask, ref, kind, beta, smoothing, average):
-        loss, rewards, saved = ops.preference_loss(z, labels, mask, ref, kind, beta, smoothing, average)
-        ctx.save_for_backward(z, labels, mask, saved)
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @staticmethod
-    def backward(ctx, grad, _):
-        none = (None,) * 7
-        if grad is None:
-            return None, *none
-        _once()
-        z, labels, mask, saved = ctx.saved_tensors
-        return ops.loss_backward(z, labels, mask, 1.0, saved, grad, N.REDUCE_SEQUENCE, coef="sequence"), *none
-
-
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor | None = None, beta: float = 0.1,
                     loss_type: str = "sigmoid", label_smoothing: float = 0.0, average: bool = False,
                     mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -218,11 +176,10 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     gradient. The loss is differentiable with respect to the logits (once)."""
     if logits.dim() != 3 or logits.shape[0] % 2:
         raise ValueError(f"logits must be [2 * pairs, tokens, vocab], got {list(logits.shape)}")
-    z, _ = _sequences(logits)
-    seqs, T, _ = z.shape
-    _integers("labels", labels, logits, logits.shape[:-1])
+    z, shape = _sequences(logits)
+    _integers("labels", labels, logits, shape)
     if ref_logps is not None:
-        _floats("ref_logps", ref_logps, logits, (seqs, T), (seqs,))
+        _floats("ref_logps", ref_logps, logits, shape, shape[:1])
     if loss_type not in _PREFERENCE:
         raise ValueError(f"loss_type must be one of {sorted(_PREFERENCE)}, got {loss_type!r}")
     if not (beta > 0 and math.isfinite(beta)):
@@ -231,17 +188,13 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"label_smoothing={label_smoothing} outside [0, 1]")
     if label_smoothing and loss_type != "sigmoid":
         raise ValueError("label_smoothing belongs to loss_type='sigmoid'")
-    m = _mask(mask, logits, seqs)
+    m = _mask(mask, logits, shape)
     kind = _PREFERENCE[loss_type]
     if not (_fits(z, 1.0, labels, m, ref_logps) and 1e-30 < beta < 1e30):
         return _preference_loss_torch(z, labels, m, ref_logps, kind, beta, label_smoothing, average)
-    z, labels, m = _rows(z), _ints(labels, seqs, T), _bools(m)
-    ref = None if ref_logps is None else _fp32(ref_logps, *ref_logps.shape)
-    args = (z, labels, m, ref, kind, float(beta), float(label_smoothing), bool(average))
-    if _differentiated(z):
-        return _Preference.apply(*args)
-    loss, rewards, _ = ops.preference_loss(*args)
-    return loss, rewards
+    ref = None if ref_logps is None else _constant(ref_logps, torch.float32, ref_logps.shape)
+    return N.torch_lib().preference_loss(_rows(z), _constant(labels, torch.int64, shape), _contiguous(m), ref, kind, beta,
+                                         label_smoothing, average)
 
 
 def _preference_loss_torch(z, labels, mask, ref, kind, beta, smoothing, average):
@@ -271,27 +224,6 @@ def _preference_loss_torch(z, labels, mask, ref, kind, beta, smoothing, average)
 # ---------------------------------------------------------------------------------- policy
 
 
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, labels, mask, old, advantages, ref, clip_lo, clip_hi, kl_coef, temperature, reduction):
-        loss, logps, saved = ops.policy_loss(z, labels, mask, old, advantages, ref, clip_lo, clip_hi, kl_coef, temperature,
-                                             reduction)
-        ctx.save_for_backward(z, labels, mask, saved)
-        ctx.temperature, ctx.reduction = temperature, reduction
-        ctx.mark_non_differentiable(logps)
-        ctx.set_materialize_grads(False)
-        return loss, logps
-
-    @staticmethod
-    def backward(ctx, grad, _):
-        none = (None,) * 10
-        if grad is None:
-            return None, *none
-        _once()
-        z, labels, mask, saved = ctx.saved_tensors
-        return ops.loss_backward(z, labels, mask, ctx.temperature, saved, grad, ctx.reduction, coef="token"), *none
-
-
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
                 ref_logps: torch.Tensor | None = None, clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0,
                 mask: torch.Tensor | None = None, temperature: float = 1.0,
@@ -304,39 +236,37 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     needs ``ref_logps``. ``reduction``: ``"mean"`` over all counted tokens (one value), ``"sequence"`` over
     each sequence's ``[...]``, ``"none"`` each token's ``[..., T]``; 0 where nothing counts. ``logps`` are constants
     to the gradient. The loss is differentiable with respect to the logits (once)."""
-    z, lead = _sequences(logits)
-    seqs, T, _ = z.shape
-    _integers("labels", labels, logits, logits.shape[:-1])
-    _floats("old_logps", old_logps, logits, logits.shape[:-1])
-    _floats("advantages", advantages, logits, lead, logits.shape[:-1])
+    z, shape = _sequences(logits)
+    _integers("labels", labels, logits, shape)
+    _floats("old_logps", old_logps, logits, shape)
+    _floats("advantages", advantages, logits, shape[:-1], shape)
     if ref_logps is not None:
-        _floats("ref_logps", ref_logps, logits, logits.shape[:-1])
+        _floats("ref_logps", ref_logps, logits, shape)
     elif kl_coef:
         raise ValueError("kl_coef needs ref_logps")
     if not math.isfinite(kl_coef):
         raise ValueError(f"kl_coef={kl_coef} is not finite")
-    lo, hi = (float(c) for c in clip)
+    lo, hi = clip
     if not (0 <= lo <= 1 and 0 <= hi and math.isfinite(hi)):
         raise ValueError(f"clip={tuple(clip)}: below in [0, 1], above not negative")
-    m, t, red = _mask(mask, logits, seqs), _temperature(temperature), _reduction(reduction)
-    ref = ref_logps if kl_coef else None
-    adv_shape = (seqs, T) if advantages.dim() > len(lead) else (seqs,)
-    if not _fits(z, t, labels, m, old_logps, advantages, ref):
-        loss, logps = _policy_loss_torch(z, labels.reshape(seqs, T), m, old_logps.reshape(seqs, T),
-                                         advantages.reshape(adv_shape), None if ref is None else ref.reshape(seqs, T),
-                                         1 - lo, 1 + hi, kl_coef, t, red)
+    m, t, red = _mask(mask, logits, shape), _temperature(temperature), _reduction(reduction)
+    ref, flat = ref_logps if kl_coef else None, z.shape[:2]
+    of_advantages = flat if advantages.dim() == len(shape) else flat[:1]
+    if _fits(z, t, labels, m, old_logps, advantages, ref):
+        loss, logps = N.torch_lib().policy_loss(
+            _rows(z), _constant(labels, torch.int64, flat), _contiguous(m), _constant(old_logps, torch.float32, flat),
+            _constant(advantages, torch.float32, of_advantages), _constant(ref, torch.float32, flat), 1 - lo, 1 + hi, kl_coef, t,
+            red)
     else:
-        z = _rows(z)
-        args = (z, _ints(labels, seqs, T), _bools(m), _fp32(old_logps, seqs, T), _fp32(advantages, *adv_shape),
-                _fp32(ref, seqs, T), 1 - lo, 1 + hi, float(kl_coef), t, red)
-        loss, logps = _Policy.apply(*args) if _differentiated(z) else ops.policy_loss(*args)[:2]
-    return _unflatten(loss, lead, T, red), logps if len(lead) == 1 else logps.view(*lead, T)
+        loss, logps = _policy_loss_torch(z, labels.reshape(flat), m, old_logps.reshape(flat), advantages.reshape(of_advantages),
+                                         None if ref is None else ref.reshape(flat), 1 - lo, 1 + hi, kl_coef, t, red)
+    return (loss, logps) if len(shape) == 2 else (_unflatten(loss, shape, red), logps.view(shape))
 
 
-def _unflatten(loss: torch.Tensor, lead, T: int, reduction: int) -> torch.Tensor:
-    if reduction == N.REDUCE_MEAN or len(lead) == 1:
+def _unflatten(loss: torch.Tensor, shape, reduction: int) -> torch.Tensor:
+    if reduction == N.REDUCE_MEAN or len(shape) == 2:
         return loss
-    return loss.view(lead if reduction == N.REDUCE_SEQUENCE else (*lead, T))
+    return loss.view(shape[:-1] if reduction == N.REDUCE_SEQUENCE else shape)
 
 
 def _reduce_torch(each, counted, reduction):
@@ -365,22 +295,6 @@ def _policy_loss_torch(z, labels, mask, old, advantages, ref, clip_lo, clip_hi, 
 # ---------------------------------------------------------------------------- distillation
 
 
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, mask, teacher, index, temperature, reduction):
-        loss, share, saved = ops.distill_loss(z, mask, teacher, index, temperature, reduction)
-        ctx.save_for_backward(z, mask, index, share, saved)
-        ctx.temperature, ctx.reduction = temperature, reduction
-        return loss
-
-    @staticmethod
-    def backward(ctx, grad):
-        _once()
-        z, mask, index, share, saved = ctx.saved_tensors
-        return (ops.loss_backward(z, None, mask, ctx.temperature, saved, grad, ctx.reduction, index=index, share=share),
-                None, None, None, None, None)
-
-
 def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                  mask: torch.Tensor | None = None, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """Distillation from a teacher's top logits: logits ``[..., T, V]``, ``teacher_logits`` and ``teacher_index`` ``[..., T,
@@ -391,25 +305,20 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     Entries whose index is outside ``[0, V)`` or whose value is ``-inf`` have no probability; a token without any has
     loss 0 (and counts, if its mask says so). ``reduction`` as in ``policy_loss``. Differentiable with respect to
     the logits (once)."""
-    z, lead = _sequences(logits)
-    seqs, T, _ = z.shape
-    if teacher_index.dim() != logits.dim() or not teacher_index.shape[-1]:
-        raise ValueError(f"teacher_index must be {list(logits.shape[:-1])} and at least one entry, got "
-                         f"{list(teacher_index.shape)}")
+    z, shape = _sequences(logits)
+    if teacher_index.dim() != len(shape) + 1 or not teacher_index.shape[-1]:
+        raise ValueError(f"teacher_index must be {list(shape)} and at least one entry, got {list(teacher_index.shape)}")
     K = teacher_index.shape[-1]
-    shape = (*logits.shape[:-1], K)
-    _integers("teacher_index", teacher_index, logits, shape)
-    _floats("teacher_logits", teacher_logits, logits, shape)
-    m, t, red = _mask(mask, logits, seqs), _temperature(temperature), _reduction(reduction)
-    if not (_fits(z, t, m, teacher_logits, teacher_index) and K <= _MAX_TOP and teacher_logits.dtype in ops._DT):
-        loss = _distill_loss_torch(z, m, teacher_logits.reshape(seqs, T, K), teacher_index.reshape(seqs, T, K), t, red)
+    _integers("teacher_index", teacher_index, logits, (*shape, K))
+    _floats("teacher_logits", teacher_logits, logits, (*shape, K))
+    m, t, red = _mask(mask, logits, shape), _temperature(temperature), _reduction(reduction)
+    flat = (*z.shape[:2], K)
+    if _fits(z, t, m, teacher_logits, teacher_index) and K <= _MAX_TOP and teacher_logits.dtype in ops._DT:
+        loss = N.torch_lib().distill_loss(_rows(z), _contiguous(m), _constant(teacher_logits, teacher_logits.dtype, flat),
+                                          _constant(teacher_index, torch.int64, flat), t, red)
     else:
-        z = _rows(z)
-        values = teacher_logits.detach()
-        args = (z, _bools(m), _aligned(values if len(lead) == 1 else values.reshape(seqs, T, K)),
-                _ints(teacher_index, seqs, T, K), t, red)
-        loss = _Distill.apply(*args) if _differentiated(z) else ops.distill_loss(*args)[0]
-    return _unflatten(loss, lead, T, red)
+        loss = _distill_loss_torch(z, m, teacher_logits.reshape(flat), teacher_index.reshape(flat), t, red)
+    return _unflatten(loss, shape, red)
 
 
 def _distill_loss_torch(z, mask, teacher, index, temperature, reduction):

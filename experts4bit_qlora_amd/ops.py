@@ -379,129 +379,6 @@ def balance_loss_backward(logits: torch.Tensor, mask: torch.Tensor | None, count
     return out
 
 
-# ------------------------------------------------------------------- losses over the vocabulary
-
-
-def _logits(z: torch.Tensor, labels, mask, temperature: float) -> N.Logits:
-    """``e4b_logits`` of ``[seqs, tokens, vocab]`` logits whose last axis is contiguous; labels ``[seqs, tokens]`` int64
-    and mask ``[tokens]`` or ``[seqs, tokens]`` bool contiguous, or None."""
-    seqs, tokens, vocab = z.shape
-    s0, s1, _ = z.stride()
-    return N.Logits(z.data_ptr(), _DT[z.dtype], temperature, seqs, tokens, vocab, s0, s1, _ptr(labels), _ptr(mask),
-                    0 if mask is None or mask.dim() == 1 else tokens)
-
-
-def token_logprobs(z: torch.Tensor, labels: torch.Tensor, mask, temperature: float, stats: bool = True):
-    """(log-probabilities of the labels fp32 ``[seqs, tokens]``, the rows' statistics fp32 ``[seqs * tokens, 4]`` for
-    ``loss_backward``, or None) by ``e4b_token_logprobs``."""
-    _require_cuda(z, labels, mask)
-    dev, (seqs, tokens, _) = z.device, z.shape
-    logps = torch.empty(seqs, tokens, dtype=torch.float32, device=dev)
-    saved = torch.empty(seqs * tokens * 4, dtype=torch.float32, device=dev) if stats else None
-    with _on(dev):
-        N.check("e4b_token_logprobs",
-                N.lib().e4b_token_logprobs(_logits(z, labels, mask, temperature), logps.data_ptr(), _ptr(saved), _stream(dev)))
-    return logps, saved
-
-
-def preference_loss(z: torch.Tensor, labels: torch.Tensor, mask, ref, kind: int, beta: float, smoothing: float,
-                    average: bool):
-    """(loss fp32 ``[seqs / 2]``, rewards fp32 ``[seqs]``, what ``loss_backward`` needs: the rows' statistics, then
-    the sequences' derivatives) by ``e4b_preference_loss``; ref fp32 ``[seqs, tokens]``, ``[seqs]`` or None."""
-    _require_cuda(z, labels, mask, ref)
-    dev, (seqs, tokens, _) = z.device, z.shape
-    loss = torch.empty(seqs // 2, dtype=torch.float32, device=dev)
-    rewards = torch.empty(seqs, dtype=torch.float32, device=dev)
-    R = seqs * tokens
-    saved = torch.empty(4 * R + seqs, dtype=torch.float32, device=dev)
-    at = saved.data_ptr()
-    with _on(dev):
-        N.check("e4b_preference_loss",
-                N.lib().e4b_preference_loss(_logits(z, labels, mask, 1.0), _ptr(ref), 0 if ref is None else ref.dim() == 2,
-                                        kind, beta, smoothing, average, loss.data_ptr(), rewards.data_ptr(), at,
-                                        at + 16 * R, _stream(dev)))
-    return loss, rewards, saved
-
-
-def _reduced(seqs: int, tokens: int, reduction: int, device):
-    """(an empty loss, the number of its means)"""
-    shape = ((seqs, tokens), (seqs,), ())[reduction]
-    return torch.empty(shape, dtype=torch.float32, device=device), (0, seqs, 1)[reduction]
-
-
-def policy_loss(z: torch.Tensor, labels: torch.Tensor, mask, old_logps: torch.Tensor, advantages: torch.Tensor, ref_logps,
-                clip_lo: float, clip_hi: float, kl_coef: float, temperature: float, reduction: int):
-    """(loss fp32, log-probabilities fp32 ``[seqs, tokens]``, what ``loss_backward`` needs: the rows' statistics,
-    the tokens' derivatives, the means' factors) by ``e4b_policy_loss``; fp32 inputs, advantages ``[seqs]`` or
-    ``[seqs, tokens]``."""
-    _require_cuda(z, labels, mask, old_logps, advantages, ref_logps)
-    dev, (seqs, tokens, _) = z.device, z.shape
-    loss, means = _reduced(seqs, tokens, reduction, dev)
-    logps = torch.empty(seqs, tokens, dtype=torch.float32, device=dev)
-    R = seqs * tokens
-    saved = torch.empty(5 * R + means + (R if means else 0), dtype=torch.float32, device=dev)
-    at = saved.data_ptr()
-    inv = at + 20 * R
-    with _on(dev):
-        N.check("e4b_policy_loss",
-                N.lib().e4b_policy_loss(_logits(z, labels, mask, temperature), old_logps.data_ptr(), advantages.data_ptr(),
-                                    advantages.dim() == 2, _ptr(ref_logps), clip_lo, clip_hi, kl_coef, reduction,
-                                    logps.data_ptr(), inv + 4 * means if means else loss.data_ptr(), at, at + 16 * R,
-                                    loss.data_ptr(), inv, _stream(dev)))
-    return loss, logps, saved
-
-
-def distill_loss(z: torch.Tensor, mask, teacher: torch.Tensor, index: torch.Tensor, temperature: float, reduction: int):
-    """(loss fp32, the teacher's probabilities fp32 ``[seqs, tokens, top]``, what ``loss_backward`` needs: the
-    rows' statistics, the means' factors) by ``e4b_distill_loss``."""
-    _require_cuda(z, mask, teacher, index)
-    dev, (seqs, tokens, _) = z.device, z.shape
-    loss, means = _reduced(seqs, tokens, reduction, dev)
-    share = torch.empty(index.shape, dtype=torch.float32, device=dev)
-    R = seqs * tokens
-    saved = torch.empty(4 * R + means + (R if means else 0), dtype=torch.float32, device=dev)
-    at = saved.data_ptr()
-    inv = at + 16 * R
-    with _on(dev):
-        N.check("e4b_distill_loss",
-                N.lib().e4b_distill_loss(_logits(z, None, mask, temperature), teacher.data_ptr(), dtype_code(teacher.dtype),
-                                     index.data_ptr(), index.shape[2], reduction, share.data_ptr(),
-                                     inv + 4 * means if means else loss.data_ptr(), at, loss.data_ptr(), inv, _stream(dev)))
-    return loss, share, saved
-
-
-_PAIR = ctypes.c_int64 * 2
-
-
-def loss_backward(z: torch.Tensor, labels, mask, temperature: float, saved: torch.Tensor, grad: torch.Tensor, reduction: int,
-                  coef: str | None = None, index=None, share=None) -> torch.Tensor:
-    """dL/dlogits from dL/dloss fp32 (any strides; one per pair serves both sequences), ``saved`` as the forward returned it (``e4b_loss_backward``).
-    reduction: what ``grad`` is the gradient of; coef: ``"token"`` or ``"sequence"`` derivatives behind the
-    rows' statistics; index, share: a teacher's entries."""
-    _require_cuda(z, labels, mask, saved, grad, index, share)
-    dev, (seqs, tokens, vocab) = z.device, z.shape
-    R = seqs * tokens
-    out = torch.empty(seqs, tokens, vocab, dtype=z.dtype, device=dev)
-    at = saved.data_ptr()
-    strides = coef_at = coef_strides = inv = None
-    if reduction == N.REDUCE_NONE:
-        strides = _PAIR(*grad.stride())
-    else:
-        strides = _PAIR(grad.stride(0) if grad.dim() else 0, 0)
-    behind = at + 16 * R
-    if coef is not None:
-        coef_at, coef_strides = behind, _PAIR(tokens, 1) if coef == "token" else _PAIR(1, 0)
-        behind += 4 * R
-    if reduction != N.REDUCE_NONE and coef != "sequence":
-        inv = behind
-    with _on(dev):
-        N.check("e4b_loss_backward",
-                N.lib().e4b_loss_backward(_logits(z, labels, mask, temperature), at, grad.data_ptr(), grad.shape[0] if grad.dim() else 1, strides,
-                                      coef_at, coef_strides, inv, int(reduction == N.REDUCE_SEQUENCE), _ptr(index), _ptr(share),
-                                      0 if index is None else index.shape[2], out.data_ptr(), _stream(dev)))
-    return out
-
-
 # -------------------------------------------------------------------------------- GEMMs
 
 

@@ -33,6 +33,23 @@ def test_exports_every_declared_symbol():
         assert hasattr(raw, name), f"{name} declared in include/e4b_amd.h but not exported"
 
 
+def test_the_torch_binding_loads_and_refuses_host_tensors():
+    import torch
+
+    ext = N.torch_lib()
+    assert ext is N.torch_lib()
+    z, labels = torch.zeros(2, 3, 4), torch.zeros(2, 3, dtype=torch.int64)
+    one = torch.zeros(2, 3)
+    for call in (lambda: ext.token_logprobs(z, labels, None, 1.0),
+                 lambda: ext.preference_loss(z, labels, None, None, 0, 0.1, 0.0, False),
+                 lambda: ext.policy_loss(z, labels, None, one, one, None, 0.8, 1.2, 0.0, 1.0, 2),
+                 lambda: ext.distill_loss(z, None, one.unsqueeze(-1), labels.unsqueeze(-1), 1.0, 2)):
+        with pytest.raises(ValueError, match="HIP device"):
+            call()
+    with pytest.raises(ValueError, match="different devices"):
+        ext.token_logprobs(z, labels.to("meta"), None, 1.0)
+
+
 def test_enums_match_header():
     src = open(HEADER).read()
     for name, val in (("E4B_FMT_NF4", N.FMT_NF4), ("E4B_FMT_NF4_DQ", N.FMT_NF4_DQ), ("E4B_FMT_MXFP4", N.FMT_MXFP4),

@@ -287,8 +287,13 @@ def test_sizes_beyond_the_kernels_take_the_torch_formulation(monkeypatch):
     """Broadcast tensors of one element, seen as device tensors: nothing of these sizes is made."""
     seen = []
     monkeypatch.setattr(L, "_on_kernel", lambda t: True)
-    monkeypatch.setattr(L, "_aligned", lambda t: t)
-    monkeypatch.setattr(L.ops, "token_logprobs", lambda z, *a, **k: seen.append("kernel") or (torch.zeros(1, 1).expand(z.shape[:2]), None))
+    monkeypatch.setattr(L, "_constant", lambda t, *a: t)
+
+    class Kernels:
+        token_logprobs = staticmethod(lambda z, *a: seen.append("kernel") or torch.zeros(1, 1).expand(z.shape[:2]))
+        distill_loss = staticmethod(lambda *a: seen.append("kernel") or torch.zeros(()))
+
+    monkeypatch.setattr(L.N, "torch_lib", lambda: Kernels)
     monkeypatch.setattr(L, "_token_logprobs_torch", lambda z, *a: seen.append("torch") or (torch.zeros(1, 1).expand(z.shape[:2]), None))
     z, labels = torch.zeros(1, 1, 1), torch.zeros(1, 1, dtype=torch.int64)
     for shape in ((1, 5, 4), (1 << 21, 2, 4), (1, (1 << 31) - 1, 4), (1, 2, 1 << 30)):
@@ -298,7 +303,6 @@ def test_sizes_beyond_the_kernels_take_the_torch_formulation(monkeypatch):
         e4b.token_logprobs(z.expand(shape), labels.expand(shape[:2]))
     e4b.token_logprobs(z, labels, temperature=1e-31)
     assert seen[4:] == ["torch"] * 5
-    monkeypatch.setattr(L.ops, "distill_loss", lambda *a: seen.append("kernel") or (torch.zeros(()), None, None))
     monkeypatch.setattr(L, "_distill_loss_torch", lambda *a: seen.append("torch") or torch.zeros(()))
     for k, dtype in ((1024, torch.float32), (1025, torch.float32), (4, torch.float64)):
         e4b.distill_loss(z, torch.zeros(1, 1, 1, dtype=dtype).expand(1, 1, k), labels.unsqueeze(-1).expand(1, 1, k))
