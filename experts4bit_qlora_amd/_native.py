@@ -49,6 +49,7 @@ EXPORTS = (
     "e4b_balance_workspace_bytes",
     "e4b_balance_loss",
     "e4b_balance_loss_backward",
+    "e4b_loss_workspace_bytes",
     "e4b_token_logprobs",
     "e4b_preference_loss",
     "e4b_policy_loss",
@@ -151,6 +152,8 @@ class Logits(ctypes.Structure):
         ("labels", ctypes.c_void_p),
         ("mask", ctypes.c_void_p),
         ("mask_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -192,6 +195,8 @@ def _bind(L):
     L.e4b_balance_loss_backward.restype = ctypes.c_int
     L.e4b_balance_loss_backward.argtypes = [P, I32, I32, I64, I32, P, I64, P, P, P, P, P]
     LG, PAIR = ctypes.POINTER(Logits), ctypes.POINTER(ctypes.c_int64)
+    L.e4b_loss_workspace_bytes.restype = ctypes.c_size_t
+    L.e4b_loss_workspace_bytes.argtypes = [LG]
     L.e4b_token_logprobs.restype = ctypes.c_int
     L.e4b_token_logprobs.argtypes = [LG, P, P, P]
     L.e4b_preference_loss.restype = ctypes.c_int

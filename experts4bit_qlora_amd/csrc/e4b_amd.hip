@@ -310,10 +310,20 @@ float2 exponent_scale(float temperature) {
   return make_float2(hi, static_cast<float>(k - hi));
 }
 
+// A forward's workspace.
+int check_loss_workspace(const e4b_logits& z) {
+  const size_t need = e4b_loss_workspace_bytes(&z);
+  if (need && (!z.workspace || z.workspace_bytes < need))
+    return fail(E4B_ESPACE, "workspace %zu bytes < %zu needed", z.workspace ? z.workspace_bytes : 0, need);
+  if (reinterpret_cast<uintptr_t>(z.workspace) & 7) return fail(E4B_EINVAL, "workspace must be 8-byte aligned");
+  return E4B_OK;
+}
+
 e4b::LossArgs loss_args(const e4b_logits& z, float* stats) {
   e4b::LossArgs a{};
   a.z = z;
   a.k = exponent_scale(z.temperature);
+  a.parts = e4b::loss_parts(z);
   a.stats = reinterpret_cast<float4*>(stats);
   return a;
 }
@@ -770,14 +780,22 @@ int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers,
   return check_launch("balance_backward_kernel");
 }
 
+size_t e4b_loss_workspace_bytes(const e4b_logits* z) {
+  if (!z || z->seqs <= 0 || z->tokens <= 0 || z->seqs > e4b::kLossMaxSeqs || z->tokens > 0x7fffffffLL ||
+      z->vocab > e4b::kLossMaxVocab)
+    return 0;
+  return sizeof(float2) * z->seqs * z->tokens * e4b::loss_parts(*z);
+}
+
 int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream) {
   alignas(16) const char none[16] = {};  // stats may be NULL here
   const int rc = check_logits(z, true, stats ? static_cast<const void*>(stats) : none);
   if (rc || z->seqs * z->tokens == 0) return rc;
   if (!logps) return fail(E4B_EINVAL, "logps is NULL");
+  if (const int bad = check_loss_workspace(*z)) return bad;
   e4b::LossArgs a = loss_args(*z, stats);
   a.logps = logps;
-  e4b::launch_loss_rows(e4b::kLogprobs, a, stream);
+  e4b::launch_loss_rows(stats ? e4b::kLogprobs : e4b::kScore, a, stream);
   return check_launch("loss_rows_kernel");
 }
 
@@ -792,6 +810,7 @@ int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_t
   if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return fail(E4B_EINVAL, "smoothing outside [0, 1]");
   if (z->seqs == 0) return E4B_OK;
   if (!loss || !rewards || !coef) return fail(E4B_EINVAL, "loss/rewards/coef is NULL");
+  if ((rc = check_loss_workspace(*z))) return rc;
   e4b::LossArgs a = loss_args(*z, stats);
   if (z->tokens) e4b::launch_loss_rows(e4b::kStats, a, stream);
   const e4b::PairArgs p{z->seqs, z->tokens, a.stats, ref, ref_per_token, kind, beta, smoothing, average, loss, rewards, coef};
@@ -809,6 +828,7 @@ int e4b_policy_loss(const e4b_logits* z, const float* old_logps, const float* ad
   if (!std::isfinite(kl_coef)) return fail(E4B_EINVAL, "kl_coef is not finite");
   if (z->seqs * z->tokens) {
     if (!old_logps || !advantages || !logps || !coef) return fail(E4B_EINVAL, "old_logps/advantages/logps/coef is NULL");
+    if ((rc = check_loss_workspace(*z))) return rc;
     e4b::LossArgs a = loss_args(*z, stats);
     a.logps = logps;
     a.old_logps = old_logps;
@@ -838,6 +858,7 @@ int e4b_distill_loss(const e4b_logits* z, const void* teacher, int32_t teacher_d
   if (top > e4b::kLossMaxTop) return fail(E4B_EUNSUPPORTED, "top=%d > %d", top, e4b::kLossMaxTop);
   if (z->seqs * z->tokens) {
     if (!teacher || !index || !share) return fail(E4B_EINVAL, "teacher/index/share is NULL");
+    if ((rc = check_loss_workspace(*z))) return rc;
     e4b::LossArgs a = loss_args(*z, stats);
     a.z.labels = nullptr;
     a.teacher = teacher;

@@ -80,9 +80,10 @@ struct Split {
   }
 };
 
-// 16 bytes at any address that the type's values may have, and to an aligned one. The backward's logits are read for the
-// last time and its gradient is larger than the caches: past them, both (1,500 x 128,000 bf16: 143 -> 122 us, the stores
-// alone 125; 5,500 x 50,257: 184 -> 185; 252 x 50,257, which the caches would hold: 13.7 -> 12.2).
+// 16 bytes at any address that the type's values may have, and to an aligned one, past the caches: logits that are read for the
+// last time, gradients, which are as large. Backward of 1,500 x 128,000 bf16: 143 -> 122 us (the stores alone 125), of
+// 5,500 x 50,257 184 -> 185, of 252 x 50,257 13.7 -> 12.2. A forward that no backward follows: 5,500 x 128,000 232 -> 214, 252 x
+// 50,257 9.6 -> 10.0; one that a backward follows leaves it what the caches hold (both, 5,500 x 128,000: 668 -> 682).
 E4B_DEV uint4 load16_once(const void* p) {
   typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
   const Any v = __builtin_nontemporal_load(static_cast<const Any*>(p));
@@ -99,13 +100,23 @@ E4B_DEV void store16_once(uint4* p, const uint4& v) {
 // their size, which a sequence's sum of log-probabilities adds up (820 tokens: 2e-4).
 E4B_DEV float exp_of(float d, float2 k) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.x, d * k.y)); }
 
-struct Run {
-  float m = kLowest, s = 0.0f;
-  E4B_DEV void join(float om, float os, float2 k) {
+// S: the sum's type. A thread's own is fp32; the joins are in 64 bits where a sequence's sum follows (kStats): each of nine
+// roundings of a row's whole sum would be one of its log-probability, and 60 tokens' are as large as 1e-6 of their ratio.
+template <class S>
+struct RunOf {
+  float m = kLowest;
+  S s = 0;
+  E4B_DEV void join(float om, S os, float2 k) {
     const float n = fmaxf(m, om);
     s = s * exp_of(m - n, k) + os * exp_of(om - n, k);
     m = n;
   }
+  E4B_DEV void join_lanes(int lanes, float2 k) {
+    for (int off = 1; off < lanes; off *= 2) join(__shfl_xor(m, off), __shfl_xor(s, off), k);
+  }
+};
+
+struct Run : RunOf<float> {
   template <int N>
   E4B_DEV void add(const float (&x)[N], float2 k) {
     float n = m;
@@ -120,18 +131,24 @@ struct Run {
 };
 
 constexpr int kRowUnroll = 4;  // pieces in flight per thread
+constexpr int kPartThreads = 256;
+template <int DT>
+constexpr int kPartPieces = kPartValues / Piece<DT>::kCount;
 
-// The maximum and the sum of a row without its element `skip` (-1: of all), in every lane of the first wave.
-template <int DT, int NT, int U>
-E4B_DEV Run row_run(const void* row, int V, int skip, float2 k) {
+// The maximum and the sum of a row without its element `skip` (-1: of all), in every lane of the first wave; of its pieces
+// [begin, end) alone where it is split (the first of the parts takes the single values at the row's ends).
+template <int DT, int NT, int U, bool ONCE, class S>
+E4B_DEV RunOf<S> row_run(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
   using P = Piece<DT>;
   const typename P::T* p = static_cast<const typename P::T*>(row);
   const Split<DT> at(row, V);
   const int tid = threadIdx.x;
   Run r;
   float edge[2] = {-__builtin_inff(), -__builtin_inff()};
-  if (tid < at.head && tid != skip) edge[0] = P::one(p[tid]);
-  if (tid < V - at.tail && at.tail + tid != skip) edge[1] = P::one(p[at.tail + tid]);
+  if (begin == 0) {
+    if (tid < at.head && tid != skip) edge[0] = P::one(p[tid]);
+    if (tid < V - at.tail && at.tail + tid != skip) edge[1] = P::one(p[at.tail + tid]);
+  }
   // the skipped element's piece (one that no thread takes where it is none) and its place there
   const int skip_at = skip < at.head ? -1 : (skip - at.head) / P::kCount, skip_off = (skip - at.head) % P::kCount;
   auto take = [&](const uint4& w, int i) {
@@ -145,31 +162,43 @@ E4B_DEV Run row_run(const void* row, int V, int skip, float2 k) {
     return r.add(x, k);
   };
   const uint4* v = reinterpret_cast<const uint4*>(p + at.head);
-  int i = tid;
-  for (; i + (U - 1) * NT < at.pieces; i += U * NT) {
+  const int last = min(end, at.pieces);
+  int i = begin + tid;
+  for (; i + (U - 1) * NT < last; i += U * NT) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = v[i + u * NT];
+    for (int u = 0; u < U; ++u) w[u] = ONCE ? load16_once(v + i + u * NT) : v[i + u * NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) take(w[u], i + u * NT);
   }
-  for (; i < at.pieces; i += NT) take(v[i], i);
+  for (; i < last; i += NT) take(v[i], i);
   r.add(edge, k);
-#pragma unroll
-  for (int off = 1; off < kWave; off *= 2) r.join(__shfl_xor(r.m, off), __shfl_xor(r.s, off), k);
+  RunOf<S> all{r.m, static_cast<S>(r.s)};
+  all.join_lanes(kWave, k);
   if constexpr (NT > kWave) {
     constexpr int W = NT / kWave;
-    __shared__ float2 part[W];
-    if ((tid & (kWave - 1)) == 0) part[tid / kWave] = make_float2(r.m, r.s);
+    __shared__ float part_m[W];
+    __shared__ S part_s[W];
+    if ((tid & (kWave - 1)) == 0) {
+      part_m[tid / kWave] = all.m;
+      part_s[tid / kWave] = all.s;
+    }
     __syncthreads();
     if (tid < kWave) {
-      const float2 o = part[tid & (W - 1)];
-      r.m = o.x;
-      r.s = o.y;
-#pragma unroll
-      for (int off = 1; off < W; off *= 2) r.join(__shfl_xor(r.m, off), __shfl_xor(r.s, off), k);
+      all.m = part_m[tid & (W - 1)];
+      all.s = part_s[tid & (W - 1)];
+      all.join_lanes(W, k);
     }
   }
+  return all;
+}
+
+// The same of a split row, from its parts.
+template <class S>
+E4B_DEV RunOf<S> joined_run(const float2* parts, int count, float2 k) {
+  RunOf<S> r;
+  for (int i = threadIdx.x; i < count; i += kWave) r.join(parts[i].x, parts[i].y, k);
+  r.join_lanes(kWave, k);
   return r;
 }
 
@@ -207,39 +236,48 @@ struct Token {
 // The teacher's part of a row, by the first wave: probabilities over its usable entries (an index inside the
 // vocabulary, a value above -inf) and tau^2 sum_k p_k (log p_k - log q_k); zero where no entry is usable.
 template <int DT>
-E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, Run& r) {
+E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, RunOf<float>& r) {
   const float tau = a.z.temperature, per = 1.0f / tau;
   const int lane = threadIdx.x;
   const int64_t first = at * a.top;
-  float most = -__builtin_inff();
-  bool bad = false;
-  for (int k = lane; k < a.top; k += kWave) {
-    const int64_t j = a.index[first + k];
-    if (j >= 0 && j < a.z.vocab) {
-      const float w = any_float(a.teacher, a.teacher_dtype, first + k);
-      most = fmaxf(most, w);
-      bad |= w != w;
-    }
+  struct Entry {
+    int64_t j;
+    float w;  // -inf where the index is outside
+  };
+  auto load = [&](int k) {
+    Entry e{k < a.top ? a.index[first + k] : -1, -__builtin_inff()};
+    if (e.j >= 0 && e.j < a.z.vocab) e.w = any_float(a.teacher, a.teacher_dtype, first + k);
+    else e.j = -1;
+    return e;
+  };
+  const Entry own = load(lane);  // the others are loaded again in each pass
+  auto entry = [&](int k) { return k == lane ? own : load(k); };
+  float most = own.w;
+  bool bad = own.w != own.w;
+  for (int k = lane + kWave; k < a.top; k += kWave) {
+    const float w = load(k).w;
+    most = fmaxf(most, w);
+    bad |= w != w;
   }
   most = wave_max(most);
   const bool none = most == -__builtin_inff() && !__any(bad);
   float norm = 0.0f;
   if (!none)
     for (int k = lane; k < a.top; k += kWave) {
-      const int64_t j = a.index[first + k];
-      if (j >= 0 && j < a.z.vocab) norm += expf((any_float(a.teacher, a.teacher_dtype, first + k) - most) * per);
+      const Entry e = entry(k);
+      if (e.j >= 0) norm += expf((e.w - most) * per);
     }
   norm = wave_sum(norm);
   const float log_norm = logf(norm), log_s = logf(r.s), inv = 1.0f / norm;
   float sum = 0.0f;
   for (int k = lane; k < a.top; k += kWave) {
-    const int64_t j = a.index[first + k];
+    const Entry e = entry(k);
     float p = 0.0f;
-    if (!none && j >= 0 && j < a.z.vocab) {
-      const float w = (any_float(a.teacher, a.teacher_dtype, first + k) - most) * per;
+    if (!none && e.j >= 0) {
+      const float w = (e.w - most) * per;
       p = expf(w) * inv;
       // log p - log q; an entry without probability adds nothing, whatever the student holds there
-      const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[j]) - r.m) * per - log_s;
+      const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[e.j]) - r.m) * per - log_s;
       if (!(p == 0.0f)) sum += p * ((w - log_norm) - lq);
     }
     a.share[first + k] = p;
@@ -248,6 +286,21 @@ E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<D
   return tau * tau * wave_sum(sum);
 }
 
+// A workgroup per part of a row, where there are few rows.
+template <int KIND, int DT>
+__global__ __launch_bounds__(kPartThreads) void loss_parts_kernel(LossArgs a) {
+  using P = Piece<DT>;
+  const int64_t at = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts, step = kPartPieces<DT>;
+  const Token tok(a.z, at, P::kBytes);
+  if (!tok.counts) return;
+  const RunOf<float> r = row_run<DT, kPartThreads, kRowUnroll, KIND == kScore, float>(tok.row, static_cast<int>(a.z.vocab),
+                                                      KIND == kDistill ? -1 : static_cast<int>(tok.label), a.k, part * step,
+                                                      (part + 1) * step);
+  if (threadIdx.x == 0) static_cast<float2*>(a.z.workspace)[blockIdx.x] = make_float2(r.m, r.s);
+}
+
+// A workgroup per row, or a wave that joins a split row's parts (NT = 64).
 template <int KIND, int DT, int NT, int U>
 __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin) {
   using P = Piece<DT>;
@@ -256,8 +309,8 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   const bool lead = threadIdx.x == 0;
   if (!tok.counts) {
     if (lead) {
-      if (a.stats) a.stats[at] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);
-      if (KIND == kLogprobs || KIND == kPolicy) a.logps[at] = 0.0f;
+      if (KIND != kScore) a.stats[at] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);
+      if (KIND == kLogprobs || KIND == kScore || KIND == kPolicy) a.logps[at] = 0.0f;
       if (KIND == kPolicy || KIND == kDistill) a.token_loss[at] = 0.0f;
       if (KIND == kPolicy) a.coef[at] = 0.0f;
     }
@@ -266,7 +319,10 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   const typename P::T* row = reinterpret_cast<const typename P::T*>(tok.row);
   float own = 0.0f;
   if (KIND != kDistill) own = P::one(row[tok.label]);
-  Run r = row_run<DT, NT, U>(row, static_cast<int>(a.z.vocab), KIND == kDistill ? -1 : static_cast<int>(tok.label), a.k);
+  const int V = static_cast<int>(a.z.vocab), skip = KIND == kDistill ? -1 : static_cast<int>(tok.label);
+  using S = std::conditional_t<KIND == kStats, double, float>;
+  RunOf<S> r = NT == kWave ? joined_run<S>(static_cast<const float2*>(a.z.workspace) + at * a.parts, a.parts, a.k)
+                           : row_run<DT, NT, U, KIND == kScore, S>(row, V, skip, a.k);
   if (threadIdx.x >= kWave) return;
   if constexpr (KIND == kDistill) {
     const float loss = teacher_loss<DT>(a, at, row, r);
@@ -275,11 +331,13 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   } else if (lead) {
     // join the label; (own - m) / tau also where it is 0, for a label of +inf. The sum is 0 where every logit is -inf: each
     // label has probability 0
-    const float m = fmaxf(r.m, own), rest = r.s * exp_of(r.m - m, a.k), s = rest + exp_of(own - m, a.k);
+    const float m = fmaxf(r.m, own);
+    const S rest = r.s * exp_of(r.m - m, a.k);
+    const float s = static_cast<float>(rest + exp_of(own - m, a.k));
     float lp, low = 0.0f;
     if constexpr (KIND == kStats) {  // for long sums, in 64 bits
       const double d = (static_cast<double>(own) - m) / a.z.temperature;
-      const double l = d - (own == m ? log1p(static_cast<double>(rest)) : log(rest + exp(d)));
+      const double l = d - (own == m ? log1p(rest) : log(rest + exp(d)));
       lp = static_cast<float>(l);
       low = lp - lp == 0.0f ? static_cast<float>(l - lp) : 0.0f;
     } else {
@@ -287,7 +345,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
     }
     if (s == 0.0f) lp = -__builtin_inff();
     if (KIND != kStats) a.logps[at] = lp;
-    if (a.stats) a.stats[at] = make_float4(m, s, lp, low);
+    if (KIND != kScore) a.stats[at] = make_float4(m, s, lp, low);
     if constexpr (KIND == kPolicy) {
       const float adv = a.advantages[a.adv_per_token ? at : tok.n];
       const float ratio = expf(lp - a.old_logps[at]);

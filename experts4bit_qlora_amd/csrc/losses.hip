@@ -18,6 +18,12 @@ void by_launch(int64_t rows, int64_t per, int threads, F&& f) {
 
 template <int KIND, int DT>
 void rows_of(const LossArgs& a, hipStream_t s) {
+  if (a.parts) {
+    const unsigned rows = static_cast<unsigned>(a.z.seqs * a.z.tokens);
+    hipLaunchKernelGGL((loss_parts_kernel<KIND, DT>), dim3(rows * a.parts), dim3(kPartThreads), 0, s, a);
+    hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, kWave, kRowUnroll>), dim3(rows), dim3(kWave), 0, s, a, int64_t(0));
+    return;
+  }
   const auto with = [&](auto nt) {
     by_launch(a.z.seqs * a.z.tokens, 1, nt(), [&](int64_t first, int64_t rows) {
       hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, nt(), kRowUnroll>), dim3(static_cast<unsigned>(rows)), dim3(nt()), 0, s, a,
@@ -64,9 +70,18 @@ void backward_of(const LossBackwardArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// One CU takes 8 us over the exponentials of 128,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
+// joined in a second launch (~3 us). Whole rows / split, us: 1 row of 50,257 bf16 6.8 / 7.2, of 65,536 7.3 / 7.1, of
+// 128,000 12.0 / 6.4; 37 rows of 65,536 7.9 / 7.3, of 128,000 14.3 / 8.6; 64 of 65,536 9.0 / 8.0, of 128,000 14.3 / 10.0; 128 of
+// 65,536 9.5 / 10.1, of 128,000 14.8 / 13.1 and fp32 17.1 / 18.6; 252 of 128,000 16.5 / 20.8.
+int loss_parts(const e4b_logits& z) {
+  return z.seqs * z.tokens <= 64 && z.vocab >= 65536 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
+}
+
 void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s) {
   switch (kind) {
     case kStats: return rows_of<kStats>(a, s);
+    case kScore: return rows_of<kScore>(a, s);
     case kLogprobs: return rows_of<kLogprobs>(a, s);
     case kPolicy: return rows_of<kPolicy>(a, s);
     default: return rows_of<kDistill>(a, s);

@@ -13,13 +13,20 @@ constexpr int kLossMaxTop = 1024;
 constexpr int64_t kLossMaxSeqs = int64_t(1) << 21;
 constexpr int64_t kLossMaxVocab = int64_t(1) << 30;  // a row's indexes stay in 32 bits
 
+constexpr int kPartValues = 8192;  // of a split row
+
+// Parts of a row in the forward: 0 (a workgroup takes the whole) or the workgroups that share it.
+int loss_parts(const e4b_logits& z);
+
 // What a token's loss is made of.
-enum LossKind { kStats = 0, kLogprobs = 1, kPolicy = 2, kDistill = 3 };
+// kScore: log-probabilities that no backward follows; kStats: the same, in 64 bits and into stats alone.
+enum LossKind { kStats = 0, kLogprobs = 1, kPolicy = 2, kDistill = 3, kScore = 4 };
 
 struct LossArgs {
   e4b_logits z;
   float2 k;         // log2(e) / temperature, its high and low part
-  float* logps;     // [R] log-probabilities of the labels, 0 where a token does not count (kLogprobs, kPolicy)
+  int parts;        // loss_parts(z)
+  float* logps;     // [R] log-probabilities of the labels, 0 where a token does not count (kLogprobs, kScore, kPolicy)
   // [R] (row maximum, sum of the row's exponentials, label's log-probability in two parts: the second for kStats only);
   // (0, -1, 0, 0) where a token does not count
   float4* stats;

@@ -64,6 +64,15 @@ e4b_logits describe(const Tensor& z, const Tensor& labels, const Tensor& mask, d
   return d;
 }
 
+// A forward's workspace, where it needs one.
+Tensor workspace_of(e4b_logits& d, const Tensor& z) {
+  d.workspace_bytes = e4b_loss_workspace_bytes(&d);
+  if (!d.workspace_bytes) return Tensor();
+  Tensor ws = at::empty({static_cast<int64_t>(d.workspace_bytes)}, z.options().dtype(torch::kByte));
+  d.workspace = ws.data_ptr();
+  return ws;
+}
+
 hipStream_t stream_of(const Tensor& z) { return c10::hip::getCurrentHIPStream(z.device().index()).stream(); }
 
 Tensor floats(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options().dtype(torch::kFloat)); }
@@ -124,7 +133,8 @@ struct Logprobs : Function<Logprobs> {
     const Tensor mask = or_undefined(mask_);
     on_device({labels, mask}, z);
     const c10::OptionalDeviceGuard guard(z.device());
-    const e4b_logits d = describe(z, labels, mask, temperature);
+    e4b_logits d = describe(z, labels, mask, temperature);
+    const Tensor workspace = workspace_of(d, z);
     const Tensor logps = floats({d.seqs, d.tokens}, z);
     Tensor saved;
     if (graph) saved = floats({4 * d.seqs * d.tokens}, z);
@@ -147,7 +157,8 @@ struct Preference : Function<Preference> {
     const Tensor mask = or_undefined(mask_), ref = or_undefined(ref_);
     on_device({labels, mask, ref}, z);
     const c10::OptionalDeviceGuard guard(z.device());
-    const e4b_logits d = describe(z, labels, mask, 1.0);
+    e4b_logits d = describe(z, labels, mask, 1.0);
+    const Tensor workspace = workspace_of(d, z);
     const int64_t rows = d.seqs * d.tokens;
     const Tensor loss = floats({d.seqs / 2}, z), rewards = floats({d.seqs}, z), saved = floats({4 * rows + d.seqs}, z);
     float* at = ptr<float>(saved);
@@ -175,7 +186,8 @@ struct Policy : Function<Policy> {
     const Tensor mask = or_undefined(mask_), ref = or_undefined(ref_);
     on_device({labels, mask, old, advantages, ref}, z);
     const c10::OptionalDeviceGuard guard(z.device());
-    const e4b_logits d = describe(z, labels, mask, temperature);
+    e4b_logits d = describe(z, labels, mask, temperature);
+    const Tensor workspace = workspace_of(d, z);
     const int64_t rows = d.seqs * d.tokens;
     const auto [loss, means] = reduced(z, reduction);
     const Tensor logps = floats({d.seqs, d.tokens}, z), saved = floats({5 * rows + means + (means ? rows : 0)}, z);
@@ -204,7 +216,8 @@ struct Distill : Function<Distill> {
     const Tensor mask = or_undefined(mask_);
     on_device({mask, teacher, index}, z);
     const c10::OptionalDeviceGuard guard(z.device());
-    const e4b_logits d = describe(z, Tensor(), mask, temperature);
+    e4b_logits d = describe(z, Tensor(), mask, temperature);
+    const Tensor workspace = workspace_of(d, z);
     const int64_t rows = d.seqs * d.tokens;
     const auto [loss, means] = reduced(z, reduction);
     const Tensor share = floats(index.sizes(), z), saved = floats({4 * rows + means + (means ? rows : 0)}, z);

@@ -110,6 +110,8 @@ typedef struct e4b_logits {
   const int64_t* labels; /* [seqs, tokens]; a token whose label is outside [0, vocab) does not count */
   const uint8_t* mask;   /* token (n, t) counts iff mask[n * mask_stride + t] != 0 (NULL: all do) */
   int64_t mask_stride;   /* 0 shares one mask */
+  void* workspace;       /* e4b_loss_workspace_bytes(z) bytes for a forward, 8-byte aligned (NULL where that is 0) */
+  size_t workspace_bytes;
 } e4b_logits;
 
 /* Library version string and the last error message of the calling host thread. */
@@ -218,6 +220,10 @@ int e4b_balance_loss(const void* logits, int32_t dtype, int32_t layers, int64_t 
 int e4b_balance_loss_backward(const void* logits, int32_t dtype, int32_t layers, int64_t tokens, int32_t num_experts,
                               const uint8_t* mask, int64_t mask_stride, const int64_t* counts, const int64_t* valid,
                               const float* grad_loss, void* grad_logits, hipStream_t stream);
+
+/* Bytes of workspace that a forward over these logits needs (few rows of a large vocabulary are shared by several
+ * workgroups), 0 for most; by the sizes alone. */
+size_t e4b_loss_workspace_bytes(const e4b_logits* z);
 
 /* Log-probabilities of the labels: logps[n, t] = (z_l - max z) / temperature - log sum_j exp((z_j - max z) /
  * temperature), 0 where the token does not count (its row is not read), -inf where the row's logits are all -inf.

@@ -418,10 +418,11 @@ def test_quantize_mxfp4_refuses_more_than_a_launch_covers():
 def test_loss_entry_points_reject_bad_arguments():
     """Everything is refused before a launch; the sizes and NULLs that are allowed return 0 without one."""
     L = N.lib()
-    assert ctypes.sizeof(N.Logits) == 8 + 4 + 4 + 5 * 8 + 3 * 8
+    assert ctypes.sizeof(N.Logits) == 8 + 4 + 4 + 5 * 8 + 5 * 8
 
-    def z(p=4096, dt=N.BF16, tau=1.0, seqs=2, tokens=3, vocab=10, s0=30, s1=10, labels=4096, mask=None, stride=0):
-        return ctypes.byref(N.Logits(p, dt, tau, seqs, tokens, vocab, s0, s1, labels, mask, stride))
+    def z(p=4096, dt=N.BF16, tau=1.0, seqs=2, tokens=3, vocab=10, s0=30, s1=10, labels=4096, mask=None, stride=0,
+          ws=None, ws_bytes=0):
+        return ctypes.byref(N.Logits(p, dt, tau, seqs, tokens, vocab, s0, s1, labels, mask, stride, ws, ws_bytes))
 
     def logprobs(d, out=4096, stats=4096):
         return L.e4b_token_logprobs(d, out, stats, None)
@@ -458,6 +459,13 @@ def test_loss_entry_points_reject_bad_arguments():
         assert f(z(), stats=4104) == -1 and "stats" in _err()
         if f is not distill:
             assert f(z(labels=None)) == -1 and "labels" in _err()
+    large = dict(seqs=2, tokens=1, vocab=100000)  # few rows of a large vocabulary need a workspace
+    need = L.e4b_loss_workspace_bytes(z(**large))
+    assert need > 0 and L.e4b_loss_workspace_bytes(z()) == L.e4b_loss_workspace_bytes(z(seqs=0, vocab=100000)) == 0
+    assert L.e4b_loss_workspace_bytes(None) == L.e4b_loss_workspace_bytes(z(tokens=-1)) == 0
+    for f in (logprobs, pref, policy, distill):
+        assert f(z(**large)) == f(z(**large, ws=4096, ws_bytes=need - 1)) == -4 and "workspace" in _err()
+        assert f(z(**large, ws=4100, ws_bytes=need)) == -1 and "aligned" in _err()
     assert logprobs(z(), out=None) == -1 and logprobs(z(seqs=0, p=None), None, None) == 0
     assert pref(z(seqs=3)) == -1 and "odd" in _err()
     assert pref(z(), kind=3) == -1 and pref(z(), kind=-1) == -1 and "kind" in _err()

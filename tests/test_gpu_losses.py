@@ -121,6 +121,25 @@ def test_logprobs_lengths_and_masks(seqs, tokens):
         _check_logprobs(_logits((seqs, tokens, V), DTYPES[i % 3], i), labels, mask)
 
 
+@pytest.mark.parametrize("V", (65535, 65536, 73728, 73729, 100003, 152064))
+@pytest.mark.parametrize("rows", (1, 9, 64, 65))
+def test_few_long_rows(rows, V):
+    """Rows shared by several workgroups, and one row or logit short of it; labels and the largest logit at the parts'
+    borders, uncounted rows between."""
+    for i, dtype in enumerate(DTYPES):
+        z = _logits((rows, 1, V), dtype, V + rows + i)
+        edges = torch.tensor([0, 8191, 8192, 8193, V - 1, 65535 % V, 65536 % V, 16383, 3])
+        labels = edges[torch.arange(rows) % 9].unsqueeze(-1)
+        z[torch.arange(rows), 0, edges.flip(0)[torch.arange(rows) % 9]] += 12
+        if rows > 4:
+            labels[3], z[3] = -100, float("nan")
+        if rows > 9:
+            z[5] = -INF
+        _check_logprobs(z.nan_to_num(0.0, posinf=INF, neginf=-INF), labels, tau=(1.0, 0.7, 2.0)[i])
+        teacher, index = _teacher(z.nan_to_num(0.0, neginf=-INF)[:9], 6, V)
+        _check_distill(z[:9].nan_to_num(0.0, neginf=-INF), teacher.clamp(min=-50), index, None, 1.0, "none")
+
+
 def test_logprobs_label_types_and_far_labels():
     z = _logits((2, 5, 100), torch.float32, 1)
     labels = torch.tensor([[0, 99, 100, -1, 1 << 40], [-(1 << 40), 50, -100, 3, 2 ** 63 - 1]])
