@@ -50,6 +50,13 @@ def test_the_torch_binding_loads_and_refuses_host_tensors():
         ext.token_logprobs(z, labels.to("meta"), None, 1.0)
 
 
+def test_a_missing_torch_binding_is_an_error(monkeypatch):
+    monkeypatch.setattr(N, "_torch_lib", None)
+    monkeypatch.setattr(N, "TORCH_LIB_PATH", N.TORCH_LIB_PATH + ".missing")
+    with pytest.raises(N.NativeUnavailable, match="libe4b_torch"):
+        N.torch_lib()
+
+
 def test_enums_match_header():
     src = open(HEADER).read()
     for name, val in (("E4B_FMT_NF4", N.FMT_NF4), ("E4B_FMT_NF4_DQ", N.FMT_NF4_DQ), ("E4B_FMT_MXFP4", N.FMT_MXFP4),

@@ -643,6 +643,60 @@ def test_backward_twice_and_other_gradients():
         assert not zero.any()
 
 
+def test_gradients_by_differences():
+    """Central differences of the kernels' own values along v in {-1, 1}^V, a token each. A row's log-probability moves along v
+    with first to third derivatives of at most 2, 1 and 0.77 (mean, variance and third cumulant of values in [-1, 1]); a
+    difference is off by h^2 / 6 of the loss's third derivative and by the values' own errors over h."""
+    N_, V, h = 24, 50, 2.0 ** -5
+    z = _logits((N_, 1, V), torch.float32, 90, 1.5)
+    v = torch.where(torch.rand(N_, 1, V, generator=_gen(91)) < 0.5, -1.0, 1.0)
+    labels = torch.randint(0, V, (N_, 1), generator=_gen(92)).to(DEV)
+    adv = torch.randn(N_, generator=_gen(93)).to(DEV)
+    teacher, index = (t.to(DEV) for t in _teacher(z, 5, 94))
+    with torch.no_grad():
+        start = e4b.token_logprobs(z.to(DEV), labels)
+    # third derivatives: of A e^(lp - old) (r below 1.1 here: no ratio reaches the clip within h), |A| r (2^3 + 3 2 1 + 0.77),
+    # of the KL term 0.1 e^x of the same (e^x below 2) and 0.1 0.77; of the pair's sigmoid at beta = 0.1, whose derivatives by d
+    # are at most 0.1, 0.1^2 / 4 and 0.1^3 / 8, with d's at most 4, 2 and 1.54
+    calls = (("logprobs", lambda a: e4b.token_logprobs(a, labels), 0.77),
+             ("preference", lambda a: e4b.preference_loss(a, labels, start)[0], 0.008 + 0.06 + 0.154),
+             ("policy", lambda a: e4b.policy_loss(a, labels, start, adv, start - 0.5, kl_coef=0.1, reduction="none")[0],
+              1.1 * 14.8 * adv.abs().max().item() + 0.1 * (2 * 14.8 + 0.77)),
+             ("distill", lambda a: e4b.distill_loss(a, teacher, index, temperature=2.0, reduction="none"), 0.77 / 2))
+    for name, f, third in calls:
+        leaf = z.to(DEV).requires_grad_()
+        out = f(leaf)
+        (grad,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        along = (grad.cpu().double() * v).sum((1, 2))
+        with torch.no_grad():
+            ends = [f((z + s * h * v).to(DEV)).cpu().double() for s in (1, -1)]
+        diff = ((ends[0] - ends[1]) / (2 * h)).flatten()
+        if name == "preference":
+            along = along[:N_ // 2] + along[N_ // 2:]
+        # a value's error: a row's (Row64's E at R = 10, twice in a pair), and z + h v's rounding, all times a slope of at most 4
+        slack = 4 * 2 * ((40 + 4 * 104) + 60) * U / h + third * h * h / 6 + 1e-4
+        assert ((along - diff).abs() <= slack).all(), (name, (along - diff).abs().max().item(), slack)
+
+
+def test_saved_tensors_elsewhere_and_recomputed():
+    """Saved tensors kept on the host between the passes, and a forward computed again in the backward."""
+    from torch.utils.checkpoint import checkpoint
+
+    z, labels, mask, index, teacher, old = _inputs()
+    for f in (lambda a: e4b.token_logprobs(a, labels, mask).sum(), lambda a: e4b.preference_loss(a, labels, old)[0].sum(),
+              lambda a: e4b.policy_loss(a, labels, old, old, mask=mask)[0], lambda a: e4b.distill_loss(a, teacher, index)):
+        leaf = z.detach().requires_grad_()
+        (want,) = torch.autograd.grad(f(leaf), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            loss = f(leaf)
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+        assert torch.equal(torch.autograd.grad(checkpoint(f, leaf, use_reentrant=False), leaf)[0], want)
+        with pytest.raises(RuntimeError, match="second time"):
+            loss = f(leaf)
+            torch.autograd.grad(loss, leaf)
+            torch.autograd.grad(loss, leaf)
+
+
 def test_leaf_gradients_accumulate():
     z, labels, mask, index, teacher, old = _inputs(torch.float32)
     leaf = z.detach().requires_grad_()
