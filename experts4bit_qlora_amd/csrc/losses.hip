@@ -30,9 +30,9 @@ void rows_of(const LossArgs& a, hipStream_t s) {
                          first);
     });
   };
-  // Threads a row by its bytes, us by 128 / 256 / 512 / 1,024 threads: 5,500 rows of 1,000 bf16 logits 6.2 / 7.7 / 12.2 / 23;
-  // of 8,000 21.9 / 21.1 / 25.8 / 33; of 32,000 70 / 66 / 61 / 80; of 50,257 104 / 98 / 93.5 / 99; of 128,000 260 / 240 / 236 /
-  // 223 (6.3 TB/s); of 32,000 fp32 - / 118 / 116 / 111. Few rows: one of 128,000 takes 26 / 14 / 11.6 / 10.6.
+  // Threads a row by its bytes, us by 128 / 256 / 512 / 1,024 threads: 5,500 rows of 1,000 bf16 logits 7.3 / 9.8 / 15 / 27; of
+  // 8,000 23 / 23.5 / 28 / 45; of 32,000 76 / 69 / 69 / 85; of 50,257 114 / 109 / 106 / 105; of 128,000 283 / 269 / 268 / 253. 37
+  // rows of 50,257: - / 7.4 / 6.3 / 6.4, of 128,000: - / 13.6 / 11.5 / 10.6.
   using std::integral_constant;
   const int64_t bytes = a.z.vocab * Piece<DT>::kBytes;
   if (bytes <= 4096) return with(integral_constant<int, 128>{});
@@ -70,12 +70,14 @@ void backward_of(const LossBackwardArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// One CU takes 8 us over the exponentials of 128,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
-// joined in a second launch (~3 us). Whole rows / split, us: 1 row of 50,257 bf16 6.8 / 7.2, of 65,536 7.3 / 7.1, of
-// 128,000 12.0 / 6.4; 37 rows of 65,536 7.9 / 7.3, of 128,000 14.3 / 8.6; 64 of 65,536 9.0 / 8.0, of 128,000 14.3 / 10.0; 128 of
-// 65,536 9.5 / 10.1, of 128,000 14.8 / 13.1 and fp32 17.1 / 18.6; 252 of 128,000 16.5 / 20.8.
+// One CU takes ~7 us over the exponentials of 128,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
+// joined in a second launch. Whole rows / split, us: 1 row of 50,257 bf16 5.8 / 6.7, of 100,003 7.6 / 7.1, of 128,000 9.5 / 6.9;
+// 37 rows of 80,000 8.1 / 8.3, of 100,003 8.5 / 7.3, of 128,000 11.1 / 7.6; 64 of 100,003 8.7 / 8.1; 128 of 100,003 9.2 / 10.3, of
+// 128,000 11.6 / 11.1. fp32: 1 row of 50,257 5.8 / 5.6, of 65,536 6.5 / 5.8; 64 of 50,257 7.4 / 8.0, of 65,536 8.5 / 8.3, of
+// 128,000 14.1 / 11.2; 128 of 128,000 16.2 / 16.6.
 int loss_parts(const e4b_logits& z) {
-  return z.seqs * z.tokens <= 64 && z.vocab >= 65536 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
+  const int64_t bytes = z.vocab * (z.dtype == E4B_FP32 ? 4 : 2);
+  return z.seqs * z.tokens <= 64 && bytes >= 200000 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
 }
 
 void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s) {

@@ -27,7 +27,7 @@ struct LossArgs {
   float2 k;         // log2(e) / temperature, its high and low part
   int parts;        // loss_parts(z)
   float* logps;     // [R] log-probabilities of the labels, 0 where a token does not count (kLogprobs, kScore, kPolicy)
-  // [R] (row maximum, sum of the row's exponentials, label's log-probability in two parts: the second for kStats only);
+  // [R] (reference, sum of the row's exponentials against it, label's log-probability in two parts: the second for kStats only);
   // (0, -1, 0, 0) where a token does not count
   float4* stats;
   // kPolicy

@@ -2,9 +2,10 @@
 
 Tolerances, with u = 2^-24, D = (max z - z_j) / temperature and R the row's largest D at most 104 (beyond, an exponential is
 below fp32's smallest value and its error below 2^-149): a difference to the maximum, its factor log2(e) / temperature and
-their product make an exponential's argument off by at most 4 u D, the exponential by 2 u more. A row's sum has at most
-n = max(64, V / 256) + 40 additions one after the other, each of which may be followed by a rescaling of 3 roundings, so it is
-off by E = (4 R + 4 n) u relative. A log-probability D_l - log s is off by E + (3 D_l + 2 |log s| + |lp|) u; a
+their product make an exponential's argument off by at most 4 u D, the exponential by 2 u more (where the difference is to
+the label instead, two multiply-adds round an argument of at most D_j + D_l <= 2 R: 1.4 u of that, no more). A row's sum has
+at most n = max(64, V / 256) + 40 additions one after the other, each of which may be followed by a rescaling of 3
+roundings, so it is off by E = (4 R + 4 n) u relative. A log-probability D_l - log s is off by E + (3 D_l + 2 |log s| + |lp|) u; a
 probability by E + (4 D + 8) u relative; a result rounded into a 16-bit type by half a step of it, or of its smallest
 normal value."""
 import pytest
@@ -121,11 +122,11 @@ def test_logprobs_lengths_and_masks(seqs, tokens):
         _check_logprobs(_logits((seqs, tokens, V), DTYPES[i % 3], i), labels, mask)
 
 
-@pytest.mark.parametrize("V", (65535, 65536, 73728, 73729, 100003, 152064))
+@pytest.mark.parametrize("V", (49999, 50000, 65536, 73729, 99999, 100000, 106496, 106497, 152064))
 @pytest.mark.parametrize("rows", (1, 9, 64, 65))
 def test_few_long_rows(rows, V):
-    """Rows shared by several workgroups, and one row or logit short of it; labels and the largest logit at the parts'
-    borders, uncounted rows between."""
+    """Rows shared by several workgroups (from 200,000 bytes on), and one row or logit short of it; labels and the largest logit
+    at the parts' borders, uncounted rows and ones of a very wide range between."""
     for i, dtype in enumerate(DTYPES):
         z = _logits((rows, 1, V), dtype, V + rows + i)
         edges = torch.tensor([0, 8191, 8192, 8193, V - 1, 65535 % V, 65536 % V, 16383, 3])
@@ -133,9 +134,14 @@ def test_few_long_rows(rows, V):
         z[torch.arange(rows), 0, edges.flip(0)[torch.arange(rows) % 9]] += 12
         if rows > 4:
             labels[3], z[3] = -100, float("nan")
+            z[4] *= 100
         if rows > 9:
             z[5] = -INF
         _check_logprobs(z.nan_to_num(0.0, posinf=INF, neginf=-INF), labels, tau=(1.0, 0.7, 2.0)[i])
+        if rows > 4:
+            pairs = z[:2 * (rows // 2)].clamp(min=-50, max=50).nan_to_num(0.0)
+            _check_preference(pairs, labels[:len(pairs)], None, beta=0.01)
+            _check_policy(pairs, labels[:len(pairs)].clamp(min=0), torch.ones(len(pairs)), kl=0.05)
         teacher, index = _teacher(z.nan_to_num(0.0, neginf=-INF)[:9], 6, V)
         _check_distill(z[:9].nan_to_num(0.0, neginf=-INF), teacher.clamp(min=-50), index, None, 1.0, "none")
 
@@ -193,6 +199,10 @@ def test_nan_and_infinity_stay_in_their_rows():
     labels = torch.full((1, 5), 9, device=DEV)
     lp = e4b.token_logprobs(leaf, labels)
     assert lp[0, 1:4].isnan().all() and torch.isfinite(lp[0, [0, 4]]).all()
+    at_label = z.clone()
+    at_label[0, 0, 9], at_label[0, 4, 9] = INF, float("nan")
+    got = e4b.token_logprobs(at_label.to(DEV), labels)
+    assert got.isnan().all()
     (grad,) = torch.autograd.grad(lp.sum(), leaf)
     assert grad[0, 1].isnan().all() and torch.isfinite(grad[0, [0, 4]]).all() and grad[0, 3].isnan().all()
 
