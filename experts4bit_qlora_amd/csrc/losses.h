@@ -266,29 +266,31 @@ struct Token {
   }
 };
 
+// Entry k of a token's teacher: an index inside the vocabulary and its value, or -1 and -inf.
+struct Entry {
+  int64_t j = -1;
+  float w = -__builtin_inff();
+  E4B_DEV Entry(const LossArgs& a, int64_t at, int k) {
+    if (k >= a.top) return;
+    j = a.index[at * a.top + k];
+    const float v = any_float(a.teacher, a.teacher_dtype, at * a.top + k);
+    if (j >= 0 && j < a.z.vocab) w = v;
+    else j = -1;
+  }
+};
+
 // The teacher's part of a row, by the first wave: probabilities over its usable entries (an index inside the
-// vocabulary, a value above -inf) and tau^2 sum_k p_k (log p_k - log q_k); zero where no entry is usable.
+// vocabulary, a value above -inf) and tau^2 sum_k p_k (log p_k - log q_k); zero where no entry is usable. `own`: entry
+// `lane`; the others are loaded in each pass.
 template <int DT>
-E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, RunOf<float>& r) {
+E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, const Entry& own, RunOf<float>& r) {
   const float tau = a.z.temperature, per = 1.0f / tau;
   const int lane = threadIdx.x;
-  const int64_t first = at * a.top;
-  struct Entry {
-    int64_t j;
-    float w;  // -inf where the index is outside
-  };
-  auto load = [&](int k) {
-    Entry e{k < a.top ? a.index[first + k] : -1, -__builtin_inff()};
-    if (e.j >= 0 && e.j < a.z.vocab) e.w = any_float(a.teacher, a.teacher_dtype, first + k);
-    else e.j = -1;
-    return e;
-  };
-  const Entry own = load(lane);  // the others are loaded again in each pass
-  auto entry = [&](int k) { return k == lane ? own : load(k); };
+  auto entry = [&](int k) { return k == lane ? own : Entry(a, at, k); };
   float most = own.w;
   bool bad = own.w != own.w;
   for (int k = lane + kWave; k < a.top; k += kWave) {
-    const float w = load(k).w;
+    const float w = entry(k).w;
     most = fmaxf(most, w);
     bad |= w != w;
   }
@@ -313,7 +315,7 @@ E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<D
       const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[e.j]) - r.m) * per - log_s;
       if (!(p == 0.0f)) sum += p * ((w - log_norm) - lq);
     }
-    a.share[first + k] = p;
+    a.share[at * a.top + k] = p;
   }
   if (none) r.s = 0.0f;  // nothing to differentiate
   return tau * tau * wave_sum(sum);
@@ -402,6 +404,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
     low = lp - lp == 0.0f ? static_cast<float>(l - lp) : 0.0f;
   } else {
     float sum = 0.0f;
+    const Entry teacher(a, at, KIND == kDistill ? static_cast<int>(threadIdx.x) : a.top);
     if constexpr (NT == kWave) {
       own = P::one(row[first]);
       for (int i = threadIdx.x; i < a.parts; i += kWave) sum += static_cast<const float*>(a.z.workspace)[at * a.parts + i];
@@ -422,7 +425,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
       RunOf<float> r;
       r.m = m;
       r.s = s;
-      const float loss = teacher_loss<DT>(a, at, row, r);
+      const float loss = teacher_loss<DT>(a, at, row, teacher, r);
       if (lead) a.token_loss[at] = loss;
       if (lead) a.stats[at] = make_float4(m, r.s, 0.0f, 0.0f);
       return;
