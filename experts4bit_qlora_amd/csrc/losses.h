@@ -103,10 +103,10 @@ constexpr int kPartThreads = 256;
 template <int DT>
 constexpr int kPartPieces = kPartValues / Piece<DT>::kCount;
 
-// f(values) over a row without its element `skip` (-1: over all) by NT threads, of its pieces [begin, end) alone where it is
+// f(values) over a row, without its element `skip` if SKIP, by NT threads, of its pieces [begin, end) alone where it is
 // split (the first of the parts takes the single values at the row's ends); -inf in the place of what is skipped. ready() is
 // called once the first pieces are on their way.
-template <int DT, int NT, int U, bool ONCE, class G, class F>
+template <int DT, int NT, int U, bool ONCE, bool SKIP, class G, class F>
 E4B_DEV void over_row(const void* row, int V, int skip, int begin, int end, G&& ready, F&& f) {
   using P = Piece<DT>;
   const typename P::T* p = static_cast<const typename P::T*>(row);
@@ -117,10 +117,10 @@ E4B_DEV void over_row(const void* row, int V, int skip, int begin, int end, G&& 
   auto take = [&](const uint4& w, int i) {
     float x[P::kCount];
     P::unpack(w, x);
-    if (i == skip_at) {
+    if (SKIP && __any(i == skip_at)) {  // a branch of the wave: under a lane's mask the selections would cost every piece
 #pragma unroll
       for (int c = 0; c < P::kCount; ++c)
-        if (c == skip_off) x[c] = -__builtin_inff();
+        if (i == skip_at && c == skip_off) x[c] = -__builtin_inff();
     }
     f(x);
   };
@@ -147,8 +147,8 @@ E4B_DEV void over_row(const void* row, int V, int skip, int begin, int end, G&& 
   for (; i < last; i += NT) take(v[i], i);
   if (begin == 0) {
     float edge[2] = {-__builtin_inff(), -__builtin_inff()};
-    if (tid < at.head && tid != skip) edge[0] = P::one(p[tid]);
-    if (tid < V - at.tail && at.tail + tid != skip) edge[1] = P::one(p[at.tail + tid]);
+    if (tid < at.head && !(SKIP && tid == skip)) edge[0] = P::one(p[tid]);
+    if (tid < V - at.tail && !(SKIP && at.tail + tid == skip)) edge[1] = P::one(p[at.tail + tid]);
     f(edge);
   }
 }
@@ -168,20 +168,20 @@ E4B_DEV T of_waves(T mine) {
   return part[threadIdx.x & (NT / kWave - 1)];
 }
 
-// sum_j exp((z_j - ref) / tau) by the whole workgroup, in every lane of the first wave; ref is the row's element `first`, a logit
-// that is likely among the largest, not the maximum: fp32 has 2^126 of room on either side, so a maximum that is kept while
+// sum_j exp((z_j - ref) / tau) by the whole workgroup, in every lane of the first wave; ref is the row's element `first`, which
+// is left out if SKIP: a logit that is likely among the largest, not the maximum. fp32 has 2^126 of room on either side, so a maximum kept while
 // the sum runs, with a rescaling at every step, is only needed where a row leaves that room (row_run). It costs two
 // multiply-adds a value, x k - ref k with the factor's second part added in the same way; the rounding of ref k is taken out
 // of the sum. With a running maximum / so, us: 5,500 rows of 128,000 bf16 logits 268 / 253, of 50,257 111 / 106; 37 rows of
 // 128,000 13.6 / 10.6, of 50,257 7.8 / 6.3 (the reference is loaded behind a row's first pieces: before them 5 % more).
-template <int DT, int NT, int U, bool ONCE>
-E4B_DEV float row_sum(const void* row, int V, int skip, int first, float& ref, float2 k, int begin = 0, int end = 0x7fffffff) {
+template <int DT, int NT, int U, bool ONCE, bool SKIP>
+E4B_DEV float row_sum(const void* row, int V, int first, float& ref, float2 k, int begin = 0, int end = 0x7fffffff) {
   float at, s = 0.0f;
   const auto ready = [&] {
     ref = Piece<DT>::one(static_cast<const typename Piece<DT>::T*>(row)[first]);
     at = ref * k.x;
   };
-  over_row<DT, NT, U, ONCE>(row, V, skip, begin, end, ready, [&](const auto& x) {
+  over_row<DT, NT, U, ONCE, SKIP>(row, V, first, begin, end, ready, [&](const auto& x) {
     float sum = 0.0f;
     for (float v : x) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v, k.y, __builtin_fmaf(v, k.x, -at)));
     s += sum;
@@ -225,10 +225,10 @@ struct RunOf {
   }
 };
 
-template <int DT, int NT, class S>
+template <int DT, int NT, bool SKIP, class S>
 E4B_DEV RunOf<S> row_run(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
   RunOf<float> r;
-  over_row<DT, NT, kRowUnroll, false>(row, V, skip, begin, end, [] {}, [&](const auto& x) { r.add(x, k); });
+  over_row<DT, NT, kRowUnroll, false, SKIP>(row, V, skip, begin, end, [] {}, [&](const auto& x) { r.add(x, k); });
   RunOf<S> all;
   all.m = r.m;
   all.s = r.s;
@@ -338,13 +338,14 @@ __global__ __launch_bounds__(kPartThreads) void loss_parts_kernel(LossArgs a) {
   const Token tok(a.z, at, P::kBytes);
   if (!tok.counts) return;
   const int V = static_cast<int>(a.z.vocab), own = static_cast<int>(reference_of<KIND>(a, at, tok));
-  const int skip = KIND == kDistill ? -1 : own, begin = part * step;
+  const int begin = part * step;
   if constexpr (KIND == kStats) {
-    const RunOf<float> r = row_run<DT, kPartThreads, float>(tok.row, V, skip, a.k, begin, begin + step);
+    const RunOf<float> r = row_run<DT, kPartThreads, true, float>(tok.row, V, own, a.k, begin, begin + step);
     if (threadIdx.x == 0) static_cast<float2*>(a.z.workspace)[blockIdx.x] = make_float2(r.m, r.s);
   } else {
     float ref;
-    const float s = row_sum<DT, kPartThreads, kRowUnroll, KIND == kScore>(tok.row, V, skip, own, ref, a.k, begin, begin + step);
+    const float s = row_sum<DT, kPartThreads, kRowUnroll, KIND == kScore, KIND != kDistill>(tok.row, V, own, ref, a.k, begin,
+                                                                                             begin + step);
     if (threadIdx.x == 0) static_cast<float*>(a.z.workspace)[blockIdx.x] = s;
   }
 }
@@ -380,7 +381,6 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   }
   const typename P::T* row = reinterpret_cast<const typename P::T*>(tok.row);
   const int V = static_cast<int>(a.z.vocab), first = static_cast<int>(reference_of<KIND>(a, at, tok));
-  const int skip = KIND == kDistill ? -1 : first;
   float adv = 0.0f, old = 0.0f, ref = 0.0f;  // on their way while the row is read
   if constexpr (KIND == kPolicy) {
     adv = a.advantages[a.adv_per_token ? at : tok.n];
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
       for (int i = threadIdx.x; i < a.parts; i += kWave) r.join(parts[i].x, parts[i].y, a.k);
       r.join_lanes(kWave, a.k);
     } else {
-      r = row_run<DT, NT, double>(row, V, skip, a.k);
+      r = row_run<DT, NT, true, double>(row, V, first, a.k);
     }
     if (threadIdx.x >= kWave) return;
     const double l = join_label(own, r, a, m, s);
@@ -410,14 +410,14 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
       for (int i = threadIdx.x; i < a.parts; i += kWave) sum += static_cast<const float*>(a.z.workspace)[at * a.parts + i];
       sum = wave_sum(sum);
     } else {
-      sum = row_sum<DT, NT, U, KIND == kScore>(row, V, skip, first, own, a.k);
+      sum = row_sum<DT, NT, U, KIND == kScore, KIND != kDistill>(row, V, first, own, a.k);
     }
     if (threadIdx.x >= kWave) return;
     m = own;
     s = KIND == kDistill ? sum : 1.0f + sum;
     lp = -log1pf(sum);
     if (!in_room(own, sum)) {  // by the first wave alone: rows of -inf, labels less likely than 1e-18
-      RunOf<float> r = row_run<DT, kWave, float>(row, V, skip, a.k);
+      RunOf<float> r = row_run<DT, kWave, KIND != kDistill, float>(row, V, first, a.k);
       lp = KIND == kDistill ? 0.0f : join_label(own, r, a, m, s);
       if (KIND == kDistill) m = r.m, s = r.s;
     }
