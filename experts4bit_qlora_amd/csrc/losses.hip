@@ -71,13 +71,13 @@ void backward_of(const LossBackwardArgs& a, hipStream_t s) {
 }  // namespace
 
 // One CU takes ~7 us over the exponentials of 128,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
-// joined in a second launch. Whole rows / split, us: 1 row of 50,257 bf16 5.8 / 6.7, of 100,003 7.6 / 7.1, of 128,000 9.5 / 6.9;
-// 37 rows of 80,000 8.1 / 8.3, of 100,003 8.5 / 7.3, of 128,000 11.1 / 7.6; 64 of 100,003 8.7 / 8.1; 128 of 100,003 9.2 / 10.3, of
-// 128,000 11.6 / 11.1. fp32: 1 row of 50,257 5.8 / 5.6, of 65,536 6.5 / 5.8; 64 of 50,257 7.4 / 8.0, of 65,536 8.5 / 8.3, of
-// 128,000 14.1 / 11.2; 128 of 128,000 16.2 / 16.6.
+// joined in a second launch, which costs the host 2.4 us with its workspace: rows where the GPU gains as much. Whole / split, us
+// on the GPU: 1 row of 100,003 bf16 7.6 / 7.1, of 128,000 9.5 / 6.9 (a call: 8.4 / 10.7), of 152,000 10.3 / 6.9; 64 of 128,000
+// 11.1 / 8.5, of 152,000 11.9 / 9.5; 128 of 152,000 12.4 / 12.4. fp32: 1 row of 50,257 5.8 / 5.6, of 80,000 8.1 / 5.8, of 128,000
+// 10.7 / 5.7; 64 of 80,000 10.7 / 10.0, of 128,000 14.1 / 11.2; 128 of 128,000 16.2 / 16.6.
 int loss_parts(const e4b_logits& z) {
   const int64_t bytes = z.vocab * (z.dtype == E4B_FP32 ? 4 : 2);
-  return z.seqs * z.tokens <= 64 && bytes >= 200000 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
+  return z.seqs * z.tokens <= 64 && bytes >= 300000 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
 }
 
 void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s) {

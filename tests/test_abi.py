@@ -466,9 +466,9 @@ def test_loss_entry_points_reject_bad_arguments():
         assert f(z(), stats=4104) == -1 and "stats" in _err()
         if f is not distill:
             assert f(z(labels=None)) == -1 and "labels" in _err()
-    large = dict(seqs=2, tokens=1, vocab=100000)  # few rows of a large vocabulary need a workspace
+    large = dict(seqs=2, tokens=1, vocab=160000)  # few rows of a large vocabulary need a workspace
     need = L.e4b_loss_workspace_bytes(z(**large))
-    assert need > 0 and L.e4b_loss_workspace_bytes(z()) == L.e4b_loss_workspace_bytes(z(seqs=0, vocab=100000)) == 0
+    assert need > 0 and L.e4b_loss_workspace_bytes(z()) == L.e4b_loss_workspace_bytes(z(seqs=0, vocab=160000)) == 0
     assert L.e4b_loss_workspace_bytes(None) == L.e4b_loss_workspace_bytes(z(tokens=-1)) == 0
     for f in (logprobs, pref, policy, distill):
         assert f(z(**large)) == f(z(**large, ws=4096, ws_bytes=need - 1)) == -4 and "workspace" in _err()

@@ -122,10 +122,10 @@ def test_logprobs_lengths_and_masks(seqs, tokens):
         _check_logprobs(_logits((seqs, tokens, V), DTYPES[i % 3], i), labels, mask)
 
 
-@pytest.mark.parametrize("V", (49999, 50000, 65536, 73729, 99999, 100000, 106496, 106497, 152064))
+@pytest.mark.parametrize("V", (74999, 75000, 81920, 81921, 149999, 150000, 152064, 155648, 155649))
 @pytest.mark.parametrize("rows", (1, 9, 64, 65))
 def test_few_long_rows(rows, V):
-    """Rows shared by several workgroups (from 200,000 bytes on), and one row or logit short of it; labels and the largest logit
+    """Rows shared by several workgroups (from 300,000 bytes on), and one row or logit short of it; labels and the largest logit
     at the parts' borders, uncounted rows and ones of a very wide range between."""
     for i, dtype in enumerate(DTYPES):
         z = _logits((rows, 1, V), dtype, V + rows + i)
