@@ -15,6 +15,11 @@
 //
 // One workgroup takes a row: its threads sum over 16-byte pieces, the sums are joined; a row's logits are read once in the
 // forward and once in the backward, tokens that do not count are not read.
+//
+// Bound by HBM from a few hundred rows on: 5,369 counted of 8,192 rows of 128,000 bf16 logits take 222 us forward (6.2 TB/s,
+// the vector units 80 % busy) and 575-585 us backward (1.4 GB in, 2.1 GB out: 6.0 TB/s, where a copy reaches 4.9). Computing
+// the gradient while the forward holds the row would save the second read, but what the loss is multiplied by is known only in
+// the backward: a third fewer bytes where that is exactly one, a third more where it is not.
 #pragma once
 
 #include "common.h"
@@ -22,7 +27,6 @@
 
 namespace e4b {
 
-constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLowest = -3.402823466e38f;
 
 // ---- 16-byte pieces of a row
@@ -31,7 +35,6 @@ template <int DT>
 struct Piece {
   static constexpr int kBytes = DT == E4B_FP32 ? 4 : 2;
   static constexpr int kCount = 16 / kBytes;
-  static constexpr uint32_t kEmpty = DT == E4B_FP32 ? 0xff800000u : DT == E4B_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
   using T = std::conditional_t<DT == E4B_FP32, float, uint16_t>;
 
   static E4B_DEV float one(T v) {
@@ -159,21 +162,12 @@ E4B_DEV float wave_sum(float v) {
   return v;
 }
 
-// A value per wave to the first wave's lanes: lane l has that of wave l mod (NT / 64).
-template <int NT, class T>
-E4B_DEV T of_waves(T mine) {
-  __shared__ T part[NT / kWave];
-  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = mine;
-  __syncthreads();
-  return part[threadIdx.x & (NT / kWave - 1)];
-}
-
 // sum_j exp((z_j - ref) / tau) by the whole workgroup, in every lane of the first wave; ref is the row's element `first`, which
-// is left out if SKIP: a logit that is likely among the largest, not the maximum. fp32 has 2^126 of room on either side, so a maximum kept while
-// the sum runs, with a rescaling at every step, is only needed where a row leaves that room (row_run). It costs two
-// multiply-adds a value, x k - ref k with the factor's second part added in the same way; the rounding of ref k is taken out
-// of the sum. With a running maximum / so, us: 5,500 rows of 128,000 bf16 logits 268 / 253, of 50,257 111 / 106; 37 rows of
-// 128,000 13.6 / 10.6, of 50,257 7.8 / 6.3 (the reference is loaded behind a row's first pieces: before them 5 % more).
+// is left out if SKIP: a logit that is likely among the largest, not the maximum. fp32 has 2^126 of room on either side, so a
+// maximum kept while the sum runs, with a rescaling at every step, is only needed where a row leaves that room (row_run). It
+// costs two multiply-adds a value, x k - ref k with the factor's second part added in the same way; the rounding of ref k is
+// taken out of the sum. With a running maximum / so, us: 5,500 rows of 128,000 bf16 logits 268 / 253, of 50,257 111 / 106; 37
+// rows of 128,000 13.6 / 10.6, of 50,257 7.8 / 6.3 (the reference is loaded behind a row's first pieces: before them 5 % more).
 template <int DT, int NT, int U, bool ONCE, bool SKIP>
 E4B_DEV float row_sum(const void* row, int V, int first, float& ref, float2 k, int begin = 0, int end = 0x7fffffff) {
   float at, s = 0.0f;
@@ -188,16 +182,20 @@ E4B_DEV float row_sum(const void* row, int V, int first, float& ref, float2 k, i
   });
   s = wave_sum(s * __builtin_amdgcn_exp2f(-__builtin_fmaf(ref, k.y, __builtin_fmaf(ref, k.x, -at))));
   if constexpr (NT > kWave) {
-    s = of_waves<NT>(s);
+    constexpr int W = NT / kWave;
+    __shared__ float part[W];
+    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = s;
+    __syncthreads();
+    s = part[threadIdx.x & (W - 1)];
 #pragma unroll
-    for (int off = 1; off < NT / kWave; off *= 2) s += __shfl_xor(s, off);
+    for (int off = 1; off < W; off *= 2) s += __shfl_xor(s, off);
   }
   return s;
 }
 
-// Whether a row's sum kept to that room. Up to here the backward's quotient by it is a normal number.
-constexpr float kMostSum = 1e18f;
-E4B_DEV bool in_room(float ref, float sum) { return fabsf(ref) < 1e37f && sum < kMostSum; }  // no NaN
+// Whether a row's reference, scaled, and its sum kept to that room (a NaN does not). Up to this sum the backward's quotient
+// by it is a normal number.
+E4B_DEV bool in_room(float ref, float2 k, float sum) { return fabsf(ref * k.x) < 1e37f && sum < 1e18f; }
 
 // Running maximum m and sum s of exp((x - m) / tau), for any finite logits: differences to the maximum are taken before they
 // are scaled, and the type's lowest value stays finite. The largest terms' exponents are the smallest, and so are their
@@ -234,9 +232,17 @@ E4B_DEV RunOf<S> row_run(const void* row, int V, int skip, float2 k, int begin =
   all.s = r.s;
   all.join_lanes(kWave, k);
   if constexpr (NT > kWave) {
-    all.m = of_waves<NT>(all.m);
-    all.s = of_waves<NT>(all.s);
-    all.join_lanes(NT / kWave, k);
+    constexpr int W = NT / kWave;
+    __shared__ float part_m[W];
+    __shared__ S part_s[W];
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+      part_m[threadIdx.x / kWave] = all.m;
+      part_s[threadIdx.x / kWave] = all.s;
+    }
+    __syncthreads();
+    all.m = part_m[threadIdx.x & (W - 1)];
+    all.s = part_s[threadIdx.x & (W - 1)];
+    all.join_lanes(W, k);
   }
   return all;
 }
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
     m = own;
     s = KIND == kDistill ? sum : 1.0f + sum;
     lp = -log1pf(sum);
-    if (!in_room(own, sum)) {  // by the first wave alone: rows of -inf, labels less likely than 1e-18
+    if (!in_room(own, a.k, sum)) {  // by the first wave alone: rows of -inf, labels less likely than 1e-18
       RunOf<float> r = row_run<DT, kWave, KIND != kDistill, float>(row, V, first, a.k);
       lp = KIND == kDistill ? 0.0f : join_label(own, r, a, m, s);
       if (KIND == kDistill) m = r.m, s = r.s;
@@ -552,7 +558,9 @@ __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
 // ---- backward
 
 constexpr int kBackThreads = 256;
-constexpr int kBackUnroll = 2;  // 5,500 x 128,000 bf16: 1 / 2 / 4 / 8 pieces a thread 505 / 509 / 542 / 554 us, 50,257: 210 / 184 / 200 / 226
+// Pieces a thread, 1 / 2 / 4 / 8 (before the accesses went past the caches): 5,500 x 128,000 bf16 505 / 509 / 542 / 554 us, 5,500
+// x 50,257 210 / 184 / 200 / 226.
+constexpr int kBackUnroll = 2;
 
 // A workgroup takes kBackThreads * kBackUnroll pieces of one row's gradient: A q_j - A p_k at the row's entries (a label:
 // one entry with p = 1, A = -derivative / tau; a teacher: p_k, A = derivative * tau). Entries inside the workgroup's part are
@@ -598,7 +606,9 @@ __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwar
   }
   // the entries of this part: positions relative to its first value, head and tail among them in part 0
   const int lo = sp.head + first * C, hi = min(sp.tail, lo + kBackThreads * kBackUnroll * C);
-  auto mine = [&](int64_t j) { return (j >= lo && j < hi) || (part == 0 && ((j >= 0 && j < sp.head) || (j >= sp.tail && j < V))); };
+  auto mine = [&](int64_t j) {
+    return (j >= lo && j < hi) || (part == 0 && ((j >= 0 && j < sp.head) || (j >= sp.tail && j < V)));
+  };
   __shared__ int where[TEACHER ? kLossMaxTop : 1];
   __shared__ float what[TEACHER ? kLossMaxTop : 1];
   __shared__ int listed;

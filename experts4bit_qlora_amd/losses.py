@@ -12,7 +12,8 @@ Logits are ``[..., tokens, vocab]``; the leading axes are sequences. They may be
 labels instead (the last one ``-100``) saves that. A token counts iff its mask is nonzero (where a mask is given) and, in
 the three losses with labels, its label is inside ``[0, vocab)``; other tokens' logits have no influence, whatever they
 are, and get a zero gradient. A row whose logits are all ``-inf`` gives every label probability 0 and gets a zero
-gradient. Everything but the logits is a constant to the gradient.
+gradient. Everything but the logits is a constant to the gradient. A backward pass is captured into a graph like any other of
+torch's: with no eager graph of the same leaves alive.
 
 The reference has no losses of its own (its training lane starts at a model's, ``experts4bit_qlora/engines/fast.py:453-674``).
 """

@@ -234,19 +234,19 @@ int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStrea
 /* Preference loss of the pairs (sequence b, chosen; sequence b + seqs / 2, rejected): S_i the sum of the counted
  * tokens' log-probabilities (their mean where `average`), d = (S_c - r_c) - (S_r - r_r). ref: log-probabilities under
  * the reference model, per token [seqs, tokens] (then summed, or averaged, over the counted tokens like the model's) or
- * per sequence [seqs] (taken as they are), NULL: zeros. loss fp32 [seqs / 2], rewards fp32 [seqs] = beta (S_i - r_i), coef fp32 [seqs]
- * = the loss's derivative by each of a sequence's log-probabilities, stats as above (required). seqs is even. Sums in 64 bits, deterministic.
- * Has no counterpart in the reference. */
+ * per sequence [seqs] (taken as they are), NULL: zeros. loss fp32 [seqs / 2], rewards fp32 [seqs] = beta (S_i - r_i),
+ * coef fp32 [seqs] = the loss's derivative by each of a sequence's log-probabilities, stats as above (required). seqs is
+ * even. Sums in 64 bits, deterministic. Has no counterpart in the reference. */
 int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_token, int32_t kind, float beta,
                         float smoothing, int32_t average, float* loss, float* rewards, float* stats, float* coef,
                         hipStream_t stream);
 
 /* Clipped policy loss: with lp a token's log-probability, r = exp(lp - old_logps) and x = ref_logps - lp,
  * -min(r A, min(max(r, clip_lo), clip_hi) A) + kl_coef (e^x - x - 1) at counted tokens, 0 elsewhere. advantages
- * [seqs], or [seqs, tokens] with adv_per_token; ref_logps may be NULL (no KL term). loss: [seqs * tokens], [seqs] or one
- * value by `reduction` (0 where nothing counts). logps, token_loss, coef (the derivative by lp) fp32 [seqs, tokens], stats as above; with a
- * reduction, inv fp32 [seqs] or one value: 1 / the number of counted tokens. With E4B_REDUCE_NONE loss is
- * token_loss and inv is not written. Has no counterpart in the reference. */
+ * [seqs], or [seqs, tokens] with adv_per_token; ref_logps may be NULL (no KL term). logps, token_loss, coef (the
+ * derivative by lp) fp32 [seqs, tokens], stats as above; loss fp32 [seqs] or one value by `reduction` (0 where nothing
+ * counts) and inv as many: 1 / the number of counted tokens. With E4B_REDUCE_NONE neither is written: token_loss is the
+ * loss. Has no counterpart in the reference. */
 int e4b_policy_loss(const e4b_logits* z, const float* old_logps, const float* advantages, int32_t adv_per_token,
                     const float* ref_logps, float clip_lo, float clip_hi, float kl_coef, int32_t reduction, float* logps,
                     float* token_loss, float* stats, float* coef, float* loss, float* inv, hipStream_t stream);
@@ -265,7 +265,8 @@ int e4b_distill_loss(const e4b_logits* z, const void* teacher, int32_t teacher_d
  * coef_strides[1]] * inv[n * inv_stride] (coef and inv may be NULL: 1), and with q the row's softmax
  *   labels (index NULL):  w / temperature ([j = label] - q_j)
  *   a teacher:            w temperature (q_j - sum of share_k with index_k = j).
- * Zero, without reading the row, where the token does not count or w is 0. stats, coef, inv, share: as the forward wrote them, z as it read it. */
+ * Zero, without reading the row, where the token does not count or w is 0. stats, coef, inv, share as the forward wrote
+ * them, z as it read it. */
 int e4b_loss_backward(const e4b_logits* z, const float* stats, const float* grad_loss, int64_t grad_seqs,
                       const int64_t grad_strides[2], const float* coef, const int64_t coef_strides[2], const float* inv,
                       int64_t inv_stride, const int64_t* index, const float* share, int32_t top, void* grad_logits,

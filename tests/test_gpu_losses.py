@@ -179,6 +179,22 @@ def test_logprobs_ranges_and_extremes(dtype):
         _check_logprobs(_logits((1, 12, V), dtype, 5, spread), labels)
 
 
+def test_temperatures_at_the_ends():
+    """So low that a scaled logit leaves fp32, so high that all are alike."""
+    z = _logits((1, 6, 300), torch.float32, 71, 1e9)
+    labels = torch.randint(0, 300, (1, 6), generator=_gen(72))
+    labels[0, :3] = z[0, :3].argmax(-1)
+    lp = e4b.token_logprobs(z.to(DEV), labels.to(DEV), temperature=2e-30).cpu()
+    # the largest logit has all the probability; the others' are -(max - z) / 2e-30, from 3.4e38 on an infinity
+    away = (z.double().gather(-1, labels.unsqueeze(-1)).squeeze(-1) - z.double().amax(-1)) / 2e-30
+    assert torch.equal(lp[0, :3], torch.zeros(3)) and (lp[0, 3:] < -1e36).all()
+    assert torch.allclose(lp, away.float(), rtol=1e-6)
+    lp = e4b.token_logprobs(z.to(DEV), labels.to(DEV), temperature=5e29)
+    assert torch.allclose(lp.cpu(), torch.full((1, 6), -5.703782474656201))
+    for tau in (1e-6, 1e6):
+        _check_logprobs(_logits((1, 6, 300), torch.float32, 73, tau), labels, tau=tau)
+
+
 def test_label_without_probability():
     """A label at -inf, beside finite logits: log-probability -inf, a finite gradient."""
     z = _logits((1, 2, 50), torch.float32, 6)
@@ -533,7 +549,8 @@ def test_distill_entries_outside_repeated_and_empty():
     for red in ("none", "mean"):
         _check_distill(z, teacher.nan_to_num(0.0, neginf=-INF), index, red=red)
     leaf = z.to(DEV).requires_grad_()
-    a, b = (e4b.distill_loss(leaf, t.to(DEV), index.to(DEV), reduction="none") for t in (teacher, teacher.nan_to_num(0.0, neginf=-INF)))
+    a, b = (e4b.distill_loss(leaf, t.to(DEV), index.to(DEV), reduction="none")
+            for t in (teacher, teacher.nan_to_num(0.0, neginf=-INF)))
     assert torch.equal(a, b)
     lone = z.to(DEV)
     teacher[0, 5, 3] = float("nan")

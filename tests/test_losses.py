@@ -294,7 +294,8 @@ def test_sizes_beyond_the_kernels_take_the_torch_formulation(monkeypatch):
         distill_loss = staticmethod(lambda *a: seen.append("kernel") or torch.zeros(()))
 
     monkeypatch.setattr(L.N, "torch_lib", lambda: Kernels)
-    monkeypatch.setattr(L, "_token_logprobs_torch", lambda z, *a: seen.append("torch") or (torch.zeros(1, 1).expand(z.shape[:2]), None))
+    monkeypatch.setattr(L, "_token_logprobs_torch",
+                        lambda z, *a: seen.append("torch") or (torch.zeros(1, 1).expand(z.shape[:2]), None))
     z, labels = torch.zeros(1, 1, 1), torch.zeros(1, 1, dtype=torch.int64)
     for shape in ((1, 5, 4), (1 << 21, 2, 4), (1, (1 << 31) - 1, 4), (1, 2, 1 << 30)):
         e4b.token_logprobs(z.expand(shape), labels.expand(shape[:2]))
