@@ -21,12 +21,12 @@ void rows_of(const LossArgs& a, hipStream_t s) {
   if (a.parts) {
     const unsigned rows = static_cast<unsigned>(a.z.seqs * a.z.tokens);
     hipLaunchKernelGGL((loss_parts_kernel<KIND, DT>), dim3(rows * a.parts), dim3(kPartThreads), 0, s, a);
-    hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, kWave, kRowUnroll>), dim3(rows), dim3(kWave), 0, s, a, int64_t(0));
+    hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, 512, kRowUnroll, true>), dim3(rows), dim3(512), 0, s, a, int64_t(0));
     return;
   }
   const auto with = [&](auto nt) {
     by_launch(a.z.seqs * a.z.tokens, 1, nt(), [&](int64_t first, int64_t rows) {
-      hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, nt(), kRowUnroll>), dim3(static_cast<unsigned>(rows)), dim3(nt()), 0, s, a,
+      hipLaunchKernelGGL((loss_rows_kernel<KIND, DT, nt(), kRowUnroll, false>), dim3(static_cast<unsigned>(rows)), dim3(nt()), 0, s, a,
                          first);
     });
   };
