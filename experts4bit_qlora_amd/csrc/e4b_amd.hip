@@ -302,11 +302,19 @@ int check_logits(const e4b_logits* z, bool labels, const void* stats) {
   return E4B_OK;
 }
 
-// log2(e) / temperature in two parts, both positive: a difference of -inf keeps its sign in either product.
+// log2(e) / temperature in two parts: a head of 12 bits, whose products with 16-bit logits are exact, and the rest. Both are
+// positive: a difference of -inf keeps its sign in either product.
 float2 exponent_scale(float temperature) {
   const double k = 1.4426950408889634 / temperature;
   float hi = static_cast<float>(k);
-  if (hi >= k) hi = std::nextafterf(hi, 0.0f);
+  uint32_t bits;
+  std::memcpy(&bits, &hi, 4);
+  bits &= ~0xfffu;
+  std::memcpy(&hi, &bits, 4);
+  if (hi >= k) {
+    bits -= 0x1000u;
+    std::memcpy(&hi, &bits, 4);
+  }
   return make_float2(hi, static_cast<float>(k - hi));
 }
 

@@ -98,8 +98,10 @@ E4B_DEV void store16_once(uint4* p, const uint4& v) {
 // ---- sums over a row
 
 // k = log2(e) / temperature in two parts: with one, the exponents of all rows are off the same way by 2^-25 or so of
-// their size, which a sequence's sum of log-probabilities adds up (820 tokens: 2e-4).
-E4B_DEV float exp_of(float d, float2 k) { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, k.x, d * k.y)); }
+// their size, which a sequence's sum of log-probabilities adds up (820 tokens: 2e-4). The first has 12 bits, so that what the
+// second adds to x k.x - n is not below that's last bit: rounded away, it would be missing as if there were one part.
+E4B_DEV float times(float d, float2 k) { return __builtin_fmaf(d, k.x, d * k.y); }
+E4B_DEV float exp_of(float d, float2 k) { return __builtin_amdgcn_exp2f(times(d, k)); }
 
 constexpr int kRowUnroll = 4;  // pieces in flight per thread
 constexpr int kPartThreads = 256;
@@ -164,16 +166,15 @@ E4B_DEV float wave_sum(float v) {
 
 // sum_j exp((z_j - ref) / tau) by the whole workgroup, in every lane; ref is the row's element `first`, which
 // is left out if SKIP: a logit that is likely among the largest, not the maximum. fp32 has 2^126 of room on either side, so a
-// maximum kept while the sum runs, with a rescaling at every step, is only needed where a row leaves that room (row_run). It
-// costs two multiply-adds a value, x k - ref k with the factor's second part added in the same way; the rounding of ref k is
-// taken out of the sum. With a running maximum / so, us: 5,500 rows of 128,000 bf16 logits 268 / 253, of 50,257 111 / 106; 37
+// maximum kept while the sum runs, with a rescaling at every step, is only needed where a row leaves that room (Run). It
+// costs two multiply-adds a value, x k.x - ref k and x k.y added to it; the rounding of ref k is taken out of the sum. With a running maximum / so, us: 5,500 rows of 128,000 bf16 logits 268 / 253, of 50,257 111 / 106; 37
 // rows of 128,000 13.6 / 10.6, of 50,257 7.8 / 6.3 (the reference is loaded behind a row's first pieces: before them 5 % more).
 template <int DT, int NT, int U, bool ONCE, bool SKIP>
 E4B_DEV float row_sum(const void* row, int V, int first, float& ref, float2 k, int begin = 0, int end = 0x7fffffff) {
   float at, s = 0.0f;
   const auto ready = [&] {
     ref = Piece<DT>::one(static_cast<const typename Piece<DT>::T*>(row)[first]);
-    at = ref * k.x;
+    at = times(ref, k);
   };
   over_row<DT, NT, U, ONCE, SKIP>(row, V, first, begin, end, ready, [&](const auto& x) {
     float sum = 0.0f;
@@ -193,58 +194,103 @@ E4B_DEV float row_sum(const void* row, int V, int first, float& ref, float2 k, i
   return s;
 }
 
-// Whether a row's reference, scaled, and its sum kept to that room (a NaN does not). Up to this sum the backward's quotient
-// by it is a normal number.
-E4B_DEV bool in_room(float ref, float2 k, float sum) { return fabsf(ref * k.x) < 1e37f && sum < 1e18f; }
+// Whether a row's reference, scaled, and its sum kept to that room (a NaN does not). Up to this reference the two parts of a
+// product, 2^-11 of it, are added to within 1e-6; up to this sum the backward's quotient by it is a normal number.
+E4B_DEV bool in_room(float ref, float2 k, float sum) { return fabsf(ref * k.x) < 65536.0f && sum < 1e18f; }
 
-// Running maximum m and sum s of exp((x - m) / tau), for any finite logits: differences to the maximum are taken before they
-// are scaled, and the type's lowest value stays finite. The largest terms' exponents are the smallest, and so are their
-// roundings: sequences' sums are made of these (kStats). S: the joins' type, 64 bits there: each of nine roundings of a row's
-// whole sum would be one of its log-probability, and 60 tokens' are as large as 1e-6 of their ratio.
+// A sum s of 2^(x k - n) whose reference n is the running maximum of x k rounded up to a whole number: the largest terms' exponents
+// are the smallest, and so are their roundings, and a change of the reference is exact. Sequences' sums are made of these
+// (kStats): a rescaling by a rounded exponential is 3e-9 too small in the mean, and a row's ten of them added up over 2,048
+// tokens to 3e-6 of their ratio; the label as reference rounds the largest terms (60 tokens: 1.4e-6). Joins in 64 bits.
+constexpr float kNoPower = -1e30f;  // nothing summed yet
 template <class S>
-struct RunOf {
-  float m = kLowest;
+struct PowerOf {
+  float n = kNoPower;
   S s = 0;
-  E4B_DEV void join(float om, S os, float2 k) {
-    const float n = fmaxf(m, om);
-    s = s * exp_of(m - n, k) + os * exp_of(om - n, k);
-    m = n;
+  static E4B_DEV S scaled(S v, float by) {  // by: a whole number, not positive
+    const int e = static_cast<int>(fmaxf(by, -2000.0f));
+    if constexpr (sizeof(S) == 8) return __builtin_amdgcn_ldexp(v, e);
+    else return __builtin_amdgcn_ldexpf(v, e);
   }
-  E4B_DEV void join_lanes(int lanes, float2 k) {
-    for (int off = 1; off < lanes; off *= 2) join(__shfl_xor(m, off), __shfl_xor(s, off), k);
+  E4B_DEV void join(float on, S os) {
+    const float to = fmaxf(n, on);
+    s = scaled(s, n - to) + scaled(os, on - to);
+    n = to;
+  }
+  E4B_DEV void join_lanes(int lanes) {
+    for (int off = 1; off < lanes; off *= 2) join(__shfl_xor(n, off), __shfl_xor(s, off));
   }
   template <int N>
   E4B_DEV void add(const float (&x)[N], float2 k) {
-    float n = m, sum = 0.0f;
-    for (float v : x) n = fmaxf(n, v);
-    for (float v : x) sum += exp_of(v - n, k);
-    s = s * exp_of(m - n, k) + sum;
-    m = n;
+    float most = x[0], sum = 0.0f;
+    for (float v : x) most = fmaxf(most, v);
+    const float to = fmaxf(n, __builtin_ceilf(times(most, k)));
+    for (float v : x) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v, k.y, __builtin_fmaf(v, k.x, -to)));
+    s = scaled(s, n - to) + sum;
+    n = to;
   }
 };
 
-template <int DT, int NT, bool SKIP, class S>
-E4B_DEV RunOf<S> row_run(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
-  RunOf<float> r;
-  over_row<DT, NT, kRowUnroll, false, SKIP>(row, V, skip, begin, end, [] {}, [&](const auto& x) { r.add(x, k); });
-  RunOf<S> all;
-  all.m = r.m;
-  all.s = r.s;
-  all.join_lanes(kWave, k);
-  if constexpr (NT > kWave) {
-    constexpr int W = NT / kWave;
-    __shared__ float part_m[W];
-    __shared__ S part_s[W];
-    if ((threadIdx.x & (kWave - 1)) == 0) {
-      part_m[threadIdx.x / kWave] = all.m;
-      part_s[threadIdx.x / kWave] = all.s;
-    }
-    __syncthreads();
-    all.m = part_m[threadIdx.x & (W - 1)];
-    all.s = part_s[threadIdx.x & (W - 1)];
-    all.join_lanes(W, k);
+// A value of each of a workgroup's waves to every lane: lane l has those of wave l mod (NT / 64).
+template <int NT, class R>
+E4B_DEV R of_waves(const R& mine) {
+  constexpr int W = NT / kWave;
+  __shared__ decltype(R::n) part_n[W];
+  __shared__ decltype(R::s) part_s[W];
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    part_n[threadIdx.x / kWave] = mine.n;
+    part_s[threadIdx.x / kWave] = mine.s;
   }
+  __syncthreads();
+  R r;
+  r.n = part_n[threadIdx.x & (W - 1)];
+  r.s = part_s[threadIdx.x & (W - 1)];
+  return r;
+}
+
+template <int DT, int NT, class S>
+E4B_DEV PowerOf<S> row_power(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
+  PowerOf<float> r;
+  over_row<DT, NT, kRowUnroll, false, true>(row, V, skip, begin, end, [] {}, [&](const auto& x) { r.add(x, k); });
+  PowerOf<S> all;
+  all.n = r.n;
+  all.s = r.s;
+  all.join_lanes(kWave);
+  all = of_waves<NT>(all);
+  all.join_lanes(NT / kWave);
   return all;
+}
+
+// The same for any finite logits: running maximum n and sum s of exp((x - n) / tau). Differences to the maximum are taken before
+// they are scaled, and the type's lowest value stays finite.
+struct Run {
+  float n = kLowest, s = 0.0f;
+  E4B_DEV void join(float on, float os, float2 k) {
+    const float to = fmaxf(n, on);
+    s = s * exp_of(n - to, k) + os * exp_of(on - to, k);
+    n = to;
+  }
+  E4B_DEV void join_lanes(int lanes, float2 k) {
+    for (int off = 1; off < lanes; off *= 2) join(__shfl_xor(n, off), __shfl_xor(s, off), k);
+  }
+  template <int N>
+  E4B_DEV void add(const float (&x)[N], float2 k) {
+    float to = n, sum = 0.0f;
+    for (float v : x) to = fmaxf(to, v);
+    for (float v : x) sum += exp_of(v - to, k);
+    s = s * exp_of(n - to, k) + sum;
+    n = to;
+  }
+};
+
+template <int DT, int NT, bool SKIP>
+E4B_DEV Run row_run(const void* row, int V, int skip, float2 k) {
+  Run r;
+  over_row<DT, NT, kRowUnroll, false, SKIP>(row, V, skip, 0, 0x7fffffff, [] {}, [&](const auto& x) { r.add(x, k); });
+  r.join_lanes(kWave, k);
+  r = of_waves<NT>(r);
+  r.join_lanes(NT / kWave, k);
+  return r;
 }
 
 E4B_DEV float any_float(const void* p, int dtype, int64_t i) {
@@ -289,7 +335,7 @@ struct Entry {
 // vocabulary, a value above -inf) and tau^2 sum_k p_k (log p_k - log q_k); zero where no entry is usable. `own`: entry
 // `lane`; the others are loaded in each pass.
 template <int DT>
-E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, const Entry& own, RunOf<float>& r) {
+E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<DT>::T* row, const Entry& own, Run& r) {
   const float tau = a.z.temperature, per = 1.0f / tau;
   const int lane = threadIdx.x;
   auto entry = [&](int k) { return k == lane ? own : Entry(a, at, k); };
@@ -318,7 +364,7 @@ E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<D
       const float w = (e.w - most) * per;
       p = expf(w) * inv;
       // log p - log q; an entry without probability adds nothing, whatever the student holds there
-      const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[e.j]) - r.m) * per - log_s;
+      const float lq = r.s == 0.0f ? -__builtin_inff() : (Piece<DT>::one(row[e.j]) - r.n) * per - log_s;
       if (!(p == 0.0f)) sum += p * ((w - log_norm) - lq);
     }
     a.share[at * a.top + k] = p;
@@ -346,8 +392,8 @@ __global__ __launch_bounds__(kPartThreads) void loss_parts_kernel(LossArgs a) {
   const int V = static_cast<int>(a.z.vocab), own = static_cast<int>(reference_of<KIND>(a, at, tok));
   const int begin = part * step;
   if constexpr (KIND == kStats) {
-    const RunOf<float> r = row_run<DT, kPartThreads, true, float>(tok.row, V, own, a.k, begin, begin + step);
-    if (threadIdx.x == 0) static_cast<float2*>(a.z.workspace)[blockIdx.x] = make_float2(r.m, r.s);
+    const PowerOf<float> r = row_power<DT, kPartThreads, float>(tok.row, V, own, a.k, begin, begin + step);
+    if (threadIdx.x == 0) static_cast<float2*>(a.z.workspace)[blockIdx.x] = make_float2(r.n, r.s);
   } else {
     float ref;
     const float s = row_sum<DT, kPartThreads, kRowUnroll, KIND == kScore, KIND != kDistill>(tok.row, V, own, ref, a.k, begin,
@@ -357,16 +403,13 @@ __global__ __launch_bounds__(kPartThreads) void loss_parts_kernel(LossArgs a) {
 }
 
 // A label's log-probability from its logit and the running sum of the others, with the statistics (m, s) of the whole row.
-template <class S>
-E4B_DEV S join_label(float own, const RunOf<S>& r, const LossArgs& a, float& m, float& s) {
-  m = fmaxf(r.m, own);
-  const S rest = r.s * exp_of(r.m - m, a.k);
-  s = static_cast<float>(rest + exp_of(own - m, a.k));
+E4B_DEV float join_label(float own, const Run& r, const LossArgs& a, float& m, float& s) {
+  m = fmaxf(r.n, own);
+  const float rest = r.s * exp_of(r.n - m, a.k);
+  s = rest + exp_of(own - m, a.k);
   // the sum is 0 where every logit is -inf: each label has probability 0
   if (s == 0.0f) return -__builtin_inff();
-  const S d = (static_cast<S>(own) - m) / a.z.temperature;  // also where it is 0, for a label of +inf
-  if constexpr (sizeof(S) == 8) return d - (own == m ? log1p(rest) : log(rest + exp(d)));
-  else return d - (own == m ? log1pf(rest) : logf(s));
+  return (own - m) / a.z.temperature - (own == m ? log1pf(rest) : logf(s));  // the first also where it is 0, for a label of +inf
 }
 
 // A workgroup per row; SPLIT: one that joins a split row's parts, each wave for itself.
@@ -396,49 +439,53 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
     old = a.old_logps[u];
     if (a.ref_logps) ref = a.ref_logps[u];
   }
-  float own, m, s, lp, low = 0.0f;
+  float own, sum = 0.0f;  // sum of the others' exponentials against own (a teacher: of all)
+  PowerOf<double> power;
+  const Entry teacher(a, at, KIND == kDistill ? static_cast<int>(threadIdx.x) : a.top);
   const int lane = threadIdx.x & (kWave - 1);
   if constexpr (KIND == kStats) {
     own = P::one(row[first]);
-    RunOf<double> r;
     if constexpr (SPLIT) {
       const float2* parts = static_cast<const float2*>(a.z.workspace) + at * a.parts;
-      for (int i = lane; i < a.parts; i += kWave) r.join(parts[i].x, parts[i].y, a.k);
-      r.join_lanes(kWave, a.k);
+      for (int i = lane; i < a.parts; i += kWave) power.join(parts[i].x, parts[i].y);
+      power.join_lanes(kWave);
     } else {
-      r = row_run<DT, NT, true, double>(row, V, first, a.k);
+      power = row_power<DT, NT, double>(row, V, first, a.k);
     }
-    if (threadIdx.x >= kWave) return;
-    const double l = join_label(own, r, a, m, s);
-    lp = static_cast<float>(l);
-    low = lp - lp == 0.0f ? static_cast<float>(l - lp) : 0.0f;
+    // nothing summed: row_run decides
+    sum = power.n == kNoPower ? __builtin_nanf("")
+                              : static_cast<float>(power.s) * __builtin_amdgcn_exp2f(power.n - times(own, a.k));
+  } else if constexpr (SPLIT) {
+    own = P::one(row[first]);
+    for (int i = lane; i < a.parts; i += kWave) sum += static_cast<const float*>(a.z.workspace)[at * a.parts + i];
+    sum = wave_sum(sum);
   } else {
-    float sum = 0.0f;
-    const Entry teacher(a, at, KIND == kDistill ? static_cast<int>(threadIdx.x) : a.top);
-    if constexpr (SPLIT) {
-      own = P::one(row[first]);
-      for (int i = lane; i < a.parts; i += kWave) sum += static_cast<const float*>(a.z.workspace)[at * a.parts + i];
-      sum = wave_sum(sum);
-    } else {
-      sum = row_sum<DT, NT, U, KIND == kScore, KIND != kDistill>(row, V, first, own, a.k);
-    }
-    RunOf<float> r;
-    r.m = m = own;
-    r.s = sum;
-    // rows of -inf, labels less likely than 1e-18: read once more, from the caches (all of 8,192 rows of 128,000: 321 -> 605 us,
-    // of 64 10 -> 18, of 800 of 50,257 16 -> 31)
-    const bool again = !in_room(own, a.k, sum);
-    if (again) r = row_run<DT, NT, KIND != kDistill, float>(row, V, first, a.k);
-    if (threadIdx.x >= kWave) return;
-    if constexpr (KIND == kDistill) {
-      const float loss = teacher_loss<DT>(a, at, row, teacher, r);
-      if (lead) a.token_loss[at] = loss;
-      if (lead) a.stats[at] = make_float4(r.m, r.s, 0.0f, 0.0f);
-      return;
-    } else {
-      s = 1.0f + sum;
-      lp = again ? join_label(own, r, a, m, s) : -log1pf(sum);
-    }
+    sum = row_sum<DT, NT, U, KIND == kScore, KIND != kDistill>(row, V, first, own, a.k);
+  }
+  Run r;
+  r.n = own;
+  r.s = sum;
+  // rows of -inf, labels less likely than 1e-18: read once more, from the caches (all of 8,192 rows of 128,000: 321 -> 605 us,
+  // of 64 10 -> 18, of 800 of 50,257 16 -> 31)
+  const bool again = !in_room(own, a.k, sum);
+  if (again) r = row_run<DT, NT, KIND != kDistill>(row, V, first, a.k);
+  if (threadIdx.x >= kWave) return;
+  if constexpr (KIND == kDistill) {
+    const float loss = teacher_loss<DT>(a, at, row, teacher, r);
+    if (lead) a.token_loss[at] = loss;
+    if (lead) a.stats[at] = make_float4(r.n, r.s, 0.0f, 0.0f);
+    return;
+  }
+  float m = own, s = 1.0f + sum, lp, low = 0.0f;
+  if (again) {
+    lp = join_label(own, r, a, m, s);
+  } else if constexpr (KIND == kStats) {
+    const double rest = power.s * exp2(power.n - own * (static_cast<double>(a.k.x) + a.k.y)), l = -log1p(rest);
+    s = static_cast<float>(1.0 + rest);
+    lp = static_cast<float>(l);
+    low = static_cast<float>(l - lp);
+  } else {
+    lp = -log1pf(sum);
   }
   if (lead) {
     if (KIND != kStats) a.logps[at] = lp;

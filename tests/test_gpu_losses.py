@@ -3,7 +3,8 @@
 Tolerances, with u = 2^-24, D = (max z - z_j) / temperature and R the row's largest D at most 104 (beyond, an exponential is
 below fp32's smallest value and its error below 2^-149): a difference to the maximum, its factor log2(e) / temperature and
 their product make an exponential's argument off by at most 4 u D, the exponential by 2 u more (where the difference is to
-the label instead, two multiply-adds round an argument of at most D_j + D_l <= 2 R: 1.4 u of that, no more). A row's sum has
+the label instead, two multiply-adds round an argument of at most D_j + D_l <= 2 R: 1.4 u of that, no more; and the first's result
+may be larger than that by the product with the factor's small part, 2^-11 of at most 2^16: 22 u, which n has room for). A row's sum has
 at most n = max(64, V / 256) + 40 additions one after the other, each of which may be followed by a rescaling of 3
 roundings, so it is off by E = (4 R + 4 n) u relative. A log-probability D_l - log s is off by E + (3 D_l + 2 |log s| + |lp|) u; a
 probability by E + (4 D + 8) u relative; a result rounded into a 16-bit type by half a step of it, or of its smallest
@@ -177,6 +178,38 @@ def test_logprobs_ranges_and_extremes(dtype):
         _check_logprobs(z, labels, tau=tau)
     for spread in (1e-4, 30.0, 300.0):
         _check_logprobs(_logits((1, 12, V), dtype, 5, spread), labels)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_logits_far_from_zero(dtype):
+    """The same rows moved up and down: on both sides of where the reference leaves fp32's room, and far behind it."""
+    V = 5000
+    z = _logits((2, 4, V), torch.float32, 81, 2.0)
+    labels = torch.randint(0, V, (2, 4), generator=_gen(82))
+    for off in (3e2, -3e3, 4e4, 4.5e4, -4.55e4, -4.6e4, 6e4, 1e6, -1e6, 1e10, -1e10):
+        if dtype != torch.float16 or abs(off) <= 6e4:
+            moved = (z + off).to(dtype)
+            _check_logprobs(moved, labels)
+            want = torch.log_softmax(moved.double(), -1).gather(-1, labels.unsqueeze(-1)).double()[..., 0]
+            rewards = e4b.preference_loss(moved.to(DEV), labels.to(DEV), beta=1.0)[1].cpu()
+            r = Row64(moved, 1.0)
+            bound = r.lp_bound().gather(-1, labels.unsqueeze(-1))[..., 0]
+            _near(rewards, want.sum(-1), bound.sum(-1) + 2 * U * want.sum(-1).abs(), f"rewards at {off}")
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("V", (1000, 32000))
+def test_rewards_errors_do_not_add_up(dtype, V):
+    """A sequence's log-probabilities summed: rounded to the nearest, their errors are as often up as down. 2,048 of them are off
+    by 2^-26 each in the mean at most, a quarter of the half step of one rounding that always goes the same way."""
+    T = 2048
+    z = _logits((2, T, V), dtype, 83, 2.0)
+    labels = torch.randint(0, V, (2, T), generator=_gen(84))
+    lp = torch.log_softmax(z.double(), -1).gather(-1, labels.unsqueeze(-1))[..., 0]
+    ref = lp.float()
+    rewards = e4b.preference_loss(z.to(DEV), labels.to(DEV), ref.to(DEV), beta=1.0)[1].cpu().double()
+    off = rewards - (lp - ref.double()).sum(-1)
+    assert (off.abs() <= T * 2.0 ** -26).all(), off / T
 
 
 def test_temperatures_at_the_ends():
