@@ -3,7 +3,7 @@
 ``token_logprobs`` (the log-probability of each label: what serving reports for a generated token, and what the losses take
 from an older or a reference model), ``preference_loss`` (paired log ratios of chosen and rejected answers),
 ``policy_loss`` (clipped ratios with a KL term) and ``distill_loss`` (divergence from a teacher's top logits). On a HIP
-device each reads the logits once forward and once backward (``csrc/losses.h``) and keeps two floats per token
+device each reads the logits once forward and once backward (``csrc/losses.h``) and keeps a few floats per token
 between; tensors elsewhere, other dtypes, sizes beyond the kernels' limits, and tensors that a transform, a trace or
 forward-mode differentiation follows take the torch formulation, which is the definition.
 
