@@ -87,12 +87,13 @@ def _reduction(name: str) -> int:
 
 
 def _fits(z: torch.Tensor, temperature: float, *others) -> bool:
-    """Whether the kernels may take these: plain device tensors within the limits of ``e4b_logits``."""
-    if not _on_kernel(z):
+    """Whether the kernels may take these: plain device tensors, in memory as they are to be read, within the limits of
+    ``e4b_logits``."""
+    if not _on_kernel(z) or z.is_neg():
         return False
     wrapped = torch._C._functorch.is_functorch_wrapped_tensor
     for t in others:
-        if t is not None and wrapped(t):
+        if t is not None and (wrapped(t) or t.is_neg()):
             return False
     seqs, tokens, vocab = z.shape
     return seqs <= 2 ** 21 and seqs * tokens < 2 ** 31 and vocab <= 2 ** 30 and 1e-30 < temperature < 1e30

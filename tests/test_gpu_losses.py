@@ -768,6 +768,24 @@ def test_leaf_gradients_accumulate():
     assert torch.equal(leaf.grad, parts[0] + parts[1])
 
 
+def test_views_with_a_pending_sign():
+    """Real tensors whose memory holds their negative (the imaginary part of a conjugate)."""
+    z, labels = _logits((2, 5, 300), torch.float32, 91).to(DEV), torch.randint(0, 300, (2, 5), generator=_gen(92)).to(DEV)
+    old, adv = _logits((2, 5), torch.float32, 93).to(DEV), _logits((2,), torch.float32, 94).to(DEV)
+    index, teacher = torch.randint(0, 300, (2, 5, 7), generator=_gen(95)).to(DEV), _logits((2, 5, 7), torch.float32, 96).to(DEV)
+
+    def negative(t):
+        out = torch.complex(t, -t).conj().imag
+        assert out.is_neg() and torch.equal(out, t)
+        return out
+
+    for a, b in ((e4b.token_logprobs(z, labels), e4b.token_logprobs(negative(z), labels)),
+                 (e4b.policy_loss(z, labels, old, adv)[0], e4b.policy_loss(z, labels, negative(old), negative(adv))[0]),
+                 (e4b.preference_loss(z, labels, old)[0], e4b.preference_loss(z, labels, negative(old))[0]),
+                 (e4b.distill_loss(z, teacher, index), e4b.distill_loss(z, negative(teacher), index))):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)  # the wrong sign is off by the values themselves
+
+
 def test_outputs_changed_in_place_leave_the_gradient():
     z, labels, mask, index, teacher, old = _inputs()
     leaf = z.detach().requires_grad_()
