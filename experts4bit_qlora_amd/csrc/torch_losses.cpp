@@ -90,10 +90,11 @@ void keep(AutogradContext* ctx, const Kept& k) {
   ctx->saved_data["k"] = c10::IValue(std::make_tuple(k.temperature, k.reduction, k.coef));
 }
 
-Tensor backward_of(AutogradContext* ctx, const Tensor& grad) {
-  if (!grad.defined()) return Tensor();
+Tensor backward_of(AutogradContext* ctx, const Tensor& upstream) {
+  if (!upstream.defined()) return Tensor();
   if (at::GradMode::is_enabled())
     throw std::runtime_error("the losses over logits are differentiable once: no create_graph=True on the device");
+  const Tensor grad = upstream.resolve_neg();  // complex products' backwards pass tensors whose memory holds their negative
   const auto t = ctx->get_saved_variables();
   const Tensor &z = t[0], &labels = t[1], &mask = t[2], &index = t[3], &share = t[4], &saved = t[5];
   const auto k = ctx->saved_data["k"].toTuple();

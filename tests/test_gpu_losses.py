@@ -968,3 +968,36 @@ def test_a_training_step_with_the_adapters():
             assert torch.isfinite(a).all() and a.any()
             assert (a - b).norm() <= 2e-2 * b.norm()
     e4b.disable_fast_train(lora)
+
+
+def _every_loss(labels, old, teacher, index):
+    """The losses as functions of the logits, every reduction among them."""
+    adv = old.sum(-1) + 9
+    return {"logprobs": lambda a: e4b.token_logprobs(a, labels), "preference": lambda a: e4b.preference_loss(a, labels, old)[0],
+            "policy, each": lambda a: e4b.policy_loss(a, labels, old, adv, old, kl_coef=0.1, reduction="none")[0],
+            "policy, sequences": lambda a: e4b.policy_loss(a, labels, old, adv, reduction="sequence")[0],
+            "distill, mean": lambda a: e4b.distill_loss(a, teacher, index),
+            "distill, each": lambda a: e4b.distill_loss(a, teacher, index, reduction="none")}
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_upstream_gradients_with_a_pending_sign(dtype):
+    """Upstream gradients whose memory holds their negative: given by the caller, and as torch's complex products pass them."""
+    z, labels, mask, index, teacher, old = _inputs(dtype, 4, 6, 300)
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        leaf = z.detach().requires_grad_()
+        loss = f(leaf)
+        up = torch.randn(loss.shape, generator=_gen(97)).to(DEV)
+        (want,) = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+        negative = torch.complex(up, -up).conj().imag
+        assert negative.is_neg() and torch.equal(negative, up) and want.any()
+        assert torch.equal(torch.autograd.grad(loss, leaf, negative)[0], want), name
+        seen = []
+        loss = f(leaf)
+        loss.register_hook(lambda g: seen.append(g))
+        w = torch.complex(up, up * 0.5 + 1)
+        total = (torch.complex(torch.ones_like(loss), loss).conj() * w).sum().real
+        (got,) = torch.autograd.grad(total, leaf)
+        assert seen[0].is_neg(), name
+        (want,) = torch.autograd.grad(f(leaf), leaf, seen[0].resolve_neg().clone())
+        assert torch.equal(got, want), name
