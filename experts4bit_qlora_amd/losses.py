@@ -153,10 +153,11 @@ def _log_softmax(z: torch.Tensor, counted: torch.Tensor, temperature: float) -> 
 
 
 def _token_logprobs_torch(z, labels, mask, temperature):
+    labels = labels.to(torch.int64)  # the vocabulary's size may lie outside their own type, where it would wrap
     counted = (labels >= 0) & (labels < z.shape[-1])
     if mask is not None:
         counted = counted & mask
-    at = torch.where(counted, labels, 0).to(torch.int64).unsqueeze(-1)
+    at = torch.where(counted, labels, 0).unsqueeze(-1)
     logps = _log_softmax(z, counted, temperature).gather(-1, at).squeeze(-1)
     return torch.where(counted, logps, 0.0), counted
 
@@ -325,6 +326,7 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
 
 def _distill_loss_torch(z, mask, teacher, index, temperature, reduction):
     counted = torch.ones(z.shape[:2], dtype=torch.bool, device=z.device) if mask is None else mask.expand(z.shape[:2])
+    index = index.to(torch.int64)
     log_q = _log_softmax(z, counted, temperature)
     w = teacher.detach().to(log_q.dtype)
     usable = (index >= 0) & (index < z.shape[-1]) & counted.unsqueeze(-1)
@@ -334,6 +336,6 @@ def _distill_loss_torch(z, mask, teacher, index, temperature, reduction):
     y = (w - top) / temperature
     log_p = torch.log_softmax(torch.where(none, 0.0, y), -1)
     p = torch.exp(log_p).masked_fill(none, 0.0)
-    away = log_p - log_q.gather(-1, torch.where(usable, index, 0).to(torch.int64))
+    away = log_p - log_q.gather(-1, torch.where(usable, index, 0))
     each = temperature ** 2 * torch.where(p == 0, 0.0, p * torch.where(p == 0, 0.0, away)).sum(-1)
     return _reduce_torch(torch.where(counted, each, 0.0), counted, reduction)

@@ -308,3 +308,24 @@ def test_sizes_beyond_the_kernels_take_the_torch_formulation(monkeypatch):
     for k, dtype in ((1024, torch.float32), (1025, torch.float32), (4, torch.float64)):
         e4b.distill_loss(z, torch.zeros(1, 1, 1, dtype=dtype).expand(1, 1, k), labels.unsqueeze(-1).expand(1, 1, k))
     assert seen[9:] == ["kernel", "torch", "torch"]
+
+
+@pytest.mark.parametrize("vocab", (300, 50257))
+@pytest.mark.parametrize("dtype", (torch.uint8, torch.int8, torch.int16, torch.int32, torch.uint16, torch.uint32, torch.uint64))
+def test_narrow_and_unsigned_labels_and_indexes(dtype, vocab):
+    """Integer types that do not hold the vocabulary's size, or that torch does not compare: as int64."""
+    z = (2 * torch.randn(2, 4, vocab, generator=_gen(7))).requires_grad_()
+    top = min(vocab, torch.iinfo(dtype).max + 1)
+    labels = torch.randint(0, top, (2, 4), generator=_gen(8))
+    labels[0, 0], labels[0, 1] = 0, top - 1
+    if dtype.is_signed:
+        labels[1, 0] = -100
+    index = torch.randint(0, top, (2, 4, 3), generator=_gen(9))
+    teacher = torch.randn(2, 4, 3, generator=_gen(10))
+    old, adv = torch.full((2, 4), -9.0), torch.tensor([1.0, -1.0])
+    for f, i in ((lambda i: e4b.token_logprobs(z, i), labels), (lambda i: e4b.preference_loss(z, i)[0], labels),
+                 (lambda i: e4b.policy_loss(z, i, old, adv)[0], labels), (lambda i: e4b.distill_loss(z, teacher, i), index)):
+        want, got = f(i), f(i.to(dtype))
+        assert torch.equal(got, want) and want.any()
+        ours, theirs = (torch.autograd.grad(v.sum(), z)[0] for v in (got, want))
+        assert torch.equal(ours, theirs) and theirs.any()
