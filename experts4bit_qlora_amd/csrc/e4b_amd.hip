@@ -807,13 +807,16 @@ int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStrea
   return check_launch("loss_rows_kernel");
 }
 
-int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_token, int32_t kind, float beta,
+int e4b_preference_loss(const e4b_logits* z, const void* ref, int32_t ref_kind, int32_t kind, float beta,
                         float smoothing, int32_t average, float* loss, float* rewards, float* stats, float* coef,
                         hipStream_t stream) {
   int rc = check_logits(z, true, stats);
   if (rc) return rc;
   if (z->seqs % 2) return fail(E4B_EINVAL, "seqs=%lld is odd", (long long)z->seqs);
   if (kind < E4B_PREFERENCE_SIGMOID || kind > E4B_PREFERENCE_IPO) return fail(E4B_EINVAL, "bad preference kind %d", kind);
+  if (ref_kind < E4B_REF_SEQUENCE || ref_kind > E4B_REF_TOKEN_FP64) return fail(E4B_EINVAL, "bad ref_kind %d", ref_kind);
+  if (reinterpret_cast<uintptr_t>(ref) & (ref_kind >= E4B_REF_SEQUENCE_FP64 ? 7 : 3))
+    return fail(E4B_EINVAL, "ref is not aligned to its dtype");
   if (!(beta > 0.0f) || !std::isfinite(beta)) return fail(E4B_EINVAL, "beta must be positive and finite");
   if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return fail(E4B_EINVAL, "smoothing outside [0, 1]");
   if (z->seqs == 0) return E4B_OK;
@@ -821,7 +824,7 @@ int e4b_preference_loss(const e4b_logits* z, const float* ref, int32_t ref_per_t
   if ((rc = check_loss_workspace(*z))) return rc;
   e4b::LossArgs a = loss_args(*z, stats);
   if (z->tokens) e4b::launch_loss_rows(e4b::kStats, a, stream);
-  const e4b::PairArgs p{z->seqs, z->tokens, a.stats, ref, ref_per_token, kind, beta, smoothing, average, loss, rewards, coef};
+  const e4b::PairArgs p{z->seqs, z->tokens, a.stats, ref, ref_kind, kind, beta, smoothing, average, loss, rewards, coef};
   e4b::launch_pairs(p, stream);
   return check_launch("pairs_kernel");
 }

@@ -562,6 +562,11 @@ __global__ __launch_bounds__(kJoin) void loss_mean_kernel(MeanArgs a) {
 // differences short.
 __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
   const int64_t half = a.seqs / 2, b = blockIdx.x;
+  const bool ref_of_tokens = a.ref_kind == E4B_REF_TOKEN || a.ref_kind == E4B_REF_TOKEN_FP64;
+  // in the type that they come in: of two sums of thousands the difference is left
+  auto ref = [&](int64_t i) -> double {
+    return a.ref_kind >= E4B_REF_SEQUENCE_FP64 ? static_cast<const double*>(a.ref)[i] : static_cast<const float*>(a.ref)[i];
+  };
   double v[4] = {0.0, 0.0, 0.0, 0.0};  // sum of lp - ref over the counted tokens, their number; of both sequences
   for (int64_t i = threadIdx.x; i < 2 * a.tokens; i += kJoin) {
     const bool second = i >= a.tokens;
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
     const float4 st = a.stats[at];
     if (st.y < 0.0f) continue;
     double lp = static_cast<double>(st.z) + st.w;
-    if (a.ref && a.ref_per_token) lp -= a.ref[at];
+    if (a.ref && ref_of_tokens) lp -= ref(at);
     v[0] += second ? 0.0 : lp;
     v[1] += second ? 0.0 : 1.0;
     v[2] += second ? lp : 0.0;
@@ -585,7 +590,7 @@ __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
       each[i] = 1.0 / n;
       ratio[i] *= each[i];
     }
-    if (a.ref && !a.ref_per_token) ratio[i] -= a.ref[b + i * half];
+    if (a.ref && !ref_of_tokens) ratio[i] -= ref(b + i * half);
     a.rewards[b + i * half] = static_cast<float>(a.beta * ratio[i]);
   }
   const double d = ratio[0] - ratio[1], beta = a.beta, h = beta * d, eps = a.smoothing;

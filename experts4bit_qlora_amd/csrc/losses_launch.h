@@ -61,8 +61,8 @@ void launch_loss_mean(const MeanArgs& a, hipStream_t s);
 struct PairArgs {
   int64_t seqs, tokens;  // the first half of the sequences are the chosen ones
   const float4* stats;
-  const float* ref;  // [R], [seqs] or NULL
-  int ref_per_token;
+  const void* ref;  // [R], [seqs] or NULL
+  int ref_kind;     // e4b_reference
   int kind;  // e4b_preference
   float beta, smoothing;
   int average;

@@ -152,6 +152,13 @@ struct Logprobs : Function<Logprobs> {
   }
 };
 
+int32_t reference_kind(const Tensor& ref) {
+  if (!ref.defined()) return E4B_REF_SEQUENCE;
+  const bool wide = ref.scalar_type() == torch::kDouble;
+  if (ref.dim() == 2) return wide ? E4B_REF_TOKEN_FP64 : E4B_REF_TOKEN;
+  return wide ? E4B_REF_SEQUENCE_FP64 : E4B_REF_SEQUENCE;
+}
+
 struct Preference : Function<Preference> {
   static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& labels, const Maybe& mask_,
                                const Maybe& ref_, int64_t kind, double beta, double smoothing, bool average) {
@@ -164,7 +171,7 @@ struct Preference : Function<Preference> {
     const Tensor loss = floats({d.seqs / 2}, z), rewards = floats({d.seqs}, z), saved = floats({4 * rows + d.seqs}, z);
     float* at = ptr<float>(saved);
     check("e4b_preference_loss",
-          e4b_preference_loss(&d, ptr<const float>(ref), ref.defined() && ref.dim() == 2, static_cast<int32_t>(kind),
+          e4b_preference_loss(&d, ptr<const void>(ref), reference_kind(ref), static_cast<int32_t>(kind),
                               static_cast<float>(beta), static_cast<float>(smoothing), average, ptr<float>(loss),
                               ptr<float>(rewards), at, at + 4 * rows, stream_of(z)));
     ctx->save_for_backward({z, labels, mask, Tensor(), Tensor(), saved});

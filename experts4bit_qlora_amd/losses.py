@@ -175,7 +175,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     reference model, ``d = (S_c - r_c) - (S_r - r_r)`` and ``h = beta d``: ``"sigmoid"`` ``-(1 - e) log sigmoid(h) - e
     log sigmoid(-h)`` with ``e = label_smoothing``, ``"hinge"`` ``max(0, 1 - h)``, ``"ipo"`` ``(d - 1 / (2 beta))^2``.
     ``ref_logps``: per token ``[2B, T]`` as ``token_logprobs`` gives them (the difference is then summed in 64 bits
-    token by token), or the answers' sums (means) ``[2B]``; None: zeros. ``rewards = beta (S - r)``, constants to the
+    token by token), or the answers' sums (means) ``[2B]``, fp64 ones as they are; None: zeros. ``rewards = beta (S - r)``, constants to the
     gradient. The loss is differentiable with respect to the logits (once)."""
     if logits.dim() != 3 or logits.shape[0] % 2:
         raise ValueError(f"logits must be [2 * pairs, tokens, vocab], got {list(logits.shape)}")
@@ -195,7 +195,9 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     kind = _PREFERENCE[loss_type]
     if not (_fits(z, 1.0, labels, m, ref_logps) and 1e-30 < beta < 1e30):
         return _preference_loss_torch(z, labels, m, ref_logps, kind, beta, label_smoothing, average)
-    ref = None if ref_logps is None else _constant(ref_logps, torch.float32, ref_logps.shape)
+    ref = ref_logps
+    if ref is not None:
+        ref = _constant(ref, ref.dtype if ref.dtype == torch.float64 else torch.float32, ref.shape)
     return N.torch_lib().preference_loss(_rows(z), _constant(labels, torch.int64, shape), _contiguous(m), ref, kind, beta,
                                          label_smoothing, average)
 
@@ -237,8 +239,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     With ``lp`` a token's log-probability at the temperature, ``r = exp(lp - old_logps)`` and ``x = ref_logps - lp``, a
     counted token's loss is ``-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (e^x - x - 1)``; the KL term
     needs ``ref_logps``. ``reduction``: ``"mean"`` over all counted tokens (one value), ``"sequence"`` over
-    each sequence's ``[...]``, ``"none"`` each token's ``[..., T]``; 0 where nothing counts. ``logps`` are constants
-    to the gradient. The loss is differentiable with respect to the logits (once)."""
+    each sequence's ``[...]``, ``"none"`` each token's ``[..., T]``; 0 where nothing counts. ``old_logps``,
+    ``advantages`` and ``ref_logps`` are taken in fp32 (fp64 for fp64 logits). ``logps`` are constants to the gradient. The
+    loss is differentiable with respect to the logits (once)."""
     z, shape = _sequences(logits)
     _integers("labels", labels, logits, shape)
     _floats("old_logps", old_logps, logits, shape)

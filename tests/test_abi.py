@@ -493,3 +493,18 @@ def test_loss_entry_points_reject_bad_arguments():
     assert back(z(), seqs=0) == -1 and back(z(), index=4096, share=None, top=4) == back(z(), index=4096, share=4096) == -1
     assert back(z(), index=4096, share=4096, top=1025) == -2 and back(z(), out=4104) == -1 and "16-byte" in _err()
     assert back(z(tokens=0, p=None)) == 0
+
+
+def test_preference_reference_kinds():
+    L = N.lib()
+    z = ctypes.byref(N.Logits(4096, N.BF16, 1.0, 2, 3, 10, 30, 10, 4096, None, 0, None, 0))
+
+    def pref(ref, kind):
+        return L.e4b_preference_loss(z, ref, kind, 0, 0.1, 0.0, 0, None, 4096, 4096, 4096, None)
+
+    for kind in (-1, 4):
+        assert pref(4096, kind) == -1 and "ref_kind" in _err()
+    for kind, bad in ((0, 4098), (1, 4097), (2, 4100), (3, 4100)):
+        assert pref(bad, kind) == -1 and "aligned" in _err()
+    for kind, good in ((0, 4100), (1, 4100), (2, 4104), (3, 4104), (3, None)):
+        assert pref(good, kind) == -1 and "loss" in _err()  # what is refused next

@@ -1001,3 +1001,50 @@ def test_upstream_gradients_with_a_pending_sign(dtype):
         assert seen[0].is_neg(), name
         (want,) = torch.autograd.grad(f(leaf), leaf, seen[0].resolve_neg().clone())
         assert torch.equal(got, want), name
+
+
+@pytest.mark.parametrize("loss_type", ("sigmoid", "ipo"))
+def test_references_in_64_bits(loss_type, monkeypatch):
+    """References whose values lie between fp32's: the rewards move by just what was added to an fp32 reference, up to their own
+    rounding; per token and per sequence, without the torch formulation."""
+    monkeypatch.setattr(L, "_preference_loss_torch", None)
+    z = _logits((4, 1500, 500), torch.float32, 98).to(DEV)
+    labels = torch.randint(0, 500, (4, 1500), generator=_gen(99)).to(DEV)
+    lp = torch.log_softmax(z.cpu().double(), -1).gather(-1, labels.cpu().unsqueeze(-1))[..., 0]
+    for ref, move in ((lp.float(), lp.abs() * 2.0 ** -26),  # a quarter of their spacing at most
+                      (lp.sum(-1).float(), torch.tensor([2e-4, -1e-4, 3e-4, 1e-4], dtype=torch.float64))):
+        fine = ref.double() + move
+        assert torch.equal(fine.float(), ref)  # rounded to fp32, nothing of it is left
+        kw = dict(beta=1.0, loss_type=loss_type)
+        base = e4b.preference_loss(z, labels, ref.to(DEV), **kw)[1].cpu().double()
+        leaf = z.detach().requires_grad_()
+        loss, got = e4b.preference_loss(leaf, labels, fine.to(DEV), **kw)
+        want = base - (move.sum(-1) if move.dim() == 2 else move)
+        # the rewards' two roundings, and the 64-bit sums of 1,500 terms below 32
+        assert ((got.cpu().double() - want).abs() <= U * (base.abs() + want.abs()) + 1500 * 1500 * 32 * 2.0 ** -53).all()
+        d = want[:2] - want[2:]
+        value = (d - 0.5) ** 2 if loss_type == "ipo" else -torch.nn.functional.logsigmoid(d)
+        slope = 2 * (d - 0.5) if loss_type == "ipo" else -torch.sigmoid(-d)
+        slack = U * (base.abs() + want.abs()).sum() + 1e-9
+        assert ((loss.detach().cpu().double() - value).abs() <= 2 * U * value + 2 * slope.abs() * slack).all()
+        # the gradients along the label's row are the slope's: their ratio to the slope is that of the fp32 reference's
+        (grad,) = torch.autograd.grad(loss.sum(), leaf)
+        q = torch.softmax(z.cpu().double(), -1)
+        pull = torch.cat([slope, -slope])[:, None] * (1 - q.gather(-1, labels.cpu().unsqueeze(-1))[..., 0])
+        r = Row64(z, 1.0)
+        bound = r.q_bound().gather(-1, labels.cpu().unsqueeze(-1))[..., 0] * torch.cat([slope, slope]).abs()[:, None]
+        _near(grad.gather(-1, labels.unsqueeze(-1))[..., 0], pull, bound + 8 * U * pull.abs() + 2 * slack, "gradient")
+
+
+def test_references_in_64_bits_behind_the_mask():
+    z, labels, mask, index, teacher, old = _inputs(torch.float32)
+    counted = mask & (labels >= 0)
+    bad = old.double().masked_fill(~counted, float("nan"))
+    for average in (False, True):
+        for a, b in zip(e4b.preference_loss(z, labels, old, mask=mask, average=average),
+                        e4b.preference_loss(z, labels, bad, mask=mask, average=average)):
+            assert torch.equal(a, b)
+        sums = old.sum(-1)
+        for a, b in zip(e4b.preference_loss(z, labels, sums, mask=mask, average=average),
+                        e4b.preference_loss(z, labels, sums.double(), mask=mask, average=average)):
+            assert torch.equal(a, b)
