@@ -4,12 +4,16 @@
 // A backward pass runs on autograd's own thread of the device. With the functions here it needs no interpreter lock there:
 // in Python the two threads hand the lock and its objects' cache lines back and forth, and a small call's forward and
 // backward took 105 us of host time, of which torch's own engine is about 45.
+#include <ATen/functorch/BatchedTensorImpl.h>
+// behind the one above, whose own calls it would make ambiguous
+#include <ATen/LegacyBatchedTensorImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "e4b_amd.h"
 
@@ -90,35 +94,69 @@ void keep(AutogradContext* ctx, const Kept& k) {
   ctx->saved_data["k"] = c10::IValue(std::make_tuple(k.temperature, k.reduction, k.coef));
 }
 
+template <class F>
+Tensor of_each(const Tensor& grad, const F& f);
+
+// f of each slice all[i]
+template <class F>
+Tensor stack_of(const Tensor& all, const F& f) {
+  std::vector<Tensor> out;
+  for (int64_t i = 0; i < all.size(0); ++i) out.push_back(of_each(all.select(0, i), f));
+  return at::stack(out);
+}
+
+// f(grad); where torch hands over several gradients as one, f of each: the kernels read memory. A vectorised Jacobian
+// (is_grads_batched) and torch.func.vmap wrap them in two different ways.
+template <class F>
+Tensor of_each(const Tensor& grad, const F& f) {
+  if (const auto* batch = at::functorch::maybeGetBatchedImpl(grad))
+    return at::functorch::makeBatched(stack_of(batch->value().movedim(batch->bdim(), 0), f), 0, batch->level());
+  if (const auto* batch = at::maybeGetBatchedImpl(grad)) {
+    std::vector<int64_t> from, to, sizes;
+    at::BatchDims dims;
+    for (const at::BatchDim& b : batch->bdims()) {
+      from.push_back(b.dim());
+      sizes.push_back(batch->value().size(b.dim()));
+      to.push_back(static_cast<int64_t>(to.size()));
+      dims.emplace_back(b.level(), to.back());
+    }
+    const Tensor out = stack_of(batch->value().movedim(from, to).flatten(0, to.back()), f);
+    return at::makeBatched(out.unflatten(0, sizes), dims);
+  }
+  return f(grad);
+}
+
 Tensor backward_of(AutogradContext* ctx, const Tensor& upstream) {
   if (!upstream.defined()) return Tensor();
   if (at::GradMode::is_enabled())
     throw std::runtime_error("the losses over logits are differentiable once: no create_graph=True on the device");
-  const Tensor grad = upstream.resolve_neg();  // complex products' backwards pass tensors whose memory holds their negative
   const auto t = ctx->get_saved_variables();
   const Tensor &z = t[0], &labels = t[1], &mask = t[2], &index = t[3], &share = t[4], &saved = t[5];
   const auto k = ctx->saved_data["k"].toTuple();
   const double temperature = k->elements()[0].toDouble();
   const int64_t reduction = k->elements()[1].toInt(), coef = k->elements()[2].toInt();
-  on_device({labels, mask, index, share, saved, grad}, z);
+  on_device({labels, mask, index, share, saved, upstream}, z);
   const c10::OptionalDeviceGuard guard(z.device());
   const e4b_logits d = describe(z, labels, mask, temperature);
   const int64_t rows = d.seqs * d.tokens;
-  const Tensor out = at::empty(z.sizes(), z.options().memory_format(c10::MemoryFormat::Contiguous));
   float* at = ptr<float>(saved);
   float* behind = at + 4 * rows;
-  const int64_t grad_strides[2] = {grad.dim() > 0 ? grad.stride(0) : 0, grad.dim() > 1 ? grad.stride(1) : 0};
   const int64_t coef_strides[2] = {coef == 2 ? d.tokens : 1, coef == 2 ? 1 : 0};
   const float* coef_at = coef ? behind : nullptr;
   if (coef == 2) behind += rows;
   // the means' factors, where the loss is one of means over tokens
   const bool means = reduction != E4B_REDUCE_NONE && coef != 1;
-  check("e4b_loss_backward",
-        e4b_loss_backward(&d, at, ptr<const float>(grad), grad.dim() > 0 ? grad.size(0) : 1, grad_strides, coef_at,
-                          coef_strides, means ? behind : nullptr, reduction == E4B_REDUCE_SEQUENCE, ptr<const int64_t>(index),
-                          ptr<const float>(share), index.defined() ? static_cast<int32_t>(index.size(2)) : 0, out.data_ptr(),
-                          stream_of(z)));
-  return out;
+  return of_each(upstream, [&](const Tensor& one) {
+    const Tensor grad = one.resolve_neg();  // complex products' backwards pass tensors whose memory holds their negative
+    const Tensor out = at::empty(z.sizes(), z.options().memory_format(c10::MemoryFormat::Contiguous));
+    const int64_t grad_strides[2] = {grad.dim() > 0 ? grad.stride(0) : 0, grad.dim() > 1 ? grad.stride(1) : 0};
+    check("e4b_loss_backward",
+          e4b_loss_backward(&d, at, ptr<const float>(grad), grad.dim() > 0 ? grad.size(0) : 1, grad_strides, coef_at,
+                            coef_strides, means ? behind : nullptr, reduction == E4B_REDUCE_SEQUENCE, ptr<const int64_t>(index),
+                            ptr<const float>(share), index.defined() ? static_cast<int32_t>(index.size(2)) : 0, out.data_ptr(),
+                            stream_of(z)));
+    return out;
+  });
 }
 
 // An empty loss of the reduction's shape, and the number of its means.

@@ -1048,3 +1048,27 @@ def test_references_in_64_bits_behind_the_mask():
         for a, b in zip(e4b.preference_loss(z, labels, sums, mask=mask, average=average),
                         e4b.preference_loss(z, labels, sums.double(), mask=mask, average=average)):
             assert torch.equal(a, b)
+
+
+def test_batched_upstream_gradients():
+    """Several upstream gradients at once (a vectorised Jacobian): each one's gradient as by itself."""
+    z, labels, mask, index, teacher, old = _inputs(torch.float32, 4, 3, 120)
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        leaf = z.detach().requires_grad_()
+        loss = f(leaf)
+        ups = torch.randn(5, *loss.shape, generator=_gen(100)).to(DEV)
+        want = torch.stack([torch.autograd.grad(loss, leaf, u, retain_graph=True)[0] for u in ups])
+        (got,) = torch.autograd.grad(loss, leaf, ups, is_grads_batched=True, retain_graph=True)
+        assert torch.equal(got, want), name
+        strided = ups.movedim(0, -1).contiguous().movedim(-1, 0)
+        (got,) = torch.autograd.grad(loss, leaf, strided, is_grads_batched=True, retain_graph=True)
+        assert torch.equal(got, want), name
+        jacobian = torch.autograd.functional.jacobian(f, z.detach(), vectorize=True)
+        ones = torch.autograd.functional.jacobian(f, z.detach())
+        assert torch.equal(jacobian, ones) and ones.any(), name
+    lp = e4b.token_logprobs(leaf, labels)
+    one = torch.ones_like(lp)
+    twice = torch.func.vmap(lambda a: torch.func.vmap(lambda b: torch.autograd.grad(lp, leaf, one * a * b, retain_graph=True)[0])(
+        torch.arange(1.0, 4.0, device=DEV)))(torch.arange(1.0, 3.0, device=DEV))
+    (base,) = torch.autograd.grad(lp, leaf, one * 2, retain_graph=True)
+    assert torch.equal(twice[1, 0], base) and twice.shape == (2, 3, *leaf.shape)
