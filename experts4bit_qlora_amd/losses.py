@@ -4,8 +4,8 @@
 from an older or a reference model), ``preference_loss`` (paired log ratios of chosen and rejected answers),
 ``policy_loss`` (clipped ratios with a KL term) and ``distill_loss`` (divergence from a teacher's top logits). On a HIP
 device each reads the logits once forward and once backward (``csrc/losses.h``) and keeps a few floats per token
-between; tensors elsewhere, other dtypes, sizes beyond the kernels' limits, and tensors that a transform, a trace or
-forward-mode differentiation follows take the torch formulation, which is the definition.
+between; tensors elsewhere, other dtypes, sizes beyond the kernels' limits, tensors that a trace or forward-mode differentiation
+follows, and all calls inside a transform (``torch.func``) take the torch formulation, which is the definition.
 
 Logits are ``[..., tokens, vocab]``; the leading axes are sequences. They may be a view whose rows lie at any stride
 (``logits[:, :-1]`` is not copied). The gradient of such a view is copied into the whole's by autograd: shifting the
@@ -90,6 +90,8 @@ def _fits(z: torch.Tensor, temperature: float, *others) -> bool:
     """Whether the kernels may take these: plain device tensors, in memory as they are to be read, within the limits of
     ``e4b_logits``."""
     if not _on_kernel(z) or z.is_neg():
+        return False
+    if torch._C._are_functorch_transforms_active():  # they admit no autograd function of the extension, whatever it is given
         return False
     wrapped = torch._C._functorch.is_functorch_wrapped_tensor
     for t in others:

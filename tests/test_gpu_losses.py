@@ -1072,3 +1072,16 @@ def test_batched_upstream_gradients():
         torch.arange(1.0, 4.0, device=DEV)))(torch.arange(1.0, 3.0, device=DEV))
     (base,) = torch.autograd.grad(lp, leaf, one * 2, retain_graph=True)
     assert torch.equal(twice[1, 0], base) and twice.shape == (2, 3, *leaf.shape)
+
+
+def test_logits_that_a_transform_leaves_alone():
+    """Inside vmap and grad, logits that the transform does not follow: the torch formulation, and no error."""
+    z, labels, mask, index, teacher, old = _inputs(torch.float32, 4, 6, 300)
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        leaf = z.detach().requires_grad_()
+        for logits in (z, leaf):
+            total = f(logits).detach().sum()
+            got = torch.func.vmap(lambda a: a * f(logits).sum())(torch.arange(1.0, 4.0, device=DEV)).detach()
+            assert torch.allclose(got, total * torch.arange(1.0, 4.0, device=DEV), rtol=1e-4), name
+            assert torch.allclose(torch.func.grad(lambda a: a * f(logits).detach().sum())(torch.ones((), device=DEV)), total,
+                                  rtol=1e-4), name

@@ -329,3 +329,22 @@ def test_narrow_and_unsigned_labels_and_indexes(dtype, vocab):
         assert torch.equal(got, want) and want.any()
         ours, theirs = (torch.autograd.grad(v.sum(), z)[0] for v in (got, want))
         assert torch.equal(ours, theirs) and theirs.any()
+
+
+def test_logits_that_a_transform_leaves_alone(monkeypatch):
+    """Inside vmap, grad and jvp the kernels' autograd functions may not be called, whatever tensors they are given: logits that
+    the transform does not follow (seen here as device tensors) take the torch formulation too."""
+    z, labels, mask = _batch(dtype=torch.float32)
+    ref = torch.randn(4, 5, generator=_gen(11)) - 3
+    want = [v.detach() for _, v in _every_loss(z, labels, mask, ref)]
+    monkeypatch.setattr(L, "_on_kernel", lambda t: True)
+    monkeypatch.setattr(L.N, "torch_lib", None)
+    w = torch.arange(1.0, 4.0)
+
+    def scaled(a):
+        return torch.stack([(a * v).sum() for _, v in _every_loss(z, labels, mask, ref)])
+
+    sums = torch.stack([v.sum() for v in want])
+    assert torch.allclose(torch.func.vmap(scaled)(w), w[:, None] * sums)
+    assert torch.allclose(torch.func.jacrev(scaled)(w[0]), sums)
+    assert torch.allclose(torch.func.jvp(scaled, (w[0],), (w[1],))[1], 2 * sums)
