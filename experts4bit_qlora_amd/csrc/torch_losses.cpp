@@ -7,6 +7,7 @@
 #include <ATen/functorch/BatchedTensorImpl.h>
 // behind the one above, whose own calls it would make ambiguous
 #include <ATen/LegacyBatchedTensorImpl.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -82,6 +83,11 @@ hipStream_t stream_of(const Tensor& z) { return c10::hip::getCurrentHIPStream(z.
 Tensor floats(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options().dtype(torch::kFloat)); }
 
 Tensor or_undefined(const Maybe& t) { return t ? *t : Tensor(); }
+
+// What a graph may save of a tensor made in inference mode (sampled tokens, a teacher's entries): a copy.
+Tensor keepable(const Tensor& t) {
+  return t.defined() && t.is_inference() && !c10::InferenceMode::is_enabled() ? t.clone() : t;
+}
 
 // What a backward needs beside the tensors it saves: (logits, labels, mask, index, share, saved).
 struct Kept {
@@ -179,7 +185,7 @@ struct Logprobs : Function<Logprobs> {
     if (graph) saved = floats({4 * d.seqs * d.tokens}, z);
     check("e4b_token_logprobs", e4b_token_logprobs(&d, ptr<float>(logps), ptr<float>(saved), stream_of(z)));
     if (graph) {
-      ctx->save_for_backward({z, labels, mask, Tensor(), Tensor(), saved});
+      ctx->save_for_backward({z, keepable(labels), keepable(mask), Tensor(), Tensor(), saved});
       keep(ctx, {temperature, E4B_REDUCE_NONE, 0});
       ctx->set_materialize_grads(false);
     }
@@ -212,7 +218,7 @@ struct Preference : Function<Preference> {
           e4b_preference_loss(&d, ptr<const void>(ref), reference_kind(ref), static_cast<int32_t>(kind),
                               static_cast<float>(beta), static_cast<float>(smoothing), average, ptr<float>(loss),
                               ptr<float>(rewards), at, at + 4 * rows, stream_of(z)));
-    ctx->save_for_backward({z, labels, mask, Tensor(), Tensor(), saved});
+    ctx->save_for_backward({z, keepable(labels), keepable(mask), Tensor(), Tensor(), saved});
     keep(ctx, {1.0, E4B_REDUCE_SEQUENCE, 1});
     ctx->mark_non_differentiable({rewards});
     ctx->set_materialize_grads(false);
@@ -243,7 +249,7 @@ struct Policy : Function<Policy> {
                           static_cast<float>(clip_lo), static_cast<float>(clip_hi), static_cast<float>(kl_coef),
                           static_cast<int32_t>(reduction), ptr<float>(logps), means ? inv + means : ptr<float>(loss), at, coef,
                           ptr<float>(loss), inv, stream_of(z)));
-    ctx->save_for_backward({z, labels, mask, Tensor(), Tensor(), saved});
+    ctx->save_for_backward({z, keepable(labels), keepable(mask), Tensor(), Tensor(), saved});
     keep(ctx, {temperature, reduction, 2});
     ctx->mark_non_differentiable({logps});
     ctx->set_materialize_grads(false);
@@ -272,7 +278,7 @@ struct Distill : Function<Distill> {
           e4b_distill_loss(&d, teacher.data_ptr(), dtype_code(teacher), ptr<const int64_t>(index),
                            static_cast<int32_t>(index.size(2)), static_cast<int32_t>(reduction), ptr<float>(share),
                            means ? inv + means : ptr<float>(loss), at, ptr<float>(loss), inv, stream_of(z)));
-    ctx->save_for_backward({z, Tensor(), mask, index, share, saved});
+    ctx->save_for_backward({z, Tensor(), keepable(mask), keepable(index), share, saved});
     keep(ctx, {temperature, reduction, 0});
     ctx->set_materialize_grads(false);
     return loss;

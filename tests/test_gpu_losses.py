@@ -1085,3 +1085,23 @@ def test_logits_that_a_transform_leaves_alone():
             assert torch.allclose(got, total * torch.arange(1.0, 4.0, device=DEV), rtol=1e-4), name
             assert torch.allclose(torch.func.grad(lambda a: a * f(logits).detach().sum())(torch.ones((), device=DEV)), total,
                                   rtol=1e-4), name
+
+
+def test_tokens_and_teachers_made_in_inference_mode():
+    """Sampled tokens, masks and a teacher's entries out of torch.inference_mode, logits that are trained."""
+    z, labels, mask, index, teacher, old = _inputs(torch.float32)
+    with torch.inference_mode():
+        made = [t.clone() for t in (labels, mask, index, teacher, old)]
+    assert all(t.is_inference() for t in made)
+    want, got = _step(z, labels, mask, index, teacher, old), _step(z, *made)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        got = [e4b.token_logprobs(z, *made[:2]), e4b.preference_loss(z, made[0], made[4], mask=made[1])[0],
+               e4b.policy_loss(z, made[0], made[4], made[4].sum(-1) + 9, made[4], kl_coef=0.1, mask=made[1])[0],
+               e4b.policy_loss(z, made[0], made[4], made[4], mask=made[1], reduction="sequence")[0],
+               e4b.distill_loss(z, made[3], made[2], mask=made[1], temperature=2.0)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        made_z = z.clone()
+    got = [e4b.token_logprobs(made_z, *made[:2]), e4b.preference_loss(made_z, labels, old, mask=mask)[0]]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
