@@ -372,7 +372,8 @@ E4B_DEV float teacher_loss(const LossArgs& a, int64_t at, const typename Piece<D
     }
     a.share[at * a.top + k] = p;
   }
-  if (none) r.s = 0.0f;  // nothing to differentiate
+  if (none) r.s = 0.0f;         // nothing to differentiate
+  if (norm != norm) r.s = norm;  // a teacher without a number: nor has any of the row's gradient one
   return tau * tau * wave_sum(sum);
 }
 

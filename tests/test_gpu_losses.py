@@ -1105,3 +1105,19 @@ def test_tokens_and_teachers_made_in_inference_mode():
         made_z = z.clone()
     got = [e4b.token_logprobs(made_z, *made[:2]), e4b.preference_loss(made_z, labels, old, mask=mask)[0]]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_teacher_without_a_number_leaves_no_gradient_unmarked():
+    """A teacher's NaN or +inf makes the token's loss NaN and its whole row's gradient, as the torch formulation has it."""
+    z = _logits((1, 4, 3000), torch.float32, 101)
+    teacher, index = _teacher(z, 5, 102)
+    teacher[0, 0, 3], teacher[0, 1, 0], teacher[0, 2, 1] = float("nan"), INF, -INF
+    outs = []
+    for dev in (DEV, "cpu"):
+        leaf = z.to(dev).requires_grad_()
+        loss = e4b.distill_loss(leaf, teacher.to(dev), index.to(dev), reduction="none")
+        (grad,) = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        outs.append((loss.detach().cpu().isnan(), grad.cpu().isnan()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert outs[0][0].tolist() == [[True, True, False, False]] and outs[0][1][0, :2].all() and not outs[0][1][0, 2:].any()
