@@ -792,7 +792,7 @@ size_t e4b_loss_workspace_bytes(const e4b_logits* z) {
   if (!z || z->seqs <= 0 || z->tokens <= 0 || z->seqs > e4b::kLossMaxSeqs || z->tokens > 0x7fffffffLL ||
       z->vocab > e4b::kLossMaxVocab)
     return 0;
-  return sizeof(float2) * z->seqs * z->tokens * e4b::loss_parts(*z);
+  return sizeof(e4b::LossPart) * z->seqs * z->tokens * e4b::loss_parts(*z);
 }
 
 int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStream_t stream) {

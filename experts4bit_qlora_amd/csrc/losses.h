@@ -251,11 +251,11 @@ E4B_DEV R of_waves(const R& mine) {
   return r;
 }
 
-template <int DT, int NT, class S>
-E4B_DEV PowerOf<S> row_power(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
+template <int DT, int NT>
+E4B_DEV PowerOf<double> row_power(const void* row, int V, int skip, float2 k, int begin = 0, int end = 0x7fffffff) {
   PowerOf<float> r;
   over_row<DT, NT, kRowUnroll, false, true>(row, V, skip, begin, end, [] {}, [&](const auto& x) { r.add(x, k); });
-  PowerOf<S> all;
+  PowerOf<double> all;
   all.n = r.n;
   all.s = r.s;
   all.join_lanes(kWave);
@@ -396,8 +396,8 @@ __global__ __launch_bounds__(kPartThreads) void loss_parts_kernel(LossArgs a) {
   const int V = static_cast<int>(a.z.vocab), own = static_cast<int>(reference_of<KIND>(a, at, tok));
   const int begin = part * step;
   if constexpr (KIND == kStats) {
-    const PowerOf<float> r = row_power<DT, kPartThreads, float>(tok.row, V, own, a.k, begin, begin + step);
-    if (threadIdx.x == 0) static_cast<float2*>(a.z.workspace)[blockIdx.x] = make_float2(r.n, r.s);
+    const PowerOf<double> r = row_power<DT, kPartThreads>(tok.row, V, own, a.k, begin, begin + step);
+    if (threadIdx.x == 0) static_cast<LossPart*>(a.z.workspace)[blockIdx.x] = {r.s, r.n};
   } else {
     float ref;
     const float s = row_sum<DT, kPartThreads, kRowUnroll, KIND == kScore, KIND != kDistill>(tok.row, V, own, ref, a.k, begin,
@@ -450,11 +450,11 @@ __global__ __launch_bounds__(NT) void loss_rows_kernel(LossArgs a, int64_t begin
   if constexpr (KIND == kStats) {
     own = P::one(row[first]);
     if constexpr (SPLIT) {
-      const float2* parts = static_cast<const float2*>(a.z.workspace) + at * a.parts;
-      for (int i = lane; i < a.parts; i += kWave) power.join(parts[i].x, parts[i].y);
+      const LossPart* parts = static_cast<const LossPart*>(a.z.workspace) + at * a.parts;
+      for (int i = lane; i < a.parts; i += kWave) power.join(parts[i].n, parts[i].s);
       power.join_lanes(kWave);
     } else {
-      power = row_power<DT, NT, double>(row, V, first, a.k);
+      power = row_power<DT, NT>(row, V, first, a.k);
     }
     // nothing summed: row_run decides
     sum = power.n == kNoPower ? __builtin_nanf("")

@@ -14,6 +14,11 @@ constexpr int64_t kLossMaxSeqs = int64_t(1) << 21;
 constexpr int64_t kLossMaxVocab = int64_t(1) << 30;  // a row's indexes stay in 32 bits
 
 constexpr int kPartValues = 8192;  // of a split row
+// What a part of a row leaves in the workspace: s 2^n the sum of its exponentials (kStats; the others' sums are fp32 alone).
+struct LossPart {
+  double s;
+  float n;
+};
 
 // Parts of a row in the forward: 0 (a workgroup takes the whole) or the workgroups that share it.
 int loss_parts(const e4b_logits& z);

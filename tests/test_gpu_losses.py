@@ -1121,3 +1121,27 @@ def test_teacher_without_a_number_leaves_no_gradient_unmarked():
     for a, b in zip(*outs):
         assert torch.equal(a, b)
     assert outs[0][0].tolist() == [[True, True, False, False]] and outs[0][1][0, :2].all() and not outs[0][1][0, 2:].any()
+
+
+@pytest.mark.parametrize("dtype,V", ((torch.bfloat16, 152064), (torch.float32, 100003)))
+def test_parts_of_a_long_row_are_joined_in_64_bits(dtype, V):
+    """A row of zeros with one logit v in each part of 8,192, e^v = 0.94 of 2^-12: a thread's 32 values keep it (their partial
+    sums, below 32, round 13 times by 2^-20 or less: 1.3e-5), while beside a part's 8,191 ones it is less than half of fp32's
+    last bit and would be lost, 2.3e-4 a part and 2.7e-8 of the row's sum. The ones themselves are exact."""
+    per, v = 8192, -8.375
+    z = torch.zeros(2, 1, V, dtype=dtype)
+    parts = V // per  # whole ones
+    for i in range(2):
+        for p in range(parts):
+            z[i, 0, p * per + (377 * p + 1023 * i + 100) % per] = v
+    labels = torch.tensor([[5], [V - 1]])
+    assert not z.gather(-1, labels.unsqueeze(-1)).any()
+    few = z.double().exp().sum(-1) - 1
+    assert ((z != 0).sum(-1) == parts).all()
+    lp = -torch.log1p(few)
+    ref = lp.float()
+    rewards = e4b.preference_loss(z.to(DEV), labels.to(DEV), ref.to(DEV), beta=1.0)[1].cpu().double()
+    want = (lp - ref.double())[:, 0]
+    bound = parts * 13 * 2.0 ** -20 / few[:, 0] + 4 * U * want.abs() + parts * 2.3e-4 * 16 * U / few[:, 0]
+    assert bound.max() < 2e-9
+    assert ((rewards - want).abs() <= bound).all(), (rewards - want, bound)
