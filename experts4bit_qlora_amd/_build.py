@@ -6,7 +6,7 @@
 pair, all in parallel, then links them into ``experts4bit_qlora_amd/libe4b_amd.so``. The output is written to a temporary
 name and renamed, so a failed build never leaves a half-written library behind. ``csrc/torch_losses.cpp``, host code that calls
 the library from torch's autograd, becomes ``experts4bit_qlora_amd/libe4b_torch.so`` the same way, with the host compiler and
-torch's headers.
+torch's headers; the library is built without it where that fails or is not asked for (``build(binding=False)``).
 """
 from __future__ import annotations
 
@@ -16,6 +16,7 @@ import subprocess
 import sys
 import sysconfig
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
@@ -61,7 +62,7 @@ def _run_all(cmds):
         _, err = p.communicate()
         err = "\n".join(l for l in err.splitlines() if noise not in l)
         if p.returncode != 0:
-            failed.append(f"hipcc failed ({p.returncode}):\n{' '.join(cmd)}\n{err}")
+            failed.append(f"{os.path.basename(cmd[0])} failed ({p.returncode}):\n{' '.join(cmd)}\n{err}")
         elif err.strip():
             msgs.append(err)
     if failed:
@@ -82,32 +83,53 @@ def _torch_commands(obj: str, out: str):
     return compile_, link
 
 
-def build(verbose: bool = False) -> str:
+def _library(tmpdir: str) -> list[str]:
+    """libe4b_amd.so: the messages of its compilation. A binding of an older library goes with that library."""
     cc = hipcc()
     inc = [f"-I{CSRC}", f"-I{INCLUDE}"]
-    with tempfile.TemporaryDirectory(prefix="e4b_build_") as tmpdir:
-        objs, cmds = [], []
-        for name, src in (("e4b_amd.o", SRC), ("mx_gemm.o", MX_SRC), ("gate.o", GATE_SRC),
-                          ("losses.o", LOSSES_SRC)):
-            obj = os.path.join(tmpdir, name)
-            cmds.append([cc, *FLAGS, *inc, "-c", "-o", obj, src])
-            objs.append(obj)
-        for dt, fmt in DECODE_PAIRS:
-            obj = os.path.join(tmpdir, f"decode_{dt}_{fmt}.o")
-            cmds.append([cc, *FLAGS, *inc, f"-DE4B_INST_DT={dt}", f"-DE4B_INST_FMT={fmt}", "-c", "-o", obj,
-                         DECODE_SRC])
-            objs.append(obj)
-            obj = os.path.join(tmpdir, f"gemm_{dt}_{fmt}.o")
-            cmds.append([cc, *FLAGS, *inc, f"-DE4B_INST_DT={dt}", f"-DE4B_INST_FMT={fmt}", "-c", "-o", obj,
-                         GEMM_SRC])
-            objs.append(obj)
-        torch_compile, torch_link = _torch_commands(os.path.join(tmpdir, "torch_losses.o"), TORCH_OUT + ".tmp")
-        msgs = _run_all([torch_compile, *cmds])
-        tmp = OUT + ".tmp"
-        msgs += _run_all([[cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]])
-        os.replace(tmp, OUT)
-        msgs += _run_all([torch_link])
-        os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
+    objs, cmds = [], []
+    for name, src in (("e4b_amd.o", SRC), ("mx_gemm.o", MX_SRC), ("gate.o", GATE_SRC),
+                      ("losses.o", LOSSES_SRC)):
+        obj = os.path.join(tmpdir, name)
+        cmds.append([cc, *FLAGS, *inc, "-c", "-o", obj, src])
+        objs.append(obj)
+    for dt, fmt in DECODE_PAIRS:
+        obj = os.path.join(tmpdir, f"decode_{dt}_{fmt}.o")
+        cmds.append([cc, *FLAGS, *inc, f"-DE4B_INST_DT={dt}", f"-DE4B_INST_FMT={fmt}", "-c", "-o", obj,
+                     DECODE_SRC])
+        objs.append(obj)
+        obj = os.path.join(tmpdir, f"gemm_{dt}_{fmt}.o")
+        cmds.append([cc, *FLAGS, *inc, f"-DE4B_INST_DT={dt}", f"-DE4B_INST_FMT={fmt}", "-c", "-o", obj,
+                     GEMM_SRC])
+        objs.append(obj)
+    msgs = _run_all(cmds)
+    tmp = OUT + ".tmp"
+    msgs += _run_all([[cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]])
+    if os.path.exists(TORCH_OUT):
+        os.remove(TORCH_OUT)
+    os.replace(tmp, OUT)
+    return msgs
+
+
+def _binding_object(tmpdir: str):
+    """(link command of libe4b_torch.so, the messages of its compilation)"""
+    compile_, link = _torch_commands(os.path.join(tmpdir, "torch_losses.o"), TORCH_OUT + ".tmp")
+    return link, _run_all([compile_])
+
+
+def build(verbose: bool = False, binding: bool = True) -> str:
+    """The library and, with ``binding``, what binds it to torch's autograd. The library needs hipcc alone: where the binding
+    fails it is in place all the same, without the binding, and the error is raised then."""
+    with tempfile.TemporaryDirectory(prefix="e4b_build_") as tmpdir, ThreadPoolExecutor(1) as beside:
+        compiled = beside.submit(_binding_object, tmpdir) if binding else None
+        msgs = _library(tmpdir)
+        if binding:
+            try:
+                link, more = compiled.result()
+                msgs += more + _run_all([link])
+            except Exception as e:
+                raise RuntimeError(f"{OUT} is built, its binding to torch is not: {e}") from e
+            os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     if verbose and msgs:
         print("\n".join(msgs), file=sys.stderr)
     return OUT
