@@ -47,7 +47,7 @@ def _sequences(logits: torch.Tensor):
 
 
 def _integers(name: str, t: torch.Tensor, logits: torch.Tensor, shape) -> None:
-    if t.shape != shape or t.is_floating_point() or t.dtype == torch.bool:
+    if t.shape != shape or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{name} must be integers {list(shape)}, got {t.dtype} {list(t.shape)}")
     if t.device != logits.device:
         raise ValueError(f"logits and {name} must be on one device")

@@ -348,3 +348,12 @@ def test_logits_that_a_transform_leaves_alone(monkeypatch):
     assert torch.allclose(torch.func.vmap(scaled)(w), w[:, None] * sums)
     assert torch.allclose(torch.func.jacrev(scaled)(w[0]), sums)
     assert torch.allclose(torch.func.jvp(scaled, (w[0],), (w[1],))[1], 2 * sums)
+
+
+def test_complex_labels_are_refused():
+    z, labels, mask = _batch()
+    for f, args in ((e4b.token_logprobs, ()), (e4b.preference_loss, ()), (e4b.policy_loss, (torch.zeros(4, 5), torch.zeros(4)))):
+        with pytest.raises(ValueError, match="labels must be integers"):
+            f(z, labels.to(torch.complex64), *args)
+    with pytest.raises(ValueError, match="teacher_index must be integers"):
+        e4b.distill_loss(z, torch.zeros(4, 5, 2), torch.zeros(4, 5, 2, dtype=torch.complex64))
