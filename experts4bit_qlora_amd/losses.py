@@ -74,9 +74,11 @@ def _mask(mask, logits: torch.Tensor, shape):
     return mask if mask.dim() <= 2 else mask.reshape(shape[:-1].numel(), shape[-1])
 
 
-def _temperature(t: float) -> float:
+def _temperature(t: float, logits: torch.Tensor) -> float:
     if not (t > 0 and math.isfinite(t)):
         raise ValueError(f"temperature={t} is not positive and finite")
+    if not 2.0 ** -126 <= t <= 2.0 ** 126 and logits.dtype != torch.float64:  # rows are divided by it in fp32
+        raise ValueError(f"temperature={t}: it or its inverse is not a normal fp32 number")
     return float(t)
 
 
@@ -129,10 +131,11 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tenso
                    temperature: float = 1.0) -> torch.Tensor:
     """Log-probability of each label under ``softmax(logits / temperature)``: logits ``[..., T, V]``, labels ``[..., T]``
     integers, mask ``[T]`` or ``[..., T]`` -> fp32 ``[..., T]`` (fp64 for fp64 logits), 0 where a token does not count.
+    The temperature and its inverse are normal fp32 numbers (for fp64 logits: any positive finite one).
     Differentiable with respect to the logits (once)."""
     z, shape = _sequences(logits)
     _integers("labels", labels, logits, shape)
-    m, t = _mask(mask, logits, shape), _temperature(temperature)
+    m, t = _mask(mask, logits, shape), _temperature(temperature, logits)
     flat = z.shape[:2]
     if _fits(z, t, labels, m):
         logps = N.torch_lib().token_logprobs(_rows(z), _constant(labels, torch.int64, flat), _contiguous(m), t)
@@ -177,8 +180,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     reference model, ``d = (S_c - r_c) - (S_r - r_r)`` and ``h = beta d``: ``"sigmoid"`` ``-(1 - e) log sigmoid(h) - e
     log sigmoid(-h)`` with ``e = label_smoothing``, ``"hinge"`` ``max(0, 1 - h)``, ``"ipo"`` ``(d - 1 / (2 beta))^2``.
     ``ref_logps``: per token ``[2B, T]`` as ``token_logprobs`` gives them (the difference is then summed in 64 bits
-    token by token), or the answers' sums (means) ``[2B]``, fp64 ones as they are; None: zeros. ``rewards = beta (S - r)``, constants to the
-    gradient. The loss is differentiable with respect to the logits (once)."""
+    token by token), or the answers' sums (means) ``[2B]``, fp64 ones as they are; None: zeros. ``rewards = beta (S - r)``,
+    constants to the gradient. The loss is differentiable with respect to the logits (once)."""
     if logits.dim() != 3 or logits.shape[0] % 2:
         raise ValueError(f"logits must be [2 * pairs, tokens, vocab], got {list(logits.shape)}")
     z, shape = _sequences(logits)
@@ -257,7 +260,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     lo, hi = clip
     if not (0 <= lo <= 1 and 0 <= hi and math.isfinite(hi)):
         raise ValueError(f"clip={tuple(clip)}: below in [0, 1], above not negative")
-    m, t, red = _mask(mask, logits, shape), _temperature(temperature), _reduction(reduction)
+    m, t, red = _mask(mask, logits, shape), _temperature(temperature, logits), _reduction(reduction)
     ref, flat = ref_logps if kl_coef else None, z.shape[:2]
     of_advantages = flat if advantages.dim() == len(shape) else flat[:1]
     if _fits(z, t, labels, m, old_logps, advantages, ref):
@@ -319,7 +322,7 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     K = teacher_index.shape[-1]
     _integers("teacher_index", teacher_index, logits, (*shape, K))
     _floats("teacher_logits", teacher_logits, logits, (*shape, K))
-    m, t, red = _mask(mask, logits, shape), _temperature(temperature), _reduction(reduction)
+    m, t, red = _mask(mask, logits, shape), _temperature(temperature, logits), _reduction(reduction)
     flat = (*z.shape[:2], K)
     if _fits(z, t, m, teacher_logits, teacher_index) and K <= _MAX_TOP and teacher_logits.dtype in ops._DT:
         loss = N.torch_lib().distill_loss(_rows(z), _contiguous(m), _constant(teacher_logits, teacher_logits.dtype, flat),

@@ -357,3 +357,19 @@ def test_complex_labels_are_refused():
             f(z, labels.to(torch.complex64), *args)
     with pytest.raises(ValueError, match="teacher_index must be integers"):
         e4b.distill_loss(z, torch.zeros(4, 5, 2), torch.zeros(4, 5, 2, dtype=torch.complex64))
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_temperatures_beyond_the_32_bits_of_the_logits_are_refused(dtype):
+    """A temperature, or its inverse, that fp32 does not hold as a normal number divided rows into NaN; fp64 logits take it."""
+    z, labels, _ = _batch(dtype=dtype)
+    teacher, index = torch.zeros(4, 5, 2), torch.zeros(4, 5, 2, dtype=torch.int64)
+    for t in (1e-46, 1e-39, 3e38, 1e39):
+        for call in (lambda a: e4b.token_logprobs(a, labels, temperature=t),
+                     lambda a: e4b.policy_loss(a, labels, torch.zeros(4, 5), torch.zeros(4), temperature=t),
+                     lambda a: e4b.distill_loss(a, teacher, index, temperature=t)):
+            with pytest.raises(ValueError, match="temperature"):
+                call(z)
+        assert torch.isfinite(e4b.token_logprobs(z.double(), labels, temperature=max(t, 1e-39))).any()
+    for t in (1.2e-38, 8e37):
+        assert not e4b.token_logprobs(z, labels, temperature=t).isnan().any()
