@@ -30,14 +30,25 @@ void rows_of(const LossArgs& a, hipStream_t s) {
                          first);
     });
   };
-  // Threads a row by its bytes, us by 128 / 256 / 512 / 1,024 threads: 5,500 rows of 1,000 bf16 logits 7.3 / 9.8 / 15 / 27; of
-  // 8,000 23 / 23.5 / 28 / 45; of 32,000 76 / 69 / 69 / 85; of 50,257 114 / 109 / 106 / 105; of 128,000 283 / 269 / 268 / 253. 37
-  // rows of 50,257: - / 7.4 / 6.3 / 6.4, of 128,000: - / 13.6 / 11.5 / 10.6.
+  // Threads a row by its bytes, us by 128 / 256 / 512 / 1,024 threads for 1,000 rows and for 5,500, bf16 logits read from
+  // memory (log-probabilities that a backward follows):
+  //     4,096 bytes   4.1 /  4.3 /  4.8 /  6.9     9.1 / 10.9 / 18.8 / 30.9
+  //     6,000         4.7 /  4.7 /  5.1 /  7.2    11.4 / 13.1 / 20.2 / 33.0
+  //    32,768         8.8 /  8.8 /  9.0 / 11.6    34.7 / 32.1 / 32.5 / 54.3
+  //    48,000        12.3 / 12.3 / 11.9 / 13.9    50.1 / 47.7 / 46.1 / 62.9
+  //   114,688        22.3 / 22.9 / 22.6 / 24.1     112 /  107 /  106 /  103
+  //   144,000        27.8 / 28.2 / 27.3 / 27.3     140 /  135 /  132 /  127
+  //   256,000        46.3 / 47.8 / 46.7 / 46.1     246 /  235 /  232 /  224
+  // fp32 rows of 114,688 bytes 21.8 / 22.1 / 22.0 / 22.8 and 109 / 106 / 105 / 102, of 131,072 25.1 / 25.8 / 24.2 / 23.6 and 124 /
+  // 122 / 119 / 114, of 160,000 30.0 / 30.2 / 30.0 / 29.1 and 152 / 148 / 145 / 140; a preference's statistics, bf16, 114,688 bytes
+  // 23.6 / 24.5 / 25.7 / 26.8 and 118 / 112 / 110 / 120, 160,000 32.6 / 34.2 / 34.9 / 33.8 and 163 / 155 / 153 / 147. 37 rows of
+  // 100,514 bytes 10.0 / 6.9 / 5.6 / 5.9, of 256,000 19.3 / 12.2 / 10.0 / 9.5. Up to 300 rows 512 threads gain 0.6 us at 16,000
+  // bytes already (5.4 -> 4.7), where 5,500 rows lose 6 (21.7 -> 27.6).
   using std::integral_constant;
   const int64_t bytes = a.z.vocab * Piece<DT>::kBytes;
   if (bytes <= 4096) return with(integral_constant<int, 128>{});
   if (bytes <= 32768) return with(integral_constant<int, 256>{});
-  if (bytes < 128000) return with(integral_constant<int, 512>{});
+  if (bytes < 131072) return with(integral_constant<int, 512>{});
   with(integral_constant<int, 1024>{});
 }
 
