@@ -617,8 +617,9 @@ __global__ __launch_bounds__(kJoin) void pairs_kernel(PairArgs a) {
 // ---- backward
 
 constexpr int kBackThreads = 256;
-// Pieces a thread, 1 / 2 / 4 / 8 (before the accesses went past the caches): 5,500 x 128,000 bf16 505 / 509 / 542 / 554 us, 5,500
-// x 50,257 210 / 184 / 200 / 226.
+// Pieces a thread, 1 / 2 / 4 / 8, us: 5,500 x 128,000 bf16 480 / 459 / 519 / 521, 5,500 x 50,257 196 / 180 / 195 / 222, 1,000 x
+// 32,000 26.7 / 23.3 / 25.7 / 25.3, 250 x 50,257 12.1 / 11.7 / 11.1 / 14.0; fp32 5,500 x 128,000 910 / 935 / 1,055 / 1,040, 5,500 x
+// 50,257 378 / 368 / 421 / 438.
 constexpr int kBackUnroll = 2;
 
 // A workgroup takes kBackThreads * kBackUnroll pieces of one row's gradient: A q_j - A p_k at the row's entries (a label:

@@ -81,14 +81,20 @@ void backward_of(const LossBackwardArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// One CU takes ~7 us over the exponentials of 128,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
-// joined in a second launch, which costs the host 2.4 us with its workspace: rows where the GPU gains as much. Whole / split, us
-// on the GPU: 1 row of 100,003 bf16 7.6 / 7.1, of 128,000 9.5 / 6.9 (a call: 8.4 / 10.7), of 152,000 10.3 / 6.9; 64 of 128,000
-// 11.1 / 8.5, of 152,000 11.9 / 9.5; 128 of 152,000 12.4 / 12.4. fp32: 1 row of 50,257 5.8 / 5.6, of 80,000 8.1 / 5.8, of 128,000
-// 10.7 / 5.7; 64 of 80,000 10.7 / 10.0, of 128,000 14.1 / 11.2; 128 of 128,000 16.2 / 16.6.
+// One CU takes ~7 us over the exponentials of 100,000 logits, so few long rows are shared by a workgroup per 8,192 logits and
+// joined in a second launch, which with its workspace costs the host as much as the GPU gains on rows below this border. Whole /
+// split, us on the GPU, 1 / 37 / 64 rows: bf16 of 80,000 6.8 / 6.4, 7.2 / 7.9, 7.8 / 8.7; of 128,000 8.9 / 6.2, 10.4 / 8.0, 10.6 /
+// 8.5; of 152,000 9.7 / 6.5, 11.1 / 8.4, 11.1 / 9.5; fp32 of 80,000 7.6 / 6.2, 9.9 / 8.3, 10.4 / 9.7; of 100,003 7.9 / 6.3, 10.6 /
+// 8.2, 11.3 / 10.1; of 128,000 9.6 / 6.3, 12.9 / 9.2, 13.9 / 11.2; 128 rows gain nothing below 262,144 logits. A call whose rows
+// are split takes 10.2 us of host time, so for 1 / 8 / 37 / 64 rows a call takes at bf16 of 149,999 (whole) 9.3 / 9.5 / 9.6 / 10.0
+// and of 150,000 (split) 9.8 / 10.2 / 9.8 / 9.9; at fp32 of 99,999 (whole) 7.9 / 8.2 / 9.1 / 9.3 and of 100,000 (split) 9.7 / 10.1 /
+// 9.9 / 9.8, while of 75,000 split ones took 10.2 / 10.3 / 10.1 / 10.0 and whole ones 6.8 / 7.2 / 7.4 / 7.4: fp32 rows, half as
+// many logits to the byte, are split from 400,000 bytes on. A captured call, which waits for the GPU alone, would gain from
+// 200,000 on.
 int loss_parts(const e4b_logits& z) {
-  const int64_t bytes = z.vocab * (z.dtype == E4B_FP32 ? 4 : 2);
-  return z.seqs * z.tokens <= 64 && bytes >= 300000 ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
+  const bool wide = z.dtype == E4B_FP32;
+  const int64_t bytes = z.vocab * (wide ? 4 : 2);
+  return z.seqs * z.tokens <= 64 && bytes >= (wide ? 400000 : 300000) ? static_cast<int>(cdiv(z.vocab, kPartValues)) : 0;
 }
 
 void launch_loss_rows(LossKind kind, const LossArgs& a, hipStream_t s) {
