@@ -39,16 +39,17 @@ void rows_of(const LossArgs& a, hipStream_t s) {
   //   114,688        22.3 / 22.9 / 22.6 / 24.1     112 /  107 /  106 /  103
   //   144,000        27.8 / 28.2 / 27.3 / 27.3     140 /  135 /  132 /  127
   //   256,000        46.3 / 47.8 / 46.7 / 46.1     246 /  235 /  232 /  224
-  // fp32 rows of 114,688 bytes 21.8 / 22.1 / 22.0 / 22.8 and 109 / 106 / 105 / 102, of 131,072 25.1 / 25.8 / 24.2 / 23.6 and 124 /
-  // 122 / 119 / 114, of 160,000 30.0 / 30.2 / 30.0 / 29.1 and 152 / 148 / 145 / 140; a preference's statistics, bf16, 114,688 bytes
-  // 23.6 / 24.5 / 25.7 / 26.8 and 118 / 112 / 110 / 120, 160,000 32.6 / 34.2 / 34.9 / 33.8 and 163 / 155 / 153 / 147. 37 rows of
-  // 100,514 bytes 10.0 / 6.9 / 5.6 / 5.9, of 256,000 19.3 / 12.2 / 10.0 / 9.5. Up to 300 rows 512 threads gain 0.6 us at 16,000
-  // bytes already (5.4 -> 4.7), where 5,500 rows lose 6 (21.7 -> 27.6).
+  // fp32 rows of 114,688 bytes 21.8 / 22.1 / 22.0 / 22.8 and 109 / 106 / 105 / 102, of 128,000 25.0 / 24.8 / 24.4 / 25.4 and 123 /
+  // 119 / 116 / 112 (a training call over 2,400 of them, what the caches hold read from there: 156 by 512, 153 by 1,024), of
+  // 160,000 30.0 / 30.2 / 30.0 / 29.1 and 152 / 148 / 145 / 140; a preference's statistics, bf16, 114,688 bytes 23.6 / 24.5 / 25.7 /
+  // 26.8 and 118 / 112 / 110 / 120, 128,000 27.4 / 27.4 / 28.4 / 29.6 and 132 / 125 / 122 / 130, 160,000 32.6 / 34.2 / 34.9 / 33.8
+  // and 163 / 155 / 153 / 147. 37 rows of 100,514 bytes 10.0 / 6.9 / 5.6 / 5.9, of 256,000 19.3 / 12.2 / 10.0 / 9.5. Up to 300 rows
+  // 512 threads gain 0.6 us at 16,000 bytes already (5.4 -> 4.7), where 5,500 rows lose 6 (21.7 -> 27.6).
   using std::integral_constant;
   const int64_t bytes = a.z.vocab * Piece<DT>::kBytes;
   if (bytes <= 4096) return with(integral_constant<int, 128>{});
   if (bytes <= 32768) return with(integral_constant<int, 256>{});
-  if (bytes < 131072) return with(integral_constant<int, 512>{});
+  if (bytes < 122880) return with(integral_constant<int, 512>{});
   with(integral_constant<int, 1024>{});
 }
 
