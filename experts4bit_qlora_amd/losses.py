@@ -25,6 +25,7 @@ import torch
 
 from . import _native as N
 from . import ops
+from .quant import _forward_ad
 from .router import _on_kernel
 
 _PREFERENCE = {"sigmoid": N.PREFERENCE_SIGMOID, "hinge": N.PREFERENCE_HINGE, "ipo": N.PREFERENCE_IPO}
@@ -115,7 +116,7 @@ def _constant(t, dtype, shape):
     """A constant of the gradient, contiguous and of one dtype (or None)."""
     if t is None:
         return None
-    if t.requires_grad:
+    if t.requires_grad or _forward_ad._current_level >= 0:
         t = t.detach()
     if t.dtype != dtype:
         t = t.to(dtype)

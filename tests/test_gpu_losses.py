@@ -1145,3 +1145,18 @@ def test_parts_of_a_long_row_are_joined_in_64_bits(dtype, V):
     bound = parts * 13 * 2.0 ** -20 / few[:, 0] + 4 * U * want.abs() + parts * 2.3e-4 * 16 * U / few[:, 0]
     assert bound.max() < 2e-9
     assert ((rewards - want).abs() <= bound).all(), (rewards - want, bound)
+
+
+def test_constants_with_a_tangent():
+    """Inside forward-mode differentiation that follows everything but the logits: the values, without a tangent."""
+    import torch.autograd.forward_ad as fa
+
+    z, labels, mask, index, teacher, old = _inputs(torch.float32)
+    want = [e4b.policy_loss(z, labels, old, old.sum(-1), old, kl_coef=0.1)[0], e4b.preference_loss(z, labels, old)[0],
+            e4b.distill_loss(z, teacher, index)]
+    with fa.dual_level():
+        o, s, t = (fa.make_dual(v, torch.ones_like(v)) for v in (old, old.sum(-1), teacher))
+        got = [e4b.policy_loss(z, labels, o, s, o, kl_coef=0.1)[0], e4b.preference_loss(z, labels, o)[0],
+               e4b.distill_loss(z, t, index)]
+        assert all(fa.unpack_dual(g).tangent is None for g in got)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))

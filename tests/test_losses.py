@@ -373,3 +373,30 @@ def test_temperatures_beyond_the_32_bits_of_the_logits_are_refused(dtype):
         assert torch.isfinite(e4b.token_logprobs(z.double(), labels, temperature=max(t, 1e-39))).any()
     for t in (1.2e-38, 8e37):
         assert not e4b.token_logprobs(z, labels, temperature=t).isnan().any()
+
+
+def test_constants_with_a_tangent(monkeypatch):
+    """Forward-mode tangents of what is a constant to the gradient do not reach the extension, whose functions refuse them."""
+    import torch.autograd.forward_ad as fa
+
+    z, labels, _ = _batch(dtype=torch.float32)
+    old, adv, index = torch.randn(4, 5), torch.randn(4), torch.zeros(4, 5, 2, dtype=torch.int64)
+    seen = []
+
+    class Kernels:
+        def __getattr__(self, name):
+            def call(z, *args):
+                seen.append((name, [fa.unpack_dual(t).tangent for t in args if isinstance(t, torch.Tensor)]))
+                out = torch.zeros(())
+                return (out, torch.zeros(4, 5)) if name in ("preference_loss", "policy_loss") else out
+            return call
+
+    monkeypatch.setattr(L, "_on_kernel", lambda t: True)
+    monkeypatch.setattr(L.N, "torch_lib", lambda: Kernels())
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))  # noqa: E731
+        e4b.preference_loss(z, labels, dual(old))
+        e4b.policy_loss(z, labels, dual(old), dual(adv), dual(old), kl_coef=0.1)
+        e4b.distill_loss(z, dual(torch.randn(4, 5, 2)), index)
+    assert [n for n, _ in seen] == ["preference_loss", "policy_loss", "distill_loss"]
+    assert all(t is None for _, ts in seen for t in ts)
