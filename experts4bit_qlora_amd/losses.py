@@ -5,7 +5,8 @@ from an older or a reference model), ``preference_loss`` (paired log ratios of c
 ``policy_loss`` (clipped ratios with a KL term) and ``distill_loss`` (divergence from a teacher's top logits). On a HIP
 device each reads the logits once forward and once backward (``csrc/losses.h``) and keeps a few floats per token
 between; tensors elsewhere, other dtypes, sizes beyond the kernels' limits, tensors that a trace or forward-mode differentiation
-follows, and all calls inside a transform (``torch.func``) take the torch formulation, which is the definition.
+follows, and all calls inside a transform (``torch.func``) or a recording (``make_fx``) take the torch formulation, which is
+the definition.
 
 Logits are ``[..., tokens, vocab]``; the leading axes are sequences. They may be a view whose rows lie at any stride
 (``logits[:, :-1]`` is not copied). The gradient of such a view is copied into the whole's by autograd: shifting the
@@ -89,12 +90,23 @@ def _reduction(name: str) -> int:
     return _REDUCTION[name]
 
 
+_MODE = torch._C._TorchDispatchModeKey
+
+
+def _recorded() -> bool:
+    """Whether torch's operators are recorded or stood in for, which leaves out what a kernel does."""
+    mode = torch._C._get_dispatch_mode
+    return torch._C._len_torch_dispatch_stack() > 0 and any(mode(k) is not None for k in (_MODE.PROXY, _MODE.FAKE,
+                                                                                         _MODE.FUNCTIONAL))
+
+
 def _fits(z: torch.Tensor, temperature: float, *others) -> bool:
     """Whether the kernels may take these: plain device tensors, in memory as they are to be read, within the limits of
     ``e4b_logits``."""
     if not _on_kernel(z) or z.is_neg():
         return False
-    if torch._C._are_functorch_transforms_active():  # they admit no autograd function of the extension, whatever it is given
+    # transforms admit no autograd function of the extension, whatever it is given
+    if torch._C._are_functorch_transforms_active() or _recorded():
         return False
     wrapped = torch._C._functorch.is_functorch_wrapped_tensor
     for t in others:

@@ -1160,3 +1160,14 @@ def test_constants_with_a_tangent():
                e4b.distill_loss(z, t, index)]
         assert all(fa.unpack_dual(g).tangent is None for g in got)
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_recorded_calls_take_the_torch_formulation():
+    """A function that make_fx recorded, on other logits, forward and with its gradient."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    z, labels, mask, index, teacher, old = _inputs(torch.float32, 4, 6, 300)
+    other = z.flip(0) * 0.5
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        for g in (f, lambda a: torch.autograd.grad(f(a.requires_grad_()).sum(), a)[0]):
+            assert torch.allclose(make_fx(g)(z.clone())(other.clone()), g(other.clone()), rtol=1e-4, atol=1e-6), name

@@ -400,3 +400,19 @@ def test_constants_with_a_tangent(monkeypatch):
         e4b.distill_loss(z, dual(torch.randn(4, 5, 2)), index)
     assert [n for n, _ in seen] == ["preference_loss", "policy_loss", "distill_loss"]
     assert all(t is None for _, ts in seen for t in ts)
+
+
+def test_recorded_calls_take_the_torch_formulation(monkeypatch):
+    """make_fx records torch's operators: what a kernel writes is not among them, and the recorded function would return
+    memory that nothing fills. The logits are seen here as device tensors."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    z, labels, mask = _batch(dtype=torch.float32)
+    other = z.flip(0) * 0.5
+    want = [v for _, v in _every_loss(other, labels, mask)]
+    monkeypatch.setattr(L, "_on_kernel", lambda t: True)
+    monkeypatch.setattr(L.N, "torch_lib", None)
+    for mode in ("real", "fake", "symbolic"):
+        recorded = make_fx(lambda a: [v for _, v in _every_loss(a, labels, mask)], tracing_mode=mode,
+                           _allow_non_fake_inputs=True)(z)
+        assert all(torch.allclose(a, b, rtol=1e-5) for a, b in zip(recorded(other), want))
