@@ -8,6 +8,7 @@
 // behind the one above, whose own calls it would make ambiguous
 #include <ATen/LegacyBatchedTensorImpl.h>
 #include <c10/core/InferenceMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -100,6 +101,14 @@ void keep(AutogradContext* ctx, const Kept& k) {
   ctx->saved_data["k"] = c10::IValue(std::make_tuple(k.temperature, k.reduction, k.coef));
 }
 
+// Whether torch's operators are recorded or stood in for (make_fx): what a kernel writes is not among them.
+bool recorded() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (!Modes::any_modes_set()) return false;
+  return Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL);
+}
+
 template <class F>
 Tensor of_each(const Tensor& grad, const F& f);
 
@@ -136,6 +145,8 @@ Tensor backward_of(AutogradContext* ctx, const Tensor& upstream) {
   if (!upstream.defined()) return Tensor();
   if (at::GradMode::is_enabled())
     throw std::runtime_error("the losses over logits are differentiable once: no create_graph=True on the device");
+  if (recorded())
+    throw std::runtime_error("the losses' backward on the device cannot be recorded by itself: record the forward with it");
   const auto t = ctx->get_saved_variables();
   const Tensor &z = t[0], &labels = t[1], &mask = t[2], &index = t[3], &share = t[4], &saved = t[5];
   const auto k = ctx->saved_data["k"].toTuple();

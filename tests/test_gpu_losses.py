@@ -1171,3 +1171,16 @@ def test_recorded_calls_take_the_torch_formulation():
     for name, f in _every_loss(labels, old, teacher, index).items():
         for g in (f, lambda a: torch.autograd.grad(f(a.requires_grad_()).sum(), a)[0]):
             assert torch.allclose(make_fx(g)(z.clone())(other.clone()), g(other.clone()), rtol=1e-4, atol=1e-6), name
+
+
+def test_a_backward_recorded_by_itself_is_refused():
+    """Of a loss that was computed before the recording: what the kernel writes would not be in it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    z, labels, mask, index, teacher, old = _inputs(torch.float32, 4, 6, 300)
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        leaf = z.detach().requires_grad_()
+        loss = f(leaf)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(lambda up: torch.autograd.grad(loss, leaf, up, retain_graph=True)[0])(torch.ones_like(loss))
+        assert torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0].any(), name
