@@ -138,6 +138,9 @@ Tensor of_each(const Tensor& grad, const F& f) {
     const Tensor out = stack_of(batch->value().movedim(from, to).flatten(0, to.back()), f);
     return at::makeBatched(out.unflatten(0, sizes), dims);
   }
+  // followed by forward-mode differentiation: f is linear
+  if (const Tensor tangent = grad._fw_grad(0); tangent.defined())
+    return at::_make_dual(f(grad._fw_primal(0)), f(tangent), 0);
   return f(grad);
 }
 
@@ -164,7 +167,8 @@ Tensor backward_of(AutogradContext* ctx, const Tensor& upstream) {
   // the means' factors, where the loss is one of means over tokens
   const bool means = reduction != E4B_REDUCE_NONE && coef != 1;
   return of_each(upstream, [&](const Tensor& one) {
-    const Tensor grad = one.resolve_neg();  // complex products' backwards pass tensors whose memory holds their negative
+    // complex products' backwards pass tensors whose memory holds their negative; zeros may come without memory
+    const Tensor grad = one._is_zerotensor() ? at::zeros(one.sizes(), one.options()) : one.resolve_neg();
     const Tensor out = at::empty(z.sizes(), z.options().memory_format(c10::MemoryFormat::Contiguous));
     const int64_t grad_strides[2] = {grad.dim() > 0 ? grad.stride(0) : 0, grad.dim() > 1 ? grad.stride(1) : 0};
     check("e4b_loss_backward",

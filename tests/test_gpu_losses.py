@@ -1184,3 +1184,22 @@ def test_a_backward_recorded_by_itself_is_refused():
         with pytest.raises(RuntimeError, match="recorded"):
             make_fx(lambda up: torch.autograd.grad(loss, leaf, up, retain_graph=True)[0])(torch.ones_like(loss))
         assert torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0].any(), name
+
+
+def test_upstream_gradients_with_a_tangent():
+    """Forward-mode differentiation that follows the upstream gradient alone: the gradient is linear in it."""
+    import torch.autograd.forward_ad as fa
+
+    z, labels, mask, index, teacher, old = _inputs(torch.float32, 4, 6, 300)
+    for name, f in _every_loss(labels, old, teacher, index).items():
+        leaf = z.detach().requires_grad_()
+        loss = f(leaf)
+        up, along = (torch.randn(loss.shape, generator=_gen(103 + i)).to(DEV) for i in range(2))
+        want = [torch.autograd.grad(loss, leaf, u, retain_graph=True)[0] for u in (up, along)]
+        with fa.dual_level():
+            got = fa.unpack_dual(torch.autograd.grad(loss, leaf, fa.make_dual(up, along), retain_graph=True)[0])
+            assert torch.equal(got.primal, want[0]) and torch.equal(got.tangent, want[1]) and want[1].any(), name
+            (plain,) = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+            assert fa.unpack_dual(plain).tangent is None and torch.equal(plain, want[0])
+        (none,) = torch.autograd.grad(loss, leaf, torch._efficientzerotensor(loss.shape, device=DEV))
+        assert none.shape == leaf.shape and not none.any(), name
