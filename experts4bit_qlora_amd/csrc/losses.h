@@ -203,8 +203,9 @@ E4B_DEV bool in_room(float ref, float2 k, float sum) { return fabsf(ref * k.x) <
 // A sum s of 2^(x k - n) whose reference n is the running maximum of x k rounded up to a whole number: the largest terms' exponents
 // are the smallest, and so are their roundings, and a change of the reference is exact. Sequences' sums are made of these
 // (kStats): a rescaling by a rounded exponential is 3e-9 too small in the mean, and a row's ten of them added up over 2,048
-// tokens to 3e-6 of their ratio; the label as reference rounds the largest terms (60 tokens: 1.4e-6). Joins in 64 bits. 8,192
-// rows of 128,000: 229 us, against 222 with row_sum and 240 with a running maximum that is no power of two.
+// tokens to 3e-6 of their ratio; the label as reference rounds the largest terms (60 tokens: 1.4e-6). Lanes, waves and a split
+// row's parts are joined in 64 bits: in 32 a part's 8,192 logits lose up to 3e-8 of their sum. 8,192 rows of 128,000: 229 us,
+// against 222 with row_sum and 240 with a running maximum that is no power of two.
 constexpr float kNoPower = -1e30f;  // nothing summed yet
 template <class S>
 struct PowerOf {
@@ -542,7 +543,9 @@ E4B_DEV void block_sums(double (&v)[N]) {
   }
 }
 
-// A workgroup per group; sums in 64 bits, in an order that the sizes alone decide.
+// A workgroup per group; sums in 64 bits, in an order that the sizes alone decide. One workgroup for a mean over all tokens costs
+// 0.7 to 0.9 ns a row: a policy forward over 8,192 / 65,536 / 262,144 / 1,048,576 rows of 1,000 bf16 logits takes 17 / 94 / 420 /
+// 1,842 us with it and 11 / 57 / 237 / 916 without (a mean for each of 16 sequences: 14 / 62 / 250 / 979).
 __global__ __launch_bounds__(kJoin) void loss_mean_kernel(MeanArgs a) {
   const int64_t first = blockIdx.x * a.per;
   double v[2] = {0.0, 0.0};
@@ -624,7 +627,9 @@ constexpr int kBackUnroll = 2;
 
 // A workgroup takes kBackThreads * kBackUnroll pieces of one row's gradient: A q_j - A p_k at the row's entries (a label:
 // one entry with p = 1, A = -derivative / tau; a teacher: p_k, A = derivative * tau). Entries inside the workgroup's part are
-// listed in LDS in the order of k, and each thread takes those in its pieces before it rounds.
+// listed in LDS in the order of k, and each thread takes those in its pieces before it rounds: it walks the part's list, in the
+// order that decides the sum. 4,096 rows by 8 / 64 / 256 / 1,024 entries: of 2,000 bf16 logits 30 / 34 / 98 / 392 us, of 32,000 93 /
+// 107 / 217 / 673; of 128,000 by 64 / 1,024 356 / 1,199.
 template <int DT, bool TEACHER>
 __global__ __launch_bounds__(kBackThreads) void loss_backward_kernel(LossBackwardArgs a, int64_t begin, int parts) {
   using P = Piece<DT>;
