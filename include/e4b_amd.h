@@ -236,10 +236,11 @@ int e4b_token_logprobs(const e4b_logits* z, float* logps, float* stats, hipStrea
 
 /* Preference loss of the pairs (sequence b, chosen; sequence b + seqs / 2, rejected): S_i the sum of the counted
  * tokens' log-probabilities (their mean where `average`), d = (S_c - r_c) - (S_r - r_r). ref: log-probabilities under
- * the reference model by ref_kind (e4b_reference), per token [seqs, tokens] (then summed, or averaged, over the counted tokens
- * like the model's) or per sequence [seqs] (taken as they are), fp32 or fp64, NULL: zeros. loss fp32 [seqs / 2], rewards fp32 [seqs] = beta (S_i - r_i),
- * coef fp32 [seqs] = the loss's derivative by each of a sequence's log-probabilities, stats as above (required). seqs is
- * even. Sums in 64 bits, deterministic. Has no counterpart in the reference. */
+ * the reference model by ref_kind (e4b_reference), per token [seqs, tokens] (then summed, or averaged, over the counted
+ * tokens like the model's) or per sequence [seqs] (taken as they are), fp32 or fp64, NULL: zeros. loss fp32 [seqs / 2],
+ * rewards fp32 [seqs] = beta (S_i - r_i), coef fp32 [seqs] = the loss's derivative by each of a sequence's
+ * log-probabilities, stats as above (required). seqs is even. Sums in 64 bits, deterministic. Has no counterpart in the
+ * reference. */
 int e4b_preference_loss(const e4b_logits* z, const void* ref, int32_t ref_kind, int32_t kind, float beta,
                         float smoothing, int32_t average, float* loss, float* rewards, float* stats, float* coef,
                         hipStream_t stream);
